@@ -406,6 +406,128 @@ int32_t m1moe_dec_prefill(m1moe_dec_t dec, const int32_t* d_tokens, int32_t T,
 /* The current position (waits for the context stream). */
 int32_t m1moe_dec_position(m1moe_dec_t dec, int32_t* pos);
 
+/* ---- several conversations at once ---------------------------------------
+ * Building blocks for callers that run a batch of sequences through a layer
+ * (no counterpart in the reference, whose engine holds one conversation): a
+ * KV cache in pages, attention over it, and sampling.  Asynchronous on the
+ * context stream like the blocks above; lengths, positions and page numbers
+ * are read from device memory, so a captured graph serves later steps too. */
+
+/* A KV cache in pages, the caller's memory.  Position p of a sequence lies in
+ * page pages[p / page_size] of its page table, at slot p % page_size.
+ * Constraints: page_size is a power of two, 8 to 4096; num_pages >= 1;
+ * head_dim is 64, 128 or 256; num_kv_heads * head_dim <= 65536. */
+typedef struct {
+    void* d_k;             /* [num_pages][page_size][num_kv_heads][head_dim] */
+    void* d_v;             /* the same */
+    int32_t dtype;         /* M1MOE_F32 or M1MOE_BF16 */
+    int32_t num_pages;
+    int32_t page_size;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+} m1moe_paged_kv;
+
+/* The rows of one call: sequence s has the rows d_row_start[s] ..
+ * d_row_start[s + 1] - 1 (none, one, or a whole prompt), which are its last
+ * positions: row d_row_start[s] + i is at position d_kv_len[s] - n + i of its
+ * n rows.  num_rows is how many rows the caller's buffers hold; those outside
+ * every sequence are left as they were.
+ * prefix_len > 0: the first prefix_len positions of every sequence lie in the
+ * pages d_prefix_pages and are read there (attention computes them once for
+ * all; the sequences' own table entries of pages wholly inside the prefix are
+ * not read).  Every row is at a position past the prefix.
+ * Constraints: 1 <= num_seqs <= 1024; 1 <= num_rows <= 1048576; table_stride
+ * >= 1, table_stride * page_size <= 2^24 positions; 0 <= prefix_len <=
+ * table_stride * page_size.  In device memory: 0 <= d_row_start[s] <=
+ * d_row_start[s + 1] <= num_rows, n <= d_kv_len[s] <= table_stride *
+ * page_size, d_kv_len[s] - n >= prefix_len where n > 0.  A sequence that
+ * breaks this is skipped, a page outside the cache is not touched (attention
+ * reads page 0 in its place); either sets the device error flag, reported by
+ * the next m1moe_sync. */
+typedef struct {
+    int32_t num_seqs;
+    int32_t num_rows;
+    int32_t table_stride;           /* entries per row of d_pages */
+    int32_t prefix_len;
+    const int32_t* d_row_start;     /* [num_seqs + 1] */
+    const int32_t* d_kv_len;        /* [num_seqs], this call's rows included */
+    const int32_t* d_pages;         /* [num_seqs][table_stride] */
+    const int32_t* d_prefix_pages;  /* [ceil(prefix_len / page_size)], or NULL */
+} m1moe_paged_batch;
+
+/* What m1moe_kv_append reads and writes besides the cache.  Row strides are in
+ * elements and multiples of 16 bytes, at least a row's length (q, k and v may
+ * be columns of one matrix); pointers are 16-byte aligned. */
+typedef struct {
+    int32_t dtype;           /* of q, k, v and q_out: M1MOE_F32 or M1MOE_BF16 */
+    int32_t num_heads;       /* a multiple of the cache's num_kv_heads */
+    const void* d_q;         /* [num_rows][num_heads * head_dim], or NULL: k and v only */
+    const void* d_k;         /* [num_rows][num_kv_heads * head_dim] */
+    const void* d_v;         /* the same */
+    void* d_q_out;           /* as d_q (may be d_q itself, with its stride); NULL with d_q */
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const uint16_t* d_q_norm;  /* bf16 [head_dim] per-head RMSNorm weights, or NULL: no norm */
+    const uint16_t* d_k_norm;
+    float eps;
+    int32_t rotary_dim;      /* 0, or a multiple of 16 up to head_dim: rotated dims, from dim 0 */
+    int32_t interleaved;     /* pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2) */
+    float rope_amplitude;    /* factor of cos and sin (1 for unscaled RoPE) */
+    const float* d_inv_freq; /* f32 [rotary_dim / 2]: angle of pair i = position * inv_freq[i] */
+} m1moe_kv_append_args;
+
+/* One row of settings per row of logits, all in device memory; any but d_u may
+ * be NULL: temperature 1, no top-k, no top-p, no min-p. */
+typedef struct {
+    const float* d_u;            /* uniform draws in [0, 1) */
+    const float* d_temperature;  /* <= 0 (or NaN): the largest logit */
+    const int32_t* d_top_k;      /* <= 0: off */
+    const float* d_top_p;        /* >= 1 (or NaN): off */
+    const float* d_min_p;        /* <= 0 (or NaN): off */
+} m1moe_sample_params;
+
+/* The checks that the calls below make of these descriptions (host only). */
+int32_t m1moe_check_paged(const m1moe_paged_kv* kv, const m1moe_paged_batch* batch);
+
+/* For every row of the batch: q and k normalised per head (x * rsqrt(mean(x^2)
+ * + eps) * w, where a weight is given), their first rotary_dim dims rotated by
+ * the row's position ((a, b) -> (a cos - b sin, a sin + b cos) *
+ * rope_amplitude; the angle is formed in 64 bits, all else in f32), q written
+ * to d_q_out, k and v to their page and slot.  Two rows must not share a slot. */
+int32_t m1moe_kv_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
+                        const m1moe_paged_batch* batch,
+                        const m1moe_kv_append_args* args);
+
+/* Attention of every row of the batch over its own sequence's positions up to
+ * its own: out_h = sum_p softmax_p(q_h . k_p / sqrt(head_dim)) v_p, kv head
+ * h / (num_heads / num_kv_heads).  q and out [num_rows][num_heads * head_dim]
+ * in dtype (row strides in elements, as above; they must not overlap); scores, softmax and sums in
+ * f32 (dtype M1MOE_BF16: the softmax numerators that multiply v are rounded to
+ * bf16).  dtype M1MOE_BF16 needs a bf16 cache; num_heads is a multiple of
+ * num_kv_heads, at most 64 times it, and num_heads * head_dim <= 65536.
+ * Later positions take no part, whatever they hold.  The first call of a
+ * larger batch may grow the context's workspace (make it before capturing). */
+int32_t m1moe_paged_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
+                              const m1moe_paged_batch* batch, const void* d_q,
+                              int64_t q_stride, void* d_out, int64_t out_stride,
+                              int32_t dtype, int32_t num_heads);
+
+/* One token per row of d_logits (f32 [rows], stride elements apart, a multiple
+ * of 4, >= vocab).  With the logits of a row in descending order, ties to the
+ * lower index, and w_i = exp((x_i - x_0) / temperature): the first top_k
+ * stay; of these the fewest whose w sum to at least top_p of their total; of
+ * these the ones with w_i >= min_p (the first always stays).  With S the sum
+ * of what stayed the token is the first whose running sum reaches u * S
+ * (m1moe_amd/sampling.py with top-k and min-p; u outside [0, 1] is taken to
+ * the nearer end, NaN to 0).  Sums are of whole multiples of 2^-44, so they do
+ * not depend on an order; w below 2^-45 counts as 0 and is never drawn.  NaN
+ * logits count as -inf; a row with nothing above -inf gives token -1,
+ * probability 0.  d_probs (nullable) receives w / S of the token.
+ * 1 <= rows <= 65536, 1 <= vocab <= 262144. */
+int32_t m1moe_sample(m1moe_ctx_t ctx, const float* d_logits, int32_t rows,
+                     int32_t vocab, int64_t stride,
+                     const m1moe_sample_params* params, int32_t* d_tokens,
+                     float* d_probs);
+
 /* ---- the converted model directory on disk (host-side) -----------------
  * scripts/extract_olmoe.py writes model_weights.bin (non-expert tensors,
  * 4-byte aligned) + model_weights.json ({name: {offset, shape, dtype}}) and

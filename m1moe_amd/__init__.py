@@ -6,8 +6,8 @@ reference's MoE-block interface over that ABI (engine.py), the decoder
 around it (decoder.py: InferenceEngine.forward on the GPU), plus the seeded
 synthetic workloads (synth.py).
 """
-from ._lib import (M1MOE_BF16, M1MOE_F32, M1MoEError, MoEShape, PROJ_DOWN, PROJ_GATE,
-                   PROJ_UP, load)
+from ._lib import (KVAppend, M1MOE_BF16, M1MOE_F32, M1MoEError, MoEShape, PROJ_DOWN, PROJ_GATE,
+                   PROJ_UP, PagedBatch, PagedKV, SampleParams, load)
 from .engine import (DeviceBuffer, HIPContext, MoEBlock, ModelSpec, check_shape, expert_bytes,
                      expert_offsets, make_shape)
 from .decoder import AttentionSpec, Decoder, DecoderSpec, DenseOps
@@ -16,5 +16,5 @@ __all__ = [
     "M1MOE_BF16", "M1MOE_F32", "M1MoEError", "MoEShape", "PROJ_DOWN", "PROJ_GATE", "PROJ_UP",
     "load", "DeviceBuffer", "HIPContext", "MoEBlock", "ModelSpec", "check_shape",
     "expert_bytes", "expert_offsets", "make_shape", "AttentionSpec", "Decoder", "DecoderSpec",
-    "DenseOps",
+    "DenseOps", "KVAppend", "PagedBatch", "PagedKV", "SampleParams",
 ]

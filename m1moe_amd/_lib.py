@@ -55,6 +55,112 @@ class DecShape(ctypes.Structure):
     ]
 
 
+def _address(p):
+    """A device address (int, c_void_p, DeviceBuffer or None) as ctypes stores it."""
+    p = getattr(p, "ptr", p)
+    return p.value if isinstance(p, c_void_p) else None if p is None else int(p)
+
+
+def dtype_code(dtype) -> int:
+    """M1MOE_F32 or M1MOE_BF16 from "f32" / "bf16" or the code itself."""
+    if dtype in ("bf16", M1MOE_BF16):
+        return M1MOE_BF16
+    if dtype in ("f32", M1MOE_F32):
+        return M1MOE_F32
+    raise ValueError(f"unknown dtype {dtype!r}")
+
+
+class PagedKV(ctypes.Structure):
+    """m1moe_paged_kv: a KV cache in pages, in the caller's memory."""
+
+    _fields_ = [
+        ("d_k", c_void_p),
+        ("d_v", c_void_p),
+        ("dtype", c_int32),
+        ("num_pages", c_int32),
+        ("page_size", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+    ]
+
+    @staticmethod
+    def make(k, v, dtype, num_pages: int, page_size: int, num_kv_heads: int,
+             head_dim: int) -> "PagedKV":
+        return PagedKV(_address(k), _address(v), dtype_code(dtype), num_pages, page_size,
+                       num_kv_heads, head_dim)
+
+
+class PagedBatch(ctypes.Structure):
+    """m1moe_paged_batch: the rows, lengths and page tables of one call."""
+
+    _fields_ = [
+        ("num_seqs", c_int32),
+        ("num_rows", c_int32),
+        ("table_stride", c_int32),
+        ("prefix_len", c_int32),
+        ("d_row_start", c_void_p),
+        ("d_kv_len", c_void_p),
+        ("d_pages", c_void_p),
+        ("d_prefix_pages", c_void_p),
+    ]
+
+    @staticmethod
+    def make(num_seqs: int, num_rows: int, row_start, kv_len, pages, table_stride: int,
+             prefix_len: int = 0, prefix_pages=None) -> "PagedBatch":
+        return PagedBatch(num_seqs, num_rows, table_stride, prefix_len, _address(row_start),
+                          _address(kv_len), _address(pages), _address(prefix_pages))
+
+
+class KVAppend(ctypes.Structure):
+    """m1moe_kv_append_args: what an append reads and writes besides the cache."""
+
+    _fields_ = [
+        ("dtype", c_int32),
+        ("num_heads", c_int32),
+        ("d_q", c_void_p),
+        ("d_k", c_void_p),
+        ("d_v", c_void_p),
+        ("d_q_out", c_void_p),
+        ("q_stride", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64),
+        ("v_stride", ctypes.c_int64),
+        ("q_out_stride", ctypes.c_int64),
+        ("d_q_norm", c_void_p),
+        ("d_k_norm", c_void_p),
+        ("eps", c_float),
+        ("rotary_dim", c_int32),
+        ("interleaved", c_int32),
+        ("rope_amplitude", c_float),
+        ("d_inv_freq", c_void_p),
+    ]
+
+    @staticmethod
+    def make(dtype, num_heads: int, q, k, v, q_stride: int, k_stride: int, v_stride: int, q_out,
+             q_out_stride: int, q_norm=None, k_norm=None, eps: float = 0.0, rotary_dim: int = 0,
+             interleaved: bool = False, inv_freq=None, amplitude: float = 1.0) -> "KVAppend":
+        return KVAppend(dtype_code(dtype), num_heads, _address(q), _address(k), _address(v),
+                        _address(q_out), q_stride, k_stride, v_stride, q_out_stride,
+                        _address(q_norm), _address(k_norm), eps, rotary_dim,
+                        1 if interleaved else 0, amplitude, _address(inv_freq))
+
+
+class SampleParams(ctypes.Structure):
+    """m1moe_sample_params: per-row settings in device memory."""
+
+    _fields_ = [
+        ("d_u", c_void_p),
+        ("d_temperature", c_void_p),
+        ("d_top_k", c_void_p),
+        ("d_top_p", c_void_p),
+        ("d_min_p", c_void_p),
+    ]
+
+    @staticmethod
+    def make(u, temperature=None, top_k=None, top_p=None, min_p=None) -> "SampleParams":
+        return SampleParams(_address(u), _address(temperature), _address(top_k), _address(top_p),
+                            _address(min_p))
+
+
 # dtypes of the on-disk manifest (m1moe_store_tensor)
 DT_BF16, DT_F32, DT_U32 = 0, 1, 2
 
@@ -129,6 +235,15 @@ _PROTOTYPES = [
     ("m1moe_dec_step_seq", c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
     ("m1moe_dec_prefill", c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     ("m1moe_dec_position", c_int32, [c_void_p, POINTER(c_int32)]),
+    ("m1moe_check_paged", c_int32, [POINTER(PagedKV), POINTER(PagedBatch)]),
+    ("m1moe_kv_append", c_int32,
+     [c_void_p, POINTER(PagedKV), POINTER(PagedBatch), POINTER(KVAppend)]),
+    ("m1moe_paged_attention", c_int32,
+     [c_void_p, POINTER(PagedKV), POINTER(PagedBatch), c_void_p, ctypes.c_int64, c_void_p,
+      ctypes.c_int64, c_int32, c_int32]),
+    ("m1moe_sample", c_int32,
+     [c_void_p, c_void_p, c_int32, c_int32, ctypes.c_int64, POINTER(SampleParams), c_void_p,
+      c_void_p]),
     ("m1moe_store_open", c_int32, [c_char_p, c_char_p, POINTER(c_void_p)]),
     ("m1moe_store_close", None, [c_void_p]),
     ("m1moe_store_count", c_int32, [c_void_p, POINTER(c_int32)]),

@@ -22,6 +22,7 @@
 #include "ctx.hpp"
 #include "internal.hpp"
 #include "m1moe_hip.h"
+#include "paged.hpp"
 
 namespace m1moe {
 
@@ -482,7 +483,7 @@ void m1moe_destroy(m1moe_ctx_t ctx) {
                      ctx->topk_w,  ctx->counters, ctx->act,     ctx->sync,    ctx->err,
                      ctx->pf_xq,   ctx->pf_xinv,  ctx->pf_pos,  ctx->pf_sorted, ctx->pf_eoff,
                      ctx->pf_toff, ctx->pf_tdesc,  ctx->pf_act,  ctx->pf_y,     ctx->pf_aexp,
-                     ctx->pf_aflag, ctx->attn_part, ctx->attn_cnt};
+                     ctx->pf_aflag, ctx->attn_part, ctx->attn_cnt, ctx->paged_part};
     for (void* p : owned)
         if (p) (void)hipFree(p);
     share_leave(ctx);
@@ -777,6 +778,14 @@ int32_t m1moe_sync(m1moe_ctx_t ctx) {
             return fail(M1MOE_ERR_DEVICE,
                         "a decoder step ran with the KV cache full (position == max_seq); "
                         "nothing was stored (device flag 0x%x)", flag);
+        if (flag & kErrPagedBatch)
+            return fail(M1MOE_ERR_DEVICE,
+                        "a paged batch has a sequence whose rows, length or prefix are out of "
+                        "range; it was skipped (device flag 0x%x)", flag);
+        if (flag & kErrPagedPage)
+            return fail(M1MOE_ERR_DEVICE,
+                        "a paged batch names a page outside the cache; nothing was stored there "
+                        "(device flag 0x%x)", flag);
         return fail(M1MOE_ERR_DEVICE,
                     "a decode hand-off wait timed out (device flag 0x%x); state was reset", flag);
     }

@@ -100,6 +100,9 @@ struct m1moe_ctx {
     float* attn_part = nullptr;
     uint64_t attn_part_floats = 0;
     uint32_t* attn_cnt = nullptr;    // [kAttnCounters], zero between launches
+    // partials of m1moe_paged_attention, grown on demand
+    float* paged_part = nullptr;
+    uint64_t paged_part_floats = 0;
     std::set<void*> allocs;
 };
 

@@ -1,0 +1,64 @@
+// paged.hpp — kernel arguments of the paged KV cache (paged.hip) and of the
+// sampler (sample.hip).
+#pragma once
+
+#include <cstdint>
+
+namespace m1moe {
+
+constexpr int kPagedMaxSeqs = 1024;
+constexpr int kPagedMaxShare = 64;   // query heads per kv head
+constexpr uint32_t kErrPagedBatch = 256u, kErrPagedPage = 512u;   // device error flags
+
+// The cache and the batch (m1moe_paged_kv, m1moe_paged_batch).
+struct PagedView {
+    void *k, *v;
+    int32_t num_pages, page_shift, kv_heads;
+    int32_t num_seqs, num_rows, table_stride, prefix_len;
+    const int32_t *row_start, *kv_len, *pages, *prefix_pages;
+    uint32_t* err;
+};
+
+struct AppendArgs {
+    PagedView p;
+    const void *q, *k, *v;
+    void* q_out;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const uint16_t *q_norm, *k_norm;
+    const float* inv_freq;
+    float eps, amp;
+    int32_t heads, head_dim, rotary, interleaved;
+    int32_t x_bf16, cache_bf16;
+};
+
+struct PagedAttnArgs {
+    PagedView p;
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    int32_t heads, share, head_dim;   // share: query heads per kv head
+    int32_t x_bf16, cache_bf16;
+    float scale;
+    int32_t grid;        // workgroups the sequences' own positions are shared by
+    int32_t splits;      // pieces of the prefix, 0 without one
+    float* part;         // partials: the workgroups' (paged_attention_floats)
+    float* pre;          // and the prefix' [splits][num_rows * heads][head_dim + 2]
+};
+
+struct SampleArgs {
+    const float* logits;
+    int64_t stride;
+    int32_t rows, vocab;
+    const float *u, *temperature, *top_p, *min_p;
+    const int32_t* top_k;
+    int32_t* tokens;
+    float* probs;
+};
+
+int launch_kv_append(const AppendArgs& a, int cus, void* stream);
+// Sets grid and splits; the floats of partials (own, then the prefix') needed.
+int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats);
+int launch_paged_attention(const PagedAttnArgs& a, void* stream);
+int launch_sample(const SampleArgs& a, void* stream);
+
+}  // namespace m1moe

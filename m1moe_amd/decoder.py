@@ -21,8 +21,8 @@ from typing import Optional
 import numpy as np
 
 from . import _lib
-from ._lib import (DecShape, W_EMBED, W_FINAL_NORM, W_IN_NORM, W_K, W_K_NORM, W_LM_HEAD, W_O,
-                   W_PER_LAYER, W_POST_NORM, W_Q, W_Q_NORM, W_V, check)
+from ._lib import (DecShape, KVAppend, PagedBatch, PagedKV, SampleParams, W_EMBED, W_FINAL_NORM, W_IN_NORM, W_K, W_K_NORM, W_LM_HEAD, W_O,
+                   W_PER_LAYER, W_POST_NORM, W_Q, W_Q_NORM, W_V, check, dtype_code)
 from .engine import DeviceBuffer, HIPContext, _ptr
 from .sampling import sample_token
 
@@ -133,6 +133,26 @@ class DenseOps:
 
     def argmax(self, x, n: int, idx) -> None:
         check(self.lib.m1moe_argmax(self.ctx.handle, _ptr(x), int(n), _ptr(idx)), "m1moe_argmax")
+
+    # several conversations at once: a KV cache in pages, attention over it, sampling
+    def kv_append(self, kv: PagedKV, batch: PagedBatch, args: KVAppend) -> None:
+        """q/k norm, RoPE and the store of k and v for every row of the batch."""
+        check(self.lib.m1moe_kv_append(self.ctx.handle, ctypes.byref(kv), ctypes.byref(batch),
+                                       ctypes.byref(args)), "m1moe_kv_append")
+
+    def paged_attention(self, kv: PagedKV, batch: PagedBatch, q, q_stride: int, out,
+                        out_stride: int, dtype, num_heads: int) -> None:
+        """Every row of the batch against its own sequence's positions up to its own."""
+        check(self.lib.m1moe_paged_attention(
+            self.ctx.handle, ctypes.byref(kv), ctypes.byref(batch), _ptr(q), q_stride, _ptr(out),
+            out_stride, dtype_code(dtype), num_heads), "m1moe_paged_attention")
+
+    def sample(self, logits, rows: int, vocab: int, stride: int, params: SampleParams, tokens,
+               probs=None) -> None:
+        """One token per row of f32 logits from given random numbers."""
+        check(self.lib.m1moe_sample(self.ctx.handle, _ptr(logits), rows, vocab, stride,
+                                    ctypes.byref(params), _ptr(tokens), _ptr(probs)),
+              "m1moe_sample")
 
 
 class Decoder:
