@@ -201,14 +201,19 @@ __device__ __forceinline__ float quads_add(float v) {
 __device__ __forceinline__ float weight(float x, float unit) { return __builtin_amdgcn_exp2f(x * unit); }
 
 constexpr int kCut = 256;        // keys: where a tile's keys may be cut between workgroups
-constexpr int kFewKeys = 128;    // least keys per workgroup
+constexpr int kFewKeys = 128;    // least places on the line per workgroup
+constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 
-// How the rows and keys are shared.  A tile is up to R = 64 NT rows (token,
-// head) of one sequence and kv head, whole tokens: TT = R / share tokens.  Its
-// keys are the positions from `org` (the prefix' end rounded down to 32) to its
-// last token's; all tiles' keys, sequence by sequence, head by head, tile by
-// tile, form one line that is cut into equal shares, one per workgroup, the
-// cuts moved down to a multiple of kCut inside their tile.
+// How the rows and keys are shared.  A tile is up to R rows (token, head) of one
+// sequence and kv head, whole tokens: TT = R / share tokens.  Its keys are the
+// positions from `org` (the prefix' end rounded down to 32) to its last token's.
+// All tiles, sequence by sequence, head by head, tile by tile, form one line, each
+// with kTileKeys places for what it costs to begin and end it (about 5 us: the
+// queries, the first page and rows one after the other, the waves' join) and one
+// place per key; the line is cut into equal shares, one per workgroup, the cuts
+// moved down to a multiple of kCut keys inside their tile.  (Without the places
+// per tile the workgroups with the shortest sequences ended last: 32 steps of 60 to
+// 8100 positions, 8 kv heads, median 61 us, last 116.)
 struct Tile {
     int seq, head, r;            // sequence, kv head, tile of its rows
     int row0, n, base;           // the sequence's first row, rows, positions before them
@@ -221,12 +226,12 @@ struct Line {
     int wgs;                     // workgroups that have a share
     int org, TT, kv_heads;
 
-    // keys of the first r tiles of a head (r below the number of tiles)
+    // places of the first r tiles of a head (r below the number of tiles)
     __device__ int64_t before(int base, int r) const {
-        return (int64_t)r * (base - org) + (int64_t)TT * r * (r + 1) / 2;
+        return (int64_t)r * (base - org + kTileKeys) + (int64_t)TT * r * (r + 1) / 2;
     }
-    __device__ int64_t head_keys(int base, int n, int tiles) const {
-        return before(base, tiles - 1) + (base - org) + n;
+    __device__ int64_t head_places(int base, int n, int tiles) const {
+        return before(base, tiles - 1) + (base - org + kTileKeys) + n;
     }
     __device__ int64_t cut(int w) const {
         return w >= wgs ? total : (int64_t)((double)total * w / wgs);
@@ -239,7 +244,7 @@ struct Line {
         t.n = p.row_start[s + 1] - t.row0;
         t.base = p.kv_len[s] - t.n;
         const int tiles = (t.n + TT - 1) / TT;
-        const int64_t hk = head_keys(t.base, t.n, tiles);
+        const int64_t hk = head_places(t.base, t.n, tiles);
         int64_t off = x - cum[s];
         t.head = (int)(off / hk);
         off -= (int64_t)t.head * hk;
@@ -253,12 +258,16 @@ struct Line {
         }
         t.r = lo;
         t.start = cum[s] + (int64_t)t.head * hk + before(t.base, lo);
-        t.end = t.start + (t.base - org) + min(t.n, (lo + 1) * TT);
+        t.end = t.start + kTileKeys + (t.base - org) + min(t.n, (lo + 1) * TT);
         return t;
     }
+    // Cut x inside tile t, moved down: to the tile's start or to a place of a key.
     __device__ int64_t rounded(const Tile& t, int64_t x) const {
-        return t.start + (x - t.start) / kCut * kCut;
+        const int64_t keys = x - t.start - kTileKeys;
+        return keys < kCut ? t.start : t.start + kTileKeys + keys / kCut * kCut;
     }
+    // The key (from org on) at place x of tile t.
+    __device__ static int key(const Tile& t, int64_t x) { return (int)max((int64_t)0, x - t.start - kTileKeys); }
 };
 
 // Fills cum (and line): the whole workgroup of 256.  tmp: LDS, 4 values.
@@ -273,7 +282,7 @@ __device__ __forceinline__ void make_line(const PagedView& p, Line& ln, int64_t*
             if (!seq_ok(p, lo, hi, len)) {
                 if (flag) flag_error(p.err, kErrPagedBatch);
             } else if (n > 0) {
-                keys = ln.kv_heads * ln.head_keys(len - n, n, (n + ln.TT - 1) / ln.TT);
+                keys = ln.kv_heads * ln.head_places(len - n, n, (n + ln.TT - 1) / ln.TT);
             }
         }
         int64_t sum = keys;
@@ -311,6 +320,14 @@ __device__ __forceinline__ int find_seq(const PagedView& p, const Line& ln, int6
     return lo;
 }
 
+// The thread's number, opaque to the compiler: what depends on it is computed where
+// it is used and not kept in registers over a workgroup's tiles (50 of them).
+__device__ __forceinline__ int thread_id() {
+    int t = (int)threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 // What a workgroup computes at once: rows of one kv head over a range of keys.
 struct Work {
     int token0, tokens;       // rows of q and out
@@ -321,25 +338,78 @@ struct Work {
     int first, last;          // positions that may be read and seen (others are not)
     int head;                 // kv head
     const int32_t* table;
+
+    // (the same in every lane: into scalar registers)
+    __device__ __forceinline__ void uniform() {
+        for (int* x : {&token0, &tokens, &pos0, &head0, &lo, &hi, &last, &head}) *x = __builtin_amdgcn_readfirstlane(*x);
+        const uint64_t t = reinterpret_cast<uint64_t>(table);
+        table = reinterpret_cast<const int32_t*>(
+            (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 32)) << 32 |
+            (uint32_t)__builtin_amdgcn_readfirstlane((int)t));
+    }
 };
 
-// One wave's 16 NT rows: running softmax and transposed output.  Lane l holds
-// query column l % 16 of each group of 16 and, in row group g = l / 16, of a
-// 32-key block the scores of keys 8 g .. 8 g + 7 (S^T = K Q^T with the K rows
-// of two 16-key MFMAs chosen so: row 4 g + v of MFMA t is key 8 g + 4 t + v):
-// the lane's P is then the operand of O^T = V^T P^T as it stands.  Its V
-// operand is eight keys of one dim: the lane loads the VD = HD / 16 dims VD (l %
-// 16) .. of its eight keys and picks dim j of them for MFMA j, whose output
-// row 4 g + v is dim VD (4 g + v) + j.
-template <int HD, int QP, int KP, int NT>
-struct Wave {
+// The cache as a wave reads it: one kv head's rows.
+template <int HD, int KP>
+struct Cache {
+    static constexpr int ES = KP == 1 ? 2 : 4;    // bytes of an element
+    const uint8_t *k, *v;                         // at the kv head
+    uint32_t row, page, mask;                     // bytes of a position and of a page; slots - 1
+    int shift, pages, first, last;
+    const int32_t* table;
+
+    __device__ __forceinline__ Cache(const PagedView& p, const Work& w) {
+        k = static_cast<const uint8_t*>(p.k) + (int64_t)w.head * HD * ES;
+        v = static_cast<const uint8_t*>(p.v) + (int64_t)w.head * HD * ES;
+        row = (uint32_t)p.kv_heads * HD * ES;
+        shift = p.page_shift;
+        page = row << shift;
+        mask = (1u << shift) - 1;
+        pages = p.num_pages;
+        first = w.first;
+        last = w.last;
+        table = w.table;
+    }
+    __device__ __forceinline__ int clamp(int pos) const { return min(max(pos, first), last); }
+    // The page of the aligned eight positions from pos on: of the readable one among
+    // them, or of the nearest (page 0 for one outside the cache).
+    __device__ __forceinline__ int page_of(int pos, bool& bad) const {
+        const int x = table[clamp(pos) >> shift];
+        const bool out = (unsigned)x >= (unsigned)pages;
+        bad |= out;
+        return out ? 0 : x;
+    }
+    // Byte offset of a readable position of page x.
+    __device__ __forceinline__ int64_t at(int x, int pos) const {
+        return (int64_t)x * page + ((uint32_t)pos & mask) * row;
+    }
+    __device__ __forceinline__ bool edge(int kb, int n) const { return kb < first || kb + n - 1 > last; }
+};
+
+// The (token, query head) of row rho of the work; false past its rows.
+__device__ __forceinline__ bool row_at(const PagedAttnArgs& a, const Work& w, int rho, int& token, int& head) {
+    const int t = rho / a.share;
+    token = w.token0 + min(t, w.tokens - 1);
+    head = w.head0 + rho - t * a.share;
+    return t < w.tokens;
+}
+
+// One wave's 16 NT rows: queries, running softmax and transposed output.  Lane l
+// holds row c = l % 16 of each group of 16 and, with g = l / 16, of a 32-key block
+// the scores of keys 8 g .. 8 g + 7 (S^T = K Q^T with the K rows of two 16-key
+// MFMAs chosen so: row 4 g + v of MFMA u is key 8 g + 4 u + v): the lane's P is
+// then the operand of O^T = V^T P^T as it stands, eight keys of one dim its
+// other one.  Row 4 g + v of output MFMA j is dim VD (4 g + v) + j where a lane
+// loads the VD = HD / 16 neighbouring dims VD c .. of eight keys itself (SPREAD),
+// else dim 16 j + 4 g + v.
+template <int HD, int QP, int NT, bool SPREAD>
+struct Rows {
     static constexpr int NS = HD / 32, VD = HD / 16;
     bf16x8 q[NT][QP][NS];
     f32x4v acc[NT][VD];
     float m[NT], l[NT];
     int qpos[NT];
-    int g, c;
-    const uint8_t *kc, *vc;
+    int g, c, see, most;      // the rows' lowest and highest position
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -350,20 +420,24 @@ struct Wave {
             for (int j = 0; j < VD; ++j) acc[t][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
         }
     }
-    __device__ __forceinline__ bool row_at(const PagedAttnArgs& a, const Work& w, int rho, int& token,
-                                           int& head) const {
-        const int t = rho / a.share;
-        token = w.token0 + min(t, w.tokens - 1);
-        head = w.head0 + rho - t * a.share;
-        return t < w.tokens;
+    __device__ __forceinline__ static int dim(int g, int j, int v) {
+        return SPREAD ? VD * (4 * g + v) + j : 16 * j + 4 * g + v;
     }
     // rows rho0 ..
-    __device__ __forceinline__ void load_q(const PagedAttnArgs& a, const Work& w, int rho0) {
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, const Work& w, int rho0) {
+        const int lane = thread_id() & 63;
+        g = lane >> 4;
+        c = lane & 15;
+        clear();
+        see = w.last;
+        most = -1;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             int token, head;
             const bool on = row_at(a, w, rho0 + 16 * t + c, token, head);
             qpos[t] = w.pos0 + (token - w.token0) * w.row_pos;
+            see = min(see, qpos[t]);
+            most = max(most, qpos[t]);
             const int64_t at = (int64_t)token * a.q_stride + (int64_t)head * HD + 8 * g;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -382,166 +456,94 @@ struct Wave {
                 }
             }
         }
-    }
-
-    // The page of position pos (clamped to the readable ones).
-    __device__ __forceinline__ int page_of(const PagedView& p, const Work& w, int pos, bool& bad) const {
-        const int at = min(max(pos, w.first), w.last) >> p.page_shift;
-        int page = w.table[at];
-        if ((unsigned)page >= (unsigned)p.num_pages) {
-            bad = true;
-            page = 0;
-        }
-        return page;
-    }
-    // Element offset of position pos of page `page`.
-    __device__ __forceinline__ int64_t cell(const PagedView& p, const Work& w, int page, int pos) const {
-        const int in = min(max(pos, w.first), w.last) & ((1 << p.page_shift) - 1);
-        return ((((int64_t)page << p.page_shift) + in) * p.kv_heads + w.head) * HD;
-    }
-
-    // Keys lo, lo + step, ... of the work in blocks of 32.
-    __device__ __forceinline__ void run(const PagedAttnArgs& a, const Work& w, int lo, int step, float unit,
-                                        bool& bad) {
-        const PagedView& p = a.p;
-        // a block with a key that some row does not see, or that is not readable
-        int see = w.last;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) see = min(see, qpos[t]);
-        int most = -1;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) most = max(most, qpos[t]);
         for (int x = 1; x < 16; x <<= 1) {
             see = min(see, __shfl_xor(see, x));
             most = max(most, __shfl_xor(most, x));
         }
-        const int hi = min(w.hi, min(most, w.last) + 1);
-        for (int kb = lo; kb < hi; kb += step) {
-            const int pk = page_of(p, w, kb + 8 * (c >> 2), bad), pv = page_of(p, w, kb + 8 * g, bad);
-            f32x4v s[NT][2];
+        see = __builtin_amdgcn_readfirstlane(see);
+        most = __builtin_amdgcn_readfirstlane(most);
+    }
+
+    // Part products of a K (or V) operand with the rows' parts, small ones first: for
+    // f32 on both sides the six down to 2^-16 of the largest.  `acc` one per group.
+    template <class OP>
+    __device__ __forceinline__ static void products(const bf16x8 (&x)[1], const OP& y, int t, int s, f32x4v& o) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int64_t at = cell(p, w, pk, kb + 8 * (c >> 2) + 4 * u + (c & 3)) + 8 * g;
-#pragma unroll
-                for (int t = 0; t < NT; ++t) s[t][u] = f32x4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    if constexpr (KP == 1) {
-                        const bf16x8 k = *reinterpret_cast<const bf16x8*>(kc + 2 * (at + 32 * i));
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int b = QP - 1; b >= 0; --b) s[t][u] = mfma(k, q[t][b][i], s[t][u]);
-                    } else {
-                        const float4* x = reinterpret_cast<const float4*>(kc + 4 * (at + 32 * i));
-                        const float4 y = x[0], z = x[1];
-                        const Parts8 k = parts8({y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w});
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            s[t][u] = mfma(k.l, q[t][0][i], s[t][u]);
-                            s[t][u] = mfma(k.h, q[t][QP - 1][i], s[t][u]);
-                            s[t][u] = mfma(k.m, q[t][QP / 2][i], s[t][u]);
-                            s[t][u] = mfma(k.m, q[t][0][i], s[t][u]);
-                            s[t][u] = mfma(k.h, q[t][QP / 2][i], s[t][u]);
-                            s[t][u] = mfma(k.h, q[t][0][i], s[t][u]);
-                        }
-                    }
-                }
-            }
-            // V of the lane's eight keys
-            float vf[KP == 3 ? 8 : 1][KP == 3 ? VD : 1];
-            uint32_t vw[KP == 1 ? 8 : 1][KP == 1 ? VD / 2 : 1];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int64_t at = cell(p, w, pv, kb + 8 * g + e) + VD * c;
-                if constexpr (KP == 1) {
-                    typedef uint32_t words __attribute__((ext_vector_type(VD / 2)));
-                    const words x = *reinterpret_cast<const words*>(vc + 2 * at);
-#pragma unroll
-                    for (int i = 0; i < VD / 2; ++i) vw[e][i] = x[i];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < VD; i += 4) {
-                        const f32x4v x = *reinterpret_cast<const f32x4v*>(vc + 4 * (at + i));
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) vf[e][i + y] = x[y];
-                    }
-                }
-            }
-            bf16x8 pp[NT][QP];
-            const bool whole = kb >= w.first && kb + 31 <= see && kb + 32 <= w.hi;
+        for (int b = QP - 1; b >= 0; --b) o = mfma(x[0], y(t, b, s), o);
+    }
+    template <class OP>
+    __device__ __forceinline__ static void products(const bf16x8 (&x)[3], const OP& y, int t, int s, f32x4v& o) {
+        o = mfma(x[2], y(t, 0, s), o);
+        o = mfma(x[0], y(t, QP - 1, s), o);
+        o = mfma(x[1], y(t, QP / 2, s), o);
+        o = mfma(x[1], y(t, 0, s), o);
+        o = mfma(x[0], y(t, QP / 2, s), o);
+        o = mfma(x[0], y(t, 0, s), o);
+    }
+
+    // The running softmax over NB blocks of 32 keys from kb on: the scores s become the
+    // weights' operands pp, acc is rescaled where a maximum grew.
+    template <int NB>
+    __device__ __forceinline__ void softmax(const Work& w, int kb, f32x4v (&s)[NB][NT][2], float unit,
+                                            bf16x8 (&pp)[NB][NT][QP]) {
+        const bool whole = kb >= w.first && kb + 32 * NB - 1 <= see && kb + 32 * NB <= w.hi;
+        if (!whole) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float x[8];
+                const int top = min(min(qpos[t], w.last), w.hi - 1) - kb - 8 * g, low = w.first - kb - 8 * g;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[t][e >> 2][e & 3];
-                if (!whole) {
-                    const int top = min(min(qpos[t], w.last), w.hi - 1);
+                for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int pos = kb + 8 * g + e;
-                        x[e] = pos >= w.first && pos <= top ? x[e] : -INFINITY;
-                    }
-                }
-                float bm = x[0];
-#pragma unroll
-                for (int e = 1; e < 8; ++e) bm = fmaxf(bm, x[e]);
-                const float mn = fmaxf(m[t], quads_max(bm));
-                const float mc = mn == -INFINITY ? 0.f : mn;   // (no key seen yet: all weights 0)
-                if (__any(mn > m[t])) {
-                    const float f = weight(m[t] - mc, unit);
-                    l[t] *= f;
-#pragma unroll
-                    for (int j = 0; j < VD; ++j) acc[t][j] *= f;
-                    m[t] = mn;
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = weight(x[e] - mc, unit);
-                    l[t] += x[e];
-                }
-                if constexpr (QP == 1) {
-                    pp[t][0] = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
-                                                                     pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
-                } else {
-                    const Parts8 r = parts8(x);
-                    pp[t][0] = r.h;
-                    pp[t][QP - 2] = r.m;
-                    pp[t][QP - 1] = r.l;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < VD; ++j) {
-                if constexpr (KP == 1) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        o[i] = __builtin_amdgcn_perm(vw[2 * i + 1][j >> 1], vw[2 * i][j >> 1],
-                                                     j & 1 ? 0x07060302u : 0x05040100u);
-                    const bf16x8 v = __builtin_bit_cast(bf16x8, make_uint4(o[0], o[1], o[2], o[3]));
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int b = QP - 1; b >= 0; --b) acc[t][j] = mfma(v, pp[t][b], acc[t][j]);
-                } else {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = vf[e][j];
-                    const Parts8 v = parts8(x);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        acc[t][j] = mfma(v.l, pp[t][0], acc[t][j]);
-                        acc[t][j] = mfma(v.h, pp[t][QP - 1], acc[t][j]);
-                        acc[t][j] = mfma(v.m, pp[t][QP / 2], acc[t][j]);
-                        acc[t][j] = mfma(v.m, pp[t][0], acc[t][j]);
-                        acc[t][j] = mfma(v.h, pp[t][QP / 2], acc[t][j]);
-                        acc[t][j] = mfma(v.h, pp[t][0], acc[t][j]);
-                    }
-                }
+                    for (int e = 0; e < 8; ++e)
+                        s[b][t][e >> 2][e & 3] =
+                            32 * b + e >= low && 32 * b + e <= top ? s[b][t][e >> 2][e & 3] : -INFINITY;
             }
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) l[t] = quads_add(l[t]);
+        for (int t = 0; t < NT; ++t) {
+            float bm = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const f32x4v x = s[b][t][0], y = s[b][t][1];
+                bm = fmaxf(fmaxf(bm, x[0]), x[1]);
+                bm = fmaxf(fmaxf(bm, x[2]), x[3]);
+                bm = fmaxf(fmaxf(bm, y[0]), y[1]);
+                bm = fmaxf(fmaxf(bm, y[2]), y[3]);
+            }
+            const float mn = fmaxf(m[t], quads_max(bm));
+            const float mc = mn == -INFINITY ? 0.f : mn;   // (no key seen yet: all weights 0)
+            if (__any(mn > m[t])) {
+                const float f = weight(m[t] - mc, unit);
+                l[t] *= f;
+#pragma unroll
+                for (int j = 0; j < VD; ++j) acc[t][j] *= f;
+                m[t] = mn;
+            }
+            // (bf16 queries: one rounding more, of the row's largest exponent, against the 2^-8
+            // of the weights)
+            const float mu = mc * unit;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float x[8], sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = s[b][t][e >> 2][e & 3];
+                    x[e] = QP == 1 ? __builtin_amdgcn_exp2f(fmaf(y, unit, -mu)) : weight(y - mc, unit);
+                    sum += x[e];
+                }
+                l[t] += sum;
+                if constexpr (QP == 1) {
+                    pp[b][t][0] =
+                        __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
+                                                              pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
+                } else {
+                    const Parts8 r = parts8(x);
+                    pp[b][t][0] = r.h;
+                    pp[b][t][QP - 2] = r.m;
+                    pp[b][t][QP - 1] = r.l;
+                }
+            }
+        }
     }
 
     // Whether an infinity or a NaN came up in some row: one in q, k or v, also at a
@@ -559,13 +561,15 @@ struct Wave {
         }
         return __any(z != 0.f);
     }
-    // The same keys for such a wave, row by row and key by key in f32: positions
-    // that a row does not see are passed over.  tmp: HD floats of LDS of the wave.
+    // Keys lo .. lo + 31, lo + step .. for such a wave, row by row and key by key in
+    // f32: positions that a row does not see are passed over.  tmp: HD floats of LDS.
+    template <int KP>
     __device__ __forceinline__ void run_plain(const PagedAttnArgs& a, const Work& w, int rho0, int lo, int step,
-                                              float unit, float* tmp) {
+                                           float unit, float* tmp) {
         constexpr int PL = HD / 64;
-        const PagedView& p = a.p;
-        const int lane = threadIdx.x & 63;
+        const Cache<HD, KP> kv(a.p, w);
+        const int lane = thread_id() & 63;
+        bool bad = false;
         clear();
         for (int rr = 0; rr < 16 * NT; ++rr) {
             int token, head;
@@ -580,16 +584,14 @@ struct Wave {
             }
             for (int kb = lo; kb <= top; kb += step)
                 for (int k = max(kb, w.first); k <= min(kb + 31, top); ++k) {
-                    int page = w.table[k >> p.page_shift];
-                    if ((unsigned)page >= (unsigned)p.num_pages) page = 0;
-                    const int64_t at = cell(p, w, page, k) + PL * lane;
+                    const int64_t at = kv.at(kv.page_of(k, bad), k) + PL * lane * kv.ES;
                     float s = 0.f, v[PL];
 #pragma unroll
                     for (int i = 0; i < PL; ++i) {
-                        const float kx = KP == 1 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(kc)[at + i])
-                                                 : reinterpret_cast<const float*>(kc)[at + i];
-                        v[i] = KP == 1 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(vc)[at + i])
-                                       : reinterpret_cast<const float*>(vc)[at + i];
+                        const float kx = KP == 1 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(kv.k + at)[i])
+                                                 : reinterpret_cast<const float*>(kv.k + at)[i];
+                        v[i] = KP == 1 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(kv.v + at)[i])
+                                       : reinterpret_cast<const float*>(kv.v + at)[i];
                         s = fmaf(qr[i], kx, s);
                     }
                     s = wave_sum(s);
@@ -611,19 +613,332 @@ struct Wave {
 #pragma unroll
                     for (int j = 0; j < VD; ++j)
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[t][j][v] = tmp[VD * (4 * g + v) + j];
+                        for (int v = 0; v < 4; ++v) acc[t][j][v] = tmp[dim(g, j, v)];
                 }
             __threadfence_block();
         }
     }
 };
 
-// Sizes of a workgroup's LDS and partials.
-template <int HD, int NT>
-struct Sizes {
-    static constexpr int R = 64 * NT;                      // rows of a tile
-    static constexpr int kTile = 16 * NT * HD;             // floats of a wave's output
-    static constexpr int64_t kSlot = (int64_t)R * (HD + 2);  // a partial: o [R][HD], m [R], l [R]
+// Few rows (at most 16): the four waves hold the same ones and take every fourth
+// block of 32 keys, each straight from the cache into registers.  While one
+// block is computed the next one's rows are on their way, K's from the moment the
+// scores have used the last, V's from the end of the block, and the page numbers
+// of the one after.
+template <int HD, int QP, int KP>
+struct Deep : Rows<HD, QP, 1, true> {
+    typedef Rows<HD, QP, 1, true> R;
+    static constexpr int NS = R::NS, VD = R::VD;
+    using R::acc;
+    using R::c;
+    using R::g;
+    typedef uint32_t words __attribute__((ext_vector_type(VD / 2)));
+    uint4 kw[2][KP == 1 ? NS : 2 * NS];      // K of the lane's two rows
+    words vw[KP == 1 ? 8 : 1];               // V of its eight
+    float vf[KP == 3 ? 8 : 1][KP == 3 ? VD : 1];
+
+    __device__ __forceinline__ void load_k(const Cache<HD, KP>& kv, int kb, int page) {
+        int p0 = kb + 8 * (c >> 2) + (c & 3), p1 = p0 + 4;
+        if (kv.edge(kb, 32)) {
+            p0 = kv.clamp(p0);
+            p1 = kv.clamp(p1);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint4* x = reinterpret_cast<const uint4*>(kv.k + kv.at(page, u ? p1 : p0) + 8 * kv.ES * g);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                kw[u][KP == 1 ? i : 2 * i] = x[KP == 1 ? 4 * i : 8 * i];
+                if constexpr (KP == 3) kw[u][2 * i + 1] = x[8 * i + 1];
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const Cache<HD, KP>& kv, int kb, int page) {
+        const uint8_t* x[8];
+        const int p0 = kb + 8 * g;
+        if (kv.edge(kb, 32)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = kv.v + kv.at(page, kv.clamp(p0 + e)) + VD * kv.ES * c;
+        } else {
+            x[0] = kv.v + kv.at(page, p0) + VD * kv.ES * c;
+#pragma unroll
+            for (int e = 1; e < 8; ++e) x[e] = x[e - 1] + kv.row;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (KP == 1) {
+                vw[e] = *reinterpret_cast<const words*>(x[e]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VD; i += 4) {
+                    const f32x4v y = *reinterpret_cast<const f32x4v*>(x[e] + 4 * i);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) vf[e][i + z] = y[z];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void run(const PagedView& p, const Work& w, int lo, int step, float unit) {
+        const Cache<HD, KP> kv(p, w);
+        const int hi = min(w.hi, min(this->most, w.last) + 1);
+        if (lo < hi) {
+            bool bad = false;
+            int pk = kv.page_of(lo + 8 * (c >> 2), bad), pv = kv.page_of(lo + 8 * g, bad);
+            int pk1 = 0, pv1 = 0;
+            if (lo + step < hi) {
+                pk1 = kv.page_of(lo + step + 8 * (c >> 2), bad);
+                pv1 = kv.page_of(lo + step + 8 * g, bad);
+            }
+            load_k(kv, lo, pk);
+            load_v(kv, lo, pv);
+            for (int kb = lo; kb < hi; kb += step) {
+                const int nb = kb + step;
+                pk = pk1;
+                pv = pv1;
+                if (nb + step < hi) {
+                    pk1 = kv.page_of(nb + step + 8 * (c >> 2), bad);
+                    pv1 = kv.page_of(nb + step + 8 * g, bad);
+                }
+                f32x4v s[1][1][2];
+                s[0][0][0] = s[0][0][1] = f32x4v{0.f, 0.f, 0.f, 0.f};
+                const auto qop = [&](int t, int b, int i) { return this->q[t][b][i]; };
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if constexpr (KP == 1) {
+                            const bf16x8 x[1] = {__builtin_bit_cast(bf16x8, kw[u][i])};
+                            R::products(x, qop, 0, i, s[0][0][u]);
+                        } else {
+                            const f32x4v y = __builtin_bit_cast(f32x4v, kw[u][2 * i]);
+                            const f32x4v z = __builtin_bit_cast(f32x4v, kw[u][2 * i + 1]);
+                            const Parts8 r = parts8({y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]});
+                            const bf16x8 x[3] = {r.h, r.m, r.l};
+                            R::products(x, qop, 0, i, s[0][0][u]);
+                        }
+                    }
+                if (nb < hi) load_k(kv, nb, pk);
+                bf16x8 pp[1][1][QP];
+                this->template softmax<1>(w, kb, s, unit, pp);
+                const auto pop = [&](int t, int b, int) { return pp[0][t][b]; };
+#pragma unroll
+                for (int j = 0; j < VD; ++j) {
+                    if constexpr (KP == 1) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            o[i] = __builtin_amdgcn_perm(vw[2 * i + 1][j >> 1], vw[2 * i][j >> 1],
+                                                         j & 1 ? 0x07060302u : 0x05040100u);
+                        const bf16x8 x[1] = {__builtin_bit_cast(bf16x8, make_uint4(o[0], o[1], o[2], o[3]))};
+                        R::products(x, pop, 0, 0, acc[0][j]);
+                    } else {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = vf[e][j];
+                        const Parts8 r = parts8(y);
+                        const bf16x8 x[3] = {r.h, r.m, r.l};
+                        R::products(x, pop, 0, 0, acc[0][j]);
+                    }
+                }
+                if (nb < hi) load_v(kv, nb, pv);
+            }
+            if (bad) flag_error(p.err, kErrPagedPage);
+        }
+        this->l[0] = quads_add(this->l[0]);
+    }
+};
+
+// Many rows: the waves hold 16 NT rows each and share the keys, staged through LDS
+// in pieces of SK: K row by row (its bf16 parts), V transposed, eight keys of a
+// dim together, both in 16-byte units placed so that the eight lanes an LDS read
+// serves at once find theirs in different banks.  Waves 0 and 1 stage K, 2 and 3 V.
+// The next piece is on its way into registers while one is computed, the page
+// numbers of the one after with it (lane l: of the piece's keys 8 (l % 16) ..).
+template <int HD, int KP>
+struct Stage {
+    static constexpr int SK = KP == 1 ? 8192 / HD : HD <= 128 ? 4096 / HD : 32;   // keys
+    static constexpr int KU = HD / 8, VU = SK / 8;        // units of a K row, of a V row
+    static constexpr int kPlane = SK * HD * 2;            // bytes of a part
+    static constexpr int kBytes = 2 * KP * kPlane;
+    static constexpr int kBuffers = KP == 1 ? 2 : 1;
+    static constexpr int ES = KP == 1 ? 2 : 4;
+    static constexpr int VB = KP == 1 ? 8 : 4;            // dims of a thread's V block (16 bytes)
+    static constexpr int N = SK * HD * ES / 2048 / 8;     // K rows' or V blocks' eights of loads
+    static_assert(SK % 32 == 0 && N >= 1 && SK <= 128, "a piece is whole 32-key blocks");
+    uint4 r[N][8];
+    int pages;                                            // lane l: of group l % 16
+
+    __device__ __forceinline__ static int k_at(int key, int unit) {
+        const int z = (key & 3) | ((key >> 3) & 3) << 2;
+        return (key * KU + (unit ^ (z & (KU - 1)))) * 16;
+    }
+    __device__ __forceinline__ static int v_at(int d, int unit) {
+        const int z = VU >= 8 ? d ^ (d >> 3) : (d >> 1) ^ (d >> 3);
+        return (d * VU + (unit ^ (z & (VU - 1)))) * 16;
+    }
+    __device__ __forceinline__ void look(const Cache<HD, KP>& kv, int kb, bool& bad) {
+        pages = kv.page_of(kb + 8 * (thread_id() & 15) % SK, bad);
+    }
+    // The piece at kb, by its pages.
+    __device__ __forceinline__ void load(const Cache<HD, KP>& kv, int kb) {
+        const int t = thread_id() & 127;
+        const bool edge = kv.edge(kb, SK);
+        if (threadIdx.x < 128) {   // eight dims (f32: in two loads) of a position
+            constexpr int UL = KP == 1 ? 1 : 2;
+#pragma unroll
+            for (int n = 0; n < N * 8 / UL; ++n) {
+                const int b = t + 128 * n, key = b / KU, unit = b % KU;
+                const int page = __shfl(pages, key >> 3);
+                const int pos = edge ? kv.clamp(kb + key) : kb + key;
+                const uint4* x = reinterpret_cast<const uint4*>(kv.k + kv.at(page, pos) + 8 * ES * unit);
+#pragma unroll
+                for (int i = 0; i < UL; ++i) r[(UL * n + i) / 8][(UL * n + i) % 8] = x[i];
+            }
+        } else {                   // VB dims of eight positions
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int b = t + 128 * n, grp = b / (HD / VB), d = VB * (b % (HD / VB));
+                const int page = __shfl(pages, grp);
+                const uint8_t* x = kv.v + ES * d;
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        r[n][e] = *reinterpret_cast<const uint4*>(x + kv.at(page, kv.clamp(kb + 8 * grp + e)));
+                } else {
+                    x += kv.at(page, kb + 8 * grp);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        r[n][e] = *reinterpret_cast<const uint4*>(x);
+                        x += kv.row;
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ static void put(uint8_t* s, const Parts8& p) {
+        *reinterpret_cast<bf16x8*>(s) = p.h;
+        *reinterpret_cast<bf16x8*>(s + kPlane) = p.m;
+        *reinterpret_cast<bf16x8*>(s + 2 * kPlane) = p.l;
+    }
+    __device__ __forceinline__ void store(uint8_t* s) const {
+        const int t = thread_id() & 127;
+        if (threadIdx.x < 128) {
+            constexpr int UL = KP == 1 ? 1 : 2;
+#pragma unroll
+            for (int n = 0; n < N * 8 / UL; ++n) {
+                const int b = t + 128 * n, at = k_at(b / KU, b % KU);
+                if constexpr (KP == 1) {
+                    *reinterpret_cast<uint4*>(s + at) = r[n / 8][n % 8];
+                } else {
+                    const f32x4v y = __builtin_bit_cast(f32x4v, r[n / 4][2 * n % 8]);
+                    const f32x4v z = __builtin_bit_cast(f32x4v, r[n / 4][2 * n % 8 + 1]);
+                    put(s + at, parts8({y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]}));
+                }
+            }
+        } else {
+            uint8_t* sv = s + KP * kPlane;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int b = t + 128 * n, grp = b / (HD / VB), d = VB * (b % (HD / VB));
+#pragma unroll
+                for (int i = 0; i < VB; ++i) {
+                    const int at = v_at(d + i, grp);
+                    if constexpr (KP == 1) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+                            const u32x4 w0 = __builtin_bit_cast(u32x4, r[n][2 * y]);
+                            const u32x4 w1 = __builtin_bit_cast(u32x4, r[n][2 * y + 1]);
+                            o[y] = __builtin_amdgcn_perm(w1[i >> 1], w0[i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+                        }
+                        *reinterpret_cast<uint4*>(sv + at) = make_uint4(o[0], o[1], o[2], o[3]);
+                    } else {
+                        float y[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = __builtin_bit_cast(f32x4v, r[n][e])[i & 3];
+                        put(sv + at, parts8(y));
+                    }
+                }
+            }
+        }
+    }
+};
+
+template <int HD, int QP, int KP, int NT>
+struct Wide : Rows<HD, QP, NT, false> {
+    typedef Rows<HD, QP, NT, false> R;
+    typedef Stage<HD, KP> S;
+    static constexpr int NS = R::NS, VD = R::VD;
+    // 32-key blocks a softmax takes at once: two halve its maxima and rescalings
+    static constexpr int NB = QP == 1 && HD <= 128 ? 2 : 1;
+
+    __device__ __forceinline__ void blocks(const Work& w, int kb, int b0, float unit, const uint8_t* s_kv) {
+        const int g = this->g, c = this->c;
+        f32x4v s[NB][NT][2];
+        const auto qop = [&](int t, int x, int i) { return this->q[t][x][i]; };
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[b][t][0] = s[b][t][1] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    bf16x8 x[KP];
+#pragma unroll
+                    for (int y = 0; y < KP; ++y)
+                        x[y] = *reinterpret_cast<const bf16x8*>(
+                            s_kv + y * S::kPlane + S::k_at(32 * (b0 + b) + 8 * (c >> 2) + 4 * u + (c & 3), 4 * i + g));
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) R::products(x, qop, t, i, s[b][t][u]);
+                }
+        }
+        bf16x8 pp[NB][NT][QP];
+        this->template softmax<NB>(w, kb, s, unit, pp);
+#pragma unroll
+        for (int j = 0; j < VD; ++j)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const auto pop = [&](int t, int x, int) { return pp[b][t][x]; };
+                bf16x8 x[KP];
+#pragma unroll
+                for (int y = 0; y < KP; ++y)
+                    x[y] = *reinterpret_cast<const bf16x8*>(s_kv + (KP + y) * S::kPlane +
+                                                            S::v_at(16 * j + c, 4 * (b0 + b) + g));
+#pragma unroll
+                for (int t = 0; t < NT; ++t) R::products(x, pop, t, 0, this->acc[t][j]);
+            }
+    }
+    // `rows`: whether the wave has some (those without take part in the staging)
+    __device__ __forceinline__ void run(const PagedView& p, const Work& w, bool rows, float unit, uint8_t* s_kv) {
+        const Cache<HD, KP> kv(p, w);
+        const int hi = rows ? min(w.hi, min(this->most, w.last) + 1) : 0;
+        bool bad = false;
+        S st;
+        st.look(kv, w.lo, bad);
+        st.load(kv, w.lo);
+        if (w.lo + S::SK < w.hi) st.look(kv, w.lo + S::SK, bad);
+        int turn = 0;
+        for (int k0 = w.lo; k0 < w.hi; k0 += S::SK) {
+            uint8_t* buf = s_kv + turn * S::kBytes;
+            if (S::kBuffers == 1) __syncthreads();
+            st.store(buf);
+            __syncthreads();   // (with two buffers the other one is still read before it)
+            if (k0 + S::SK < w.hi) {
+                st.load(kv, k0 + S::SK);
+                if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK, bad);
+            }
+#pragma unroll
+            for (int b = 0; b < S::SK / 32; b += NB)
+                if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, buf);
+            if (S::kBuffers == 2) turn ^= 1;
+        }
+        if (bad) flag_error(p.err, kErrPagedPage);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) this->l[t] = quads_add(this->l[t]);
+        __syncthreads();   // (s_kv is free again)
+    }
 };
 
 // joins (m1, l1) with (m0, l0): the factors of both
@@ -635,116 +950,159 @@ __device__ __forceinline__ void join(float& m0, float& l0, float m1, float l1, f
     m0 = mn;
 }
 
-template <int HD, bool OB, int N>
-__device__ __forceinline__ void store_out(const PagedAttnArgs& a, int token, int head, int d, const float (&x)[N]) {
-    const int64_t at = (int64_t)token * a.out_stride + (int64_t)head * HD + d;
-    if constexpr (OB) {
-        uint16_t* o = static_cast<uint16_t*>(a.out) + at;
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
-            *reinterpret_cast<uint2*>(o + i) = make_uint2(pack_bf16(x[i], x[i + 1]), pack_bf16(x[i + 2], x[i + 3]));
-    } else {
-        float* o = static_cast<float*>(a.out) + at;
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
-            *reinterpret_cast<float4*>(o + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-    }
+__device__ __forceinline__ void store4(const PagedAttnArgs& a, bool bf16, int64_t at, const float (&x)[4]) {
+    if (bf16)
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+            make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
+    else
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// Adds the prefix' pieces of (token, head), dims d .., to x with m and l.
-template <int HD, int N>
-__device__ __forceinline__ void add_prefix(const PagedAttnArgs& a, int token, int head, int d, float unit, float& m,
-                                           float& l, float (&x)[N]) {
-    const int64_t rows = (int64_t)a.p.num_rows * a.heads, row = (int64_t)token * a.heads + head;
-    for (int s = 0; s < a.splits; ++s) {
-        const float* o = a.pre + ((int64_t)s * rows + row) * (HD + 2);
-        float f0, f1;
-        join(m, l, o[HD], o[HD + 1], unit, f0, f1);
+// Where a finished tile's rows go: divided by their sums to out, or as a partial (o
+// [HD] per row, m and l): row rho of a slot, or (token, head) of a piece.
+template <int HD>
+struct Sink {
+    bool out;
+    float *o, *ml;            // slot: o [R][HD], ml [R][2]; piece: o [rows][HD], ml [rows][2]
+    bool by_token;
+
+    template <int QP, int NT, bool SPREAD>
+    __device__ __forceinline__ void rows(const PagedAttnArgs& a, const Work& w, const Rows<HD, QP, NT, SPREAD>& r,
+                                         int rho0) const {
+        constexpr int VD = HD / 16;
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = x[i] * f0 + o[d + i] * f1;
+        for (int t = 0; t < NT; ++t) {
+            const int rho = rho0 + 16 * t + r.c;
+            int token, head;
+            if (!row_at(a, w, rho, token, head)) continue;
+            const int64_t row = by_token ? (int64_t)token * a.heads + head : rho;
+            const int64_t at = (int64_t)token * a.out_stride + (int64_t)head * HD;
+            const float f = out ? 1.0f / r.l[t] : 1.0f;
+            if (!out && r.g == 0) *reinterpret_cast<float2*>(ml + 2 * row) = make_float2(r.m[t], r.l[t]);
+#pragma unroll
+            for (int y = 0; y < (SPREAD ? 4 : VD); ++y)
+#pragma unroll
+                for (int z = 0; z < (SPREAD ? VD : 4); z += 4) {
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[i] = (SPREAD ? r.acc[t][SPREAD ? z + i : 0][y & 3] : r.acc[t][SPREAD ? 0 : y][i]) * f;
+                    const int d = SPREAD ? VD * (4 * r.g + y) + z : 16 * y + 4 * r.g;
+                    if (out)
+                        store4(a, QP == 1, at + d, x);
+                    else
+                        *reinterpret_cast<float4*>(o + row * HD + d) = make_float4(x[0], x[1], x[2], x[3]);
+                }
+        }
     }
+};
+
+// Groups of 16 rows that a wave of Wide holds at most.  (f32 queries: three times the
+// MFMAs per LDS read and three times the query registers)
+template <int HD, int QP>
+constexpr int tile_groups() { return HD <= 128 && QP == 1 ? 2 : 1; }
+template <int HD, int QP>
+constexpr int tile_rows() { return 64 * tile_groups<HD, QP>(); }
+// floats of a workgroup's partial: o [R][HD], (m, l) [R]
+template <int HD, int QP>
+constexpr int64_t slot_floats() { return (int64_t)tile_rows<HD, QP>() * (HD + 2); }
+
+// Workgroups that a CU holds (their registers).
+constexpr int wgs_per_cu(int hd, int kp) { return hd * kp <= 192 ? 2 : 1; }
+template <int HD, int KP>
+constexpr int wgs_per_cu() { return wgs_per_cu(HD, KP); }
+
+// bytes of LDS: a stage of Wide; two waves' results of Deep; the plain path's rows
+template <int HD, int KP>
+constexpr int work_lds() {
+    constexpr int kDeep = 2 * (16 * HD + 128) * 4, kPlain = 4 * HD * 4;
+    return std::max({Stage<HD, KP>::kBuffers * Stage<HD, KP>::kBytes, kDeep, kPlain});
 }
 
-// The work's rows over its keys by the four waves: as many waves side by side
-// over the rows as they fill (1, 2 or 4), the others taking every second or
-// fourth block of 32 keys; those are joined into the first waves' registers.
-// Returns whether this wave holds rows, from rho0 on.
+template <int HD, int QP, int KP>
+__device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
+                                         const Sink<HD>& sink) {
+    const int tid = thread_id(), wave = tid >> 6, lane = tid & 63;
+    Deep<HD, QP, KP> r;
+    r.load(a, w, 0);
+    r.run(a.p, w, w.lo + 32 * wave, 128, unit);
+    float* s = reinterpret_cast<float*>(s_buf);
+    if (r.odd()) r.template run_plain<KP>(a, w, 0, w.lo + 32 * wave, 128, unit, s + wave * HD);
+    constexpr int kWave = 16 * HD + 128, VD = HD / 16;
+#pragma unroll
+    for (int half = 2; half >= 1; half /= 2) {   // the upper waves hand theirs to the lower ones
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+            float* o = s + (wave - half) * kWave;
+            o[lane] = r.m[0];
+            o[64 + lane] = r.l[0];
+#pragma unroll
+            for (int j = 0; j < VD; ++j)
+                *reinterpret_cast<f32x4v*>(o + 128 + (j * 64 + lane) * 4) = r.acc[0][j];
+        }
+        __syncthreads();
+        if (wave < half) {
+            const float* o = s + wave * kWave;
+            float f0, f1;
+            join(r.m[0], r.l[0], o[lane], o[64 + lane], unit, f0, f1);
+#pragma unroll
+            for (int j = 0; j < VD; ++j)
+                r.acc[0][j] = r.acc[0][j] * f0 + *reinterpret_cast<const f32x4v*>(o + 128 + (j * 64 + lane) * 4) * f1;
+        }
+    }
+    if (wave == 0) sink.rows(a, w, r, 0);
+}
+
 template <int HD, int QP, int KP, int NT>
-__device__ __forceinline__ bool work_rows(const PagedAttnArgs& a, const Work& w, Wave<HD, QP, KP, NT>& wv, float unit,
-                                          float* s_buf, int& rho0) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int groups = (w.tokens * a.share + 16 * NT - 1) / (16 * NT);
-    const int side = groups <= 1 ? 1 : groups <= 2 ? 2 : 4, deep = 4 / side;
-    const int ks = wave / side;
-    rho0 = (wave % side) * 16 * NT;
-    wv.kc = static_cast<const uint8_t*>(a.p.k);
-    wv.vc = static_cast<const uint8_t*>(a.p.v);
-    wv.g = lane >> 4;
-    wv.c = lane & 15;
-    wv.clear();
+__device__ __forceinline__ void many_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
+                                          const Sink<HD>& sink) {
+    const int wave = thread_id() >> 6, rho0 = wave * 16 * NT;
     const bool rows = rho0 < w.tokens * a.share;
-    if (rows) {
-        bool bad = false;
-        wv.load_q(a, w, rho0);
-        wv.run(a, w, w.lo + 32 * ks, 32 * deep, unit, bad);
-        if (bad) flag_error(a.p.err, kErrPagedPage);
-        if (wv.odd()) wv.run_plain(a, w, rho0, w.lo + 32 * ks, 32 * deep, unit, s_buf + wave * HD);
-    }
-    if (deep == 1) return rows;
-    // halves the waves over the keys: those from `half` on hand theirs to the others
-    constexpr int kWave = Sizes<HD, NT>::kTile + 128 * NT;
-    for (int half = deep / 2; half >= 1; half /= 2) {
-        __syncthreads();
-        if (rows && ks >= half && ks < 2 * half) {
-            float* o = s_buf + ((ks - half) * side + wave % side) * kWave;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                o[(2 * t) * 64 + lane] = wv.m[t];
-                o[(2 * t + 1) * 64 + lane] = wv.l[t];
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        o[128 * NT + ((t * HD / 16 + j) * 4 + v) * 64 + lane] = wv.acc[t][j][v];
-            }
-        }
-        __syncthreads();
-        if (rows && ks < half) {
-            const float* o = s_buf + (ks * side + wave % side) * kWave;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float f0, f1;
-                join(wv.m[t], wv.l[t], o[(2 * t) * 64 + lane], o[(2 * t + 1) * 64 + lane], unit, f0, f1);
-#pragma unroll
-                for (int j = 0; j < HD / 16; ++j)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        wv.acc[t][j][v] =
-                            wv.acc[t][j][v] * f0 + o[128 * NT + ((t * HD / 16 + j) * 4 + v) * 64 + lane] * f1;
-            }
-        }
-    }
-    return rows && ks == 0;
+    Wide<HD, QP, KP, NT> r;
+    r.load(a, w, rho0);
+    r.run(a.p, w, rows, unit, s_buf);
+    if (!rows) return;
+    if (r.odd()) r.template run_plain<KP>(a, w, rho0, w.lo, 32, unit, reinterpret_cast<float*>(s_buf) + wave * HD);
+    sink.rows(a, w, r, rho0);
 }
 
-template <int HD, int NT>
-constexpr int work_lds() {   // floats: two waves' results; the plain path's rows
-    return 2 * (Sizes<HD, NT>::kTile + 128 * NT) > 4 * HD ? 2 * (Sizes<HD, NT>::kTile + 128 * NT) : 4 * HD;
+template <int HD, int QP, int KP>
+__device__ __forceinline__ void compute(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
+                                        const Sink<HD>& sink) {
+    const int n = w.tokens * a.share;
+    if (n <= 16)
+        few_rows<HD, QP, KP>(a, w, unit, s_buf, sink);
+    else if (tile_groups<HD, QP>() == 1 || n <= 64)
+        many_rows<HD, QP, KP, 1>(a, w, unit, s_buf, sink);
+    else if constexpr (tile_groups<HD, QP>() > 1)
+        many_rows<HD, QP, KP, tile_groups<HD, QP>()>(a, w, unit, s_buf, sink);
+}
+
+// Partials: the workgroups' slots; then, with a prefix, its pieces and one more for
+// the rows' own positions, each [num_rows * heads][HD] and their (m, l).
+template <int HD, int QP>
+__device__ __forceinline__ Sink<HD> slot_of(const PagedAttnArgs& a, int i) {
+    float* o = a.part + i * slot_floats<HD, QP>();
+    return {false, o, o + (int64_t)tile_rows<HD, QP>() * HD, false};
+}
+template <int HD>
+__device__ __forceinline__ Sink<HD> piece_of(const PagedAttnArgs& a, int i) {
+    const int64_t rows = (int64_t)a.p.num_rows * a.heads;
+    return {false, a.pre + i * rows * HD, a.pre + (a.splits + 1) * rows * HD + i * rows * 2, true};
 }
 
 // The sequences' own positions: one workgroup per share of the line.
-template <int HD, int QP, int KP, int NT>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
-    constexpr int R = Sizes<HD, NT>::R, VD = HD / 16;
+template <int HD, int QP, int KP>
+__global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_attn_kernel(PagedAttnArgs a) {
     __shared__ int64_t s_cum[kPagedMaxSeqs + 1];
     __shared__ int64_t s_tmp[4];
-    __shared__ __attribute__((aligned(16))) float s_buf[work_lds<HD, NT>()];
+    __shared__ __attribute__((aligned(16))) uint8_t s_buf[work_lds<HD, KP>()];
     const PagedView& p = a.p;
     const float unit = a.scale * 1.44269504f;
     Line ln;
     ln.cum = s_cum;
     ln.org = p.prefix_len & ~31;
-    ln.TT = R / a.share;
+    ln.TT = tile_rows<HD, QP>() / a.share;
     ln.kv_heads = p.kv_heads;
     make_line(p, ln, s_tmp, a.grid, blockIdx.x == 0);
     if (ln.total == 0) return;
@@ -765,48 +1123,18 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
         w.row_pos = 1;
         w.head = t.head;
         w.head0 = t.head * a.share;
-        w.lo = ln.org + (int)(x - t.start);
-        w.hi = ln.org + (int)(end - t.start);
+        w.lo = ln.org + ln.key(t, x);
+        w.hi = ln.org + ln.key(t, end);
         w.first = p.prefix_len;
         w.last = w.pos0 + w.tokens - 1;
         w.table = p.pages + (int64_t)t.seq * p.table_stride;
-        Wave<HD, QP, KP, NT> wv;
-        int rho0;
-        const bool holds = work_rows(a, w, wv, unit, s_buf, rho0);
-        const bool all = x == t.start && end == t.end;
-        float* slot = a.part + (int64_t)(2 * wg + (x > t.start ? 0 : 1)) * Sizes<HD, NT>::kSlot;
-        if (holds) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const int rho = rho0 + 16 * i + wv.c;
-                int token, head;
-                if (!wv.row_at(a, w, rho, token, head)) continue;
-                if (!all && wv.g == 0) {
-                    slot[(int64_t)R * HD + rho] = wv.m[i];
-                    slot[(int64_t)R * HD + R + rho] = wv.l[i];
-                }
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    float o[VD];
-#pragma unroll
-                    for (int j = 0; j < VD; ++j) o[j] = wv.acc[i][j][v];
-                    const int d = VD * (4 * wv.g + v);
-                    if (all) {
-                        float m = wv.m[i], l = wv.l[i];
-                        add_prefix<HD>(a, token, head, d, unit, m, l, o);
-                        const float f = 1.0f / l;
-#pragma unroll
-                        for (int j = 0; j < VD; ++j) o[j] *= f;
-                        store_out<HD, QP == 1>(a, token, head, d, o);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < VD; j += 4)
-                            *reinterpret_cast<float4*>(slot + (int64_t)rho * HD + d + j) =
-                                make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                    }
-                }
-            }
-        }
+        w.uniform();
+        Sink<HD> sink = {true, nullptr, nullptr, false};
+        if (x > t.start || end < t.end)
+            sink = slot_of<HD, QP>(a, 2 * wg + (x > t.start ? 0 : 1));
+        else if (a.splits)
+            sink = piece_of<HD>(a, a.splits);
+        compute<HD, QP, KP>(a, w, unit, s_buf, sink);
         __syncthreads();   // (s_buf is the next tile's)
         x = end;
         if (x < x1) t = ln.tile(p, find_seq(p, ln, x), x);
@@ -815,9 +1143,8 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
 
 // The tiles that several workgroups shared: workgroup w joins the tile that cut w is
 // the first inside of.
-template <int HD, int QP, int NT>
+template <int HD, int QP>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-    constexpr int R = Sizes<HD, NT>::R;
     __shared__ int64_t s_cum[kPagedMaxSeqs + 1];
     __shared__ int64_t s_tmp[4];
     const PagedView& p = a.p;
@@ -825,7 +1152,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     Line ln;
     ln.cum = s_cum;
     ln.org = p.prefix_len & ~31;
-    ln.TT = R / a.share;
+    ln.TT = tile_rows<HD, QP>() / a.share;
     ln.kv_heads = p.kv_heads;
     make_line(p, ln, s_tmp, a.grid, false);
     const int wg = (int)blockIdx.x + 1;
@@ -835,47 +1162,74 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
     if (ln.rounded(t, x) == t.start) return;                            // not cut here
     const int64_t prev = ln.cut(wg - 1);
     if (prev >= t.start && ln.rounded(t, prev) > t.start) return;       // nor first here
-    const int tokens = min(ln.TT, t.n - t.r * ln.TT);
-    for (int i = threadIdx.x; i < tokens * a.share * (HD / 4); i += 256) {
-        const int rho = i / (HD / 4), d = 4 * (i % (HD / 4));
-        const float* slot = a.part + (int64_t)(2 * (wg - 1) + 1) * Sizes<HD, NT>::kSlot;
-        float4 y = *reinterpret_cast<const float4*>(slot + (int64_t)rho * HD + d);
-        float m = slot[(int64_t)R * HD + rho], l = slot[(int64_t)R * HD + R + rho];
-        float o[4] = {y.x, y.y, y.z, y.w};
-        int64_t at = ln.rounded(t, x);
-        for (int w = wg; at < t.end; ++w) {
-            int64_t next = ln.cut(w + 1);
-            next = next >= t.end ? t.end : ln.rounded(t, next);
-            if (next > at) {
-                slot = a.part + (int64_t)(2 * w) * Sizes<HD, NT>::kSlot;
-                y = *reinterpret_cast<const float4*>(slot + (int64_t)rho * HD + d);
-                float f0, f1;
-                join(m, l, slot[(int64_t)R * HD + rho], slot[(int64_t)R * HD + R + rho], unit, f0, f1);
-                o[0] = o[0] * f0 + y.x * f1;
-                o[1] = o[1] * f0 + y.y * f1;
-                o[2] = o[2] * f0 + y.z * f1;
-                o[3] = o[3] * f0 + y.w * f1;
-            }
-            at = next;
-        }
-        const int token = t.row0 + t.r * ln.TT + rho / a.share, head = t.head * a.share + rho % a.share;
-        add_prefix<HD>(a, token, head, d, unit, m, l, o);
-        const float f = 1.0f / l;
+    // (segment by segment, a thread's values of the tile's rows in registers)
+    constexpr int R = tile_rows<HD, QP>(), NV = R * HD / 4 / 256;
+    const int rows = min(ln.TT, t.n - t.r * ln.TT) * a.share, tid = threadIdx.x;
+    float4 o[NV];
+    float m[NV], l[NV];
+    auto segment = [&](const Sink<HD>& slot, bool first) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] *= f;
-        store_out<HD, QP == 1>(a, token, head, d, o);
+        for (int k0 = 0; k0 < NV; k0 += 8) {
+            float4 y[8];
+            float2 z[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = tid + 256 * (k0 + k), rho = min(i / (HD / 4), rows - 1);
+                y[k] = *reinterpret_cast<const float4*>(slot.o + rho * HD + 4 * (i % (HD / 4)));
+                z[k] = *reinterpret_cast<const float2*>(slot.ml + 2 * rho);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                float4& q = o[k0 + k];
+                if (first) {
+                    q = y[k];
+                    m[k0 + k] = z[k].x;
+                    l[k0 + k] = z[k].y;
+                } else {
+                    float f0, f1;
+                    join(m[k0 + k], l[k0 + k], z[k].x, z[k].y, unit, f0, f1);
+                    q = make_float4(q.x * f0 + y[k].x * f1, q.y * f0 + y[k].y * f1, q.z * f0 + y[k].z * f1,
+                                    q.w * f0 + y[k].w * f1);
+                }
+            }
+            if (256 * (k0 + 8) / (HD / 4) >= rows) break;
+        }
+    };
+    segment(slot_of<HD, QP>(a, 2 * (wg - 1) + 1), true);
+    int64_t at = ln.rounded(t, x);
+    for (int w = wg; at < t.end; ++w) {
+        int64_t next = ln.cut(w + 1);
+        next = next >= t.end ? t.end : ln.rounded(t, next);
+        if (next > at) segment(slot_of<HD, QP>(a, 2 * w), false);
+        at = next;
+    }
+    const Sink<HD> own = piece_of<HD>(a, a.splits);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int i = tid + 256 * k, rho = i / (HD / 4), d = 4 * (i % (HD / 4));
+        if (rho >= rows) break;
+        const int token = t.row0 + t.r * ln.TT + rho / a.share, head = t.head * a.share + rho % a.share;
+        if (a.splits) {
+            const int64_t row = (int64_t)token * a.heads + head;
+            *reinterpret_cast<float4*>(own.o + row * HD + d) = o[k];
+            if (d == 0) *reinterpret_cast<float2*>(own.ml + 2 * row) = make_float2(m[k], l[k]);
+        } else {
+            const float f = 1.0f / l[k];
+            store4(a, QP == 1, (int64_t)token * a.out_stride + (int64_t)head * HD + d,
+                   {o[k].x * f, o[k].y * f, o[k].z * f, o[k].w * f});
+        }
     }
 }
 
 // The prefix, for all rows of the batch: workgroup = (tile of rows, kv head, piece of
 // the prefix).
-template <int HD, int QP, int KP, int NT>
-__global__ __launch_bounds__(256) void paged_prefix_kernel(PagedAttnArgs a) {
-    constexpr int R = Sizes<HD, NT>::R, VD = HD / 16;
-    __shared__ __attribute__((aligned(16))) float s_buf[work_lds<HD, NT>()];
+template <int HD, int QP, int KP>
+__global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_prefix_kernel(PagedAttnArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_buf[work_lds<HD, KP>()];
     const PagedView& p = a.p;
     const float unit = a.scale * 1.44269504f;
-    const int TT = R / a.share, head = (int)blockIdx.y % p.kv_heads, piece = (int)blockIdx.y / p.kv_heads;
+    const int TT = tile_rows<HD, QP>() / a.share, head = (int)blockIdx.y % p.kv_heads;
+    const int piece = (int)blockIdx.y / p.kv_heads;
     const int rows = min(p.row_start[p.num_seqs], p.num_rows), blocks = (p.prefix_len + 31) / 32;
     Work w;
     w.token0 = (int)blockIdx.x * TT;
@@ -890,46 +1244,69 @@ __global__ __launch_bounds__(256) void paged_prefix_kernel(PagedAttnArgs a) {
     w.first = 0;
     w.last = p.prefix_len - 1;
     w.table = p.prefix_pages;
-    Wave<HD, QP, KP, NT> wv;
-    int rho0;
-    if (!work_rows(a, w, wv, unit, s_buf, rho0)) return;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        int token, qh;
-        if (!wv.row_at(a, w, rho0 + 16 * i + wv.c, token, qh)) continue;
-        float* o = a.pre + (((int64_t)piece * p.num_rows + token) * a.heads + qh) * (HD + 2);
-        if (wv.g == 0) *reinterpret_cast<float2*>(o + HD) = make_float2(wv.m[i], wv.l[i]);
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-#pragma unroll
-            for (int j = 0; j < VD; j += 2)
-                *reinterpret_cast<float2*>(o + VD * (4 * wv.g + v) + j) =
-                    make_float2(wv.acc[i][j][v], wv.acc[i][j + 1][v]);
+    if (piece == 0) {   // the rows' own part is not there yet (nor ever, where the sequence is skipped)
+        const Sink<HD> own = piece_of<HD>(a, a.splits);
+        for (int i = threadIdx.x; i < w.tokens * a.share; i += 256)
+            own.ml[2 * ((int64_t)(w.token0 + i / a.share) * a.heads + w.head0 + i % a.share) + 1] = -1.f;
     }
+    compute<HD, QP, KP>(a, w, unit, s_buf, piece_of<HD>(a, piece));
 }
 
-template <int HD, int QP, int KP, int NT>
+// A row's pieces of the prefix and its own part: out.
+template <int HD, int QP>
+__global__ __launch_bounds__(256) void paged_pieces_kernel(PagedAttnArgs a) {
+    const float unit = a.scale * 1.44269504f;
+    const int64_t rows = (int64_t)a.p.num_rows * a.heads;
+    const int64_t row = (int64_t)blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4);
+    const int d = 4 * (threadIdx.x % (HD / 4)), token = (int)(row / a.heads), head = (int)(row % a.heads);
+    if (row >= rows || token >= a.p.row_start[a.p.num_seqs]) return;
+    const Sink<HD> all = piece_of<HD>(a, 0);
+    const float2 own = *reinterpret_cast<const float2*>(all.ml + 2 * (a.splits * rows + row));
+    if (own.y < 0.f) return;   // (a skipped sequence's)
+    float m = own.x;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, all.ml[2 * (s * rows + row)]);
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s <= a.splits; ++s) {
+        const float2 z = *reinterpret_cast<const float2*>(all.ml + 2 * (s * rows + row));
+        const float4 y = *reinterpret_cast<const float4*>(all.o + (s * rows + row) * HD + d);
+        const float f = z.x == -INFINITY ? 0.f : weight(z.x - m, unit);
+        l = fmaf(z.y, f, l);
+        o[0] = fmaf(y.x, f, o[0]);
+        o[1] = fmaf(y.y, f, o[1]);
+        o[2] = fmaf(y.z, f, o[2]);
+        o[3] = fmaf(y.w, f, o[3]);
+    }
+    const float f = 1.0f / l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] *= f;
+    store4(a, QP == 1, (int64_t)token * a.out_stride + (int64_t)head * HD + d, o);
+}
+
+template <int HD, int QP, int KP>
 void launch_attn(const PagedAttnArgs& a, hipStream_t st) {
     if (a.splits) {
-        const int TT = 64 * NT / a.share;
-        hipLaunchKernelGGL((paged_prefix_kernel<HD, QP, KP, NT>),
+        const int TT = tile_rows<HD, QP>() / a.share;
+        hipLaunchKernelGGL((paged_prefix_kernel<HD, QP, KP>),
                            dim3((unsigned)((a.p.num_rows + TT - 1) / TT), (unsigned)(a.p.kv_heads * a.splits)),
                            dim3(256), 0, st, a);
     }
-    hipLaunchKernelGGL((paged_attn_kernel<HD, QP, KP, NT>), dim3((unsigned)a.grid), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((paged_join_kernel<HD, QP, NT>), dim3((unsigned)a.grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<HD, QP, KP>), dim3((unsigned)a.grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_join_kernel<HD, QP>), dim3((unsigned)a.grid), dim3(256), 0, st, a);
+    if (a.splits)
+        hipLaunchKernelGGL((paged_pieces_kernel<HD, QP>),
+                           dim3((unsigned)(((int64_t)a.p.num_rows * a.heads + 1024 / HD - 1) / (1024 / HD))),
+                           dim3(256), 0, st, a);
 }
-
-int tile_groups(const PagedAttnArgs&) { return 1; }
 
 template <int HD>
 void launch_attn_hd(const PagedAttnArgs& a, hipStream_t st) {
     if (a.x_bf16)
-        launch_attn<HD, 1, 1, 1>(a, st);
+        launch_attn<HD, 1, 1>(a, st);
     else if (a.cache_bf16)
-        launch_attn<HD, 3, 1, 1>(a, st);
+        launch_attn<HD, 3, 1>(a, st);
     else
-        launch_attn<HD, 3, 3, 1>(a, st);
+        launch_attn<HD, 3, 3>(a, st);
 }
 
 template <int HD>
@@ -943,16 +1320,17 @@ void launch_append_hd(const AppendArgs& a, dim3 grid, hipStream_t st) {
 }  // namespace
 
 int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats) {
-    const int nt = tile_groups(a), R = 64 * nt;
-    a.grid = (2 * cus + 7) / 8 * 8;
+    const int R = a.head_dim <= 128 && a.x_bf16 ? 128 : 64;   // tile_rows
+    const int per = wgs_per_cu(a.head_dim, a.cache_bf16 ? 1 : 3);
+    a.grid = (per * cus + 7) / 8 * 8;
     a.splits = 0;
     *own_floats = (int64_t)a.grid * 2 * R * (a.head_dim + 2);
     if (a.p.prefix_len == 0) return *own_floats;
     const int TT = R / a.share, tiles = (a.p.num_rows + TT - 1) / TT;
     const int64_t wgs = (int64_t)tiles * a.p.kv_heads;
     const int64_t most = std::max(1, a.p.prefix_len / 256);
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (2 * cus + wgs - 1) / wgs, 32}));
-    return *own_floats + (int64_t)a.splits * a.p.num_rows * a.heads * (a.head_dim + 2);
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (per * cus + wgs - 1) / wgs, 32}));
+    return *own_floats + (int64_t)(a.splits + 1) * a.p.num_rows * a.heads * (a.head_dim + 2);
 }
 
 int launch_paged_attention(const PagedAttnArgs& a, void* stream) {
