@@ -53,12 +53,19 @@ struct SampleArgs {
     const int32_t* top_k;
     int32_t* tokens;
     float* probs;
+    // workgroups per row and, for more than one, their histograms ([rows * parts][2048]
+    // sums and counts) and a counter per row, zero between launches
+    int32_t parts;
+    unsigned long long* part_sum;
+    uint32_t *part_cnt, *counters;
 };
 
 int launch_kv_append(const AppendArgs& a, int cus, void* stream);
 // Sets grid and splits; the floats of partials (own, then the prefix') needed.
 int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats);
 int launch_paged_attention(const PagedAttnArgs& a, void* stream);
+int sample_parts(int rows, int vocab, int cus);
+int64_t sample_part_words(int cus);   // of part_sum, part_cnt and counters, in this order (sums as two)
 int launch_sample(const SampleArgs& a, void* stream);
 
 }  // namespace m1moe

@@ -5,10 +5,18 @@
 // filter keeps a beginning of that order, and so does all of them together:
 // the kept sum S is the smallest of theirs, and the drawn token is the first
 // whose running sum reaches u S.  Nothing is sorted: each of these places is
-// looked for by value.  The weights w = e^((x - max) / T) are computed in f64
-// and rounded to whole multiples of 2^-44, so that their sums are integer sums:
-// exact, whatever their order (2^18 logits of weight 1 stay below 2^63).
+// looked for by value, in a histogram and then among one step's logits.  The
+// weights w = e^((x - max) / T) are computed in f64 and rounded to whole
+// multiples of 2^-44, so that their sums are integer sums: exact, whatever their
+// order (2^18 logits of weight 1 stay below 2^63).
+//
+// Bound by one CU's work on a row (f64 weights, LDS atomics, the chain of
+// searches), so while rows are fewer than CUs several workgroups share a row's
+// histogram, and the last of them to end adds the others' up and searches.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "device.hpp"
 #include "paged.hpp"
@@ -19,9 +27,11 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024, kWaves = 16;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;      // steps of a histogram
+constexpr int kPer = kBins / kThreads;   // a thread's neighbouring steps
 constexpr int kList = 256;       // a step of at most so many logits is ranked in pairs
+constexpr int kFront = 1024;    // the order's beginning, kept aside where it is at most so long
 constexpr int kUnit = 44;        // weights are whole multiples of 2^-44
 
 // 2^t for t <= 0 in units of 2^-44 (0 below half a unit), and as it is.  2^f on
@@ -50,7 +60,10 @@ struct Scale {
     __device__ __forceinline__ double exponent(float x) const {   // <= 0; NaN or -inf: no weight
         return x == top ? 0.0 : ((double)x - (double)top) * c;
     }
-    __device__ __forceinline__ bool some(float x) const { return exponent(x) >= -45.0; }
+    // Weights of smaller logits are 0 (the smallest of them may be, too).
+    __device__ __forceinline__ float lowest() const {
+        return top == INFINITY ? top : (float)((double)top - 45.5 / c);   // (-inf at an infinite T)
+    }
     __device__ __forceinline__ u64 units(float x) const {
         const double t = exponent(x);
         // (adding 2^52 leaves the rounded units in the low bits)
@@ -59,61 +72,76 @@ struct Scale {
     }
 };
 
-// The thread's logits: 4 (tid + 1024 j) .. + 3 for j = 0, 1, ..., NaN and those
-// past the vocabulary as -inf; NV > 0: in registers, else read again each pass.
-template <int NV>
+// The thread's logits: the fours 4 (tid + 1024 j) .. + 3 for j = 0, 1, ... and one of
+// the vocabulary's last, fewer than four.  NaN and -inf are in no range that is asked
+// for.  Every pass reads them again, from the L2 after the first (kept in
+// registers, with 512 threads, they leave too few for the f64 weights: 36.9 against
+// 35.7 us for one row of 50304).
 struct Row {
     const float* x;
-    int vocab;
-    float4 v[NV > 0 ? NV : 1];
+    int vocab, fours;
+    float last;
 
+    // (past the end: the last four again)
     __device__ __forceinline__ float4 load(int j) const {
-        const int i = 4 * ((int)threadIdx.x + kThreads * j);
-        float e[4];
-        if (i + 3 < vocab) {
-            const float4 y = *reinterpret_cast<const float4*>(x + i);
-            e[0] = y.x;
-            e[1] = y.y;
-            e[2] = y.z;
-            e[3] = y.w;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) e[k] = i + k < vocab ? x[i + k] : -INFINITY;
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = __builtin_isnan(e[k]) ? -INFINITY : e[k];
-        return make_float4(e[0], e[1], e[2], e[3]);
+        return reinterpret_cast<const float4*>(x)[min((int)threadIdx.x + kThreads * j, fours - 1)];
     }
+    __device__ __forceinline__ bool has(int j) const { return (int)threadIdx.x + kThreads * j < fours; }
     __device__ __forceinline__ void init(const float* row, int n) {
         x = row;
         vocab = n;
-        if constexpr (NV > 0) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) v[j] = load(j);
-        }
+        fours = n >> 2;
+        const int i = 4 * fours + (int)threadIdx.x;
+        last = i < n ? x[i] : -INFINITY;
     }
-    __device__ __forceinline__ int chunks() const { return (vocab + 4 * kThreads - 1) / (4 * kThreads); }
+    __device__ __forceinline__ int chunks() const { return (fours + kThreads - 1) / kThreads; }
+    // f(four logits, the first one's index) of the thread's fours and, the last one with
+    // three times -inf, of the rest; eight loads in flight
     template <class F>
     __device__ __forceinline__ void each(F&& f) const {
-        if constexpr (NV > 0) {
+        for (int j = 0; j < chunks(); j += 8) {
+            float4 y[8];
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int i = 4 * ((int)threadIdx.x + kThreads * j);
-                f(v[j].x, i);
-                f(v[j].y, i + 1);
-                f(v[j].z, i + 2);
-                f(v[j].w, i + 3);
+            for (int k = 0; k < 8; ++k) y[k] = load(j + k);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (has(j + k)) f(y[k], 4 * ((int)threadIdx.x + kThreads * (j + k)));
+        }
+        f(make_float4(last, -INFINITY, -INFINITY, -INFINITY), 4 * fours + (int)threadIdx.x);
+    }
+    // f(logit, index) of those in [from, to], few of them (from above -inf)
+    template <class F>
+    __device__ __forceinline__ void each_in(float from, float to, F&& f) const {
+        each([&](float4 y, int i) {
+            const auto in = [&](float v) { return v >= from && v <= to; };
+            if (!(in(y.x) | in(y.y) | in(y.z) | in(y.w))) return;
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+                const float t = y.x;
+                y = make_float4(y.y, y.z, y.w, t);
+                if (in(t)) f(t, i + e);
             }
-        } else {
-            for (int j = 0; j < chunks(); ++j) {
-                const float4 y = load(j);
-                const int i = 4 * ((int)threadIdx.x + kThreads * j);
-                f(y.x, i);
-                f(y.y, i + 1);
-                f(y.z, i + 2);
-                f(y.w, i + 3);
+        });
+    }
+    // f(logit) of the chunks first, first + step, ..., one by one (the weights of several
+    // at once need more registers than there are), and of the last ones with chunk 0.
+    template <class F>
+    __device__ __forceinline__ void each_of(F&& f, int first, int step) const {
+        if (first < chunks()) {
+            float4 y = load(first);
+            for (int j = first; j < chunks(); j += step) {
+                float4 e = y;
+                y = load(j + step);   // (on its way meanwhile)
+                if (!has(j)) continue;
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    const float t = e.x;
+                    e = make_float4(e.y, e.z, e.w, t);
+                    f(t);
+                }
             }
         }
+        if (first == 0) f(last);
     }
 };
 
@@ -136,10 +164,21 @@ struct Span {
     __device__ __forceinline__ int step(float x) const {
         return x == hi ? 0 : (int)(((double)hi - (double)x) * per);
     }
+    // f32 bounds around the logits of steps a .. b, for a first glance.
+    __device__ __forceinline__ void bounds(int a, int b, float& from, float& to) const {
+        const double x0 = (double)hi - (b + 1) / per, x1 = (double)hi - a / per;
+        from = per > 0.0 ? (float)(x0 - 1e-6 * fabs(x0)) : lo;
+        to = per > 0.0 ? (float)(x1 + 1e-6 * fabs(x1)) : hi;
+        from = fmaxf(from, lo);
+        to = fminf(to, hi);
+    }
 };
 
 struct Shared {
     Bins top, sub;            // all logits with a weight; those of one step
+    float fx[kFront];         // the logits of the top steps, in any order, and their indexes
+    int fi[kFront];
+    int fn;
     float lx[kList];          // one step's logits
     int li[kList];
     u64 lw[kList];
@@ -174,27 +213,34 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     return m;
 }
 
-template <int NV>
-__device__ __forceinline__ void histogram(const Row<NV>& row, const Scale& sc, const Span& sp, Bins& b, Shared& s) {
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    for (int i = tid; i < kBins; i += kThreads) {
+__device__ __forceinline__ void fill(const Row& row, const Scale& sc, const Span& sp, Bins& b, bool counts,
+                                     int first, int step) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
         b.sum[i] = 0;
         b.cnt[i] = 0;
     }
     __syncthreads();
-    row.each([&](float x, int) {
-        if (sp.in(x)) {
-            const int k = sp.step(x);
-            atomicAdd(&b.sum[k], sc.units(x));
-            atomicAdd(&b.cnt[k], 1u);
-        }
-    });
+    row.each_of([&](float x) {
+        if (!sp.in(x)) return;
+        const int k = sp.step(x);
+        atomicAdd(&b.sum[k], sc.units(x));
+        if (counts) atomicAdd(&b.cnt[k], 1u);
+    }, first, step);
     __syncthreads();
-    // two neighbouring steps per thread, summed over the workgroup
-    const u64 s0 = b.sum[2 * tid], s1 = b.sum[2 * tid + 1];
-    const uint32_t c0 = b.cnt[2 * tid], c1 = b.cnt[2 * tid + 1];
-    u64 ss = s0 + s1;
-    uint32_t cc = c0 + c1;
+}
+
+// Turns the steps' sums and counts (of steps kPer tid ..) into what lies above each.
+__device__ __forceinline__ void scan(Bins& b, const u64 (&sum)[kPer], const uint32_t (&cnt)[kPer], Shared& s) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    u64 ss = 0;
+    uint32_t cc = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        ss += sum[i];
+        cc += cnt[i];
+    }
+    const u64 s_own = ss;
+    const uint32_t c_own = cc;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
         const u64 o = __shfl_up(ss, m);
@@ -209,23 +255,106 @@ __device__ __forceinline__ void histogram(const Row<NV>& row, const Scale& sc, c
         s.red32[wave] = cc;
     }
     __syncthreads();
-    u64 bs = 0;
-    uint32_t bc = 0;
+    ss -= s_own;
+    cc -= c_own;
     for (int w = 0; w < wave; ++w) {
-        bs += s.red[w];
-        bc += s.red32[w];
+        ss += s.red[w];
+        cc += s.red32[w];
     }
-    ss += bs;
-    cc += bc;
-    b.sum[2 * tid] = ss - s0 - s1;
-    b.sum[2 * tid + 1] = ss - s1;
-    b.cnt[2 * tid] = cc - c0 - c1;
-    b.cnt[2 * tid + 1] = cc - c1;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        b.sum[kPer * tid + i] = ss;
+        b.cnt[kPer * tid + i] = cc;
+        ss += sum[i];
+        cc += cnt[i];
+    }
     if (tid == kThreads - 1) {
         b.sum[kBins] = ss;
         b.cnt[kBins] = cc;
     }
     __syncthreads();
+}
+
+__device__ __forceinline__ void histogram(const Row& row, const Scale& sc, const Span& sp, Bins& b, bool counts,
+                                          Shared& s) {
+    fill(row, sc, sp, b, counts, 0, 1);
+    u64 sum[kPer];
+    uint32_t cnt[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        sum[i] = b.sum[kPer * (int)threadIdx.x + i];
+        cnt[i] = b.cnt[kPer * (int)threadIdx.x + i];
+    }
+    scan(b, sum, cnt, s);
+}
+
+// (Counts are kept where top-k asks for them.)
+// A row's histogram made by `parts` workgroups, part `mine` this one's: true in
+// the last of them to end, which has the whole.  Stores and loads of the parts are
+// coherent across the XCDs, and complete before the workgroup is counted.
+__device__ __forceinline__ bool gather(Bins& b, bool counts, Shared& s, const SampleArgs& a, int row, int mine) {
+    const int tid = threadIdx.x, parts = a.parts;
+    u64* sums = a.part_sum + ((int64_t)row * parts) * kBins + tid;
+    uint32_t* cnts = a.part_cnt + ((int64_t)row * parts) * kBins + tid;
+    const auto put = [](auto* p, auto v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const auto get = [](const auto* p) {
+        return __hip_atomic_load(const_cast<std::remove_const_t<std::remove_pointer_t<decltype(p)>>*>(p),
+                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    u64 sum[kPer];
+    uint32_t cnt[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {   // (neighbouring lanes, neighbouring words)
+        sum[i] = b.sum[kPer * tid + i];
+        cnt[i] = b.cnt[kPer * tid + i];
+        put(sums + mine * kBins + i * kThreads, sum[i]);
+        if (counts) put(cnts + mine * kBins + i * kThreads, cnt[i]);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+        const uint32_t before =
+            __hip_atomic_fetch_add(a.counters + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s.bin = before == (uint32_t)parts - 1u;
+        if (s.bin) put(a.counters + row, 0u);
+    }
+    __syncthreads();
+    const bool last = s.bin != 0;
+    __syncthreads();
+    if (!last) return false;
+#pragma unroll 4
+    for (int c = 0; c < parts; ++c) {
+        if (c == mine) continue;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            sum[i] += get(sums + c * kBins + i * kThreads);
+            if (counts) cnt[i] += get(cnts + c * kBins + i * kThreads);
+        }
+    }
+    scan(b, sum, cnt, s);
+    return true;
+}
+
+// The logits of the steps down to `bin` of all, kept aside by the search for the end
+// of the first top_k: the later places lie above it, and their searches need not read
+// the row again.  (Where their number is not known before, as with top-p alone, keeping
+// them costs more than a pass: 28.5 -> 31.6 us for one row.)
+struct Front {
+    int bin;         // -1: none
+};
+
+template <class F>
+__device__ __forceinline__ void each_in(const Row& row, const Front& fr, const Shared& s, float from, float to,
+                                        F&& f) {
+    if (fr.bin < 0) {
+        row.each_in(from, to, f);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kFront / kThreads; ++i) {
+        const int at = (int)threadIdx.x + kThreads * i;
+        if (at < s.fn && s.fx[at] >= from && s.fx[at] <= to) f(s.fx[at], s.fi[at]);
+    }
 }
 
 // A place in the order: the first logit at which the running count (by_count)
@@ -237,9 +366,8 @@ struct Found {
     int index;
 };
 
-template <int NV>
-__device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shared& s, bool by_count, u64 target,
-                      bool index) {
+__device__ __forceinline__ Found find(const Row& row, Front& fr, const Scale& sc, const Span& all, Shared& s,
+                                      bool counts, bool by_count, u64 target, bool index) {
     const int tid = threadIdx.x;
     Span sp = all;
     const Bins* b = &s.top;
@@ -249,8 +377,8 @@ __device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shar
         // the step that the place lies in
         const u64 want = by_count ? target - n_above : target - above;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int k = 2 * tid + i;
+        for (int i = 0; i < kPer; ++i) {
+            const int k = kPer * tid + i;
             const u64 lo = by_count ? b->cnt[k] : b->sum[k], hi = by_count ? b->cnt[k + 1] : b->sum[k + 1];
             if (lo < want && want <= hi) {
                 s.bin = k;
@@ -261,33 +389,65 @@ __device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shar
         }
         __syncthreads();
         const int bin = s.bin;
-        const uint32_t n = b->cnt[bin + 1] - b->cnt[bin];
+        uint32_t n = b->cnt[bin + 1] - b->cnt[bin];   // (0 without counts)
         above += b->sum[bin];
         n_above += b->cnt[bin];
+        float from, to;
+        if (by_count && b == &s.top && n_above + n <= kFront) {
+            if (tid == 0) s.fn = 0;
+            __syncthreads();
+            all.bounds(0, bin, from, to);
+            row.each_in(from, to, [&](float x, int i) {
+                if (all.step(x) > bin) return;
+                const int at = atomicAdd(&s.fn, 1);
+                s.fx[at] = x;
+                s.fi[at] = i;
+            });
+            __syncthreads();
+            fr.bin = bin;
+        }
+        sp.bounds(bin, bin, from, to);
         if (n <= kList) {
-            row.each([&](float x, int i) {
-                if (sp.in(x) && sp.step(x) == bin) {
+            each_in(row, fr, s, from, to, [&](float x, int i) {
+                if (sp.step(x) == bin) {
                     const int at = atomicAdd(&s.n, 1);
-                    s.lx[at] = x;
-                    s.li[at] = i;
-                    s.lw[at] = sc.units(x);
+                    if (at < kList) {
+                        s.lx[at] = x;
+                        s.li[at] = i;
+                    }
                 }
             });
             __syncthreads();
-            if (tid < (int)n) {
-                const float x = s.lx[tid];
-                const int i = s.li[tid];
-                const u64 w = s.lw[tid];
-                u64 sum = above + w;
-                uint32_t cnt = n_above + 1;
-                for (int j = 0; j < (int)n; ++j) {
+            n = s.n;
+        }
+        if (n <= kList) {
+            if (tid < (int)n) s.lw[tid] = sc.units(s.lx[tid]);
+            __syncthreads();
+            // the lanes per logit of the step that there are, up to 64, share the others
+            int shift = 2;
+            static_assert(kThreads >> 2 == kList, "four lanes per logit of a full list");
+            while (shift < 6 && (int)n << (shift + 1) <= kThreads) ++shift;
+            const int lanes = 1 << shift, mine = tid >> shift;
+            if (mine < (int)n) {
+                const float x = s.lx[mine];
+                const int i = s.li[mine];
+                const u64 w = s.lw[mine];
+                u64 sum = 0;
+                uint32_t cnt = 0;
+#pragma unroll 2
+                for (int j = tid & (lanes - 1); j < (int)n; j += lanes) {
                     const float y = s.lx[j];
-                    if (y > x || (y == x && s.li[j] < i)) {
-                        sum += s.lw[j];
-                        ++cnt;
-                    }
+                    const bool before = y > x || (y == x && s.li[j] < i);
+                    sum += before ? s.lw[j] : 0;
+                    cnt += before;
                 }
-                if (by_count ? cnt == target : sum >= target && sum - w < target) {
+                for (int m = 1; m < lanes; m <<= 1) {
+                    sum += __shfl_xor(sum, m);
+                    cnt += __shfl_xor(cnt, m);
+                }
+                sum += above + w;
+                cnt += n_above + 1;
+                if ((tid & (lanes - 1)) == 0 && (by_count ? cnt == target : sum >= target && sum - w < target)) {
                     s.sum = sum;
                     s.x = x;
                     s.at = i;
@@ -300,8 +460,8 @@ __device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shar
         }
         // narrower: from its smallest to its largest logit
         uint32_t klo = 0xFFFFFFFFu, khi = 0u;
-        row.each([&](float x, int) {
-            if (sp.in(x) && sp.step(x) == bin) {
+        each_in(row, fr, s, from, to, [&](float x, int) {
+            if (sp.step(x) == bin) {
                 klo = min(klo, order_of(x));
                 khi = max(khi, order_of(x));
             }
@@ -314,7 +474,7 @@ __device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shar
         sp.set(of_order(s.key_lo), of_order(s.key_hi));
         __syncthreads();
         if (sp.lo == sp.hi) break;
-        histogram(row, sc, sp, s.sub, s);
+        histogram(row, sc, sp, s.sub, counts, s);
         b = &s.sub;
     }
     // all of them the same logit: the j-th of them by index
@@ -324,9 +484,12 @@ __device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shar
     if (!index) return f;
     u64 seen = 0;
     const int wave = tid >> 6, lane = tid & 63;
-    for (int c = 0; c < row.chunks(); ++c) {
-        const float4 y = row.load(c);
-        const uint32_t e[4] = {y.x == sp.hi, y.y == sp.hi, y.z == sp.hi, y.w == sp.hi};
+    for (int c = 0; c <= row.chunks(); ++c) {   // (the last ones after all fours)
+        const bool end = c == row.chunks();
+        const bool on = end || row.has(c);
+        float4 y = make_float4(row.last, -INFINITY, -INFINITY, -INFINITY);
+        if (!end) y = row.load(c);
+        const uint32_t e[4] = {on && y.x == sp.hi, on && y.y == sp.hi, on && y.z == sp.hi, on && y.w == sp.hi};
         uint32_t q = e[0] + e[1] + e[2] + e[3];
         const uint32_t mine = q;
 #pragma unroll
@@ -345,7 +508,7 @@ __device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shar
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             at += e[k];
-            if (e[k] && at == j) s.at = 4 * (tid + kThreads * c) + k;
+            if (e[k] && at == j) s.at = end ? 4 * row.fours + tid : 4 * (tid + kThreads * c) + k;
         }
         __syncthreads();
         if (seen >= j) break;
@@ -355,30 +518,34 @@ __device__ Found find(const Row<NV>& row, const Scale& sc, const Span& all, Shar
     return f;
 }
 
-template <int NV>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     __shared__ Shared s;
-    const int r = (int)blockIdx.x, tid = threadIdx.x;
-    Row<NV> row;
+    const int r = (int)blockIdx.x / a.parts, part = (int)blockIdx.x % a.parts, tid = threadIdx.x;
+    Row row;
     row.init(a.logits + (int64_t)r * a.stride, a.vocab);
     const float T = a.temperature ? a.temperature[r] : 1.f;
-    float top = -INFINITY;
-    row.each([&](float x, int) { top = fmaxf(top, x); });
+    float top = -INFINITY, low = -INFINITY;   // (low: of the negated logits)
+    row.each([&](float4 y, int) {
+        // (fmaxf passes over NaN)
+        top = fmaxf(fmaxf(top, y.x), fmaxf(y.y, fmaxf(y.z, y.w)));
+        const auto neg = [](float x) { return x == -INFINITY ? x : -x; };
+        low = fmaxf(fmaxf(low, neg(y.x)), fmaxf(neg(y.y), fmaxf(neg(y.z), neg(y.w))));
+    });
     top = block_max(top, s.redf[0]);
+    low = -block_max(low, s.redf[1]);
     if (top == -INFINITY) {
-        if (tid == 0) {
+        if (tid == 0 && part == 0) {
             a.tokens[r] = -1;
             if (a.probs) a.probs[r] = 0.f;
         }
         return;
     }
     if (!(T > 0.f)) {   // the largest, at its lowest index
+        if (part) return;
         if (tid == 0) s.at = 0x7FFFFFFF;
         __syncthreads();
         int best = 0x7FFFFFFF;
-        row.each([&](float x, int i) {
-            if (x == top) best = min(best, i);
-        });
+        row.each_in(top, top, [&](float, int i) { best = min(best, i); });
         if (best != 0x7FFFFFFF) atomicMin(&s.at, best);
         __syncthreads();
         if (tid == 0) {
@@ -388,51 +555,56 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
         return;
     }
     const Scale sc{top, 1.4426950408889634 / (double)T};
-    float low = -INFINITY;   // (of the negated logits: the smallest with a weight)
-    row.each([&](float x, int) {
-        if (sc.some(x)) low = fmaxf(low, -x);
-    });
-    low = -block_max(low, s.redf[1]);
     Span all;
-    all.set(low, top);
-    histogram(row, sc, all, s.top, s);
-    u64 kept = s.top.sum[kBins];
+    all.set(fmaxf(low, sc.lowest()), top);
     const int k = a.top_k ? a.top_k[r] : 0;
-    if (k > 0 && (uint32_t)k < s.top.cnt[kBins]) kept = find(row, sc, all, s, true, (u64)k, false).sum;
-    const float mp = a.min_p ? a.min_p[r] : 0.f;
-    u64 kept_m = kept;
-    if (mp > 0.f) {
-        // weights of at least min_p: whole steps above the one that holds the border,
-        // and that one's logits
-        const double border = fmin(log2((double)mp), 0.0);
-        const double xb = (double)top + border / sc.c;
-        if (tid == 0) s.units = 0;
-        const int bin = !(xb > (double)low) ? kBins - 1
-                                           : (int)fmin(((double)top - xb) * all.per, (double)(kBins - 1));
-        __syncthreads();
-        // (a step to either side: the border's own step is rounded another way)
-        const int b0 = max(bin - 1, 0), b1 = min(bin + 1, kBins - 1);
-        row.each([&](float x, int) {
-            if (all.in(x)) {
-                const int b = all.step(x);
-                if (b >= b0 && b <= b1 && sc.exponent(x) >= border) atomicAdd(&s.units, sc.units(x));
+    const bool counts = k > 0;
+    if (a.parts == 1) {
+        histogram(row, sc, all, s.top, counts, s);
+    } else {
+        fill(row, sc, all, s.top, counts, part, a.parts);
+        if (!gather(s.top, counts, s, a, r, part)) return;
+    }
+    const float mp = a.min_p ? a.min_p[r] : 0.f, tp = a.top_p ? a.top_p[r] : 1.f, u = a.u[r];
+    u64 kept = s.top.sum[kBins];
+    // the end of the first top_k, of the fewest with top_p of what is left, the draw
+    Front fr{-1};
+    Found f{0, 0.f, 0};
+#pragma unroll 1
+    for (int phase = 0; phase < 3; ++phase) {
+        if (phase == 0 && !(k > 0 && (uint32_t)k < s.top.cnt[kBins])) continue;
+        if (phase == 1 && !(tp < 1.f)) continue;
+        if (phase == 2 && mp > 0.f) {
+            // weights of at least min_p: whole steps above the one that holds the border,
+            // and the logits of that one (and, as it is rounded another way, of the steps
+            // to either side); a border below the front leaves all that is kept
+            const double border = fmin(log2((double)mp), 0.0);
+            const double xb = (double)top + border / sc.c;
+            const int bin = !(xb > (double)all.lo) ? kBins - 1
+                                                  : (int)fmin(((double)top - xb) * all.per, (double)(kBins - 1));
+            const int b0 = max(bin - 1, 0), b1 = min(bin + 1, kBins - 1);
+            if (mp > 1.f) {
+                kept = 1ull << kUnit;
+            } else if (fr.bin < 0 || b1 <= fr.bin) {
+                if (tid == 0) s.units = 0;
+                __syncthreads();
+                float from, to;
+                all.bounds(b0, b1, from, to);
+                each_in(row, fr, s, from, to, [&](float x, int) {
+                    const int b = all.step(x);
+                    if (b >= b0 && b <= b1 && sc.exponent(x) >= border) atomicAdd(&s.units, sc.units(x));
+                });
+                __syncthreads();
+                const u64 sum = s.top.sum[b0] + s.units;
+                if (sum < kept) kept = sum;
             }
-        });
-        __syncthreads();
-        kept_m = mp > 1.f ? 1ull << kUnit : s.top.sum[b0] + s.units;
-    }
-    const float tp = a.top_p ? a.top_p[r] : 1.f;
-    if (tp < 1.f) {
-        u64 want = (u64)ceil(fmax((double)tp, 0.0) * (double)kept);
+        }
+        const double share = phase == 1 ? fmax((double)tp, 0.0) : u > 0.f ? fmin((double)u, 1.0) : 0.0;
+        u64 want = (u64)ceil(share * (double)kept);
         want = want < 1 ? 1 : want > kept ? kept : want;
-        const u64 sum = find(row, sc, all, s, false, want, false).sum;
-        kept = sum < kept ? sum : kept;
+        f = find(row, fr, sc, all, s, counts, phase == 0, phase == 0 ? (u64)k : want, phase == 2);
+        if (phase < 2 && f.sum < kept) kept = f.sum;
     }
-    kept = kept_m < kept ? kept_m : kept;
-    const float u = a.u[r];
-    u64 want = (u64)ceil((u > 0.f ? fmin((double)u, 1.0) : 0.0) * (double)kept);
-    want = want < 1 ? 1 : want > kept ? kept : want;
-    const Found f = find(row, sc, all, s, false, want, true);
     if (tid == 0) {
         a.tokens[r] = f.index;
         if (a.probs)
@@ -442,17 +614,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 
 }  // namespace
 
+// While the rows leave CUs idle, up to kMostParts workgroups per row, each with
+// at least one chunk of its logits.
+int sample_parts(int rows, int vocab, int cus) {
+    constexpr int kMostParts = 8;
+    const int chunks = (vocab + 4 * kThreads - 1) / (4 * kThreads);
+    return std::max(1, std::min({cus / rows, chunks, kMostParts}));
+}
+int64_t sample_part_words(int cus) { return (int64_t)cus * (3 * kBins + 1); }
+
 int launch_sample(const SampleArgs& a, void* stream) {
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)a.rows), block(kThreads);
-    if (a.vocab <= 4 * kThreads * 4)
-        hipLaunchKernelGGL(sample_kernel<4>, grid, block, 0, st, a);
-    else if (a.vocab <= 4 * kThreads * 8)
-        hipLaunchKernelGGL(sample_kernel<8>, grid, block, 0, st, a);
-    else if (a.vocab <= 4 * kThreads * 13)
-        hipLaunchKernelGGL(sample_kernel<13>, grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL(sample_kernel<0>, grid, block, 0, st, a);
+    const dim3 grid((unsigned)(a.rows * a.parts)), block(kThreads);
+    hipLaunchKernelGGL(sample_kernel, grid, block, 0, st, a);
     return (int)hipGetLastError();
 }
 

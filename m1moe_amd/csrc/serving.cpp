@@ -110,6 +110,21 @@ int32_t ensure_paged_scratch(m1moe_ctx_t ctx, uint64_t floats) {
     return M1MOE_OK;
 }
 
+// The histograms of m1moe_sample's workgroups.  Not there yet while the stream is
+// captured: the call does without (one workgroup per row, the same results).
+int32_t ensure_sample_scratch(m1moe_ctx_t ctx) {
+    if (ctx->sample_part) return M1MOE_OK;
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(ctx->stream, &cs));
+    if (cs != hipStreamCaptureStatusNone) return M1MOE_OK;
+    const uint64_t bytes = (uint64_t)sample_part_words(ctx->cus) * 4;
+    int32_t rc = device_alloc((void**)&ctx->sample_part, bytes, "sampling scratch");
+    if (rc) return rc;
+    // (the counters; on the launches' own stream)
+    HIP_TRY(hipMemsetAsync(ctx->sample_part, 0, bytes, ctx->stream));
+    return M1MOE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -238,6 +253,15 @@ int32_t m1moe_sample(m1moe_ctx_t ctx, const float* d_logits, int32_t rows, int32
     a.min_p = s->d_min_p;
     a.tokens = d_tokens;
     a.probs = d_probs;
+    a.parts = sample_parts(rows, vocab, ctx->cus);
+    if (a.parts > 1 && (rc = ensure_sample_scratch(ctx))) return rc;
+    if (!ctx->sample_part) a.parts = 1;
+    if (a.parts > 1) {
+        const uint64_t bins = sample_part_words(ctx->cus) / (3 * (uint64_t)ctx->cus);   // words per part
+        a.part_sum = reinterpret_cast<unsigned long long*>(ctx->sample_part);
+        a.part_cnt = ctx->sample_part + 2 * bins * ctx->cus;
+        a.counters = a.part_cnt + bins * ctx->cus;
+    }
     return launched(launch_sample(a, ctx->stream), "sample");
 }
 

@@ -590,6 +590,21 @@ def test_sample_odd_values(dev):
     check_draw(dev, x, s)
 
 
+def test_sample_dense_steps(dev):
+    """One logit far above the others, which then share few steps of a histogram over
+    all: more of them in a step than are ranked at once, with every setting's end there."""
+    rng = np.random.default_rng(44)
+    V = 30000
+    x = rng.normal(0, 1, (12, V)).astype(np.float32)
+    x[:, 777] = 1000.0
+    s = [dict(u=u, T=300.0, **k) for u in (0.2, 0.95) for k in
+         (dict(), dict(top_k=5), dict(top_k=300), dict(top_k=2000), dict(top_p=0.9), dict(top_k=900, top_p=0.97))]
+    for i in (1, 3, 7):
+        s[i]["min_p"] = float(np.exp(-1000 / 300.0) * 1.002)
+    say("sample dense steps")
+    check_draw(dev, x, s)
+
+
 def test_sample_settings_at_their_ends(dev):
     rng = np.random.default_rng(41)
     V = 9000
