@@ -103,6 +103,7 @@ struct m1moe_ctx {
     // partials of m1moe_paged_attention, grown on demand
     float* paged_part = nullptr;
     uint64_t paged_part_floats = 0;
+    uint32_t* paged_cnt = nullptr;   // its workgroups' counters, zero between launches
     // m1moe_sample's workgroups' histograms, made by its first call
     uint32_t* sample_part = nullptr;
     std::set<void*> allocs;

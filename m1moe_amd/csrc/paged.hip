@@ -201,7 +201,6 @@ __device__ __forceinline__ float quads_add(float v) {
 __device__ __forceinline__ float weight(float x, float unit) { return __builtin_amdgcn_exp2f(x * unit); }
 
 constexpr int kCut = 256;        // keys: where a tile's keys may be cut between workgroups
-constexpr int kFewKeys = 128;    // least places on the line per workgroup
 constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 
 // How the rows and keys are shared.  A tile is up to R rows (token, head) of one
@@ -217,12 +216,20 @@ constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 struct Tile {
     int seq, head, r;            // sequence, kv head, tile of its rows
     int row0, n, base;           // the sequence's first row, rows, positions before them
-    int64_t start, end;          // on the line
+    int64_t cum, start, end;     // on the line: the sequence's start, the tile's, its end
+
+    // (the sequence's are the same in every lane: into scalar registers)
+    __device__ __forceinline__ void uniform() {
+        for (int* x : {&seq, &row0, &n, &base}) *x = __builtin_amdgcn_readfirstlane(*x);
+        cum = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(cum >> 32)) << 32 |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)cum));
+    }
 };
 
 struct Line {
     int64_t* cum;                // LDS [num_seqs + 1]: the sequences' starts on the line
-    int64_t total;
+    int64_t total, share;
+    int rest;                    // the first shares have a place more
     int wgs;                     // workgroups that have a share
     int org, TT, kv_heads;
 
@@ -233,21 +240,34 @@ struct Line {
     __device__ int64_t head_places(int base, int n, int tiles) const {
         return before(base, tiles - 1) + (base - org + kTileKeys) + n;
     }
-    __device__ int64_t cut(int w) const {
-        return w >= wgs ? total : (int64_t)((double)total * w / wgs);
+    // Equal shares but for one place, at least kCut places, so that every cut inside a
+    // tile's keys begins a piece of its own.
+    __device__ int64_t cut(int w) const { return w * share + min(w, rest); }
+    // The last cut below place x > 0.
+    __device__ int below(int64_t x) const {
+        int w = min((int)((double)x / (double)share), wgs - 1);
+        while (w + 1 < wgs && cut(w + 1) < x) ++w;
+        while (w > 0 && cut(w) >= x) --w;
+        return w;
     }
-    // The tile that holds place x (0 <= x < total) of sequence s.
-    __device__ Tile tile(const PagedView& p, int s, int64_t x) const {
-        Tile t;
+    // Sequence s of the batch, and its tile that holds place x of the line.
+    __device__ void sequence(const PagedView& p, int s, Tile& t) const {
         t.seq = s;
         t.row0 = p.row_start[s];
         t.n = p.row_start[s + 1] - t.row0;
         t.base = p.kv_len[s] - t.n;
+        t.cum = cum[s];
+        t.uniform();
+    }
+    __device__ void find(int64_t x, Tile& t) const {
         const int tiles = (t.n + TT - 1) / TT;
         const int64_t hk = head_places(t.base, t.n, tiles);
-        int64_t off = x - cum[s];
-        t.head = (int)(off / hk);
-        off -= (int64_t)t.head * hk;
+        int64_t off = x - t.cum;
+        // (the quotient in f64, within one of the whole one)
+        int head = (int)((double)off / (double)hk);
+        if ((int64_t)head * hk > off) --head;
+        if ((int64_t)(head + 1) * hk <= off) ++head;
+        off -= (int64_t)head * hk;
         int lo = 0, hi = tiles - 1;       // the last tile that starts at or before off
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -256,10 +276,10 @@ struct Line {
             else
                 hi = mid - 1;
         }
+        t.head = head;
         t.r = lo;
-        t.start = cum[s] + (int64_t)t.head * hk + before(t.base, lo);
+        t.start = t.cum + (int64_t)head * hk + before(t.base, lo);
         t.end = t.start + kTileKeys + (t.base - org) + min(t.n, (lo + 1) * TT);
-        return t;
     }
     // Cut x inside tile t, moved down: to the tile's start or to a place of a key.
     __device__ int64_t rounded(const Tile& t, int64_t x) const {
@@ -270,7 +290,7 @@ struct Line {
     __device__ static int key(const Tile& t, int64_t x) { return (int)max((int64_t)0, x - t.start - kTileKeys); }
 };
 
-// Fills cum (and line): the whole workgroup of 256.  tmp: LDS, 4 values.
+// Fills cum and the line: the whole workgroup of 256.  tmp: LDS, 4 values.
 __device__ __forceinline__ void make_line(const PagedView& p, Line& ln, int64_t* tmp, int grid, bool flag) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     int64_t carry = 0;
@@ -303,7 +323,10 @@ __device__ __forceinline__ void make_line(const PagedView& p, Line& ln, int64_t*
     }
     if (tid == 0) ln.cum[p.num_seqs] = carry;
     ln.total = carry;
-    ln.wgs = (int)min((int64_t)grid, max((int64_t)1, carry / kFewKeys));
+    ln.wgs = (int)min((int64_t)grid, max((int64_t)1, carry / kCut));
+    ln.share = (int64_t)((double)carry / ln.wgs);       // (within one)
+    ln.share += ((ln.share + 1) * ln.wgs <= carry) - (ln.share * ln.wgs > carry);
+    ln.rest = (int)(carry - ln.share * ln.wgs);
     __syncthreads();
 }
 
@@ -423,11 +446,13 @@ struct Rows {
     __device__ __forceinline__ static int dim(int g, int j, int v) {
         return SPREAD ? VD * (4 * g + v) + j : 16 * j + 4 * g + v;
     }
-    // rows rho0 ..
-    __device__ __forceinline__ void load(const PagedAttnArgs& a, const Work& w, int rho0) {
+    __device__ __forceinline__ void lanes() {
         const int lane = thread_id() & 63;
         g = lane >> 4;
         c = lane & 15;
+    }
+    // rows rho0 ..
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, const Work& w, int rho0) {
         clear();
         see = w.last;
         most = -1;
@@ -678,19 +703,25 @@ struct Deep : Rows<HD, QP, 1, true> {
             }
         }
     }
-    __device__ __forceinline__ void run(const PagedView& p, const Work& w, int lo, int step, float unit) {
-        const Cache<HD, KP> kv(p, w);
-        const int hi = min(w.hi, min(this->most, w.last) + 1);
-        if (lo < hi) {
-            bool bad = false;
-            int pk = kv.page_of(lo + 8 * (c >> 2), bad), pv = kv.page_of(lo + 8 * g, bad);
-            int pk1 = 0, pv1 = 0;
-            if (lo + step < hi) {
+    // (the first block's rows are on their way before the queries are read and split)
+    __device__ __forceinline__ void run(const PagedAttnArgs& a, const Work& w, int lo, int step, float unit) {
+        const Cache<HD, KP> kv(a.p, w);
+        this->lanes();
+        bool bad = false;
+        int pk1 = 0, pv1 = 0;
+        if (lo < w.hi) {
+            const int pk = kv.page_of(lo + 8 * (c >> 2), bad), pv = kv.page_of(lo + 8 * g, bad);
+            if (lo + step < w.hi) {
                 pk1 = kv.page_of(lo + step + 8 * (c >> 2), bad);
                 pv1 = kv.page_of(lo + step + 8 * g, bad);
             }
             load_k(kv, lo, pk);
             load_v(kv, lo, pv);
+        }
+        this->load(a, w, 0);
+        const int hi = min(w.hi, min(this->most, w.last) + 1);
+        if (lo < hi) {
+            int pk, pv;
             for (int kb = lo; kb < hi; kb += step) {
                 const int nb = kb + step;
                 pk = pk1;
@@ -742,8 +773,8 @@ struct Deep : Rows<HD, QP, 1, true> {
                 }
                 if (nb < hi) load_v(kv, nb, pv);
             }
-            if (bad) flag_error(p.err, kErrPagedPage);
         }
+        if (bad) flag_error(a.p.err, kErrPagedPage);
         this->l[0] = quads_add(this->l[0]);
     }
 };
@@ -958,41 +989,48 @@ __device__ __forceinline__ void store4(const PagedAttnArgs& a, bool bf16, int64_
         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// Where a finished tile's rows go: divided by their sums to out, or as a partial (o
-// [HD] per row, m and l): row rho of a slot, or (token, head) of a piece.
+// Sixteen bytes to memory, past this XCD's L2 (sc1: for a workgroup on any XCD).
+__device__ __forceinline__ void store4_coh(float* p, const float (&x)[4]) {
+    const f32x4v v = {x[0], x[1], x[2], x[3]};
+    asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
+}
+// Eight times sixteen bytes from there, waited for.
+__device__ __forceinline__ void load8_coh(const float* const (&p)[8], f32x4v (&v)[8]) {
+    asm volatile(
+        "global_load_dwordx4 %0, %8, off sc1\n\tglobal_load_dwordx4 %1, %9, off sc1\n\t"
+        "global_load_dwordx4 %2, %10, off sc1\n\tglobal_load_dwordx4 %3, %11, off sc1\n\t"
+        "global_load_dwordx4 %4, %12, off sc1\n\tglobal_load_dwordx4 %5, %13, off sc1\n\t"
+        "global_load_dwordx4 %6, %14, off sc1\n\tglobal_load_dwordx4 %7, %15, off sc1\n\t"
+        "s_waitcnt vmcnt(0)"
+        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7])
+        : "memory");
+}
+
+// Where a finished tile's rows go: divided by their sums to out, or as they are, with
+// their maxima and sums, to a piece of the batch's rows (token, head) or, row by row, to
+// a workgroup's slot, which another workgroup reads.
+enum { kToOut, kToPiece, kToSlot };
 template <int HD>
 struct Sink {
-    bool out;
-    float *o, *ml;            // slot: o [R][HD], ml [R][2]; piece: o [rows][HD], ml [rows][2]
-    bool by_token;
+    int to;
+    float *o, *ml;            // [rows][HD], [rows][2]
 
-    template <int QP, int NT, bool SPREAD>
-    __device__ __forceinline__ void rows(const PagedAttnArgs& a, const Work& w, const Rows<HD, QP, NT, SPREAD>& r,
-                                         int rho0) const {
-        constexpr int VD = HD / 16;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int rho = rho0 + 16 * t + r.c;
-            int token, head;
-            if (!row_at(a, w, rho, token, head)) continue;
-            const int64_t row = by_token ? (int64_t)token * a.heads + head : rho;
-            const int64_t at = (int64_t)token * a.out_stride + (int64_t)head * HD;
-            const float f = out ? 1.0f / r.l[t] : 1.0f;
-            if (!out && r.g == 0) *reinterpret_cast<float2*>(ml + 2 * row) = make_float2(r.m[t], r.l[t]);
-#pragma unroll
-            for (int y = 0; y < (SPREAD ? 4 : VD); ++y)
-#pragma unroll
-                for (int z = 0; z < (SPREAD ? VD : 4); z += 4) {
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[i] = (SPREAD ? r.acc[t][SPREAD ? z + i : 0][y & 3] : r.acc[t][SPREAD ? 0 : y][i]) * f;
-                    const int d = SPREAD ? VD * (4 * r.g + y) + z : 16 * y + 4 * r.g;
-                    if (out)
-                        store4(a, QP == 1, at + d, x);
-                    else
-                        *reinterpret_cast<float4*>(o + row * HD + d) = make_float4(x[0], x[1], x[2], x[3]);
-                }
+    // dims d .. d + 3 of row rho
+    __device__ __forceinline__ void put(const PagedAttnArgs& a, bool bf16, int rho, int token, int head, int d,
+                                        float m, float l, float f, float x0, float x1, float x2, float x3) const {
+        if (to == kToOut) {
+            store4(a, bf16, (int64_t)token * a.out_stride + (int64_t)head * HD + d, {x0 * f, x1 * f, x2 * f, x3 * f});
+        } else if (to == kToPiece) {
+            const int64_t row = (int64_t)token * a.heads + head;
+            *reinterpret_cast<float4*>(o + row * HD + d) = make_float4(x0, x1, x2, x3);
+            if (d == 0) *reinterpret_cast<float2*>(ml + 2 * row) = make_float2(m, l);
+        } else {
+            store4_coh(o + rho * HD + d, {x0, x1, x2, x3});
+            if (d == 0) {
+                __hip_atomic_store(ml + 2 * rho, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(ml + 2 * rho + 1, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
         }
     }
 };
@@ -1012,45 +1050,57 @@ constexpr int wgs_per_cu(int hd, int kp) { return hd * kp <= 192 ? 2 : 1; }
 template <int HD, int KP>
 constexpr int wgs_per_cu() { return wgs_per_cu(HD, KP); }
 
-// bytes of LDS: a stage of Wide; two waves' results of Deep; the plain path's rows
+// bytes of LDS: the stages of Wide; the four waves' results of Deep (the plain path's
+// four rows are less)
 template <int HD, int KP>
 constexpr int work_lds() {
-    constexpr int kDeep = 2 * (16 * HD + 128) * 4, kPlain = 4 * HD * 4;
-    return std::max({Stage<HD, KP>::kBuffers * Stage<HD, KP>::kBytes, kDeep, kPlain});
+    return std::max(Stage<HD, KP>::kBuffers * Stage<HD, KP>::kBytes, (4 * 16 * HD + 128) * 4);
 }
 
 template <int HD, int QP, int KP>
 __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
                                          const Sink<HD>& sink) {
+    constexpr int kWave = 16 * HD, VD = HD / 16;
     const int tid = thread_id(), wave = tid >> 6, lane = tid & 63;
     Deep<HD, QP, KP> r;
-    r.load(a, w, 0);
-    r.run(a.p, w, w.lo + 32 * wave, 128, unit);
-    float* s = reinterpret_cast<float*>(s_buf);
+    r.run(a, w, w.lo + 32 * wave, 128, unit);
+    float* s = reinterpret_cast<float*>(s_buf);      // [4 waves][VD][64][4]
+    float* s_ml = s + 4 * kWave;                     // [2][4][16]
     if (r.odd()) r.template run_plain<KP>(a, w, 0, w.lo + 32 * wave, 128, unit, s + wave * HD);
-    constexpr int kWave = 16 * HD + 128, VD = HD / 16;
-#pragma unroll
-    for (int half = 2; half >= 1; half /= 2) {   // the upper waves hand theirs to the lower ones
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-            float* o = s + (wave - half) * kWave;
-            o[lane] = r.m[0];
-            o[64 + lane] = r.l[0];
-#pragma unroll
-            for (int j = 0; j < VD; ++j)
-                *reinterpret_cast<f32x4v*>(o + 128 + (j * 64 + lane) * 4) = r.acc[0][j];
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float* o = s + wave * kWave;
-            float f0, f1;
-            join(r.m[0], r.l[0], o[lane], o[64 + lane], unit, f0, f1);
-#pragma unroll
-            for (int j = 0; j < VD; ++j)
-                r.acc[0][j] = r.acc[0][j] * f0 + *reinterpret_cast<const f32x4v*>(o + 128 + (j * 64 + lane) * 4) * f1;
-        }
+    // the waves' results of a row joined, wave i of four taking a quarter of its dims
+    __syncthreads();
+    if (lane < 16) {
+        s_ml[16 * wave + lane] = r.m[0];
+        s_ml[64 + 16 * wave + lane] = r.l[0];
     }
-    if (wave == 0) sink.rows(a, w, r, 0);
+#pragma unroll
+    for (int j = 0; j < VD; ++j) *reinterpret_cast<f32x4v*>(s + wave * kWave + (j * 64 + lane) * 4) = r.acc[0][j];
+    __syncthreads();
+    int token, head;
+    const bool on = row_at(a, w, r.c, token, head);
+    float f[4], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = fmaxf(m, s_ml[16 * k + r.c]);
+    const float mc = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        f[k] = weight(s_ml[16 * k + r.c] - mc, unit);
+        l = fmaf(s_ml[64 + 16 * k + r.c], f[k], l);
+    }
+    if (!on) return;
+    // lane (g, c) of wave v: of row c the dims VD (4 g + v) .. + VD - 1
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int j0 = 0; j0 < VD; j0 += 4) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[i] = fmaf(s[k * kWave + ((j0 + i) * 64 + lane) * 4 + wave], f[k], x[i]);
+        }
+        sink.put(a, QP == 1, r.c, token, head, VD * (4 * r.g + wave) + j0, m, l, inv, x[0], x[1], x[2], x[3]);
+    }
 }
 
 template <int HD, int QP, int KP, int NT>
@@ -1059,11 +1109,22 @@ __device__ __forceinline__ void many_rows(const PagedAttnArgs& a, const Work& w,
     const int wave = thread_id() >> 6, rho0 = wave * 16 * NT;
     const bool rows = rho0 < w.tokens * a.share;
     Wide<HD, QP, KP, NT> r;
+    r.lanes();
     r.load(a, w, rho0);
     r.run(a.p, w, rows, unit, s_buf);
     if (!rows) return;
     if (r.odd()) r.template run_plain<KP>(a, w, rho0, w.lo, 32, unit, reinterpret_cast<float*>(s_buf) + wave * HD);
-    sink.rows(a, w, r, rho0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int rho = rho0 + 16 * t + r.c;
+        int token, head;
+        if (!row_at(a, w, rho, token, head)) continue;
+        const float f = 1.0f / r.l[t];
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j)
+            sink.put(a, QP == 1, rho, token, head, 16 * j + 4 * r.g, r.m[t], r.l[t], f, r.acc[t][j][0],
+                     r.acc[t][j][1], r.acc[t][j][2], r.acc[t][j][3]);
+    }
 }
 
 template <int HD, int QP, int KP>
@@ -1079,41 +1140,131 @@ __device__ __forceinline__ void compute(const PagedAttnArgs& a, const Work& w, f
 }
 
 // Partials: the workgroups' slots; then, with a prefix, its pieces and one more for
-// the rows' own positions, each [num_rows * heads][HD] and their (m, l).
+// the rows' own positions, each [num_rows * heads][HD], and their (m, l).
 template <int HD, int QP>
 __device__ __forceinline__ Sink<HD> slot_of(const PagedAttnArgs& a, int i) {
     float* o = a.part + i * slot_floats<HD, QP>();
-    return {false, o, o + (int64_t)tile_rows<HD, QP>() * HD, false};
+    return {kToSlot, o, o + (int64_t)tile_rows<HD, QP>() * HD};
 }
 template <int HD>
 __device__ __forceinline__ Sink<HD> piece_of(const PagedAttnArgs& a, int i) {
     const int64_t rows = (int64_t)a.p.num_rows * a.heads;
-    return {false, a.pre + i * rows * HD, a.pre + (a.splits + 1) * rows * HD + i * rows * 2, true};
+    return {kToPiece, a.pre + i * rows * HD, a.pre + (a.splits + 1) * rows * HD + i * rows * 2};
 }
 
-// The sequences' own positions: one workgroup per share of the line.
+// The pieces first .. last of tile w.r.t. the line, which workgroups first .. last have
+// written to their slots, joined in their order: a thread's values of the tile's rows
+// in registers.
+template <int HD, int QP>
+__device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w, int first, int last, float unit,
+                                          const Sink<HD>& sink) {
+    constexpr int NV = tile_rows<HD, QP>() * HD / 4 / 256;
+    const int rows = w.tokens * a.share, tid = thread_id();
+#pragma unroll 1
+    for (int k0 = 0; k0 < NV && 256 * k0 / (HD / 4) < rows; k0 += 8) {
+        f32x4v o[8];
+        float m[8], l[8];
+        for (int p = first; p <= last; ++p) {
+            const Sink<HD> slot = slot_of<HD, QP>(a, p == first ? 2 * p + 1 : 2 * p);
+            const float* at[8];
+            f32x4v y[8];
+            float z[8], u[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = tid + 256 * (k0 + k), rho = min(i / (HD / 4), rows - 1);
+                at[k] = slot.o + rho * HD + 4 * (i % (HD / 4));
+                z[k] = __hip_atomic_load(slot.ml + 2 * rho, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                u[k] = __hip_atomic_load(slot.ml + 2 * rho + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            load8_coh(at, y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (p == first) {
+                    o[k] = y[k];
+                    m[k] = z[k];
+                    l[k] = u[k];
+                } else {
+                    float f0, f1;
+                    join(m[k], l[k], z[k], u[k], unit, f0, f1);
+                    o[k] = o[k] * f0 + y[k] * f1;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = tid + 256 * (k0 + k), rho = i / (HD / 4);
+            int token, head;
+            if (rho < rows && row_at(a, w, rho, token, head))
+                sink.put(a, QP == 1, rho, token, head, 4 * (i % (HD / 4)), m[k], l[k], 1.0f / l[k], o[k][0], o[k][1],
+                         o[k][2], o[k][3]);
+        }
+    }
+}
+
+// The prefix, for all rows of the batch: workgroup = (tile of rows, kv head, piece of
+// the prefix).
+template <int HD, int QP, int KP>
+__device__ __forceinline__ void prefix_piece(const PagedAttnArgs& a, int id, float unit, uint8_t* s_buf) {
+    const PagedView& p = a.p;
+    const int TT = tile_rows<HD, QP>() / a.share, tiles = (p.num_rows + TT - 1) / TT;
+    const int head = id / tiles % p.kv_heads, piece = id / tiles / p.kv_heads;
+    if (piece >= a.splits) return;   // (the grid's rounding)
+    const int rows = min(p.row_start[p.num_seqs], p.num_rows), blocks = (p.prefix_len + 31) / 32;
+    Work w;
+    w.token0 = id % tiles * TT;
+    w.tokens = min(TT, rows - w.token0);
+    if (w.tokens <= 0) return;
+    w.pos0 = p.prefix_len - 1;
+    w.row_pos = 0;
+    w.head = head;
+    w.head0 = head * a.share;
+    w.lo = 32 * (int)((int64_t)blocks * piece / a.splits);
+    w.hi = min(p.prefix_len, 32 * (int)((int64_t)blocks * (piece + 1) / a.splits));
+    w.first = 0;
+    w.last = p.prefix_len - 1;
+    w.table = p.prefix_pages;
+    w.uniform();
+    compute<HD, QP, KP>(a, w, unit, s_buf, piece_of<HD>(a, piece));
+}
+
+// The first workgroups (as many as the prefix has pieces) take those; then one
+// workgroup per share of the line of the sequences' own positions.  A tile that several
+// workgroups have a share of is joined by the last of them to end: their partials are
+// stored past the L2s and complete before the workgroup is counted.
 template <int HD, int QP, int KP>
 __global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_attn_kernel(PagedAttnArgs a) {
     __shared__ int64_t s_cum[kPagedMaxSeqs + 1];
     __shared__ int64_t s_tmp[4];
+    __shared__ int s_last;
     __shared__ __attribute__((aligned(16))) uint8_t s_buf[work_lds<HD, KP>()];
     const PagedView& p = a.p;
     const float unit = a.scale * 1.44269504f;
+    const int id = (int)blockIdx.x - a.prefix_wgs;
+    if (id < 0) {
+        prefix_piece<HD, QP, KP>(a, (int)blockIdx.x, unit, s_buf);
+        return;
+    }
     Line ln;
     ln.cum = s_cum;
     ln.org = p.prefix_len & ~31;
     ln.TT = tile_rows<HD, QP>() / a.share;
     ln.kv_heads = p.kv_heads;
-    make_line(p, ln, s_tmp, a.grid, blockIdx.x == 0);
+    make_line(p, ln, s_tmp, a.grid, id == 0);
     if (ln.total == 0) return;
-    // neighbouring shares on one XCD (workgroup id mod 8)
-    const int per = (ln.wgs + 7) / 8, id = (int)blockIdx.x;
-    const int wg = (id & 7) * per + (id >> 3);
+    // neighbouring shares on one XCD (workgroup id mod 8; the prefix' are a multiple of 8)
+    const int per = (ln.wgs + 7) / 8, wg = (id & 7) * per + (id >> 3);
     if ((id >> 3) >= per || wg >= ln.wgs) return;
-    int64_t x = ln.cut(wg), x1 = ln.cut(wg + 1);
-    Tile t = ln.tile(p, find_seq(p, ln, x), x);
+    int64_t x1 = ln.cut(wg + 1);
+    Tile t;
+    if (x1 < ln.total) {
+        ln.sequence(p, find_seq(p, ln, x1), t);
+        ln.find(x1, t);
+        x1 = ln.rounded(t, x1);
+    }
+    int64_t x = ln.cut(wg);
+    if (x1 == ln.total || x < t.cum) ln.sequence(p, find_seq(p, ln, x), t);
+    ln.find(x, t);
     x = ln.rounded(t, x);
-    if (x1 < ln.total) x1 = ln.rounded(ln.tile(p, find_seq(p, ln, x1), x1), x1);
     while (x < x1) {
         const int64_t end = min(t.end, x1);
         Work w;
@@ -1129,173 +1280,80 @@ __global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_attn_kernel
         w.last = w.pos0 + w.tokens - 1;
         w.table = p.pages + (int64_t)t.seq * p.table_stride;
         w.uniform();
-        Sink<HD> sink = {true, nullptr, nullptr, false};
-        if (x > t.start || end < t.end)
-            sink = slot_of<HD, QP>(a, 2 * wg + (x > t.start ? 0 : 1));
-        else if (a.splits)
-            sink = piece_of<HD>(a, a.splits);
-        compute<HD, QP, KP>(a, w, unit, s_buf, sink);
-        __syncthreads();   // (s_buf is the next tile's)
+        const Sink<HD> done = a.splits ? piece_of<HD>(a, a.splits) : Sink<HD>{kToOut, nullptr, nullptr};
+        const bool whole = x == t.start && end == t.end;
+        compute<HD, QP, KP>(a, w, unit, s_buf, whole ? done : slot_of<HD, QP>(a, 2 * wg + (x > t.start ? 0 : 1)));
+        if (!whole) {
+            // the tile's workgroups: from the one whose cut is its start (or rounded to it)
+            // to the one with the last cut inside it
+            const int first = x == t.start ? wg : ln.below(t.start + kTileKeys + kCut);
+            const int last = end == t.end ? wg : ln.below(t.end);
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const uint32_t before = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED,
+                                                               __HIP_MEMORY_SCOPE_AGENT);
+                s_last = before == (uint32_t)(last - first);
+                if (s_last)
+                    __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (s_last) join_tile<HD, QP>(a, w, first, last, unit, done);
+        }
+        __syncthreads();   // (s_buf and s_last are the next tile's)
         x = end;
-        if (x < x1) t = ln.tile(p, find_seq(p, ln, x), x);
-    }
-}
-
-// The tiles that several workgroups shared: workgroup w joins the tile that cut w is
-// the first inside of.
-template <int HD, int QP>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
-    __shared__ int64_t s_cum[kPagedMaxSeqs + 1];
-    __shared__ int64_t s_tmp[4];
-    const PagedView& p = a.p;
-    const float unit = a.scale * 1.44269504f;
-    Line ln;
-    ln.cum = s_cum;
-    ln.org = p.prefix_len & ~31;
-    ln.TT = tile_rows<HD, QP>() / a.share;
-    ln.kv_heads = p.kv_heads;
-    make_line(p, ln, s_tmp, a.grid, false);
-    const int wg = (int)blockIdx.x + 1;
-    if (wg >= ln.wgs) return;
-    const int64_t x = ln.cut(wg);
-    const Tile t = ln.tile(p, find_seq(p, ln, x), x);
-    if (ln.rounded(t, x) == t.start) return;                            // not cut here
-    const int64_t prev = ln.cut(wg - 1);
-    if (prev >= t.start && ln.rounded(t, prev) > t.start) return;       // nor first here
-    // (segment by segment, a thread's values of the tile's rows in registers)
-    constexpr int R = tile_rows<HD, QP>(), NV = R * HD / 4 / 256;
-    const int rows = min(ln.TT, t.n - t.r * ln.TT) * a.share, tid = threadIdx.x;
-    float4 o[NV];
-    float m[NV], l[NV];
-    auto segment = [&](const Sink<HD>& slot, bool first) {
-#pragma unroll
-        for (int k0 = 0; k0 < NV; k0 += 8) {
-            float4 y[8];
-            float2 z[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int i = tid + 256 * (k0 + k), rho = min(i / (HD / 4), rows - 1);
-                y[k] = *reinterpret_cast<const float4*>(slot.o + rho * HD + 4 * (i % (HD / 4)));
-                z[k] = *reinterpret_cast<const float2*>(slot.ml + 2 * rho);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                float4& q = o[k0 + k];
-                if (first) {
-                    q = y[k];
-                    m[k0 + k] = z[k].x;
-                    l[k0 + k] = z[k].y;
-                } else {
-                    float f0, f1;
-                    join(m[k0 + k], l[k0 + k], z[k].x, z[k].y, unit, f0, f1);
-                    q = make_float4(q.x * f0 + y[k].x * f1, q.y * f0 + y[k].y * f1, q.z * f0 + y[k].z * f1,
-                                    q.w * f0 + y[k].w * f1);
-                }
-            }
-            if (256 * (k0 + 8) / (HD / 4) >= rows) break;
-        }
-    };
-    segment(slot_of<HD, QP>(a, 2 * (wg - 1) + 1), true);
-    int64_t at = ln.rounded(t, x);
-    for (int w = wg; at < t.end; ++w) {
-        int64_t next = ln.cut(w + 1);
-        next = next >= t.end ? t.end : ln.rounded(t, next);
-        if (next > at) segment(slot_of<HD, QP>(a, 2 * w), false);
-        at = next;
-    }
-    const Sink<HD> own = piece_of<HD>(a, a.splits);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int i = tid + 256 * k, rho = i / (HD / 4), d = 4 * (i % (HD / 4));
-        if (rho >= rows) break;
-        const int token = t.row0 + t.r * ln.TT + rho / a.share, head = t.head * a.share + rho % a.share;
-        if (a.splits) {
-            const int64_t row = (int64_t)token * a.heads + head;
-            *reinterpret_cast<float4*>(own.o + row * HD + d) = o[k];
-            if (d == 0) *reinterpret_cast<float2*>(own.ml + 2 * row) = make_float2(m[k], l[k]);
-        } else {
-            const float f = 1.0f / l[k];
-            store4(a, QP == 1, (int64_t)token * a.out_stride + (int64_t)head * HD + d,
-                   {o[k].x * f, o[k].y * f, o[k].z * f, o[k].w * f});
+        if (x < x1) {
+            if (x >= s_cum[t.seq + 1]) ln.sequence(p, find_seq(p, ln, x), t);
+            ln.find(x, t);
         }
     }
 }
 
-// The prefix, for all rows of the batch: workgroup = (tile of rows, kv head, piece of
-// the prefix).
-template <int HD, int QP, int KP>
-__global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_prefix_kernel(PagedAttnArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t s_buf[work_lds<HD, KP>()];
-    const PagedView& p = a.p;
-    const float unit = a.scale * 1.44269504f;
-    const int TT = tile_rows<HD, QP>() / a.share, head = (int)blockIdx.y % p.kv_heads;
-    const int piece = (int)blockIdx.y / p.kv_heads;
-    const int rows = min(p.row_start[p.num_seqs], p.num_rows), blocks = (p.prefix_len + 31) / 32;
-    Work w;
-    w.token0 = (int)blockIdx.x * TT;
-    w.tokens = min(TT, rows - w.token0);
-    if (w.tokens <= 0) return;
-    w.pos0 = p.prefix_len - 1;
-    w.row_pos = 0;
-    w.head = head;
-    w.head0 = head * a.share;
-    w.lo = 32 * (int)((int64_t)blocks * piece / a.splits);
-    w.hi = min(p.prefix_len, 32 * (int)((int64_t)blocks * (piece + 1) / a.splits));
-    w.first = 0;
-    w.last = p.prefix_len - 1;
-    w.table = p.prefix_pages;
-    if (piece == 0) {   // the rows' own part is not there yet (nor ever, where the sequence is skipped)
-        const Sink<HD> own = piece_of<HD>(a, a.splits);
-        for (int i = threadIdx.x; i < w.tokens * a.share; i += 256)
-            own.ml[2 * ((int64_t)(w.token0 + i / a.share) * a.heads + w.head0 + i % a.share) + 1] = -1.f;
-    }
-    compute<HD, QP, KP>(a, w, unit, s_buf, piece_of<HD>(a, piece));
-}
-
-// A row's pieces of the prefix and its own part: out.
+// A row's pieces of the prefix and its own part: out.  Workgroup = (token, some heads).
 template <int HD, int QP>
 __global__ __launch_bounds__(256) void paged_pieces_kernel(PagedAttnArgs a) {
+    __shared__ int s_in;
+    const PagedView& p = a.p;
     const float unit = a.scale * 1.44269504f;
-    const int64_t rows = (int64_t)a.p.num_rows * a.heads;
-    const int64_t row = (int64_t)blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4);
-    const int d = 4 * (threadIdx.x % (HD / 4)), token = (int)(row / a.heads), head = (int)(row % a.heads);
-    if (row >= rows || token >= a.p.row_start[a.p.num_seqs]) return;
+    const int token = (int)blockIdx.x, tid = threadIdx.x;
+    const int head = (int)blockIdx.y * (1024 / HD) + tid / (HD / 4), d = 4 * (tid % (HD / 4));
+    const int64_t rows = (int64_t)p.num_rows * a.heads, row = (int64_t)token * a.heads + min(head, a.heads - 1);
     const Sink<HD> all = piece_of<HD>(a, 0);
-    const float2 own = *reinterpret_cast<const float2*>(all.ml + 2 * (a.splits * rows + row));
-    if (own.y < 0.f) return;   // (a skipped sequence's)
-    float m = own.x;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, all.ml[2 * (s * rows + row)]);
+    // (a row of a sequence that was computed)
+    if (tid == 0) s_in = 0;
+    __syncthreads();
+    for (int s = tid; s < p.num_seqs; s += 256) {
+        const int lo = p.row_start[s], hi = p.row_start[s + 1];
+        if (token >= lo && token < hi && seq_ok(p, lo, hi, p.kv_len[s])) s_in = 1;
+    }
+    float m = -INFINITY;
+    for (int s = 0; s <= a.splits; ++s) m = fmaxf(m, all.ml[2 * (s * rows + row)]);
+    const float mc = m == -INFINITY ? 0.f : m;
     float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
     for (int s = 0; s <= a.splits; ++s) {
         const float2 z = *reinterpret_cast<const float2*>(all.ml + 2 * (s * rows + row));
         const float4 y = *reinterpret_cast<const float4*>(all.o + (s * rows + row) * HD + d);
-        const float f = z.x == -INFINITY ? 0.f : weight(z.x - m, unit);
+        const float f = weight(z.x - mc, unit);
         l = fmaf(z.y, f, l);
         o[0] = fmaf(y.x, f, o[0]);
         o[1] = fmaf(y.y, f, o[1]);
         o[2] = fmaf(y.z, f, o[2]);
         o[3] = fmaf(y.w, f, o[3]);
     }
+    __syncthreads();
+    if (!s_in || head >= a.heads) return;
     const float f = 1.0f / l;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) o[k] *= f;
-    store4(a, QP == 1, (int64_t)token * a.out_stride + (int64_t)head * HD + d, o);
+    store4(a, QP == 1, (int64_t)token * a.out_stride + (int64_t)head * HD + d,
+           {o[0] * f, o[1] * f, o[2] * f, o[3] * f});
 }
 
 template <int HD, int QP, int KP>
 void launch_attn(const PagedAttnArgs& a, hipStream_t st) {
-    if (a.splits) {
-        const int TT = tile_rows<HD, QP>() / a.share;
-        hipLaunchKernelGGL((paged_prefix_kernel<HD, QP, KP>),
-                           dim3((unsigned)((a.p.num_rows + TT - 1) / TT), (unsigned)(a.p.kv_heads * a.splits)),
-                           dim3(256), 0, st, a);
-    }
-    hipLaunchKernelGGL((paged_attn_kernel<HD, QP, KP>), dim3((unsigned)a.grid), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((paged_join_kernel<HD, QP>), dim3((unsigned)a.grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<HD, QP, KP>), dim3((unsigned)(a.prefix_wgs + a.grid)), dim3(256), 0, st, a);
     if (a.splits)
         hipLaunchKernelGGL((paged_pieces_kernel<HD, QP>),
-                           dim3((unsigned)(((int64_t)a.p.num_rows * a.heads + 1024 / HD - 1) / (1024 / HD))),
+                           dim3((unsigned)a.p.num_rows, (unsigned)((a.heads + 1024 / HD - 1) / (1024 / HD))),
                            dim3(256), 0, st, a);
 }
 
@@ -1323,13 +1381,14 @@ int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats) {
     const int R = a.head_dim <= 128 && a.x_bf16 ? 128 : 64;   // tile_rows
     const int per = wgs_per_cu(a.head_dim, a.cache_bf16 ? 1 : 3);
     a.grid = (per * cus + 7) / 8 * 8;
-    a.splits = 0;
+    a.splits = a.prefix_wgs = 0;
     *own_floats = (int64_t)a.grid * 2 * R * (a.head_dim + 2);
     if (a.p.prefix_len == 0) return *own_floats;
+    // about one workgroup per CU takes the prefix, pieces of at least 64 keys
     const int TT = R / a.share, tiles = (a.p.num_rows + TT - 1) / TT;
     const int64_t wgs = (int64_t)tiles * a.p.kv_heads;
-    const int64_t most = std::max(1, a.p.prefix_len / 256);
-    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (per * cus + wgs - 1) / wgs, 32}));
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({a.p.prefix_len / 64, (cus + wgs - 1) / wgs, 32}));
+    a.prefix_wgs = (int)((wgs * a.splits + 7) / 8 * 8);
     return *own_floats + (int64_t)(a.splits + 1) * a.p.num_rows * a.heads * (a.head_dim + 2);
 }
 

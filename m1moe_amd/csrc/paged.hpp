@@ -41,8 +41,10 @@ struct PagedAttnArgs {
     float scale;
     int32_t grid;        // workgroups the sequences' own positions are shared by
     int32_t splits;      // pieces of the prefix, 0 without one
-    float* part;         // partials: the workgroups' (paged_attention_floats)
-    float* pre;          // and the prefix' [splits][num_rows * heads][head_dim + 2]
+    int32_t prefix_wgs;  // and the workgroups that take them
+    float* part;         // partials: the workgroups' slots
+    float* pre;          // and the prefix' pieces, [splits + 1][num_rows * heads][head_dim + 2]
+    uint32_t* counters;  // [grid], zero between launches
 };
 
 struct SampleArgs {
@@ -61,7 +63,7 @@ struct SampleArgs {
 };
 
 int launch_kv_append(const AppendArgs& a, int cus, void* stream);
-// Sets grid and splits; the floats of partials (own, then the prefix') needed.
+// Sets grid, splits and prefix_wgs; the floats of partials (slots, then pieces) needed.
 int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats);
 int launch_paged_attention(const PagedAttnArgs& a, void* stream);
 int sample_parts(int rows, int vocab, int cus);

@@ -97,8 +97,15 @@ PagedView view(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m1moe_paged_batc
 // At least `floats` of paged attention partials.
 int32_t ensure_paged_scratch(m1moe_ctx_t ctx, uint64_t floats) {
     ctx->capture_uses_scratch = true;
-    if (floats <= ctx->paged_part_floats) return M1MOE_OK;
+    if (ctx->paged_cnt && floats <= ctx->paged_part_floats) return M1MOE_OK;
     if (int32_t rc = refuse_growth_in_capture(ctx->stream, "the paged attention scratch")) return rc;
+    if (!ctx->paged_cnt) {
+        const uint64_t bytes = 4 * (2 * (uint64_t)ctx->cus + 8);   // the largest grid
+        int32_t rc = device_alloc((void**)&ctx->paged_cnt, bytes, "paged attention counters");
+        if (rc) return rc;
+        HIP_TRY(hipMemsetAsync(ctx->paged_cnt, 0, bytes, ctx->stream));
+        if (floats <= ctx->paged_part_floats) return M1MOE_OK;
+    }
     HIP_TRY(hipStreamSynchronize(ctx->stream));
     if (ctx->paged_part) ++ctx->scratch_gen;  // earlier graphs hold the old buffer
     if (ctx->paged_part) HIP_TRY(hipFree(ctx->paged_part));
@@ -219,6 +226,7 @@ int32_t m1moe_paged_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m
     if ((rc = ensure_paged_scratch(ctx, (uint64_t)floats))) return rc;
     a.part = ctx->paged_part;
     a.pre = ctx->paged_part + own;
+    a.counters = ctx->paged_cnt;
     return launched(launch_paged_attention(a, ctx->stream), "paged_attention");
 }
 
