@@ -179,6 +179,22 @@ __device__ __forceinline__ Parts8 parts8(const float (&v)[8]) {
     return s;
 }
 
+// The same of four.
+__device__ __forceinline__ void parts4(f32x4v v, uint2& h, uint2& m, uint2& l) {
+    uint32_t a[2], b[2], c[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float x0 = v[2 * i], x1 = v[2 * i + 1];
+        a[i] = pack_bf16(x0, x1);
+        const float r0 = x0 - __uint_as_float(a[i] << 16), r1 = x1 - __uint_as_float(a[i] & 0xFFFF0000u);
+        b[i] = pack_bf16(r0, r1);
+        c[i] = pack_bf16(r0 - __uint_as_float(b[i] << 16), r1 - __uint_as_float(b[i] & 0xFFFF0000u));
+    }
+    h = make_uint2(a[0], a[1]);
+    m = make_uint2(b[0], b[1]);
+    l = make_uint2(c[0], c[1]);
+}
+
 __device__ __forceinline__ f32x4v mfma(bf16x8 a, bf16x8 b, f32x4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -394,19 +410,25 @@ struct Cache {
         table = w.table;
     }
     __device__ __forceinline__ int clamp(int pos) const { return min(max(pos, first), last); }
-    // The page of the aligned eight positions from pos on: of the readable one among
-    // them, or of the nearest (page 0 for one outside the cache).
-    __device__ __forceinline__ int page_of(int pos, bool& bad) const {
-        const int x = table[clamp(pos) >> shift];
+    // Whether some of the n positions from kb on are not readable.  Their rows are read
+    // all the same, from the slots they would have in a page that is looked up for them:
+    // K's scores are passed over, V's rows are taken as 0.
+    __device__ __forceinline__ bool edge(int kb, int n) const { return kb < first || kb + n - 1 > last; }
+    __device__ __forceinline__ bool readable(int pos) const { return pos >= first && pos <= last; }
+    // The page number of the aligned eight positions from pos on: of the readable one
+    // among them, or of the nearest.  As the table has it: it is checked (known) where
+    // it is used, as a test here would wait for it and for every load before it.
+    __device__ __forceinline__ int page_of(int pos) const { return table[clamp(pos) >> shift]; }
+    // Page 0 for one outside the cache.
+    __device__ __forceinline__ int known(int x, bool& bad) const {
         const bool out = (unsigned)x >= (unsigned)pages;
         bad |= out;
         return out ? 0 : x;
     }
-    // Byte offset of a readable position of page x.
+    // Byte offset of position pos in page x.
     __device__ __forceinline__ int64_t at(int x, int pos) const {
-        return (int64_t)x * page + ((uint32_t)pos & mask) * row;
+        return (int64_t)((uint64_t)(uint32_t)x * page + ((uint32_t)pos & mask) * row);
     }
-    __device__ __forceinline__ bool edge(int kb, int n) const { return kb < first || kb + n - 1 > last; }
 };
 
 // The (token, query head) of row rho of the work; false past its rows.
@@ -609,7 +631,7 @@ struct Rows {
             }
             for (int kb = lo; kb <= top; kb += step)
                 for (int k = max(kb, w.first); k <= min(kb + 31, top); ++k) {
-                    const int64_t at = kv.at(kv.page_of(k, bad), k) + PL * lane * kv.ES;
+                    const int64_t at = kv.at(kv.known(kv.page_of(k), bad), k) + PL * lane * kv.ES;
                     float s = 0.f, v[PL];
 #pragma unroll
                     for (int i = 0; i < PL; ++i) {
@@ -663,14 +685,10 @@ struct Deep : Rows<HD, QP, 1, true> {
     float vf[KP == 3 ? 8 : 1][KP == 3 ? VD : 1];
 
     __device__ __forceinline__ void load_k(const Cache<HD, KP>& kv, int kb, int page) {
-        int p0 = kb + 8 * (c >> 2) + (c & 3), p1 = p0 + 4;
-        if (kv.edge(kb, 32)) {
-            p0 = kv.clamp(p0);
-            p1 = kv.clamp(p1);
-        }
+        const uint8_t* y = kv.k + kv.at(page, kb + 8 * (c >> 2) + (c & 3)) + 8 * kv.ES * g;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const uint4* x = reinterpret_cast<const uint4*>(kv.k + kv.at(page, u ? p1 : p0) + 8 * kv.ES * g);
+            const uint4* x = reinterpret_cast<const uint4*>(y + 4 * u * kv.row);
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 kw[u][KP == 1 ? i : 2 * i] = x[KP == 1 ? 4 * i : 8 * i];
@@ -679,27 +697,33 @@ struct Deep : Rows<HD, QP, 1, true> {
         }
     }
     __device__ __forceinline__ void load_v(const Cache<HD, KP>& kv, int kb, int page) {
-        const uint8_t* x[8];
-        const int p0 = kb + 8 * g;
-        if (kv.edge(kb, 32)) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = kv.v + kv.at(page, kv.clamp(p0 + e)) + VD * kv.ES * c;
-        } else {
-            x[0] = kv.v + kv.at(page, p0) + VD * kv.ES * c;
-#pragma unroll
-            for (int e = 1; e < 8; ++e) x[e] = x[e - 1] + kv.row;
-        }
+        const uint8_t* x = kv.v + kv.at(page, kb + 8 * g) + VD * kv.ES * c;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if constexpr (KP == 1) {
-                vw[e] = *reinterpret_cast<const words*>(x[e]);
+                vw[e] = *reinterpret_cast<const words*>(x);
             } else {
 #pragma unroll
                 for (int i = 0; i < VD; i += 4) {
-                    const f32x4v y = *reinterpret_cast<const f32x4v*>(x[e] + 4 * i);
+                    const f32x4v y = *reinterpret_cast<const f32x4v*>(x + 4 * i);
 #pragma unroll
                     for (int z = 0; z < 4; ++z) vf[e][i + z] = y[z];
                 }
+            }
+            x += kv.row;
+        }
+    }
+    // V's rows that are not readable: 0
+    __device__ __forceinline__ void clear_v(const Cache<HD, KP>& kv, int kb) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool in = kv.readable(kb + 8 * g + e);
+            if constexpr (KP == 1) {
+#pragma unroll
+                for (int i = 0; i < VD / 2; ++i) vw[e][i] = in ? vw[e][i] : 0u;
+            } else {
+#pragma unroll
+                for (int i = 0; i < VD; ++i) vf[e][i] = in ? vf[e][i] : 0.f;
             }
         }
     }
@@ -710,13 +734,13 @@ struct Deep : Rows<HD, QP, 1, true> {
         bool bad = false;
         int pk1 = 0, pv1 = 0;
         if (lo < w.hi) {
-            const int pk = kv.page_of(lo + 8 * (c >> 2), bad), pv = kv.page_of(lo + 8 * g, bad);
+            const int pk = kv.page_of(lo + 8 * (c >> 2)), pv = kv.page_of(lo + 8 * g);
             if (lo + step < w.hi) {
-                pk1 = kv.page_of(lo + step + 8 * (c >> 2), bad);
-                pv1 = kv.page_of(lo + step + 8 * g, bad);
+                pk1 = kv.page_of(lo + step + 8 * (c >> 2));
+                pv1 = kv.page_of(lo + step + 8 * g);
             }
-            load_k(kv, lo, pk);
-            load_v(kv, lo, pv);
+            load_k(kv, lo, kv.known(pk, bad));
+            load_v(kv, lo, kv.known(pv, bad));
         }
         this->load(a, w, 0);
         const int hi = min(w.hi, min(this->most, w.last) + 1);
@@ -727,8 +751,8 @@ struct Deep : Rows<HD, QP, 1, true> {
                 pk = pk1;
                 pv = pv1;
                 if (nb + step < hi) {
-                    pk1 = kv.page_of(nb + step + 8 * (c >> 2), bad);
-                    pv1 = kv.page_of(nb + step + 8 * g, bad);
+                    pk1 = kv.page_of(nb + step + 8 * (c >> 2));
+                    pv1 = kv.page_of(nb + step + 8 * g);
                 }
                 f32x4v s[1][1][2];
                 s[0][0][0] = s[0][0][1] = f32x4v{0.f, 0.f, 0.f, 0.f};
@@ -748,10 +772,11 @@ struct Deep : Rows<HD, QP, 1, true> {
                             R::products(x, qop, 0, i, s[0][0][u]);
                         }
                     }
-                if (nb < hi) load_k(kv, nb, pk);
+                if (nb < hi) load_k(kv, nb, kv.known(pk, bad));
                 bf16x8 pp[1][1][QP];
                 this->template softmax<1>(w, kb, s, unit, pp);
                 const auto pop = [&](int t, int b, int) { return pp[0][t][b]; };
+                if (kv.edge(kb, 32)) clear_v(kv, kb);
 #pragma unroll
                 for (int j = 0; j < VD; ++j) {
                     if constexpr (KP == 1) {
@@ -771,7 +796,7 @@ struct Deep : Rows<HD, QP, 1, true> {
                         R::products(x, pop, 0, 0, acc[0][j]);
                     }
                 }
-                if (nb < hi) load_v(kv, nb, pv);
+                if (nb < hi) load_v(kv, nb, kv.known(pv, bad));
             }
         }
         if (bad) flag_error(a.p.err, kErrPagedPage);
@@ -782,9 +807,12 @@ struct Deep : Rows<HD, QP, 1, true> {
 // Many rows: the waves hold 16 NT rows each and share the keys, staged through LDS
 // in pieces of SK: K row by row (its bf16 parts), V transposed, eight keys of a
 // dim together, both in 16-byte units placed so that the eight lanes an LDS read
-// serves at once find theirs in different banks.  Waves 0 and 1 stage K, 2 and 3 V.
-// The next piece is on its way into registers while one is computed, the page
-// numbers of the one after with it (lane l: of the piece's keys 8 (l % 16) ..).
+// serves at once find theirs in different banks.  Each thread has 16 bytes of K at a
+// time (a position's neighbouring dims) and 64 of V (VB dims of eight positions).
+// The next piece is on its way into registers while one is computed, the page numbers
+// of the one after with it (lane l: of the piece's keys 8 (l % 16) ..).  The eight
+// positions that share a page number are the same for a whole wave, of K at every
+// load, so that a load's address is one scalar base and a lane's constant offset.
 template <int HD, int KP>
 struct Stage {
     static constexpr int SK = KP == 1 ? 8192 / HD : HD <= 128 ? 4096 / HD : 32;   // keys
@@ -793,58 +821,88 @@ struct Stage {
     static constexpr int kBytes = 2 * KP * kPlane;
     static constexpr int kBuffers = KP == 1 ? 2 : 1;
     static constexpr int ES = KP == 1 ? 2 : 4;
-    static constexpr int VB = KP == 1 ? 8 : 4;            // dims of a thread's V block (16 bytes)
-    static constexpr int N = SK * HD * ES / 2048 / 8;     // K rows' or V blocks' eights of loads
-    static_assert(SK % 32 == 0 && N >= 1 && SK <= 128, "a piece is whole 32-key blocks");
-    uint4 r[N][8];
+    static constexpr int VB = KP == 1 ? 4 : HD * SK / 2048;     // dims of a thread's V block: 4 or 2
+    static constexpr int NV = SK * HD / 8 / VB / 256;           // blocks of a thread
+    static constexpr int CU = HD * ES / 16;                     // 16-byte units of a position in the cache
+    static constexpr int NK = SK * CU / 256;                    // loads of K
+    static_assert(SK % 32 == 0 && SK <= 128 && NV >= 1 && NK >= 1, "a piece is whole 32-key blocks");
+    static constexpr int VW = VB * ES / 4;                      // words of a position's in it
+    typedef uint32_t vblock __attribute__((ext_vector_type(VW)));
+    f32x4v kr[NK];
+    uint32_t vr[NV][8][VW];
     int pages;                                            // lane l: of group l % 16
+    // the thread, its wave, its offsets in a position of K and of V
+    int t, wave;
+    uint32_t k_off, v_off;
 
     __device__ __forceinline__ static int k_at(int key, int unit) {
         const int z = (key & 3) | ((key >> 3) & 3) << 2;
         return (key * KU + (unit ^ (z & (KU - 1)))) * 16;
     }
     __device__ __forceinline__ static int v_at(int d, int unit) {
-        const int z = VU >= 8 ? d ^ (d >> 3) : (d >> 1) ^ (d >> 3);
+        const int z = VU >= 8 ? d ^ (d >> 2) : (d >> 1) ^ (d >> 3);
         return (d * VU + (unit ^ (z & (VU - 1)))) * 16;
     }
-    __device__ __forceinline__ void look(const Cache<HD, KP>& kv, int kb, bool& bad) {
-        pages = kv.page_of(kb + 8 * (thread_id() & 15) % SK, bad);
+    static constexpr int KS = 256 / CU;                   // positions of K the threads load at once
+    __device__ __forceinline__ void init(const Cache<HD, KP>& kv) {
+        t = thread_id();
+        wave = __builtin_amdgcn_readfirstlane(t >> 6);
+        k_off = (uint32_t)(t / CU - 64 * wave / CU) * kv.row + 16 * (t % CU);
+        v_off = (uint32_t)(ES * VB * (t % (HD / VB)));
+    }
+    __device__ __forceinline__ void look(const Cache<HD, KP>& kv, int kb) {
+        pages = kv.page_of(kb + 8 * (t & 15) % SK);
+    }
+    __device__ __forceinline__ static int64_t lane64(int64_t x, int lane) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
+    }
+    __device__ __forceinline__ static void get(uint32_t (&to)[VW], const uint8_t* x) {
+        const vblock v = *reinterpret_cast<const vblock*>(x);
+#pragma unroll
+        for (int i = 0; i < VW; ++i) to[i] = v[i];
     }
     // The piece at kb, by its pages.
-    __device__ __forceinline__ void load(const Cache<HD, KP>& kv, int kb) {
-        const int t = thread_id() & 127;
-        const bool edge = kv.edge(kb, SK);
-        if (threadIdx.x < 128) {   // eight dims (f32: in two loads) of a position
-            constexpr int UL = KP == 1 ? 1 : 2;
+    __device__ __forceinline__ void load(const Cache<HD, KP>& kv, int kb, bool& bad) {
+        // (lane l: where the group l % 16 of eight positions begins)
+        const int64_t at = kv.at(kv.known(pages, bad), kb + 8 * (t & 15) % SK);
+        const int key0 = 64 * wave / CU;   // the wave's first position of K
 #pragma unroll
-            for (int n = 0; n < N * 8 / UL; ++n) {
-                const int b = t + 128 * n, key = b / KU, unit = b % KU;
-                const int page = __shfl(pages, key >> 3);
-                const int pos = edge ? kv.clamp(kb + key) : kb + key;
-                const uint4* x = reinterpret_cast<const uint4*>(kv.k + kv.at(page, pos) + 8 * ES * unit);
+        for (int n = 0; n < NK; ++n) {
+            const int key = key0 + n * KS;
+            kr[n] = *reinterpret_cast<const f32x4v*>(kv.k + (lane64(at, key >> 3) + (uint32_t)(key & 7) * kv.row) + k_off);
+        }
+        constexpr int kGroups = 64 * VB / HD > 1 ? 64 * VB / HD : 1;   // a wave's V blocks lie in so many
 #pragma unroll
-                for (int i = 0; i < UL; ++i) r[(UL * n + i) / 8][(UL * n + i) % 8] = x[i];
+        for (int n = 0; n < NV; ++n) {
+            const int grp = (64 * wave + 256 * n) / (HD / VB);
+            int64_t base = lane64(at, grp);
+            if (kGroups == 2) {
+                const int64_t other = lane64(at, grp + 1);
+                base = (t & 63) >= HD / VB ? other : base;
+            } else if (kGroups > 2) {
+                const int mine = (t + 256 * n) / (HD / VB);
+                base = (int64_t)((uint64_t)(uint32_t)__shfl((int)(at >> 32), mine) << 32 |
+                                 (uint32_t)__shfl((int)at, mine));
             }
-        } else {                   // VB dims of eight positions
+            const uint8_t* x = kv.v + base + v_off;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int b = t + 128 * n, grp = b / (HD / VB), d = VB * (b % (HD / VB));
-                const int page = __shfl(pages, grp);
-                const uint8_t* x = kv.v + ES * d;
-                if (edge) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        r[n][e] = *reinterpret_cast<const uint4*>(x + kv.at(page, kv.clamp(kb + 8 * grp + e)));
-                } else {
-                    x += kv.at(page, kb + 8 * grp);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        r[n][e] = *reinterpret_cast<const uint4*>(x);
-                        x += kv.row;
-                    }
-                }
+            for (int e = 0; e < 8; ++e) {
+                get(vr[n][e], x);
+                x += kv.row;
             }
         }
+    }
+    // V's rows of the piece at kb that are not readable: 0
+    __device__ __forceinline__ void clear_v(const Cache<HD, KP>& kv, int kb) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool in = kv.readable(kb + (t + 256 * n) / (HD / VB) * 8 + e);
+#pragma unroll
+                for (int i = 0; i < VW; ++i) vr[n][e][i] = in ? vr[n][e][i] : 0u;
+            }
     }
     __device__ __forceinline__ static void put(uint8_t* s, const Parts8& p) {
         *reinterpret_cast<bf16x8*>(s) = p.h;
@@ -852,44 +910,39 @@ struct Stage {
         *reinterpret_cast<bf16x8*>(s + 2 * kPlane) = p.l;
     }
     __device__ __forceinline__ void store(uint8_t* s) const {
-        const int t = thread_id() & 127;
-        if (threadIdx.x < 128) {
-            constexpr int UL = KP == 1 ? 1 : 2;
 #pragma unroll
-            for (int n = 0; n < N * 8 / UL; ++n) {
-                const int b = t + 128 * n, at = k_at(b / KU, b % KU);
-                if constexpr (KP == 1) {
-                    *reinterpret_cast<uint4*>(s + at) = r[n / 8][n % 8];
-                } else {
-                    const f32x4v y = __builtin_bit_cast(f32x4v, r[n / 4][2 * n % 8]);
-                    const f32x4v z = __builtin_bit_cast(f32x4v, r[n / 4][2 * n % 8 + 1]);
-                    put(s + at, parts8({y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]}));
-                }
+        for (int n = 0; n < NK; ++n) {
+            const int key = t / CU + n * KS, unit = t % CU;
+            if constexpr (KP == 1) {
+                *reinterpret_cast<f32x4v*>(s + k_at(key, unit)) = kr[n];
+            } else {   // (half a unit of each part)
+                uint2 h, m, l;
+                parts4(kr[n], h, m, l);
+                uint8_t* at = s + k_at(key, unit >> 1) + 8 * (unit & 1);
+                *reinterpret_cast<uint2*>(at) = h;
+                *reinterpret_cast<uint2*>(at + kPlane) = m;
+                *reinterpret_cast<uint2*>(at + 2 * kPlane) = l;
             }
-        } else {
-            uint8_t* sv = s + KP * kPlane;
+        }
+        uint8_t* sv = s + KP * kPlane;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int b = t + 128 * n, grp = b / (HD / VB), d = VB * (b % (HD / VB));
+        for (int n = 0; n < NV; ++n) {
+            const int b = t + 256 * n, grp = b / (HD / VB), d = VB * (b % (HD / VB));
 #pragma unroll
-                for (int i = 0; i < VB; ++i) {
-                    const int at = v_at(d + i, grp);
-                    if constexpr (KP == 1) {
-                        uint32_t o[4];
+            for (int i = 0; i < VB; ++i) {
+                const int at = v_at(d + i, grp);
+                if constexpr (KP == 1) {
+                    uint32_t o[4];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-                            const u32x4 w0 = __builtin_bit_cast(u32x4, r[n][2 * y]);
-                            const u32x4 w1 = __builtin_bit_cast(u32x4, r[n][2 * y + 1]);
-                            o[y] = __builtin_amdgcn_perm(w1[i >> 1], w0[i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
-                        }
-                        *reinterpret_cast<uint4*>(sv + at) = make_uint4(o[0], o[1], o[2], o[3]);
-                    } else {
-                        float y[8];
+                    for (int y = 0; y < 4; ++y)
+                        o[y] = __builtin_amdgcn_perm(vr[n][2 * y + 1][i >> 1], vr[n][2 * y][i >> 1],
+                                                     i & 1 ? 0x07060302u : 0x05040100u);
+                    *reinterpret_cast<uint4*>(sv + at) = make_uint4(o[0], o[1], o[2], o[3]);
+                } else {
+                    float y[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = __builtin_bit_cast(f32x4v, r[n][e])[i & 3];
-                        put(sv + at, parts8(y));
-                    }
+                    for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(vr[n][e][i]);
+                    put(sv + at, parts8(y));
                 }
             }
         }
@@ -947,18 +1000,20 @@ struct Wide : Rows<HD, QP, NT, false> {
         const int hi = rows ? min(w.hi, min(this->most, w.last) + 1) : 0;
         bool bad = false;
         S st;
-        st.look(kv, w.lo, bad);
-        st.load(kv, w.lo);
-        if (w.lo + S::SK < w.hi) st.look(kv, w.lo + S::SK, bad);
+        st.init(kv);
+        st.look(kv, w.lo);
+        st.load(kv, w.lo, bad);
+        if (w.lo + S::SK < w.hi) st.look(kv, w.lo + S::SK);
         int turn = 0;
         for (int k0 = w.lo; k0 < w.hi; k0 += S::SK) {
             uint8_t* buf = s_kv + turn * S::kBytes;
             if (S::kBuffers == 1) __syncthreads();
+            if (kv.edge(k0, S::SK)) st.clear_v(kv, k0);
             st.store(buf);
             __syncthreads();   // (with two buffers the other one is still read before it)
             if (k0 + S::SK < w.hi) {
-                st.load(kv, k0 + S::SK);
-                if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK, bad);
+                st.load(kv, k0 + S::SK, bad);
+                if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
             }
 #pragma unroll
             for (int b = 0; b < S::SK / 32; b += NB)
