@@ -158,41 +158,42 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 
 // ---- attention -----------------------------------------------------------------------
 
-// Eight f32 values as three bf16 parts that add up to them exactly.
+// f32 values as three bf16 parts, each rounded to nearest, that add up to them
+// exactly (24 bits), a pair at a time.  The rest of a pair is two v_dot2, (hi0, hi1) .
+// (-1, 0) + x0 and (hi0, hi1) . (0, -1) + x1, exact: seven instructions a pair against
+// eleven with the parts unpacked and subtracted.  The constants live in scalar registers:
+// as literals the instruction would read them as f32.
 struct Parts8 {
     bf16x8 h, m, l;
 };
+__device__ __forceinline__ void parts2(float x0, float x1, uint32_t& h, uint32_t& m, uint32_t& l) {
+    uint32_t c0, c1;
+    asm("s_mov_b32 %0, 0xbf80" : "=s"(c0));
+    asm("s_mov_b32 %0, 0xbf800000" : "=s"(c1));
+    const bf16x2 n0 = __builtin_bit_cast(bf16x2, c0), n1 = __builtin_bit_cast(bf16x2, c1);
+    const bf16x2 hi = __builtin_convertvector(f32x2v{x0, x1}, bf16x2);
+    const float r0 = __builtin_amdgcn_fdot2_f32_bf16(hi, n0, x0, false);
+    const float r1 = __builtin_amdgcn_fdot2_f32_bf16(hi, n1, x1, false);
+    const bf16x2 mid = __builtin_convertvector(f32x2v{r0, r1}, bf16x2);
+    const float t0 = __builtin_amdgcn_fdot2_f32_bf16(mid, n0, r0, false);
+    const float t1 = __builtin_amdgcn_fdot2_f32_bf16(mid, n1, r1, false);
+    h = __builtin_bit_cast(uint32_t, hi);
+    m = __builtin_bit_cast(uint32_t, mid);
+    l = pack_bf16(t0, t1);
+}
 __device__ __forceinline__ Parts8 parts8(const float (&v)[8]) {
     uint32_t h[4], m[4], l[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float x0 = v[2 * i], x1 = v[2 * i + 1];
-        h[i] = pack_bf16(x0, x1);
-        const float r0 = x0 - __uint_as_float(h[i] << 16), r1 = x1 - __uint_as_float(h[i] & 0xFFFF0000u);
-        m[i] = pack_bf16(r0, r1);
-        l[i] = pack_bf16(r0 - __uint_as_float(m[i] << 16), r1 - __uint_as_float(m[i] & 0xFFFF0000u));
-    }
+    for (int i = 0; i < 4; ++i) parts2(v[2 * i], v[2 * i + 1], h[i], m[i], l[i]);
     Parts8 s;
     s.h = __builtin_bit_cast(bf16x8, make_uint4(h[0], h[1], h[2], h[3]));
     s.m = __builtin_bit_cast(bf16x8, make_uint4(m[0], m[1], m[2], m[3]));
     s.l = __builtin_bit_cast(bf16x8, make_uint4(l[0], l[1], l[2], l[3]));
     return s;
 }
-
-// The same of four.
 __device__ __forceinline__ void parts4(f32x4v v, uint2& h, uint2& m, uint2& l) {
-    uint32_t a[2], b[2], c[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float x0 = v[2 * i], x1 = v[2 * i + 1];
-        a[i] = pack_bf16(x0, x1);
-        const float r0 = x0 - __uint_as_float(a[i] << 16), r1 = x1 - __uint_as_float(a[i] & 0xFFFF0000u);
-        b[i] = pack_bf16(r0, r1);
-        c[i] = pack_bf16(r0 - __uint_as_float(b[i] << 16), r1 - __uint_as_float(b[i] & 0xFFFF0000u));
-    }
-    h = make_uint2(a[0], a[1]);
-    m = make_uint2(b[0], b[1]);
-    l = make_uint2(c[0], c[1]);
+    parts2(v[0], v[1], h.x, m.x, l.x);
+    parts2(v[2], v[3], h.y, m.y, l.y);
 }
 
 __device__ __forceinline__ f32x4v mfma(bf16x8 a, bf16x8 b, f32x4v c) {
@@ -511,21 +512,63 @@ struct Rows {
         most = __builtin_amdgcn_readfirstlane(most);
     }
 
-    // Part products of a K (or V) operand with the rows' parts, small ones first: for
-    // f32 on both sides the six down to 2^-16 of the largest.  `acc` one per group.
-    template <class OP>
-    __device__ __forceinline__ static void products(const bf16x8 (&x)[1], const OP& y, int t, int s, f32x4v& o) {
-#pragma unroll
-        for (int b = QP - 1; b >= 0; --b) o = mfma(x[0], y(t, b, s), o);
+    // Products of the parts of a K (or V) operand, KP of them, with the rows' QP, small
+    // ones first: product p takes parts left(p) and right(p); for f32 on both sides the six
+    // down to 2^-16 of the largest.  Those of one size (order(p)) are summed by themselves
+    // where sums are short: an MFMA waits for the one before on the same sum.
+    template <int KP>
+    static constexpr int kProducts = KP == 1 ? QP : 6;
+    static constexpr int kOrders = QP;
+    template <int KP>
+    static constexpr int left(int p) {
+        constexpr int l[6] = {2, 0, 1, 1, 0, 0};
+        return KP == 1 ? 0 : l[p];
     }
-    template <class OP>
-    __device__ __forceinline__ static void products(const bf16x8 (&x)[3], const OP& y, int t, int s, f32x4v& o) {
-        o = mfma(x[2], y(t, 0, s), o);
-        o = mfma(x[0], y(t, QP - 1, s), o);
-        o = mfma(x[1], y(t, QP / 2, s), o);
-        o = mfma(x[1], y(t, 0, s), o);
-        o = mfma(x[0], y(t, QP / 2, s), o);
-        o = mfma(x[0], y(t, 0, s), o);
+    template <int KP>
+    static constexpr int right(int p) {
+        constexpr int r[6] = {0, 2, 1, 0, 1, 0};
+        return KP == 1 ? QP - 1 - p : r[p];
+    }
+    template <int KP>
+    static constexpr int order(int p) { return left<KP>(p) + right<KP>(p); }
+
+    // Scores of a 32-key block from K's parts x[u] of dims 32 i ..
+    template <int KP>
+    __device__ __forceinline__ void scores(const bf16x8 (&x)[2][KP], int i, f32x4v (&s)[kOrders][NT][2]) const {
+#pragma unroll
+        for (int p = 0; p < kProducts<KP>; ++p)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    s[order<KP>(p)][t][u] = mfma(x[u][left<KP>(p)], q[t][right<KP>(p)][i], s[order<KP>(p)][t][u]);
+    }
+    __device__ __forceinline__ static void zero(f32x4v (&s)[kOrders][NT][2]) {
+#pragma unroll
+        for (int o = 0; o < kOrders; ++o)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[o][t][0] = s[o][t][1] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ static void total(const f32x4v (&s)[kOrders][NT][2], f32x4v (&sum)[NT][2]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                sum[t][u] = s[kOrders - 1][t][u];
+#pragma unroll
+                for (int o = kOrders - 2; o >= 0; --o) sum[t][u] += s[o][t][u];
+            }
+    }
+    // Output MFMAs j0 .. j0 + N - 1 from V's parts x[j]
+    template <int KP, int N>
+    __device__ __forceinline__ void values(const bf16x8 (&x)[N][KP], int j0, const bf16x8 (&pp)[NT][QP]) {
+#pragma unroll
+        for (int p = 0; p < kProducts<KP>; ++p)
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    acc[t][j0 + j] = mfma(x[j][left<KP>(p)], pp[t][right<KP>(p)], acc[t][j0 + j]);
     }
 
     // The running softmax over NB blocks of 32 keys from kb on: the scores s become the
@@ -754,47 +797,56 @@ struct Deep : Rows<HD, QP, 1, true> {
                     pk1 = kv.page_of(nb + step + 8 * (c >> 2));
                     pv1 = kv.page_of(nb + step + 8 * g);
                 }
-                f32x4v s[1][1][2];
-                s[0][0][0] = s[0][0][1] = f32x4v{0.f, 0.f, 0.f, 0.f};
-                const auto qop = [&](int t, int b, int i) { return this->q[t][b][i]; };
+                f32x4v part[QP][1][2], s[1][1][2];
+                R::zero(part);
 #pragma unroll
-                for (int i = 0; i < NS; ++i)
+                for (int i = 0; i < NS; ++i) {
+                    bf16x8 x[2][KP];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         if constexpr (KP == 1) {
-                            const bf16x8 x[1] = {__builtin_bit_cast(bf16x8, kw[u][i])};
-                            R::products(x, qop, 0, i, s[0][0][u]);
+                            x[u][0] = __builtin_bit_cast(bf16x8, kw[u][i]);
                         } else {
                             const f32x4v y = __builtin_bit_cast(f32x4v, kw[u][2 * i]);
                             const f32x4v z = __builtin_bit_cast(f32x4v, kw[u][2 * i + 1]);
                             const Parts8 r = parts8({y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]});
-                            const bf16x8 x[3] = {r.h, r.m, r.l};
-                            R::products(x, qop, 0, i, s[0][0][u]);
+                            x[u][0] = r.h;
+                            x[u][1] = r.m;
+                            x[u][2] = r.l;
                         }
                     }
+                    this->template scores<KP>(x, i, part);
+                }
+                R::total(part, s[0]);
                 if (nb < hi) load_k(kv, nb, kv.known(pk, bad));
                 bf16x8 pp[1][1][QP];
                 this->template softmax<1>(w, kb, s, unit, pp);
-                const auto pop = [&](int t, int b, int) { return pp[0][t][b]; };
                 if (kv.edge(kb, 32)) clear_v(kv, kb);
+                constexpr int JG = KP == 1 ? 4 : 2;
 #pragma unroll
-                for (int j = 0; j < VD; ++j) {
-                    if constexpr (KP == 1) {
-                        uint32_t o[4];
+                for (int j0 = 0; j0 < VD; j0 += JG) {
+                    bf16x8 x[JG][KP];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            o[i] = __builtin_amdgcn_perm(vw[2 * i + 1][j >> 1], vw[2 * i][j >> 1],
-                                                         j & 1 ? 0x07060302u : 0x05040100u);
-                        const bf16x8 x[1] = {__builtin_bit_cast(bf16x8, make_uint4(o[0], o[1], o[2], o[3]))};
-                        R::products(x, pop, 0, 0, acc[0][j]);
-                    } else {
-                        float y[8];
+                    for (int jj = 0; jj < JG; ++jj) {
+                        const int j = j0 + jj;
+                        if constexpr (KP == 1) {
+                            uint32_t o[4];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = vf[e][j];
-                        const Parts8 r = parts8(y);
-                        const bf16x8 x[3] = {r.h, r.m, r.l};
-                        R::products(x, pop, 0, 0, acc[0][j]);
+                            for (int i = 0; i < 4; ++i)
+                                o[i] = __builtin_amdgcn_perm(vw[2 * i + 1][j >> 1], vw[2 * i][j >> 1],
+                                                             j & 1 ? 0x07060302u : 0x05040100u);
+                            x[jj][0] = __builtin_bit_cast(bf16x8, make_uint4(o[0], o[1], o[2], o[3]));
+                        } else {
+                            float y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = vf[e][j];
+                            const Parts8 r = parts8(y);
+                            x[jj][0] = r.h;
+                            x[jj][1] = r.m;
+                            x[jj][2] = r.l;
+                        }
                     }
+                    this->template values<KP>(x, j0, pp[0]);
                 }
                 if (nb < hi) load_v(kv, nb, kv.known(pv, bad));
             }
@@ -955,44 +1007,49 @@ struct Wide : Rows<HD, QP, NT, false> {
     typedef Stage<HD, KP> S;
     static constexpr int NS = R::NS, VD = R::VD;
     // 32-key blocks a softmax takes at once: two halve its maxima and rescalings
-    static constexpr int NB = QP == 1 && HD <= 128 ? 2 : 1;
+    static constexpr int NB = S::SK >= 64 ? 2 : 1;
 
     __device__ __forceinline__ void blocks(const Work& w, int kb, int b0, float unit, const uint8_t* s_kv) {
         const int g = this->g, c = this->c;
         f32x4v s[NB][NT][2];
-        const auto qop = [&](int t, int x, int i) { return this->q[t][x][i]; };
+        // (the SIMD's other wave's vector work fits between the MFMAs, not they between it)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            f32x4v part[QP][NT][2];
+            R::zero(part);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) s[b][t][0] = s[b][t][1] = f32x4v{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < NS; ++i) {
+                bf16x8 x[2][KP];
 #pragma unroll
-            for (int i = 0; i < NS; ++i)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    bf16x8 x[KP];
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int y = 0; y < KP; ++y)
-                        x[y] = *reinterpret_cast<const bf16x8*>(
+                        x[u][y] = *reinterpret_cast<const bf16x8*>(
                             s_kv + y * S::kPlane + S::k_at(32 * (b0 + b) + 8 * (c >> 2) + 4 * u + (c & 3), 4 * i + g));
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) R::products(x, qop, t, i, s[b][t][u]);
-                }
+                this->template scores<KP>(x, i, part);
+            }
+            R::total(part, s[b]);
         }
+        __builtin_amdgcn_s_setprio(0);
         bf16x8 pp[NB][NT][QP];
         this->template softmax<NB>(w, kb, s, unit, pp);
+        __builtin_amdgcn_s_setprio(1);
+        constexpr int JG = KP == 1 ? 4 : 2;
 #pragma unroll
-        for (int j = 0; j < VD; ++j)
+        for (int j0 = 0; j0 < VD; j0 += JG)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const auto pop = [&](int t, int x, int) { return pp[b][t][x]; };
-                bf16x8 x[KP];
+                bf16x8 x[JG][KP];
 #pragma unroll
-                for (int y = 0; y < KP; ++y)
-                    x[y] = *reinterpret_cast<const bf16x8*>(s_kv + (KP + y) * S::kPlane +
-                                                            S::v_at(16 * j + c, 4 * (b0 + b) + g));
+                for (int j = 0; j < JG; ++j)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) R::products(x, pop, t, 0, this->acc[t][j]);
+                    for (int y = 0; y < KP; ++y)
+                        x[j][y] = *reinterpret_cast<const bf16x8*>(
+                            s_kv + (KP + y) * S::kPlane + S::v_at(16 * (j0 + j) + c, 4 * (b0 + b) + g));
+                this->template values<KP>(x, j0, pp[b]);
             }
+        __builtin_amdgcn_s_setprio(0);
     }
     // `rows`: whether the wave has some (those without take part in the staging)
     __device__ __forceinline__ void run(const PagedView& p, const Work& w, bool rows, float unit, uint8_t* s_kv) {
