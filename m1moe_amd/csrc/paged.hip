@@ -217,7 +217,9 @@ __device__ __forceinline__ float quads_add(float v) {
 // e^(x scale) of a difference of raw scores, as the hardware exp2.
 __device__ __forceinline__ float weight(float x, float unit) { return __builtin_amdgcn_exp2f(x * unit); }
 
-constexpr int kCut = 256;        // keys: where a tile's keys may be cut between workgroups
+constexpr int kCut = 64;         // keys: where a tile's keys may be cut between workgroups
+constexpr int kWhole = 512;      // keys of a tile that is not cut
+constexpr int kFewKeys = 128;    // least places on the line per workgroup
 constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 
 // How the rows and keys are shared.  A tile is up to R rows (token, head) of one
@@ -227,7 +229,8 @@ constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 // with kTileKeys places for what it costs to begin and end it (about 5 us: the
 // queries, the first page and rows one after the other, the waves' join) and one
 // place per key; the line is cut into equal shares, one per workgroup, the cuts
-// moved down to a multiple of kCut keys inside their tile.  (Without the places
+// moved down to a multiple of kCut keys inside their tile, or to its start where it has
+// at most kWhole keys (to join two pieces of one takes longer than to read it).  (Without the places
 // per tile the workgroups with the shortest sequences ended last: 32 steps of 60 to
 // 8100 positions, 8 kv heads, median 61 us, last 116.)
 struct Tile {
@@ -257,8 +260,8 @@ struct Line {
     __device__ int64_t head_places(int base, int n, int tiles) const {
         return before(base, tiles - 1) + (base - org + kTileKeys) + n;
     }
-    // Equal shares but for one place, at least kCut places, so that every cut inside a
-    // tile's keys begins a piece of its own.
+    // Equal shares but for one place, at least kFewKeys >= kCut places, so that every cut
+    // inside a cut tile's keys begins a piece of its own.
     __device__ int64_t cut(int w) const { return w * share + min(w, rest); }
     // The last cut below place x > 0.
     __device__ int below(int64_t x) const {
@@ -301,7 +304,8 @@ struct Line {
     // Cut x inside tile t, moved down: to the tile's start or to a place of a key.
     __device__ int64_t rounded(const Tile& t, int64_t x) const {
         const int64_t keys = x - t.start - kTileKeys;
-        return keys < kCut ? t.start : t.start + kTileKeys + keys / kCut * kCut;
+        return keys < kCut || t.end - t.start <= kTileKeys + kWhole ? t.start
+                                                                    : t.start + kTileKeys + keys / kCut * kCut;
     }
     // The key (from org on) at place x of tile t.
     __device__ static int key(const Tile& t, int64_t x) { return (int)max((int64_t)0, x - t.start - kTileKeys); }
@@ -340,7 +344,8 @@ __device__ __forceinline__ void make_line(const PagedView& p, Line& ln, int64_t*
     }
     if (tid == 0) ln.cum[p.num_seqs] = carry;
     ln.total = carry;
-    ln.wgs = (int)min((int64_t)grid, max((int64_t)1, carry / kCut));
+    ln.wgs = (int)min((int64_t)grid, max((int64_t)1, carry / kFewKeys));
+    static_assert(kFewKeys >= kCut, "a cut per piece");
     ln.share = (int64_t)((double)carry / ln.wgs);       // (within one)
     ln.share += ((ln.share + 1) * ln.wgs <= carry) - (ln.share * ln.wgs > carry);
     ln.rest = (int)(carry - ln.share * ln.wgs);
@@ -1264,20 +1269,69 @@ __device__ __forceinline__ Sink<HD> piece_of(const PagedAttnArgs& a, int i) {
     return {kToPiece, a.pre + i * rows * HD, a.pre + (a.splits + 1) * rows * HD + i * rows * 2};
 }
 
-// The pieces first .. last of tile w.r.t. the line, which workgroups first .. last have
-// written to their slots, joined in their order: a thread's values of the tile's rows
-// in registers.
+// The pieces of a tile that workgroups first .. last have written to their slots, joined.
+// Few values: the threads that they leave share the pieces, eight loads of each in
+// flight, and join theirs through LDS.  Many: eight values of a thread in flight, piece
+// after piece.  Either way in an order that does not depend on who is last.
 template <int HD, int QP>
 __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w, int first, int last, float unit,
-                                          const Sink<HD>& sink) {
+                                          uint8_t* s_buf, const Sink<HD>& sink) {
     constexpr int NV = tile_rows<HD, QP>() * HD / 4 / 256;
-    const int rows = w.tokens * a.share, tid = thread_id();
+    const int rows = w.tokens * a.share, tid = thread_id(), values = rows * (HD / 4);
+    const auto piece = [&](int p) { return slot_of<HD, QP>(a, p == first ? 2 * p + 1 : 2 * p); };
+    const auto coh = [](const float* p) {
+        return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    if (values <= 256) {
+        const int groups = 256 / values, grp = tid / values, i = tid - grp * values;
+        const int rho = i / (HD / 4), d = 4 * (i % (HD / 4));
+        f32x4v o = {0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        if (grp < groups) {
+            for (int p0 = first + 8 * grp; p0 <= last; p0 += 8 * groups) {
+                const float* at[8];
+                f32x4v y[8];
+                float z[8], u[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const Sink<HD> slot = piece(min(p0 + k, last));
+                    at[k] = slot.o + rho * HD + d;
+                    z[k] = coh(slot.ml + 2 * rho);
+                    u[k] = coh(slot.ml + 2 * rho + 1);
+                }
+                load8_coh(at, y);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (p0 + k > last) break;
+                    float f0, f1;
+                    join(m, l, z[k], u[k], unit, f0, f1);
+                    o = o * f0 + y[k] * f1;
+                }
+            }
+        }
+        float* s = reinterpret_cast<float*>(s_buf) + 8 * tid;
+        *reinterpret_cast<f32x4v*>(s) = o;
+        s[4] = m;
+        s[5] = l;
+        __syncthreads();
+        int token, head;
+        if (grp == 0 && row_at(a, w, rho, token, head)) {
+            for (int k = 1; k < groups; ++k) {
+                const float* y = reinterpret_cast<const float*>(s_buf) + 8 * (tid + k * values);
+                float f0, f1;
+                join(m, l, y[4], y[5], unit, f0, f1);
+                o = o * f0 + *reinterpret_cast<const f32x4v*>(y) * f1;
+            }
+            sink.put(a, QP == 1, rho, token, head, d, m, l, 1.0f / l, o[0], o[1], o[2], o[3]);
+        }
+        return;
+    }
 #pragma unroll 1
-    for (int k0 = 0; k0 < NV && 256 * k0 / (HD / 4) < rows; k0 += 8) {
+    for (int k0 = 0; k0 < NV && 256 * k0 < values; k0 += 8) {
         f32x4v o[8];
         float m[8], l[8];
         for (int p = first; p <= last; ++p) {
-            const Sink<HD> slot = slot_of<HD, QP>(a, p == first ? 2 * p + 1 : 2 * p);
+            const Sink<HD> slot = piece(p);
             const float* at[8];
             f32x4v y[8];
             float z[8], u[8];
@@ -1285,8 +1339,8 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
             for (int k = 0; k < 8; ++k) {
                 const int i = tid + 256 * (k0 + k), rho = min(i / (HD / 4), rows - 1);
                 at[k] = slot.o + rho * HD + 4 * (i % (HD / 4));
-                z[k] = __hip_atomic_load(slot.ml + 2 * rho, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                u[k] = __hip_atomic_load(slot.ml + 2 * rho + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                z[k] = coh(slot.ml + 2 * rho);
+                u[k] = coh(slot.ml + 2 * rho + 1);
             }
             load8_coh(at, y);
 #pragma unroll
@@ -1410,7 +1464,7 @@ __global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_attn_kernel
                     __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
-            if (s_last) join_tile<HD, QP>(a, w, first, last, unit, done);
+            if (s_last) join_tile<HD, QP>(a, w, first, last, unit, s_buf, done);
         }
         __syncthreads();   // (s_buf and s_last are the next tile's)
         x = end;
