@@ -238,11 +238,14 @@ struct Tile {
     int row0, n, base;           // the sequence's first row, rows, positions before them
     int64_t cum, start, end;     // on the line: the sequence's start, the tile's, its end
 
-    // (the sequence's are the same in every lane: into scalar registers)
-    __device__ __forceinline__ void uniform() {
-        for (int* x : {&seq, &row0, &n, &base}) *x = __builtin_amdgcn_readfirstlane(*x);
-        cum = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(cum >> 32)) << 32 |
-                        (uint32_t)__builtin_amdgcn_readfirstlane((int)cum));
+    // Lane `lane`'s in every lane, in scalar registers.
+    __device__ __forceinline__ static int64_t lane64(int64_t x, int lane) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
+    }
+    __device__ __forceinline__ void of_lane(int lane) {
+        for (int* x : {&seq, &head, &r, &row0, &n, &base}) *x = __builtin_amdgcn_readlane(*x, lane);
+        for (int64_t* x : {&cum, &start, &end}) *x = lane64(*x, lane);
     }
 };
 
@@ -270,14 +273,14 @@ struct Line {
         while (w > 0 && cut(w) >= x) --w;
         return w;
     }
-    // Sequence s of the batch, and its tile that holds place x of the line.
+    // Sequence s of the batch, and its tile that holds place x of the line (all of a lane's
+    // own: two places take no longer than one).
     __device__ void sequence(const PagedView& p, int s, Tile& t) const {
         t.seq = s;
         t.row0 = p.row_start[s];
         t.n = p.row_start[s + 1] - t.row0;
         t.base = p.kv_len[s] - t.n;
         t.cum = cum[s];
-        t.uniform();
     }
     __device__ void find(int64_t x, Tile& t) const {
         const int tiles = (t.n + TT - 1) / TT;
@@ -479,9 +482,10 @@ struct Rows {
         g = lane >> 4;
         c = lane & 15;
     }
-    // rows rho0 ..
-    __device__ __forceinline__ void load(const PagedAttnArgs& a, const Work& w, int rho0) {
-        clear();
+    // Rows rho0 ..: read (raw, 16 bytes at a time), then split.
+    static constexpr int kRaw = QP == 1 ? 1 : 2;
+    __device__ __forceinline__ void read(const PagedAttnArgs& a, const Work& w, int rho0,
+                                         f32x4v (&raw)[NT][NS][kRaw]) {
         see = w.last;
         most = -1;
 #pragma unroll
@@ -492,23 +496,33 @@ struct Rows {
             see = min(see, qpos[t]);
             most = max(most, qpos[t]);
             const int64_t at = (int64_t)token * a.q_stride + (int64_t)head * HD + 8 * g;
+            const f32x4v* x = QP == 1 ? reinterpret_cast<const f32x4v*>(static_cast<const uint16_t*>(a.q) + at)
+                                      : reinterpret_cast<const f32x4v*>(static_cast<const float*>(a.q) + at);
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int i = 0; i < kRaw; ++i) {
+                    raw[t][s][i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+                    if (on) raw[t][s][i] = x[4 * kRaw * s + i];
+                }
+        }
+    }
+    __device__ __forceinline__ void split(const f32x4v (&raw)[NT][NS][kRaw]) {
+        clear();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 if constexpr (QP == 1) {
-                    uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at + 32 * s);
-                    if (!on) x = make_uint4(0, 0, 0, 0);
-                    q[t][0][s] = __builtin_bit_cast(bf16x8, x);
+                    q[t][0][s] = __builtin_bit_cast(bf16x8, raw[t][s][0]);
                 } else {
-                    const float4* x = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at + 32 * s);
-                    float4 y = x[0], z = x[1];
-                    if (!on) y = z = make_float4(0.f, 0.f, 0.f, 0.f);
-                    const Parts8 r = parts8({y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w});
+                    const f32x4v y = raw[t][s][0], z = raw[t][s][1];
+                    const Parts8 r = parts8({y[0], y[1], y[2], y[3], z[0], z[1], z[2], z[3]});
                     q[t][0][s] = r.h;
                     q[t][QP - 2][s] = r.m;
                     q[t][QP - 1][s] = r.l;
                 }
             }
-        }
         for (int x = 1; x < 16; x <<= 1) {
             see = min(see, __shfl_xor(see, x));
             most = max(most, __shfl_xor(most, x));
@@ -775,22 +789,28 @@ struct Deep : Rows<HD, QP, 1, true> {
             }
         }
     }
-    // (the first block's rows are on their way before the queries are read and split)
+    // (the queries are read before the first block's rows and split while those are on
+    // their way: loads come back in their order)
     __device__ __forceinline__ void run(const PagedAttnArgs& a, const Work& w, int lo, int step, float unit) {
         const Cache<HD, KP> kv(a.p, w);
         this->lanes();
         bool bad = false;
-        int pk1 = 0, pv1 = 0;
+        int pk0 = 0, pv0 = 0, pk1 = 0, pv1 = 0;
         if (lo < w.hi) {
-            const int pk = kv.page_of(lo + 8 * (c >> 2)), pv = kv.page_of(lo + 8 * g);
+            pk0 = kv.page_of(lo + 8 * (c >> 2));
+            pv0 = kv.page_of(lo + 8 * g);
             if (lo + step < w.hi) {
                 pk1 = kv.page_of(lo + step + 8 * (c >> 2));
                 pv1 = kv.page_of(lo + step + 8 * g);
             }
-            load_k(kv, lo, kv.known(pk, bad));
-            load_v(kv, lo, kv.known(pv, bad));
         }
-        this->load(a, w, 0);
+        f32x4v raw[1][NS][R::kRaw];
+        this->read(a, w, 0, raw);
+        if (lo < w.hi) {
+            load_k(kv, lo, kv.known(pk0, bad));
+            load_v(kv, lo, kv.known(pv0, bad));
+        }
+        this->split(raw);
         const int hi = min(w.hi, min(this->most, w.last) + 1);
         if (lo < hi) {
             int pk, pv;
@@ -910,10 +930,6 @@ struct Stage {
     __device__ __forceinline__ void look(const Cache<HD, KP>& kv, int kb) {
         pages = kv.page_of(kb + 8 * (t & 15) % SK);
     }
-    __device__ __forceinline__ static int64_t lane64(int64_t x, int lane) {
-        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
-    }
     __device__ __forceinline__ static void get(uint32_t (&to)[VW], const uint8_t* x) {
         const vblock v = *reinterpret_cast<const vblock*>(x);
 #pragma unroll
@@ -927,15 +943,15 @@ struct Stage {
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
             const int key = key0 + n * KS;
-            kr[n] = *reinterpret_cast<const f32x4v*>(kv.k + (lane64(at, key >> 3) + (uint32_t)(key & 7) * kv.row) + k_off);
+            kr[n] = *reinterpret_cast<const f32x4v*>(kv.k + (Tile::lane64(at, key >> 3) + (uint32_t)(key & 7) * kv.row) + k_off);
         }
         constexpr int kGroups = 64 * VB / HD > 1 ? 64 * VB / HD : 1;   // a wave's V blocks lie in so many
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int grp = (64 * wave + 256 * n) / (HD / VB);
-            int64_t base = lane64(at, grp);
+            int64_t base = Tile::lane64(at, grp);
             if (kGroups == 2) {
-                const int64_t other = lane64(at, grp + 1);
+                const int64_t other = Tile::lane64(at, grp + 1);
                 base = (t & 63) >= HD / VB ? other : base;
             } else if (kGroups > 2) {
                 const int mine = (t + 256 * n) / (HD / VB);
@@ -1227,7 +1243,9 @@ __device__ __forceinline__ void many_rows(const PagedAttnArgs& a, const Work& w,
     const bool rows = rho0 < w.tokens * a.share;
     Wide<HD, QP, KP, NT> r;
     r.lanes();
-    r.load(a, w, rho0);
+    f32x4v raw[NT][HD / 32][Wide<HD, QP, KP, NT>::R::kRaw];
+    r.read(a, w, rho0, raw);
+    r.split(raw);
     r.run(a.p, w, rows, unit, s_buf);
     if (!rows) return;
     if (r.odd()) r.template run_plain<KP>(a, w, rho0, w.lo, 32, unit, reinterpret_cast<float*>(s_buf) + wave * HD);
@@ -1420,17 +1438,18 @@ __global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_attn_kernel
     // neighbouring shares on one XCD (workgroup id mod 8; the prefix' are a multiple of 8)
     const int per = (ln.wgs + 7) / 8, wg = (id & 7) * per + (id >> 3);
     if ((id >> 3) >= per || wg >= ln.wgs) return;
-    int64_t x1 = ln.cut(wg + 1);
+    // (lane 0: the share's first place, lane 1: the next one's)
+    const int lane = threadIdx.x & 63;
+    int64_t x = ln.cut(wg + (lane == 1));
+    const bool all = x >= ln.total;
+    if (all) x = ln.total - 1;
     Tile t;
-    if (x1 < ln.total) {
-        ln.sequence(p, find_seq(p, ln, x1), t);
-        ln.find(x1, t);
-        x1 = ln.rounded(t, x1);
-    }
-    int64_t x = ln.cut(wg);
-    if (x1 == ln.total || x < t.cum) ln.sequence(p, find_seq(p, ln, x), t);
+    ln.sequence(p, find_seq(p, ln, x), t);
     ln.find(x, t);
-    x = ln.rounded(t, x);
+    x = all ? ln.total : ln.rounded(t, x);
+    const int64_t x1 = Tile::lane64(x, 1);
+    x = Tile::lane64(x, 0);
+    t.of_lane(0);
     while (x < x1) {
         const int64_t end = min(t.end, x1);
         Work w;
@@ -1471,6 +1490,7 @@ __global__ __launch_bounds__(256, (wgs_per_cu<HD, KP>())) void paged_attn_kernel
         if (x < x1) {
             if (x >= s_cum[t.seq + 1]) ln.sequence(p, find_seq(p, ln, x), t);
             ln.find(x, t);
+            t.of_lane(0);
         }
     }
 }
@@ -1492,20 +1512,35 @@ __global__ __launch_bounds__(256) void paged_pieces_kernel(PagedAttnArgs a) {
         const int lo = p.row_start[s], hi = p.row_start[s + 1];
         if (token >= lo && token < hi && seq_ok(p, lo, hi, p.kv_len[s])) s_in = 1;
     }
-    float m = -INFINITY;
-    for (int s = 0; s <= a.splits; ++s) m = fmaxf(m, all.ml[2 * (s * rows + row)]);
-    const float mc = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s <= a.splits; ++s) {
-        const float2 z = *reinterpret_cast<const float2*>(all.ml + 2 * (s * rows + row));
-        const float4 y = *reinterpret_cast<const float4*>(all.o + (s * rows + row) * HD + d);
-        const float f = weight(z.x - mc, unit);
-        l = fmaf(z.y, f, l);
-        o[0] = fmaf(y.x, f, o[0]);
-        o[1] = fmaf(y.y, f, o[1]);
-        o[2] = fmaf(y.z, f, o[2]);
-        o[3] = fmaf(y.w, f, o[3]);
+    // (eight pieces in flight)
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 <= a.splits; s0 += 8) {
+        float2 z[8];
+        float4 y[8];
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t at = min(s0 + k, a.splits) * rows + row;
+            z[k] = *reinterpret_cast<const float2*>(all.ml + 2 * at);
+            y[k] = *reinterpret_cast<const float4*>(all.o + at * HD + d);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, z[k].x);
+        const float mc = top == -INFINITY ? 0.f : top, f0 = weight(m - mc, unit);
+        m = top;
+        l *= f0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= f0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (s0 + k > a.splits) break;   // (the last one again)
+            const float f = weight(z[k].x - mc, unit);
+            l = fmaf(z[k].y, f, l);
+            o[0] = fmaf(y[k].x, f, o[0]);
+            o[1] = fmaf(y[k].y, f, o[1]);
+            o[2] = fmaf(y[k].z, f, o[2]);
+            o[3] = fmaf(y[k].w, f, o[3]);
+        }
     }
     __syncthreads();
     if (!s_in || head >= a.heads) return;
