@@ -1122,10 +1122,12 @@ __device__ __forceinline__ void store4(const PagedAttnArgs& a, bool bf16, int64_
         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// Sixteen bytes to memory, past this XCD's L2 (sc1: for a workgroup on any XCD).
+// Sixteen bytes to memory, past this XCD's L2 (sc1: for a workgroup on any XCD).  (The
+// s_nop: a store of more than 8 bytes may still read its registers when the next
+// instruction writes them, and the compiler does not see a store here.)
 __device__ __forceinline__ void store4_coh(float* p, const float (&x)[4]) {
     const f32x4v v = {x[0], x[1], x[2], x[3]};
-    asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
 }
 // Eight times sixteen bytes from there, waited for.
 __device__ __forceinline__ void load8_coh(const float* const (&p)[8], f32x4v (&v)[8]) {

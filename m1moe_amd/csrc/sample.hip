@@ -164,11 +164,13 @@ struct Span {
     __device__ __forceinline__ int step(float x) const {
         return x == hi ? 0 : (int)(((double)hi - (double)x) * per);
     }
-    // f32 bounds around the logits of steps a .. b, for a first glance.
+    // f32 bounds around the logits of steps a .. b, for a first glance: wider than they
+    // can be off (a step's border by 2^-52 of hi and the range, an f32 by 2^-24).
     __device__ __forceinline__ void bounds(int a, int b, float& from, float& to) const {
         const double x0 = (double)hi - (b + 1) / per, x1 = (double)hi - a / per;
-        from = per > 0.0 ? (float)(x0 - 1e-6 * fabs(x0)) : lo;
-        to = per > 0.0 ? (float)(x1 + 1e-6 * fabs(x1)) : hi;
+        const double eps = 1e-12 * (fabs((double)hi) + fabs((double)lo));
+        from = per > 0.0 ? (float)(x0 - 1e-6 * fabs(x0) - eps) : lo;
+        to = per > 0.0 ? (float)(x1 + 1e-6 * fabs(x1) + eps) : hi;
         from = fmaxf(from, lo);
         to = fminf(to, hi);
     }

@@ -1,6 +1,8 @@
 """GPU parity of the paged KV cache, attention over it and the sampler against
 f64 references (serving_cases.py), through the C ABI.  Bounds are elementwise
 and derived there (attention_bound) or beside the test; sampled tokens are equal."""
+import ctypes
+import gc
 import math
 
 import numpy as np
@@ -356,6 +358,234 @@ def test_attention_in_a_graph(dev):
         ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
         check_close(got.astype(np.float64), ref, attention_bound(ref, mag, top, hd, "f32"), "f32")
     d.free()
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd", [(2, 1, 64), (2, 2, 128), (3, 1, 256)])
+def test_attention_many_rows_shared_by_workgroups(dev, types, heads, kv_heads, hd):
+    """Tiles of many rows, few and one whose keys several workgroups share, alone on the
+    device and beside short ones."""
+    rng = np.random.default_rng(60)
+    for rows, past in (([130], [3000]), ([100, 1, 9, 64], [900, 5, 4000, 0])):
+        b = Batch(rng, rows, past, 16)
+        say(f"attention cut tiles {types} {heads}/{kv_heads}x{hd} {rows}")
+        got, _, ref, bound = attend(dev, b, heads, kv_heads, hd, types, 61)
+        check_close(got, ref, bound, types[0])
+
+
+@pytest.mark.parametrize("types", TYPES)
+def test_attention_infinities_in_pieces(dev, types):
+    """An infinity that only some of a row's pieces meet, in the prefix or behind it."""
+    ctx, ops = dev
+    rng = np.random.default_rng(62)
+    heads, kv_heads, hd, prefix = 2, 2, 64, 600
+    x, cache = types
+    for where in (100, 2500):
+        b = Batch(rng, [1, 40, 2], [4000, 3000, 700], 16, prefix=prefix)
+        q = as_dtype(rng.normal(0, 1, (b.T, heads * hd)), x)
+        kc, vc = cache_of(rng, b, kv_heads, hd, cache)
+        pg, sl = b.cell(1, np.array([where]))
+        vc[pg, sl, 0, 3] = as_dtype(np.full(1, np.inf), cache)[0]
+        vc[pg, sl, 1, 9] = as_dtype(np.full(1, np.nan), cache)[0]
+        d = Held(ctx, b, kc, vc, cache, kv_heads, hd)
+        out = d.up(np.zeros((b.T, heads * hd), np.uint16 if x == "bf16" else np.float32))
+        say(f"attention infinity at {where} {types}")
+        ops.paged_attention(d.kv, d.batch, d.up(q), heads * hd, out, heads * hd, x, heads)
+        ctx.sync()
+        got = f64(out.download(np.uint16 if x == "bf16" else np.float32)).reshape(-1, heads, hd)
+        d.free()
+        ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
+        bound = attention_bound(ref, mag, top, hd, x)
+        fine = np.isfinite(ref)
+        hit = slice(0, b.T) if where < prefix else slice(1, 41)
+        assert np.isposinf(ref[hit, 0, 3]).all() and np.isnan(ref[hit, 1, 9]).all()
+        assert (~fine).sum() == 2 * (hit.stop - hit.start)
+        assert np.array_equal(np.isnan(got), np.isnan(ref)) and np.isposinf(got[hit, 0, 3]).all()
+        assert np.all(np.abs(got[fine] - ref[fine]) <= bound[fine])
+
+
+def test_two_graphs_share_the_partials(dev):
+    """Graphs of two batches captured on one context and replayed in turn, eager calls of
+    a third between them: all use the context's partials and counters."""
+    ctx, ops = dev
+    rng = np.random.default_rng(63)
+    heads, kv_heads, hd = 4, 1, 128
+    held, calls = [], []
+    for rows, past, prefix in (([1, 1], [9000, 40], 0), ([70], [2000], 0), ([1, 3], [3000, 900], 500)):
+        b = Batch(rng, rows, past, 32, prefix=prefix)
+        q = rng.normal(0, 1, (b.T, heads * hd)).astype(np.float32)
+        kc, vc = cache_of(rng, b, kv_heads, hd, "bf16")
+        d = Held(ctx, b, kc, vc, "bf16", kv_heads, hd)
+        dq, out = d.up(q), d.up(np.zeros_like(q))
+        ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
+        held.append((d, out, ref, attention_bound(ref, mag, top, hd, "f32")))
+        calls.append(lambda d=d, dq=dq, out=out: ops.paged_attention(d.kv, d.batch, dq, heads * hd, out, heads * hd,
+                                                                     "f32", heads))
+    for c in calls:
+        c()
+    ctx.sync()
+    first = [out.download(np.float32).copy() for _, out, _, _ in held]
+    graphs = []
+    for c in calls[:2]:
+        ctx.graph_begin()
+        c()
+        graphs.append(ctx.graph_end())
+    for rep in range(3):
+        for _, out, _, _ in held:
+            out.upload(np.zeros(out.nbytes // 4, np.float32))
+        say(f"two graphs in turn {rep}")
+        graphs[0].launch()
+        graphs[1].launch()
+        calls[2]()
+        graphs[0].launch()
+        ctx.sync()
+        for (d, out, ref, bound), want in zip(held, first):
+            got = out.download(np.float32)
+            assert np.array_equal(got, want)
+            check_close(got.reshape(-1, heads, hd).astype(np.float64), ref, bound, "f32")
+    del graphs
+    for d, _, _, _ in held:
+        d.free()
+
+
+def test_attention_scratch_grows_between_captures():
+    """A first call inside a capture is refused, a graph from before the partials grew as
+    well; sampling's first call inside one gives the same tokens."""
+    rng = np.random.default_rng(64)
+    ctx = m.HIPContext(m.make_shape(64, 1, 1, 64))
+    ops = DenseOps(ctx)
+    heads, kv_heads, hd = 4, 2, 64
+    b = Batch(rng, [1, 1], [300, 40], 16)
+    q = rng.normal(0, 1, (2, heads * hd)).astype(np.float32)
+    kc, vc = cache_of(rng, b, kv_heads, hd, "f32")
+    d = Held(ctx, b, kc, vc, "f32", kv_heads, hd)
+    dq, out = d.up(q), d.up(np.zeros_like(q))
+    V = 9001
+    x, u = rng.normal(0, 2, (2, 9004)).astype(np.float32), rng.random(2).astype(np.float32)
+    dx, du, tok = d.up(x), d.up(u), d.up(np.zeros(2, np.int32))
+    want = [sample_ref(x[r, :V], u[r])[0] for r in range(2)]
+
+    def call():
+        ops.paged_attention(d.kv, d.batch, dq, heads * hd, out, heads * hd, "f32", heads)
+    say("first calls inside a capture")
+    ctx.graph_begin()
+    with pytest.raises(M1MoEError) as e:
+        call()
+    assert e.value.code == _lib.M1MOE_ERR_INVALID and "capture" in str(e.value)
+    ops.sample(dx, 2, V, 9004, SampleParams.make(du), tok)
+    g = ctx.graph_end()
+    for _ in range(2):
+        tok.upload(np.zeros(2, np.int32))
+        g.launch()
+        ctx.sync()
+        assert tok.download(np.int32).tolist() == want
+        ops.sample(dx, 2, V, 9004, SampleParams.make(du), tok)
+        ctx.sync()
+        assert tok.download(np.int32).tolist() == want
+    call()
+    ctx.graph_begin()
+    call()
+    g = ctx.graph_end()
+    g.launch()
+    ctx.sync()
+    ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
+    bound = attention_bound(ref, mag, top, hd, "f32")
+    check_close(out.download(np.float32).reshape(2, heads, hd).astype(np.float64), ref, bound, "f32")
+    b2 = Batch(rng, [400], [100], 16, prefix=64)
+    q2 = rng.normal(0, 1, (400, heads * hd)).astype(np.float32)
+    k2, v2 = cache_of(rng, b2, kv_heads, hd, "f32")
+    d2 = Held(ctx, b2, k2, v2, "f32", kv_heads, hd)
+    o2 = d2.up(np.zeros_like(q2))
+    say("the partials grow")
+    ops.paged_attention(d2.kv, d2.batch, d2.up(q2), heads * hd, o2, heads * hd, "f32", heads)
+    ctx.sync()
+    with pytest.raises(M1MoEError) as e:
+        g.launch()
+    assert "capture it again" in str(e.value)
+    out.upload(np.zeros_like(q))
+    call()
+    ctx.sync()
+    check_close(out.download(np.float32).reshape(2, heads, hd).astype(np.float64), ref, bound, "f32")
+    ref, mag, top = attention_ref(b2, q2, k2, v2, heads, kv_heads, hd)
+    check_close(o2.download(np.float32).reshape(400, heads, hd).astype(np.float64), ref,
+                attention_bound(ref, mag, top, hd, "f32"), "f32")
+    del g
+    d.free()
+    d2.free()
+    ctx.close()
+
+
+def test_two_contexts_in_turn(dev):
+    """Calls of two contexts of one device, none waited for: each has its own partials."""
+    a, ops = dev
+    c = m.HIPContext(m.make_shape(64, 1, 1, 64))
+    rng = np.random.default_rng(65)
+    heads, hd = 4, 64
+    held = []
+    for ctx in (a, c):
+        b = Batch(rng, [1, 20], [5000, 700], 16)
+        q = rng.normal(0, 1, (b.T, heads * hd)).astype(np.float32)
+        kc, vc = cache_of(rng, b, 1, hd, "f32")
+        d = Held(ctx, b, kc, vc, "f32", 1, hd)
+        ref, mag, top = attention_ref(b, q, kc, vc, heads, 1, hd)
+        x = rng.normal(0, 2, (3, 20000)).astype(np.float32)
+        u = rng.random(3).astype(np.float32)
+        held.append((ctx, DenseOps(ctx), d, d.up(q), d.up(np.zeros_like(q)), ref,
+                     attention_bound(ref, mag, top, hd, "f32"), d.up(x), d.up(u), d.up(np.zeros(3, np.int32)),
+                     [sample_ref(x[r], u[r], top_p=0.9)[0] for r in range(3)], d.up(np.full(3, 0.9, np.float32))))
+    say("two contexts in turn")
+    for _ in range(3):
+        for ctx, o, d, dq, out, _, _, dx, du, tok, _, dp in held:
+            o.paged_attention(d.kv, d.batch, dq, heads * hd, out, heads * hd, "f32", heads)
+            o.sample(dx, 3, 20000, 20000, SampleParams.make(du, top_p=dp), tok)
+    for ctx, o, d, dq, out, ref, bound, _, _, tok, want, _ in held:
+        ctx.sync()
+        check_close(out.download(np.float32).reshape(-1, heads, hd).astype(np.float64), ref, bound, "f32")
+        assert tok.download(np.int32).tolist() == want
+        d.free()
+    c.close()
+
+
+def test_a_caller_stream(dev):
+    """The operators on a stream of the caller's, captured and replayed there."""
+    ctx, ops = dev
+    gc.collect()
+    ctx.sync()
+    hip = ctypes.CDLL("libamdhip64.so")
+    s = ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(s)) == 0
+    try:
+        if ctx.lib.m1moe_set_stream(ctx.handle, s) != _lib.M1MOE_OK:
+            assert "share device" in _lib.last_error()
+            pytest.skip("another context is alive on the device")
+        rng = np.random.default_rng(66)
+        heads, kv_heads, hd = 4, 2, 128
+        b = Batch(rng, [1, 30], [2000, 10], 16)
+        q = rng.normal(0, 1, (b.T, heads * hd)).astype(np.float32)
+        kc, vc = cache_of(rng, b, kv_heads, hd, "bf16")
+        d = Held(ctx, b, kc, vc, "bf16", kv_heads, hd)
+        dq, out = d.up(q), d.up(np.zeros_like(q))
+        ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
+        bound = attention_bound(ref, mag, top, hd, "f32")
+
+        def call():
+            ops.paged_attention(d.kv, d.batch, dq, heads * hd, out, heads * hd, "f32", heads)
+        say("a caller stream")
+        call()
+        ctx.graph_begin()
+        call()
+        g = ctx.graph_end()
+        for _ in range(3):
+            ctx.sync()
+            check_close(out.download(np.float32).reshape(-1, heads, hd).astype(np.float64), ref, bound, "f32")
+            out.upload(np.zeros_like(q))
+            g.launch()
+        ctx.sync()
+        del g
+        d.free()
+    finally:
+        ctx.lib.m1moe_set_stream(ctx.handle, None)
+        assert hip.hipStreamDestroy(s) == 0
 
 
 # ---- append ------------------------------------------------------------------------------
