@@ -10,11 +10,12 @@ from ._lib import (KVAppend, M1MOE_BF16, M1MOE_F32, M1MoEError, MoEShape, PROJ_D
                    PROJ_UP, PagedBatch, PagedKV, SampleParams, load)
 from .engine import (DeviceBuffer, HIPContext, MoEBlock, ModelSpec, check_shape, expert_bytes,
                      expert_offsets, make_shape)
-from .decoder import AttentionSpec, Decoder, DecoderSpec, DenseOps
+from .decoder import AttentionSpec, Decoder, DecoderSpec, DenseOps, rope_frequencies
 
 __all__ = [
     "M1MOE_BF16", "M1MOE_F32", "M1MoEError", "MoEShape", "PROJ_DOWN", "PROJ_GATE", "PROJ_UP",
     "load", "DeviceBuffer", "HIPContext", "MoEBlock", "ModelSpec", "check_shape",
     "expert_bytes", "expert_offsets", "make_shape", "AttentionSpec", "Decoder", "DecoderSpec",
     "DenseOps", "KVAppend", "PagedBatch", "PagedKV", "SampleParams",
+    "rope_frequencies",
 ]

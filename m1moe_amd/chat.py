@@ -1,7 +1,8 @@
 """Interactive multi-turn chat over the decoder (Sources/chat/main.swift).
 
   python -m m1moe_amd.chat --config PATH [--model DIR] [--system TEXT]
-                           [--temp T] [--top-p P] [--max-ctx N]
+                           [--temp T] [--top-p P] [--top-k K] [--min-p P]
+                           [--max-ctx N]
 
 Commands during chat: /reset, /system TEXT, /stats, /quit (also /exit, /q).
 
@@ -21,7 +22,8 @@ What differs is where the work runs: every prefill (system prompt, user
 turn, assistant prefix and suffix, the re-prefill after a trim) is one
 batched m1moe_dec_prefill on the GPU instead of one forward per token, and
 each generated token is one m1moe_dec_step (greedy on the GPU at
-temperature 0, else sampled on the host from its logits).
+temperature 0, else sampled on the host from its logits; with --top-k or
+--min-p, which the reference does not have, on the GPU).
 """
 from __future__ import annotations
 
@@ -80,9 +82,10 @@ def split_command(text: str):
 class DecoderEngine:
     """InferenceEngine's forward / reset over a Decoder, with batched prefill."""
 
-    def __init__(self, decoder, seed: Optional[int] = None):
+    def __init__(self, decoder, seed: Optional[int] = None, top_k: int = 0, min_p: float = 0.0):
         self.dec = decoder
         self.rng = np.random.default_rng(seed)
+        self.more = dict(top_k=int(top_k), min_p=float(min_p)) if top_k > 0 or min_p > 0 else {}
 
     def reset(self) -> None:
         self.dec.reset()
@@ -93,7 +96,7 @@ class DecoderEngine:
 
     def forward(self, token: int, temperature: float, top_p: float) -> int:
         return int(self.dec.forward(int(token), temperature=temperature, top_p=top_p,
-                                    rng=self.rng))
+                                    rng=self.rng, **self.more))
 
 
 class ChatSession:
@@ -233,6 +236,8 @@ M1MoE chat — interactive multi-turn conversation
 --system  TEXT   System prompt text
 --temp    T      Sampling temperature (default: 0.7)
 --top-p   P      Nucleus threshold (default: 0.9)
+--top-k   K      Most likely tokens to draw from (default: all)
+--min-p   P      Least probability, as a share of the largest (default: 0)
 --max-ctx N      Max context tokens before sliding window (default: 2048)
 
 During chat:
@@ -246,9 +251,10 @@ def parse_args(argv: Sequence[str]) -> dict:
     """The reference's argument loop (:24-56): a flag whose value is missing
     or does not parse is skipped and the value is read as the next flag."""
     a = {"config": None, "model": None, "system": None, "temp": 0.7, "top_p": 0.9,
-         "max_ctx": 2048, "help": False}
+         "top_k": 0, "min_p": 0.0, "max_ctx": 2048, "help": False}
     rest = list(argv)
-    conv = {"--temp": ("temp", float), "--top-p": ("top_p", float), "--max-ctx": ("max_ctx", int),
+    conv = {"--temp": ("temp", float), "--top-p": ("top_p", float), "--top-k": ("top_k", int),
+            "--min-p": ("min_p", float), "--max-ctx": ("max_ctx", int),
             "--config": ("config", str), "--model": ("model", str), "--system": ("system", str)}
     while rest:
         f = rest.pop(0)
@@ -342,7 +348,8 @@ def serve(config: dict, model_dir: str, args: dict, stdin, stdout) -> ChatSessio
                 system = f.read().strip(_WHITESPACE + _NEWLINES)
             stdout.write(f"[chat] system prompt loaded from ~/.m1moe/system.md "
                          f"({len(system)} chars)\n")
-        session = ChatSession(DecoderEngine(dec), tok, chat_template(config),
+        engine = DecoderEngine(dec, top_k=args.get("top_k", 0), min_p=args.get("min_p", 0.0))
+        session = ChatSession(engine, tok, chat_template(config),
                               st.get("eos", []), int(st.get("bos", 1)), args["temp"],
                               args["top_p"], args["max_ctx"], out=stdout)
         session.start(system)

@@ -109,6 +109,34 @@ def weight_count(which: int, hidden: int, s: DecShape) -> int:
             W_K_NORM: s.head_dim}[which]
 
 
+def rope_frequencies(theta: float, rotary_dim: int, factor: float = 1.0, kind: str = "parts",
+                     trained_len: int = 0, slow: float = 1.0, fast: float = 32.0):
+    """(inv_freq f32 [rotary_dim / 2], amplitude) for KVAppend: theta^(-2i / rotary_dim),
+    for contexts `factor` times the trained one: "linear" divides every frequency by it,
+    "base" raises theta so that only the slowest pair's is, "parts" divides those of pairs
+    with at most `slow` turns over trained_len positions, keeps those with `fast` or more,
+    blends between, and scales cos and sin by 0.1 ln(factor) + 1."""
+    if rotary_dim <= 0 or rotary_dim % 2 or not theta > 0 or not factor >= 1:
+        raise ValueError(f"rotary_dim {rotary_dim} / theta {theta} / factor {factor}: need an even "
+                         "positive rotary_dim, theta > 0 and factor >= 1")
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    if kind == "base":
+        if rotary_dim > 2:
+            theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+        return (theta ** (-2 * i / rotary_dim)).astype(np.float32), 1.0
+    f = theta ** (-2 * i / rotary_dim)
+    if kind == "linear":
+        return (f / factor).astype(np.float32), 1.0
+    if kind != "parts":
+        raise ValueError(f"unknown kind {kind!r}: linear, base or parts")
+    if factor == 1:
+        return f.astype(np.float32), 1.0
+    if trained_len <= 0 or not 0 <= slow < fast:
+        raise ValueError("kind \"parts\" needs trained_len > 0 and 0 <= slow < fast")
+    keep = np.clip((trained_len * f / (2 * np.pi) - slow) / (fast - slow), 0, 1)
+    return (f * keep + f / factor * (1 - keep)).astype(np.float32), 0.1 * float(np.log(factor)) + 1
+
+
 class DenseOps:
     """The dense kernels one by one (asynchronous on the context stream)."""
 
@@ -172,6 +200,7 @@ class Decoder:
         self.handle = h
         self._tok = ctx.alloc(16)     # token in/out of forward()
         self._logits = ctx.alloc(4 * shape.vocab)
+        self._draw = ctx.alloc(32)    # a sampled step's settings and random number
 
     def close(self) -> None:
         if self.handle:
@@ -261,16 +290,65 @@ class Decoder:
         seq.free()
         return out
 
+    def _sample_params(self, buf: DeviceBuffer, u, temperature, top_k, top_p, min_p):
+        """Copies n draws and the settings (one each) to buf, 4 + n words; what makes
+        SampleParams of draw i."""
+        words = np.zeros(4 + np.size(u), np.float32)
+        words[:4] = [temperature, 0, top_p, min_p]
+        words[1:2].view(np.int32)[0] = top_k
+        words[4:] = u
+        at = buf.upload(words).addr
+        return lambda i: SampleParams.make(at + 16 + 4 * i, at, at + 4, at + 8, at + 12)
+
+    def generate_sampled(self, prompt, n_gen: int, temperature: float, top_p: float = 1.0,
+                         top_k: int = 0, min_p: float = 0.0, u=None,
+                         rng: Optional[np.random.Generator] = None):
+        """generate() with every token drawn on the GPU (m1moe_sample) from the
+        n_gen + 1 uniform numbers u (from rng when None): the prompt in one batch, then
+        a step per token, and no host round trip between them."""
+        prompt = np.ascontiguousarray(prompt, dtype=np.int32)
+        n, V = n_gen + 1, self.shape.vocab
+        if u is None:
+            u = (rng or np.random.default_rng()).random(n, dtype=np.float32)
+        if np.size(u) != n:
+            raise ValueError(f"{np.size(u)} random numbers for {n} tokens")
+        ops = DenseOps(self.ctx)
+        buf = self.ctx.alloc(4 * (4 + n))
+        params = self._sample_params(buf, u, temperature, top_k, top_p, min_p)
+        toks, d = self.ctx.alloc(4 * n), self.ctx.to_device(prompt)
+        self.reset()
+        self.prefill_device(d, prompt.size, self._tok, self._logits)
+        for i in range(n):
+            if i:
+                self.step_device(toks.addr + 4 * (i - 1), self._tok, self._logits)
+            ops.sample(self._logits, 1, V, (V + 3) // 4 * 4, params(i), toks.addr + 4 * i)
+        self.ctx.sync()
+        out = toks.download(np.int32)
+        for b in (buf, toks, d):
+            b.free()
+        return out
+
     def forward(self, token: int, return_logits: bool = False, temperature: float = 0.0,
-                top_p: float = 1.0, rng: Optional[np.random.Generator] = None):
+                top_p: float = 1.0, rng: Optional[np.random.Generator] = None, top_k: int = 0,
+                min_p: float = 0.0):
         """InferenceEngine.forward(token:temperature:topP:) (:125-156): the next
         token — greedy on the GPU at temperature <= 0, else sampled on the host
         from the step's logits as the reference does (sampling.sample_token) —
-        and the f32 logits when asked."""
+        and the f32 logits when asked.  With top_k or min_p, which the reference
+        does not have, the token is drawn on the GPU (m1moe_sample) and only it
+        is read back."""
         self._tok.upload(np.array([token, 0, 0, 0], dtype=np.int32))
         self.step_device(self._tok, self._tok, self._logits)
-        self.ctx.sync()
         logits = None
+        if temperature > 0 and (top_k > 0 or min_p > 0):
+            V = self.shape.vocab
+            u = (rng or np.random.default_rng()).random(1, dtype=np.float32)
+            params = self._sample_params(self._draw, u, temperature, top_k, top_p, min_p)
+            DenseOps(self.ctx).sample(self._logits, 1, V, (V + 3) // 4 * 4, params(0), self._tok)
+            self.ctx.sync()
+            nxt = int(self._tok.download(np.int32, 1)[0])
+            return (nxt, self._logits.download(np.float32, V)) if return_logits else nxt
+        self.ctx.sync()
         if temperature > 0:
             logits = self._logits.download(np.float32, self.shape.vocab)
             nxt = sample_token(logits, temperature, top_p, rng=rng)
@@ -283,5 +361,5 @@ class Decoder:
         return nxt
 
 
-__all__ = ["AttentionSpec", "DecoderSpec", "DenseOps", "Decoder", "DeviceBuffer",
+__all__ = ["rope_frequencies", "AttentionSpec", "DecoderSpec", "DenseOps", "Decoder", "DeviceBuffer",
            "WEIGHT_NAMES", "weight_count"]

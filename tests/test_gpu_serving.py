@@ -962,3 +962,45 @@ def test_a_batch_decodes_step_by_step(dev):
         assert tokens.tolist() == want
     assert b.kv_len.tolist() == ends
     d.free()
+
+
+# ---- the decoder's sampler -----------------------------------------------------------------
+
+def test_decoder_draws_on_the_gpu():
+    """generate_sampled and forward with top_k / min_p give the tokens that the f64
+    sampler draws from the same steps' logits."""
+    from m1moe_amd.decoder import Decoder
+    wl = synth.DECODERS["tiny_dec"]
+    L, seed = wl.num_layers, 78
+    shape = wl.moe.shape(L)
+    with m.HIPContext(shape) as ctx:
+        for layer in range(L):
+            ctx.upload_layer_experts(layer, synth.layer_image(shape, seed, layer))
+            ctx.upload_router(layer, synth.router(shape, seed, layer))
+        dec = Decoder(ctx, wl.dec_shape(64))
+        dec.upload_all(lambda w, layer: synth.dense_weight(wl, seed, w, layer))
+        rng = np.random.default_rng(51)
+        prompt, n = rng.integers(0, wl.vocab, 11), 12
+        u = rng.random(n + 1).astype(np.float32)
+        for k in (dict(temperature=0.9, top_p=0.95, top_k=20, min_p=0.01), dict(temperature=1.3), dict(temperature=0.0)):
+            say(f"decoder draws {k}")
+            got = dec.generate_sampled(prompt, n, u=u, **k)
+            dec.reset()
+            _, logits = dec.prefill(prompt, return_logits=True)
+            for i in range(n + 1):
+                want, _ = sample_ref(logits, u[i], k["temperature"], k.get("top_k", 0), k.get("top_p", 1.0),
+                                     k.get("min_p", 0.0))
+                assert got[i] == want, (k, i)
+                if i < n:
+                    _, logits = dec.forward(int(got[i]), return_logits=True)
+        dec.reset()
+        r1, r2 = np.random.default_rng(5), np.random.default_rng(5)
+        tok = 3
+        for _ in range(4):
+            nxt, logits = dec.forward(tok, return_logits=True, temperature=0.8, top_p=0.9, rng=r1, top_k=30, min_p=0.02)
+            want, _ = sample_ref(logits, r2.random(1, dtype=np.float32)[0], 0.8, 30, 0.9, 0.02)
+            assert nxt == want
+            tok = nxt
+        with pytest.raises(ValueError):
+            dec.generate_sampled(prompt, 3, 1.0, u=u)
+        dec.close()
