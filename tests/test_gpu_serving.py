@@ -491,13 +491,13 @@ def test_attention_scratch_grows_between_captures():
     ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
     bound = attention_bound(ref, mag, top, hd, "f32")
     check_close(out.download(np.float32).reshape(2, heads, hd).astype(np.float64), ref, bound, "f32")
-    b2 = Batch(rng, [400], [100], 16, prefix=64)
-    q2 = rng.normal(0, 1, (400, heads * hd)).astype(np.float32)
-    k2, v2 = cache_of(rng, b2, kv_heads, hd, "f32")
-    d2 = Held(ctx, b2, k2, v2, "f32", kv_heads, hd)
+    b2 = Batch(rng, [40], [100], 16, prefix=64)
+    q2 = rng.normal(0, 1, (40, heads * 256)).astype(np.float32)
+    k2, v2 = cache_of(rng, b2, kv_heads, 256, "f32")
+    d2 = Held(ctx, b2, k2, v2, "f32", kv_heads, 256)
     o2 = d2.up(np.zeros_like(q2))
     say("the partials grow")
-    ops.paged_attention(d2.kv, d2.batch, d2.up(q2), heads * hd, o2, heads * hd, "f32", heads)
+    ops.paged_attention(d2.kv, d2.batch, d2.up(q2), heads * 256, o2, heads * 256, "f32", heads)
     ctx.sync()
     with pytest.raises(M1MoEError) as e:
         g.launch()
@@ -506,9 +506,9 @@ def test_attention_scratch_grows_between_captures():
     call()
     ctx.sync()
     check_close(out.download(np.float32).reshape(2, heads, hd).astype(np.float64), ref, bound, "f32")
-    ref, mag, top = attention_ref(b2, q2, k2, v2, heads, kv_heads, hd)
-    check_close(o2.download(np.float32).reshape(400, heads, hd).astype(np.float64), ref,
-                attention_bound(ref, mag, top, hd, "f32"), "f32")
+    ref, mag, top = attention_ref(b2, q2, k2, v2, heads, kv_heads, 256)
+    check_close(o2.download(np.float32).reshape(40, heads, 256).astype(np.float64), ref,
+                attention_bound(ref, mag, top, 256, "f32"), "f32")
     del g
     d.free()
     d2.free()
