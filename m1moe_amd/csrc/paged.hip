@@ -900,33 +900,105 @@ struct Deep : Rows<HD, QP, 1, true> {
     }
 };
 
-// Many rows: the waves hold 16 NT rows each and share the keys, staged through LDS
-// in pieces of SK: K row by row (its bf16 parts), V transposed, eight keys of a
-// dim together, both in 16-byte units placed so that the eight lanes an LDS read
-// serves at once find theirs in different banks.  Each thread has 16 bytes of K at a
-// time (a position's neighbouring dims) and 64 of V (VB dims of eight positions).
-// The next piece is on its way into registers while one is computed, the page numbers
-// of the one after with it (lane l: of the piece's keys 8 (l % 16) ..).  The eight
-// positions that share a page number are the same for a whole wave, of K at every
-// load, so that a load's address is one scalar base and a lane's constant offset.
+// Many rows: the waves hold 16 NT rows each and share the keys, staged through LDS in
+// pieces of SK.  The page numbers of the piece after the next are looked up while one
+// is computed (lane l: of the piece's keys 8 (l % 16) ..).  The eight positions that share
+// a page number are the same for a whole wave at every load, so that a load's address is
+// one scalar base and a lane's constant offset.
 template <int HD, int KP>
-struct Stage {
-    static constexpr int SK = KP == 1 ? 8192 / HD : HD <= 128 ? 4096 / HD : 32;   // keys
+struct Stage;
+
+// A bf16 cache: K and V row by row as the cache has them, copied by the loads themselves
+// (no registers, no vector instruction), V's operands (eight keys of a dim) made by LDS reads
+// that transpose, 4 keys x 16 dims at a time in 16 lanes.  A row's 16-byte units are placed
+// so that the eight lanes of a K read, or the 32-byte pairs of the eight rows of 32 lanes
+// of a V read, find theirs in different banks: the lane that copies a place takes the
+// unit that belongs there.
+template <int HD>
+struct Stage<HD, 1> {
+    static constexpr int SK = 8192 / HD;                  // keys
+    static constexpr int KU = HD / 8;                     // 16-byte units of a row
+    static constexpr int kPlane = SK * HD * 2;            // bytes of K, of V
+    static constexpr int kBytes = 2 * kPlane;
+    static constexpr int kBuffers = 2;
+    static constexpr int N = SK * KU / 256, KS = 256 / KU;   // copies of K (and V), positions of one
+    static_assert(SK % 32 == 0 && SK <= 128 && N >= 1, "a piece is whole 32-key blocks");
+    int pages, t, wave;
+    uint32_t off, k_unit, v_unit;   // the lane's position in the wave's, its units at it, in bytes
+
+    __device__ __forceinline__ static constexpr int k_turn(int key) {
+        return ((key & 3) | ((key >> 3) & 3) << 2) & (KU - 1);
+    }
+    __device__ __forceinline__ static constexpr int v_turn(int key) {   // of pairs
+        return HD == 64 ? ((key >> 1) & 1) | ((key >> 3) & 1) << 1 : (key & 3) | ((key >> 3) & 1) << 2;
+    }
+    __device__ __forceinline__ static int k_at(int key, int unit) { return (key * KU + (unit ^ k_turn(key))) * 16; }
+    // Of the wave's keys key0 + 8 g .. + 7, dims 16 j + c.
+    __device__ __forceinline__ static bf16x8 v_operand(const uint8_t* v, int key0, int j, int g, int c) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) s16x4* lds_p;
+        const int key = 8 * g + (c >> 2);
+        const uint8_t* at = v + key0 * HD * 2 + key * HD * 2 + 32 * (j ^ v_turn(key)) + 8 * (c & 3);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)at);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(at + 4 * HD * 2));
+        return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    __device__ __forceinline__ void init(const Cache<HD, 1>& kv) {
+        t = thread_id();
+        wave = __builtin_amdgcn_readfirstlane(t >> 6);
+        const int key = t / KU;
+        off = (uint32_t)(key - 64 * wave / KU) * kv.row;
+        k_unit = 16 * (t % KU ^ k_turn(key));
+        v_unit = 16 * (t % KU ^ 2 * v_turn(key));
+    }
+    __device__ __forceinline__ void look(const Cache<HD, 1>& kv, int kb) {
+        pages = kv.page_of(kb + 8 * (t & 15) % SK);
+    }
+    // The piece at kb, by its pages, to the buffer s: on its way until waited for.
+    __device__ __forceinline__ void load(const Cache<HD, 1>& kv, int kb, uint8_t* s, bool& bad) {
+        // (lane l: where the group l % 16 of eight positions begins)
+        const int64_t at = kv.at(kv.known(pages, bad), kb + 8 * (t & 15) % SK);
+        const uint32_t lds = lds_addr(s) + 1024 * wave;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int key = 64 * wave / KU + n * KS;   // the wave's first; (the lane's: its own turn, n's added)
+            const int64_t base = Tile::lane64(at, key >> 3) + (uint32_t)(key & 7) * kv.row;
+            lds_copy16(off + (k_unit ^ 16 * k_turn(n * KS)), kv.k + base, lds + 4096 * n);
+            lds_copy16(off + (v_unit ^ 32 * v_turn(n * KS)), kv.v + base, lds + kPlane + 4096 * n);
+        }
+    }
+    // V's rows of the piece at kb (there, as far as the thread copied it) that are not
+    // readable: 0
+    __device__ __forceinline__ void clear_v(const Cache<HD, 1>& kv, int kb, uint8_t* s) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (!kv.readable(kb + t / KU + n * KS))
+                *reinterpret_cast<uint4*>(s + kPlane + 16 * t + 4096 * n) = make_uint4(0, 0, 0, 0);
+    }
+};
+
+// An f32 cache: K row by row as bf16 parts, V's parts transposed, eight keys of a dim
+// together, both in 16-byte units placed so that the eight lanes an LDS read serves at
+// once find theirs in different banks.  Each thread has 16 bytes of K at a time (a
+// position's neighbouring dims) and VB dims of eight positions of V; the next piece is on
+// its way into registers while one is computed.
+template <int HD>
+struct Stage<HD, 3> {
+    static constexpr int SK = HD <= 128 ? 4096 / HD : 32;   // keys
     static constexpr int KU = HD / 8, VU = SK / 8;        // units of a K row, of a V row
     static constexpr int kPlane = SK * HD * 2;            // bytes of a part
-    static constexpr int kBytes = 2 * KP * kPlane;
-    static constexpr int kBuffers = KP == 1 ? 2 : 1;
-    static constexpr int ES = KP == 1 ? 2 : 4;
-    static constexpr int VB = KP == 1 ? 4 : HD * SK / 2048;     // dims of a thread's V block: 4 or 2
+    static constexpr int kBytes = 6 * kPlane;
+    static constexpr int kBuffers = 1;
+    static constexpr int VB = HD * SK / 2048;                   // dims of a thread's V block: 4 or 2
     static constexpr int NV = SK * HD / 8 / VB / 256;           // blocks of a thread
-    static constexpr int CU = HD * ES / 16;                     // 16-byte units of a position in the cache
+    static constexpr int CU = HD / 4;                           // 16-byte units of a position in the cache
     static constexpr int NK = SK * CU / 256;                    // loads of K
     static_assert(SK % 32 == 0 && SK <= 128 && NV >= 1 && NK >= 1, "a piece is whole 32-key blocks");
-    static constexpr int VW = VB * ES / 4;                      // words of a position's in it
-    typedef uint32_t vblock __attribute__((ext_vector_type(VW)));
+    typedef float vblock __attribute__((ext_vector_type(VB)));
     f32x4v kr[NK];
-    uint32_t vr[NV][8][VW];
-    int pages;                                            // lane l: of group l % 16
+    float vr[NV][8][VB];
+    int pages;
     // the thread, its wave, its offsets in a position of K and of V
     int t, wave;
     uint32_t k_off, v_off;
@@ -940,22 +1012,17 @@ struct Stage {
         return (d * VU + (unit ^ (z & (VU - 1)))) * 16;
     }
     static constexpr int KS = 256 / CU;                   // positions of K the threads load at once
-    __device__ __forceinline__ void init(const Cache<HD, KP>& kv) {
+    __device__ __forceinline__ void init(const Cache<HD, 3>& kv) {
         t = thread_id();
         wave = __builtin_amdgcn_readfirstlane(t >> 6);
         k_off = (uint32_t)(t / CU - 64 * wave / CU) * kv.row + 16 * (t % CU);
-        v_off = (uint32_t)(ES * VB * (t % (HD / VB)));
+        v_off = (uint32_t)(4 * VB * (t % (HD / VB)));
     }
-    __device__ __forceinline__ void look(const Cache<HD, KP>& kv, int kb) {
+    __device__ __forceinline__ void look(const Cache<HD, 3>& kv, int kb) {
         pages = kv.page_of(kb + 8 * (t & 15) % SK);
     }
-    __device__ __forceinline__ static void get(uint32_t (&to)[VW], const uint8_t* x) {
-        const vblock v = *reinterpret_cast<const vblock*>(x);
-#pragma unroll
-        for (int i = 0; i < VW; ++i) to[i] = v[i];
-    }
     // The piece at kb, by its pages.
-    __device__ __forceinline__ void load(const Cache<HD, KP>& kv, int kb, bool& bad) {
+    __device__ __forceinline__ void load(const Cache<HD, 3>& kv, int kb, bool& bad) {
         // (lane l: where the group l % 16 of eight positions begins)
         const int64_t at = kv.at(kv.known(pages, bad), kb + 8 * (t & 15) % SK);
         const int key0 = 64 * wave / CU;   // the wave's first position of K
@@ -965,6 +1032,7 @@ struct Stage {
             kr[n] = *reinterpret_cast<const f32x4v*>(kv.k + (Tile::lane64(at, key >> 3) + (uint32_t)(key & 7) * kv.row) + k_off);
         }
         constexpr int kGroups = 64 * VB / HD > 1 ? 64 * VB / HD : 1;   // a wave's V blocks lie in so many
+        static_assert(kGroups <= 2, "one group or two");
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int grp = (64 * wave + 256 * n) / (HD / VB);
@@ -972,70 +1040,53 @@ struct Stage {
             if (kGroups == 2) {
                 const int64_t other = Tile::lane64(at, grp + 1);
                 base = (t & 63) >= HD / VB ? other : base;
-            } else if (kGroups > 2) {
-                const int mine = (t + 256 * n) / (HD / VB);
-                base = (int64_t)((uint64_t)(uint32_t)__shfl((int)(at >> 32), mine) << 32 |
-                                 (uint32_t)__shfl((int)at, mine));
             }
             const uint8_t* x = kv.v + base + v_off;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                get(vr[n][e], x);
+                const vblock v = *reinterpret_cast<const vblock*>(x);
+#pragma unroll
+                for (int i = 0; i < VB; ++i) vr[n][e][i] = v[i];
                 x += kv.row;
             }
         }
     }
     // V's rows of the piece at kb that are not readable: 0
-    __device__ __forceinline__ void clear_v(const Cache<HD, KP>& kv, int kb) {
+    __device__ __forceinline__ void clear_v(const Cache<HD, 3>& kv, int kb) {
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const bool in = kv.readable(kb + (t + 256 * n) / (HD / VB) * 8 + e);
 #pragma unroll
-                for (int i = 0; i < VW; ++i) vr[n][e][i] = in ? vr[n][e][i] : 0u;
+                for (int i = 0; i < VB; ++i) vr[n][e][i] = in ? vr[n][e][i] : 0.f;
             }
-    }
-    __device__ __forceinline__ static void put(uint8_t* s, const Parts8& p) {
-        *reinterpret_cast<bf16x8*>(s) = p.h;
-        *reinterpret_cast<bf16x8*>(s + kPlane) = p.m;
-        *reinterpret_cast<bf16x8*>(s + 2 * kPlane) = p.l;
     }
     __device__ __forceinline__ void store(uint8_t* s) const {
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
+        for (int n = 0; n < NK; ++n) {   // (half a unit of each part)
             const int key = t / CU + n * KS, unit = t % CU;
-            if constexpr (KP == 1) {
-                *reinterpret_cast<f32x4v*>(s + k_at(key, unit)) = kr[n];
-            } else {   // (half a unit of each part)
-                uint2 h, m, l;
-                parts4(kr[n], h, m, l);
-                uint8_t* at = s + k_at(key, unit >> 1) + 8 * (unit & 1);
-                *reinterpret_cast<uint2*>(at) = h;
-                *reinterpret_cast<uint2*>(at + kPlane) = m;
-                *reinterpret_cast<uint2*>(at + 2 * kPlane) = l;
-            }
+            uint2 h, m, l;
+            parts4(kr[n], h, m, l);
+            uint8_t* at = s + k_at(key, unit >> 1) + 8 * (unit & 1);
+            *reinterpret_cast<uint2*>(at) = h;
+            *reinterpret_cast<uint2*>(at + kPlane) = m;
+            *reinterpret_cast<uint2*>(at + 2 * kPlane) = l;
         }
-        uint8_t* sv = s + KP * kPlane;
+        uint8_t* sv = s + 3 * kPlane;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int b = t + 256 * n, grp = b / (HD / VB), d = VB * (b % (HD / VB));
 #pragma unroll
             for (int i = 0; i < VB; ++i) {
-                const int at = v_at(d + i, grp);
-                if constexpr (KP == 1) {
-                    uint32_t o[4];
+                float y[8];
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        o[y] = __builtin_amdgcn_perm(vr[n][2 * y + 1][i >> 1], vr[n][2 * y][i >> 1],
-                                                     i & 1 ? 0x07060302u : 0x05040100u);
-                    *reinterpret_cast<uint4*>(sv + at) = make_uint4(o[0], o[1], o[2], o[3]);
-                } else {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(vr[n][e][i]);
-                    put(sv + at, parts8(y));
-                }
+                for (int e = 0; e < 8; ++e) y[e] = vr[n][e][i];
+                const Parts8 p = parts8(y);
+                uint8_t* at = sv + v_at(d + i, grp);
+                *reinterpret_cast<bf16x8*>(at) = p.h;
+                *reinterpret_cast<bf16x8*>(at + kPlane) = p.m;
+                *reinterpret_cast<bf16x8*>(at + 2 * kPlane) = p.l;
             }
         }
     }
@@ -1084,9 +1135,13 @@ struct Wide : Rows<HD, QP, NT, false> {
 #pragma unroll
                 for (int j = 0; j < JG; ++j)
 #pragma unroll
-                    for (int y = 0; y < KP; ++y)
-                        x[j][y] = *reinterpret_cast<const bf16x8*>(
-                            s_kv + (KP + y) * S::kPlane + S::v_at(16 * (j0 + j) + c, 4 * (b0 + b) + g));
+                    for (int y = 0; y < KP; ++y) {
+                        if constexpr (KP == 1)
+                            x[j][y] = S::v_operand(s_kv + S::kPlane, 32 * (b0 + b), j0 + j, g, c);
+                        else
+                            x[j][y] = *reinterpret_cast<const bf16x8*>(
+                                s_kv + (KP + y) * S::kPlane + S::v_at(16 * (j0 + j) + c, 4 * (b0 + b) + g));
+                    }
                 this->template values<KP>(x, j0, pp[b]);
             }
         __builtin_amdgcn_s_setprio(0);
@@ -1099,23 +1154,40 @@ struct Wide : Rows<HD, QP, NT, false> {
         S st;
         st.init(kv);
         st.look(kv, w.lo);
-        st.load(kv, w.lo, bad);
-        if (w.lo + S::SK < w.hi) st.look(kv, w.lo + S::SK);
-        int turn = 0;
-        for (int k0 = w.lo; k0 < w.hi; k0 += S::SK) {
-            uint8_t* buf = s_kv + turn * S::kBytes;
-            if (S::kBuffers == 1) __syncthreads();
-            if (kv.edge(k0, S::SK)) st.clear_v(kv, k0);
-            st.store(buf);
-            __syncthreads();   // (with two buffers the other one is still read before it)
-            if (k0 + S::SK < w.hi) {
-                st.load(kv, k0 + S::SK, bad);
-                if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
-            }
+        if constexpr (KP == 1) {
+            st.load(kv, w.lo, s_kv, bad);
+            if (w.lo + S::SK < w.hi) st.look(kv, w.lo + S::SK);
+            int turn = 0;
+            for (int k0 = w.lo; k0 < w.hi; k0 += S::SK) {
+                uint8_t* buf = s_kv + turn * S::kBytes;
+                turn ^= 1;
+                wait_vm<0>();
+                if (kv.edge(k0, S::SK)) st.clear_v(kv, k0, buf);
+                __syncthreads();   // (the piece is there, and the other buffer read)
+                if (k0 + S::SK < w.hi) {
+                    st.load(kv, k0 + S::SK, s_kv + turn * S::kBytes, bad);
+                    if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
+                }
 #pragma unroll
-            for (int b = 0; b < S::SK / 32; b += NB)
-                if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, buf);
-            if (S::kBuffers == 2) turn ^= 1;
+                for (int b = 0; b < S::SK / 32; b += NB)
+                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, buf);
+            }
+        } else {
+            st.load(kv, w.lo, bad);
+            if (w.lo + S::SK < w.hi) st.look(kv, w.lo + S::SK);
+            for (int k0 = w.lo; k0 < w.hi; k0 += S::SK) {
+                __syncthreads();
+                if (kv.edge(k0, S::SK)) st.clear_v(kv, k0);
+                st.store(s_kv);
+                __syncthreads();
+                if (k0 + S::SK < w.hi) {
+                    st.load(kv, k0 + S::SK, bad);
+                    if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
+                }
+#pragma unroll
+                for (int b = 0; b < S::SK / 32; b += NB)
+                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, s_kv);
+            }
         }
         if (bad) flag_error(p.err, kErrPagedPage);
 #pragma unroll
