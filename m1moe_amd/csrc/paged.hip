@@ -591,7 +591,10 @@ struct Rows {
     }
 
     // The running softmax over NB blocks of 32 keys from kb on: the scores s become the
-    // weights' operands pp, acc is rescaled where a maximum grew.
+    // weights' operands pp.  m, the score of weight 1, follows the maximum (and acc and l are
+    // rescaled) only where that grew by more than kGrown in the exponent of 2: no weight
+    // is above 2^kGrown, and all are rounded relative to themselves.
+    static constexpr float kGrown = 8.f;
     template <int NB>
     __device__ __forceinline__ void softmax(const Work& w, int kb, f32x4v (&s)[NB][NT][2], float unit,
                                             bf16x8 (&pp)[NB][NT][QP]) {
@@ -620,14 +623,14 @@ struct Rows {
                 bm = fmaxf(fmaxf(bm, y[2]), y[3]);
             }
             const float mn = fmaxf(m[t], quads_max(bm));
-            const float mc = mn == -INFINITY ? 0.f : mn;   // (no key seen yet: all weights 0)
-            if (__any(mn > m[t])) {
-                const float f = weight(m[t] - mc, unit);
+            if (__any((mn - m[t]) * unit > kGrown)) {   // (from -infinity: so it is)
+                const float f = mn == -INFINITY ? 1.f : weight(m[t] - mn, unit);
                 l[t] *= f;
 #pragma unroll
                 for (int j = 0; j < VD; ++j) acc[t][j] *= f;
                 m[t] = mn;
             }
+            const float mc = m[t] == -INFINITY ? 0.f : m[t];   // (no key seen yet: all weights 0)
             // (bf16 queries: one rounding more, of the row's largest exponent, against the 2^-8
             // of the weights)
             const float mu = mc * unit;
@@ -922,7 +925,7 @@ struct Stage<HD, 1> {
     static constexpr int kBytes = 2 * kPlane;
     static constexpr int kBuffers = 2;
     static constexpr int N = SK * KU / 256, KS = 256 / KU;   // copies of K (and V), positions of one
-    static_assert(SK % 32 == 0 && SK <= 128 && N >= 1, "a piece is whole 32-key blocks");
+    static_assert(SK % 32 == 0 && SK <= 128 && N == 4, "a piece is whole 32-key blocks, in quarters");
     int pages, t, wave;
     uint32_t off, k_unit, v_unit;   // the lane's position in the wave's, its units at it, in bytes
 
@@ -955,18 +958,17 @@ struct Stage<HD, 1> {
     __device__ __forceinline__ void look(const Cache<HD, 1>& kv, int kb) {
         pages = kv.page_of(kb + 8 * (t & 15) % SK);
     }
-    // The piece at kb, by its pages, to the buffer s: on its way until waited for.
-    __device__ __forceinline__ void load(const Cache<HD, 1>& kv, int kb, uint8_t* s, bool& bad) {
-        // (lane l: where the group l % 16 of eight positions begins)
-        const int64_t at = kv.at(kv.known(pages, bad), kb + 8 * (t & 15) % SK);
-        const uint32_t lds = lds_addr(s) + 1024 * wave;
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int key = 64 * wave / KU + n * KS;   // the wave's first; (the lane's: its own turn, n's added)
-            const int64_t base = Tile::lane64(at, key >> 3) + (uint32_t)(key & 7) * kv.row;
-            lds_copy16(off + (k_unit ^ 16 * k_turn(n * KS)), kv.k + base, lds + 4096 * n);
-            lds_copy16(off + (v_unit ^ 32 * v_turn(n * KS)), kv.v + base, lds + kPlane + 4096 * n);
-        }
+    // Where the piece at kb is, by its pages (lane l: its group l % 16 of eight positions).
+    __device__ __forceinline__ int64_t places(const Cache<HD, 1>& kv, int kb, bool& bad) const {
+        return kv.at(kv.known(pages, bad), kb + 8 * (t & 15) % SK);
+    }
+    // A quarter of it to the buffer s: on its way until waited for.
+    __device__ __forceinline__ void load(const Cache<HD, 1>& kv, int64_t at, int n, uint8_t* s) {
+        const uint32_t lds = lds_addr(s) + 1024 * wave + 4096 * n;
+        const int key = 64 * wave / KU + n * KS;   // the wave's first; (the lane's: its own turn, n's added)
+        const int64_t base = Tile::lane64(at, key >> 3) + (uint32_t)(key & 7) * kv.row;
+        lds_copy16(off + (k_unit ^ 16 * k_turn(n * KS)), kv.k + base, lds);
+        lds_copy16(off + (v_unit ^ 32 * v_turn(n * KS)), kv.v + base, lds + kPlane);
     }
     // V's rows of the piece at kb (there, as far as the thread copied it) that are not
     // readable: 0
@@ -1100,7 +1102,11 @@ struct Wide : Rows<HD, QP, NT, false> {
     // 32-key blocks a softmax takes at once: two halve its maxima and rescalings
     static constexpr int NB = S::SK >= 64 ? 2 : 1;
 
-    __device__ __forceinline__ void blocks(const Work& w, int kb, int b0, float unit, const uint8_t* s_kv) {
+    // between(i): called in the course of it, i = 0 .. kBreaks - 1
+    static constexpr int kBreaks = NB + 1;
+    template <class F>
+    __device__ __forceinline__ void blocks(const Work& w, int kb, int b0, float unit, const uint8_t* s_kv,
+                                           F&& between) {
         const int g = this->g, c = this->c;
         f32x4v s[NB][NT][2];
         // (the SIMD's other wave's vector work fits between the MFMAs, not they between it)
@@ -1121,10 +1127,12 @@ struct Wide : Rows<HD, QP, NT, false> {
                 R::template scores<KP>(x, [&](int t, int y) { return this->q[t][y][i]; }, part);
             }
             R::total(part, s[b]);
+            between(b);
         }
         __builtin_amdgcn_s_setprio(0);
         bf16x8 pp[NB][NT][QP];
         this->template softmax<NB>(w, kb, s, unit, pp);
+        between(NB);
         __builtin_amdgcn_s_setprio(1);
         constexpr int JG = KP == 1 ? 4 : 2;
 #pragma unroll
@@ -1155,22 +1163,35 @@ struct Wide : Rows<HD, QP, NT, false> {
         st.init(kv);
         st.look(kv, w.lo);
         if constexpr (KP == 1) {
-            st.load(kv, w.lo, s_kv, bad);
+            int64_t at = st.places(kv, w.lo, bad);
+#pragma unroll
+            for (int n = 0; n < S::N; ++n) st.load(kv, at, n, s_kv);
             if (w.lo + S::SK < w.hi) st.look(kv, w.lo + S::SK);
             int turn = 0;
             for (int k0 = w.lo; k0 < w.hi; k0 += S::SK) {
                 uint8_t* buf = s_kv + turn * S::kBytes;
                 turn ^= 1;
+                uint8_t* other = s_kv + turn * S::kBytes;
                 wait_vm<0>();
                 if (kv.edge(k0, S::SK)) st.clear_v(kv, k0, buf);
+                const bool more = k0 + S::SK < w.hi;
+                if (more) at = st.places(kv, k0 + S::SK, bad);
                 __syncthreads();   // (the piece is there, and the other buffer read)
-                if (k0 + S::SK < w.hi) {
-                    st.load(kv, k0 + S::SK, s_kv + turn * S::kBytes, bad);
-                    if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
-                }
+                // the next piece's copies, spread over this one's first blocks
+                const auto rest = [&](int n0, int n1) {
+                    if (!more) return;
 #pragma unroll
-                for (int b = 0; b < S::SK / 32; b += NB)
-                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, buf);
+                    for (int n = 0; n < S::N; ++n)
+                        if (n >= n0 && n < n1) st.load(kv, at, n, other);
+                };
+                const bool on = k0 < hi;
+                rest(0, on ? 1 : S::N);
+                if (on)
+                    blocks(w, k0, 0, unit, buf, [&](int i) { rest(i + 1, i + 1 < kBreaks ? i + 2 : S::N); });
+                if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
+#pragma unroll
+                for (int b = NB; b < S::SK / 32; b += NB)
+                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, buf, [](int) {});
             }
         } else {
             st.load(kv, w.lo, bad);
@@ -1186,7 +1207,7 @@ struct Wide : Rows<HD, QP, NT, false> {
                 }
 #pragma unroll
                 for (int b = 0; b < S::SK / 32; b += NB)
-                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, s_kv);
+                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, s_kv, [](int) {});
             }
         }
         if (bad) flag_error(p.err, kErrPagedPage);
