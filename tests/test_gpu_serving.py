@@ -374,6 +374,35 @@ def test_attention_many_rows_shared_by_workgroups(dev, types, heads, kv_heads, h
 
 
 @pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("slope", [0.02, 0.08, 0.3, -0.3])
+def test_attention_scores_that_rise(dev, types, slope):
+    """Scores that rise (or fall) with the position, by less and by more per block than what
+    a softmax's reference may lag behind its maximum."""
+    ctx, ops = dev
+    rng = np.random.default_rng(67)
+    heads, kv_heads, hd = 4, 2, 64
+    x, cache = types
+    b = Batch(rng, [1, 90], [900, 300], 16)
+    q = as_dtype(np.full((b.T, heads * hd), 0.5) + rng.normal(0, 0.02, (b.T, heads * hd)), x)
+    kc, vc = (rng.normal(0, 0.05, (b.num_pages, 16, kv_heads, hd)) for _ in range(2))
+    for s in range(2):
+        pos = np.arange(int(b.kv_len[s]))
+        pg, sl = b.cell(s, pos)
+        kc[pg, sl] += (pos * slope / 4)[:, None, None]     # (hd 0.5 / sqrt(hd) = 4)
+    kc, vc = as_dtype(kc, cache), as_dtype(vc, cache)
+    d = Held(ctx, b, kc, vc, cache, kv_heads, hd)
+    out = d.up(np.zeros((b.T, heads * hd), np.uint16 if x == "bf16" else np.float32))
+    say(f"attention slope {slope} {types}")
+    ops.paged_attention(d.kv, d.batch, d.up(q), heads * hd, out, heads * hd, x, heads)
+    ctx.sync()
+    got = f64(out.download(np.uint16 if x == "bf16" else np.float32)).reshape(-1, heads, hd)
+    d.free()
+    ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
+    assert np.all(np.isfinite(got))
+    assert np.all(np.abs(got - ref) <= attention_bound(ref, mag, top, hd, x))
+
+
+@pytest.mark.parametrize("types", TYPES)
 def test_attention_infinities_in_pieces(dev, types):
     """An infinity that only some of a row's pieces meet, in the prefix or behind it."""
     ctx, ops = dev
