@@ -48,6 +48,14 @@ __device__ __forceinline__ void store_vec(void* base, int64_t at, const float (&
     }
 }
 
+// q and k of a head are divided by their root mean square (and multiplied by a
+// weight), pairs of their dims are turned by the position's angles, then k and v go
+// to the row's place in the cache, q to its output: every element is read and
+// written once.  Prompts are bound by memory (five of 37 to 1900 tokens, 32 + 2 x 8 heads
+// of 128, bf16: 28.8 us, of which 26.4 at the rate of a large copy), steps by the
+// launch and the chain sequence - page - store (64 tokens 4.3 us; one workgroup for all
+// heads of a row 5.9).
+//
 // Workgroup = (row, a share of its q, k and v heads).  A lane holds VEC
 // neighbouring dims (16 bytes) of a head; the head's sum of squares and, in
 // the half layout, a pair's other dim come from the head's other lanes.  The
@@ -157,6 +165,21 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 }
 
 // ---- attention -----------------------------------------------------------------------
+//
+// out = sum_p e^(s_p - m) v_p / sum_p e^(s_p - m), s_p = q . k_p / sqrt(head_dim), over the
+// positions p up to the row's own, in one pass over them with a running m.  Scores and
+// weighted sums are MFMAs of bf16 operands with f32 sums.  bf16 queries and
+// cache: the weights are rounded to bf16 (their sum is not), as v is.  f32 ones are taken
+// apart into three bf16 parts, whose products down to 2^-16 of the largest are formed, so
+// that the result is as good as f32 arithmetic's.
+//
+// Steps are bound by reading the cache once (32 heads over 8, f32 queries, bf16 cache:
+// 32 tokens behind 60 to 8100 positions 80.6 us, 4.5 TB/s; 16 heads, all bf16: 48 behind
+// 100 to 4000 117 us, 4.8 TB/s), prompts and turns by a SIMD's two waves, whose MFMAs,
+// softmax and LDS reads overlap only in part (2500 positions, all bf16: 84 us, 608 TFLOP/s;
+// six turns of 9 to 400 tokens behind up to 4000, f32 queries: 73 us, of which 55 are
+// the three products at a large matrix product's rate), one token behind few positions by
+// the chain launch - lengths - page - rows - join (14.8 us).
 
 // f32 values as three bf16 parts, each rounded to nearest, that add up to them
 // exactly (24 bits), a pair at a time.  The rest of a pair is two v_dot2, (hi0, hi1) .
@@ -230,7 +253,9 @@ constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 // queries, the first page and rows one after the other, the waves' join) and one
 // place per key; the line is cut into equal shares, one per workgroup, the cuts
 // moved down to a multiple of kCut keys inside their tile, or to its start where it has
-// at most kWhole keys (to join two pieces of one takes longer than to read it).  (Without the places
+// at most kWhole keys: to join two pieces of one takes longer than to read it (a prompt of
+// 2500 and turns behind up to 4000: 104 and 88 us with every tile cut, 98 and 79 with
+// 512 whole; as they are now, 84.2 and 73.2, with 768 whole 87.2 and 83.5).  (Without the places
 // per tile the workgroups with the shortest sequences ended last: 32 steps of 60 to
 // 8100 positions, 8 kv heads, median 61 us, last 116.)
 struct Tile {
@@ -794,7 +819,8 @@ struct Deep : Rows<HD, QP, 1, true> {
     }
     // (the queries are read before the first block's rows and split while those are on
     // their way: loads come back in their order)
-    // s_q: LDS of the wave's own, kQueries bytes.
+    // s_q: LDS of the wave's own, kQueries bytes: beside the rows of an f32 cache the queries'
+    // parts leave too few registers for two workgroups per CU (104 spilled).
     static constexpr int kQueries = KP == 1 ? 0 : QP * NS * 1024;
     __device__ __forceinline__ void run(const PagedAttnArgs& a, const Work& w, int lo, int step, float unit,
                                         uint8_t* s_q) {
@@ -916,7 +942,8 @@ struct Stage;
 // that transpose, 4 keys x 16 dims at a time in 16 lanes.  A row's 16-byte units are placed
 // so that the eight lanes of a K read, or the 32-byte pairs of the eight rows of 32 lanes
 // of a V read, find theirs in different banks: the lane that copies a place takes the
-// unit that belongs there.
+// unit that belongs there.  (By way of registers, V's operands put together from words
+// by v_perm: a prompt of 2500 positions 103 against 90 us.)
 template <int HD>
 struct Stage<HD, 1> {
     static constexpr int SK = 8192 / HD;                  // keys
@@ -1177,7 +1204,8 @@ struct Wide : Rows<HD, QP, NT, false> {
                 const bool more = k0 + S::SK < w.hi;
                 if (more) at = st.places(kv, k0 + S::SK, bad);
                 __syncthreads();   // (the piece is there, and the other buffer read)
-                // the next piece's copies, spread over this one's first blocks
+                // the next piece's copies, spread over this one's first blocks (at once a wave
+                // waits 1000 of the piece's 5250 clocks to issue them)
                 const auto rest = [&](int n0, int n1) {
                     if (!more) return;
 #pragma unroll
@@ -1292,7 +1320,8 @@ constexpr int tile_rows() { return 64 * tile_groups<HD, QP>(); }
 template <int HD, int QP>
 constexpr int64_t slot_floats() { return (int64_t)tile_rows<HD, QP>() * (HD + 2); }
 
-// Workgroups that a CU holds (their registers).
+// Workgroups that a CU holds (their registers).  (f32 cache, head_dim 128, eight turns of 1 to
+// 30 tokens behind a prefix of 500: 39.3 us with one, 29.5 with two.)
 constexpr int wgs_per_cu(int hd) { return hd <= 128 ? 2 : 1; }
 
 // bytes of LDS: the stages of Wide; the four waves' results of Deep, or before them its
