@@ -169,7 +169,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // out = sum_p e^(s_p - m) v_p / sum_p e^(s_p - m), s_p = q . k_p / sqrt(head_dim), over the
 // positions p up to the row's own, in one pass over them with a running m.  Scores and
 // weighted sums are MFMAs of bf16 operands with f32 sums.  bf16 queries and
-// cache: the weights are rounded to bf16 (their sum is not), as v is.  f32 ones are taken
+// cache: the weights are rounded to bf16, as v is, and summed as rounded, so that what
+// rounding adds to them all cancels.  f32 ones are taken
 // apart into three bf16 parts, whose products down to 2^-16 of the largest are formed, so
 // that the result is as good as f32 arithmetic's.
 //
@@ -487,6 +488,7 @@ struct Rows {
     bf16x8 q[NT][QP][NS];
     f32x4v acc[NT][VD];
     float m[NT], l[NT];
+    f32x4v lv[QP == 1 ? NT : 1];   // bf16 weights: l, four times, as an MFMA sums it
     int qpos[NT];
     int g, c, see, most;      // the rows' lowest and highest position
 
@@ -495,6 +497,7 @@ struct Rows {
         for (int t = 0; t < NT; ++t) {
             m[t] = -INFINITY;
             l[t] = 0.f;
+            if constexpr (QP == 1) lv[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < VD; ++j) acc[t][j] = f32x4v{0.f, 0.f, 0.f, 0.f};
         }
@@ -650,7 +653,10 @@ struct Rows {
             const float mn = fmaxf(m[t], quads_max(bm));
             if (__any((mn - m[t]) * unit > kGrown)) {   // (from -infinity: so it is)
                 const float f = mn == -INFINITY ? 1.f : weight(m[t] - mn, unit);
-                l[t] *= f;
+                if constexpr (QP == 1)
+                    lv[t] *= f;
+                else
+                    l[t] *= f;
 #pragma unroll
                 for (int j = 0; j < VD; ++j) acc[t][j] *= f;
                 m[t] = mn;
@@ -661,25 +667,40 @@ struct Rows {
             const float mu = mc * unit;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float x[8], sum = 0.f;
+                float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float y = s[b][t][e >> 2][e & 3];
                     x[e] = QP == 1 ? __builtin_amdgcn_exp2f(fmaf(y, unit, -mu)) : weight(y - mc, unit);
-                    sum += x[e];
                 }
-                l[t] += sum;
                 if constexpr (QP == 1) {
                     pp[b][t][0] =
                         __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
                                                               pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
+                    lv[t] = mfma(__builtin_bit_cast(bf16x8, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u)),
+                                 pp[b][t][0], lv[t]);
                 } else {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum += x[e];
+                    l[t] += sum;
                     const Parts8 r = parts8(x);
                     pp[b][t][0] = r.h;
                     pp[b][t][QP - 2] = r.m;
                     pp[b][t][QP - 1] = r.l;
                 }
             }
+        }
+    }
+
+    // l, a lane's own so far, of the whole row.
+    __device__ __forceinline__ void close() {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if constexpr (QP == 1)
+                l[t] = lv[t][0];
+            else
+                l[t] = quads_add(l[t]);
         }
     }
 
@@ -925,7 +946,7 @@ struct Deep : Rows<HD, QP, 1, true> {
             }
         }
         if (bad) flag_error(a.p.err, kErrPagedPage);
-        this->l[0] = quads_add(this->l[0]);
+        this->close();
     }
 };
 
@@ -1239,8 +1260,7 @@ struct Wide : Rows<HD, QP, NT, false> {
             }
         }
         if (bad) flag_error(p.err, kErrPagedPage);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) this->l[t] = quads_add(this->l[t]);
+        this->close();
         __syncthreads();   // (s_kv is free again)
     }
 };
