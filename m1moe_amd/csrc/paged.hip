@@ -453,7 +453,10 @@ struct Cache {
     // The page number of the aligned eight positions from pos on: of the readable one
     // among them, or of the nearest.  As the table has it: it is checked (known) where
     // it is used, as a test here would wait for it and for every load before it.
-    __device__ __forceinline__ int page_of(int pos) const { return table[clamp(pos) >> shift]; }
+    // (a global load: a generic one would hold up the LDS reads that follow it)
+    __device__ __forceinline__ int page_of(int pos) const {
+        return ((const __attribute__((address_space(1))) int32_t*)table)[clamp(pos) >> shift];
+    }
     // Page 0 for one outside the cache.
     __device__ __forceinline__ int known(int x, bool& bad) const {
         const bool out = (unsigned)x >= (unsigned)pages;
@@ -1233,11 +1236,11 @@ struct Wide : Rows<HD, QP, NT, false> {
                     for (int n = 0; n < S::N; ++n)
                         if (n >= n0 && n < n1) st.load(kv, at, n, other);
                 };
+                if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
                 const bool on = k0 < hi;
                 rest(0, on ? 1 : S::N);
                 if (on)
                     blocks(w, k0, 0, unit, buf, [&](int i) { rest(i + 1, i + 1 < kBreaks ? i + 2 : S::N); });
-                if (k0 + 2 * S::SK < w.hi) st.look(kv, k0 + 2 * S::SK);
 #pragma unroll
                 for (int b = NB; b < S::SK / 32; b += NB)
                     if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, buf, [](int) {});
