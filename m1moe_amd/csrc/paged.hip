@@ -1268,13 +1268,20 @@ struct Wide : Rows<HD, QP, NT, false> {
     }
 };
 
-// joins (m1, l1) with (m0, l0): the factors of both
+// joins (m1, l1) with (m0, l0): the factors of both.  (Here and in mix the roundings are
+// written out: the same wherever it is compiled.)
 __device__ __forceinline__ void join(float& m0, float& l0, float m1, float l1, float unit, float& f0, float& f1) {
     const float mn = fmaxf(m0, m1), mc = mn == -INFINITY ? 0.f : mn;
     f0 = weight(m0 - mc, unit);
     f1 = weight(m1 - mc, unit);
-    l0 = l0 * f0 + l1 * f1;
+    l0 = __builtin_fmaf(l0, f0, __fmul_rn(l1, f1));
     m0 = mn;
+}
+__device__ __forceinline__ f32x4v mix(f32x4v x, float f0, f32x4v y, float f1) {
+    f32x4v o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(x[i], f0, __fmul_rn(y[i], f1));
+    return o;
 }
 
 __device__ __forceinline__ void store4(const PagedAttnArgs& a, bool bf16, int64_t at, const float (&x)[4]) {
@@ -1402,21 +1409,30 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const Work& w, 
     }
 }
 
-template <int HD, int QP, int KP, int NT>
-__device__ __forceinline__ void many_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
-                                          const Sink<HD>& sink) {
-    const int wave = thread_id() >> 6, rho0 = wave * 16 * NT;
-    const bool rows = rho0 < w.tokens * a.share;
-    Wide<HD, QP, KP, NT> r;
-    r.lanes();
-    f32x4v raw[NT][HD / 32][Wide<HD, QP, KP, NT>::R::kRaw];
-    r.read(a, w, rho0, raw);
-    r.split(raw);
-    r.run(a.p, w, rows, unit, s_buf);
-    if (!rows) return;
-    if (r.odd()) r.template run_plain<KP>(a, w, rho0, w.lo, 32, unit, reinterpret_cast<float*>(s_buf) + wave * HD);
+// Partials: the workgroups' slots; then, with a prefix, its pieces and one more for
+// the rows' own positions, each [num_rows * heads][HD], and their (m, l).
+template <int HD, int QP>
+__device__ __forceinline__ Sink<HD> slot_of(const PagedAttnArgs& a, int i) {
+    float* o = a.part + i * slot_floats<HD, QP>();
+    return {kToSlot, o, o + (int64_t)tile_rows<HD, QP>() * HD};
+}
+// Workgroup p's piece of a tile that begins in workgroup `first` (it may have two pieces: of
+// the tile that ends its share, and of the one that begins it).
+template <int HD, int QP>
+__device__ __forceinline__ Sink<HD> piece_slot(const PagedAttnArgs& a, int p, int first) {
+    return slot_of<HD, QP>(a, p == first ? 2 * p + 1 : 2 * p);
+}
+template <int HD>
+__device__ __forceinline__ Sink<HD> piece_of(const PagedAttnArgs& a, int i) {
+    const int64_t rows = (int64_t)a.p.num_rows * a.heads;
+    return {kToPiece, a.pre + i * rows * HD, a.pre + (a.splits + 1) * rows * HD + i * rows * 2};
+}
+
+template <int HD, int QP, class R>
+__device__ __forceinline__ void many_out(const PagedAttnArgs& a, const Work& w, int rho0, const R& r,
+                                         const Sink<HD>& sink) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < (int)(sizeof(r.m) / sizeof(float)); ++t) {
         const int rho = rho0 + 16 * t + r.c;
         int token, head;
         if (!row_at(a, w, rho, token, head)) continue;
@@ -1428,29 +1444,102 @@ __device__ __forceinline__ void many_rows(const PagedAttnArgs& a, const Work& w,
     }
 }
 
-template <int HD, int QP, int KP>
-__device__ __forceinline__ void compute(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
-                                        const Sink<HD>& sink) {
-    const int n = w.tokens * a.share;
-    if (n <= 16)
-        few_rows<HD, QP, KP>(a, w, unit, s_buf, sink);
-    else if (tile_groups<HD, QP>() == 1 || n <= 64)
-        many_rows<HD, QP, KP, 1>(a, w, unit, s_buf, sink);
-    else if constexpr (tile_groups<HD, QP>() > 1)
-        many_rows<HD, QP, KP, tile_groups<HD, QP>()>(a, w, unit, s_buf, sink);
+// A tile that workgroups first .. last have a piece of, this one `mine`: the counter of
+// those that have stored theirs (null: no such tile), and where the tile's rows go.
+template <int HD>
+struct Cut {
+    uint32_t* counter;
+    int first, last, mine;
+    Sink<HD> done;
+};
+
+// True if a cut tile is done: all its other workgroups had ended, so that this one's rows
+// need not go through memory.  (Joined in the order of the pieces, as join_tile does.)
+template <int HD, int QP, int KP, int NT>
+__device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
+                                          const Sink<HD>& sink, const Cut<HD>& cut) {
+    const int wave = thread_id() >> 6, rho0 = wave * 16 * NT;
+    const bool rows = rho0 < w.tokens * a.share;
+    Wide<HD, QP, KP, NT> r;
+    r.lanes();
+    f32x4v raw[NT][HD / 32][Wide<HD, QP, KP, NT>::R::kRaw];
+    r.read(a, w, rho0, raw);
+    r.split(raw);
+    r.run(a.p, w, rows, unit, s_buf);
+    if (rows && r.odd())
+        r.template run_plain<KP>(a, w, rho0, w.lo, 32, unit, reinterpret_cast<float*>(s_buf) + wave * HD);
+    if (cut.counter) {
+        uint32_t* s_there = reinterpret_cast<uint32_t*>(s_buf + 16 * HD);   // (behind run_plain's)
+        if (threadIdx.x == 0)
+            *s_there = __hip_atomic_load(cut.counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (*s_there == (uint32_t)(cut.last - cut.first)) {
+            if (threadIdx.x == 0) __hip_atomic_store(cut.counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (rows) {
+                constexpr int VD = HD / 16, V = VD < 8 ? VD : 8;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int rho = rho0 + 16 * t + r.c;
+                    float m = -INFINITY, l = 0.f;
+#pragma unroll
+                    for (int j0 = 0; j0 < VD; j0 += V) {
+                        f32x4v o[V];
+                        for (int p = cut.first; p <= cut.last; ++p) {
+                            float mp = r.m[t], lp = r.l[t];
+                            f32x4v y[8];
+#pragma unroll
+                            for (int k = 0; k < V; ++k) y[k] = r.acc[t][j0 + k];
+                            if (p != cut.mine) {
+                                const Sink<HD> slot = piece_slot<HD, QP>(a, p, cut.first);
+                                const unsigned long long z =
+                                    __hip_atomic_load(reinterpret_cast<unsigned long long*>(slot.ml + 2 * rho),
+                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                                const float* at[8];
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) at[k] = slot.o + rho * HD + 16 * (j0 + k % V) + 4 * r.g;
+                                load8_coh(at, y);
+                                mp = __uint_as_float((uint32_t)z);
+                                lp = __uint_as_float((uint32_t)(z >> 32));
+                            }
+                            if (p == cut.first) {
+                                m = mp;
+                                l = lp;
+#pragma unroll
+                                for (int k = 0; k < V; ++k) o[k] = y[k];
+                            } else {
+                                float f0, f1;
+                                join(m, l, mp, lp, unit, f0, f1);
+#pragma unroll
+                                for (int k = 0; k < V; ++k) o[k] = mix(o[k], f0, y[k], f1);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < V; ++k) r.acc[t][j0 + k] = o[k];
+                    }
+                    r.m[t] = m;
+                    r.l[t] = l;
+                }
+                many_out<HD, QP>(a, w, rho0, r, cut.done);
+            }
+            return true;
+        }
+    }
+    if (rows) many_out<HD, QP>(a, w, rho0, r, sink);
+    return false;
 }
 
-// Partials: the workgroups' slots; then, with a prefix, its pieces and one more for
-// the rows' own positions, each [num_rows * heads][HD], and their (m, l).
-template <int HD, int QP>
-__device__ __forceinline__ Sink<HD> slot_of(const PagedAttnArgs& a, int i) {
-    float* o = a.part + i * slot_floats<HD, QP>();
-    return {kToSlot, o, o + (int64_t)tile_rows<HD, QP>() * HD};
-}
-template <int HD>
-__device__ __forceinline__ Sink<HD> piece_of(const PagedAttnArgs& a, int i) {
-    const int64_t rows = (int64_t)a.p.num_rows * a.heads;
-    return {kToPiece, a.pre + i * rows * HD, a.pre + (a.splits + 1) * rows * HD + i * rows * 2};
+template <int HD, int QP, int KP>
+__device__ __forceinline__ bool compute(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
+                                        const Sink<HD>& sink, const Cut<HD>& cut) {
+    const int n = w.tokens * a.share;
+    if (n <= 16) {
+        few_rows<HD, QP, KP>(a, w, unit, s_buf, sink);
+        return false;
+    }
+    if (tile_groups<HD, QP>() == 1 || n <= 64) return many_rows<HD, QP, KP, 1>(a, w, unit, s_buf, sink, cut);
+    if constexpr (tile_groups<HD, QP>() > 1)
+        return many_rows<HD, QP, KP, tile_groups<HD, QP>()>(a, w, unit, s_buf, sink, cut);
+    return false;
 }
 
 // The pieces of a tile that workgroups first .. last have written to their slots, joined.
@@ -1462,7 +1551,7 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
                                           uint8_t* s_buf, const Sink<HD>& sink) {
     constexpr int NV = tile_rows<HD, QP>() * HD / 4 / 256;
     const int rows = w.tokens * a.share, tid = thread_id(), values = rows * (HD / 4);
-    const auto piece = [&](int p) { return slot_of<HD, QP>(a, p == first ? 2 * p + 1 : 2 * p); };
+    const auto piece = [&](int p) { return piece_slot<HD, QP>(a, p, first); };
     const auto coh = [](const float* p) {
         return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
@@ -1489,7 +1578,7 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
                     if (p0 + k > last) break;
                     float f0, f1;
                     join(m, l, z[k], u[k], unit, f0, f1);
-                    o = o * f0 + y[k] * f1;
+                    o = mix(o, f0, y[k], f1);
                 }
             }
         }
@@ -1504,7 +1593,7 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
                 const float* y = reinterpret_cast<const float*>(s_buf) + 8 * (tid + k * values);
                 float f0, f1;
                 join(m, l, y[4], y[5], unit, f0, f1);
-                o = o * f0 + *reinterpret_cast<const f32x4v*>(y) * f1;
+                o = mix(o, f0, *reinterpret_cast<const f32x4v*>(y), f1);
             }
             sink.put(a, QP == 1, rho, token, head, d, m, l, 1.0f / l, o[0], o[1], o[2], o[3]);
         }
@@ -1536,7 +1625,7 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
                 } else {
                     float f0, f1;
                     join(m[k], l[k], z[k], u[k], unit, f0, f1);
-                    o[k] = o[k] * f0 + y[k] * f1;
+                    o[k] = mix(o[k], f0, y[k], f1);
                 }
             }
         }
@@ -1573,7 +1662,7 @@ __device__ __forceinline__ void prefix_piece(const PagedAttnArgs& a, int id, flo
     w.last = p.prefix_len - 1;
     w.table = p.prefix_pages;
     w.uniform();
-    compute<HD, QP, KP>(a, w, unit, s_buf, piece_of<HD>(a, piece));
+    compute<HD, QP, KP>(a, w, unit, s_buf, piece_of<HD>(a, piece), Cut<HD>{});
 }
 
 // The first workgroups take a share each of the line of the sequences' own positions, the
@@ -1632,12 +1721,17 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAt
         w.uniform();
         const Sink<HD> done = a.splits ? piece_of<HD>(a, a.splits) : Sink<HD>{kToOut, nullptr, nullptr};
         const bool whole = x == t.start && end == t.end;
-        compute<HD, QP, KP>(a, w, unit, s_buf, whole ? done : slot_of<HD, QP>(a, 2 * wg + (x > t.start ? 0 : 1)));
+        // the workgroups of a cut tile: from the one whose cut is its start (or rounded to
+        // it) to the one with the last cut inside it
+        int first = wg, last = wg;
         if (!whole) {
-            // the tile's workgroups: from the one whose cut is its start (or rounded to it)
-            // to the one with the last cut inside it
-            const int first = x == t.start ? wg : ln.below(t.start + kTileKeys + kCut);
-            const int last = end == t.end ? wg : ln.below(t.end);
+            if (x != t.start) first = ln.below(t.start + kTileKeys + kCut);
+            if (end != t.end) last = ln.below(t.end);
+        }
+        const Cut<HD> cut{whole ? nullptr : a.counters + first, first, last, wg, done};
+        const bool joined =
+            compute<HD, QP, KP>(a, w, unit, s_buf, whole ? done : piece_slot<HD, QP>(a, wg, first), cut);
+        if (!whole && !joined) {
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
             if (threadIdx.x == 0) {
