@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // Steps are bound by reading the cache once (32 heads over 8, f32 queries, bf16 cache:
 // 32 tokens behind 60 to 8100 positions 80.6 us, 4.5 TB/s; 16 heads, all bf16: 48 behind
 // 100 to 4000 117 us, 4.8 TB/s), prompts and turns by a SIMD's two waves, whose MFMAs,
-// softmax and LDS reads overlap only in part (2500 positions, all bf16: 84 us, 608 TFLOP/s;
+// softmax and LDS reads overlap only in part (2500 positions, all bf16: 80 us, 640 TFLOP/s;
 // six turns of 9 to 400 tokens behind up to 4000, f32 queries: 73 us, of which 55 are
 // the three products at a large matrix product's rate), one token behind few positions by
 // the chain launch - lengths - page - rows - join (14.8 us).
@@ -256,7 +256,7 @@ constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 // moved down to a multiple of kCut keys inside their tile, or to its start where it has
 // at most kWhole keys: to join two pieces of one takes longer than to read it (a prompt of
 // 2500 and turns behind up to 4000: 104 and 88 us with every tile cut, 98 and 79 with
-// 512 whole; as they are now, 84.2 and 73.2, with 768 whole 87.2 and 83.5).  (Without the places
+// 512 whole; later 84.2 and 73.2, with 768 whole 87.2 and 83.5).  (Without the places
 // per tile the workgroups with the shortest sequences ended last: 32 steps of 60 to
 // 8100 positions, 8 kv heads, median 61 us, last 116.)
 struct Tile {
@@ -1454,7 +1454,8 @@ struct Cut {
 };
 
 // True if a cut tile is done: all its other workgroups had ended, so that this one's rows
-// need not go through memory.  (Joined in the order of the pieces, as join_tile does.)
+// need not go through memory (a prompt of 2500 positions 83.9 -> 79.9 us).  Joined in the
+// order of the pieces, as join_tile does.
 template <int HD, int QP, int KP, int NT>
 __device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
                                           const Sink<HD>& sink, const Cut<HD>& cut) {
