@@ -88,8 +88,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     if (tid < a.rotary / 2) {
         const double ang = (double)pos * (double)a.inv_freq[tid];
         const double k = rint(ang * 0.15915494309189533577);
-        const float r = (float)fma(-k, 2.4492935982947064e-16, fma(-k, 6.283185307179586232, ang));
-        s_cs[tid] = make_float2(cosf(r) * a.amp, sinf(r) * a.amp);
+        const double rest = fma(-k, 2.4492935982947064e-16, fma(-k, 6.283185307179586232, ang));
+        // (what its rounding to f32 leaves, up to 2^-23, turns the pair once more)
+        const float r = (float)rest, e = (float)(rest - (double)r), c = cosf(r), s = sinf(r);
+        s_cs[tid] = make_float2(fmaf(-e, s, c) * a.amp, fmaf(e, c, s) * a.amp);
     }
     __syncthreads();
     const bool page_ok = page >= 0 && page < p.num_pages;
