@@ -433,6 +433,30 @@ def test_attention_infinities_in_pieces(dev, types):
         assert np.all(np.abs(got[fine] - ref[fine]) <= bound[fine])
 
 
+@pytest.mark.parametrize("types", TYPES)
+def test_attention_sequences_share_pages(dev, types):
+    """Sequences whose tables name the same pages (a conversation continued twice), and a
+    page named twice in one table."""
+    ctx, ops = dev
+    b = Batch(np.random.default_rng(68), [1, 1, 20], [600, 600, 581], 16)
+    b.table[1] = b.table[0]
+    b.table[2, :30] = b.table[0, :30]
+    b.table[2, 31] = b.table[2, 30]
+    say(f"attention shared pages {types}")
+    got, _, ref, bound = attend(dev, b, 4, 2, 128, types, 69)
+    check_close(got, ref, bound, types[0])
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd", [(1024, 16, 64), (256, 256, 256), (512, 8, 128)])
+def test_attention_most_heads(dev, types, heads, kv_heads, hd):
+    """num_heads * head_dim at its limit."""
+    b = Batch(np.random.default_rng(70), [3, 1], [5, 70], 8, prefix=4)
+    say(f"attention most heads {types} {heads}/{kv_heads}x{hd}")
+    got, _, ref, bound = attend(dev, b, heads, kv_heads, hd, types, 71)
+    check_close(got, ref, bound, types[0])
+
+
 def test_two_graphs_share_the_partials(dev):
     """Graphs of two batches captured on one context and replayed in turn, eager calls of
     a third between them: all use the context's partials and counters."""
