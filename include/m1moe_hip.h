@@ -502,7 +502,7 @@ int32_t m1moe_kv_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
  * h / (num_heads / num_kv_heads).  q and out [num_rows][num_heads * head_dim]
  * in dtype (row strides in elements, as above; they must not overlap); scores, softmax and sums in
  * f32 (dtype M1MOE_BF16: the softmax numerators that multiply v are rounded to
- * bf16).  dtype M1MOE_BF16 needs a bf16 cache; num_heads is a multiple of
+ * bf16, or to two bf16 parts for the few rows of a step).  dtype M1MOE_BF16 needs a bf16 cache; num_heads is a multiple of
  * num_kv_heads, at most 64 times it, and num_heads * head_dim <= 65536.
  * Later positions take no part, whatever they hold.  The first call of a
  * larger batch may grow the context's workspace (make it before capturing). */
