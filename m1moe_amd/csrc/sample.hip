@@ -582,15 +582,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
         if (phase == 2 && mp > 0.f) {
             // weights of at least min_p: whole steps above the one that holds the border,
             // and the logits of that one (and, as it is rounded another way, of the steps
-            // to either side); a border below the front leaves all that is kept
+            // to either side).  A front holds its steps whole, and nothing behind it is kept:
+            // of these steps those in the front count, and a border below all of it leaves
+            // what is kept.
             const double border = fmin(log2((double)mp), 0.0);
             const double xb = (double)top + border / sc.c;
             const int bin = !(xb > (double)all.lo) ? kBins - 1
                                                   : (int)fmin(((double)top - xb) * all.per, (double)(kBins - 1));
-            const int b0 = max(bin - 1, 0), b1 = min(bin + 1, kBins - 1);
+            const int b0 = max(bin - 1, 0), b1 = min(bin + 1, fr.bin < 0 ? kBins - 1 : fr.bin);
             if (mp > 1.f) {
                 kept = 1ull << kUnit;
-            } else if (fr.bin < 0 || b1 <= fr.bin) {
+            } else if (b0 <= b1) {
                 if (tid == 0) s.units = 0;
                 __syncthreads();
                 float from, to;

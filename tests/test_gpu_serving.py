@@ -888,6 +888,91 @@ def test_sample_dense_steps(dev):
     check_draw(dev, x, s)
 
 
+def kept_count(x, T, top_k=0, min_p=0.0):
+    """How many logits of a row top-k and min-p leave (f64)."""
+    x = -np.sort(-x.astype(np.float64), kind="stable")
+    x = x[:top_k] if top_k else x
+    return max(1, int(np.count_nonzero(np.exp((x - x[0]) / T) >= float(np.float32(min_p)))))
+
+
+def test_sample_min_p_among_equal_logits(dev):
+    """Two crowded values below the first logit, the border of min-p just above the one
+    that top-k ends in: only the first logit stays.  And three candidates of which the border
+    parts the last two."""
+    x = np.concatenate([[10.0], np.full(200, 5.0), np.zeros(1000)]).astype(np.float32)
+    s = [dict(u=u, top_k=k, min_p=float(np.exp(-5.0) * 1.0005)) for u in (0.0, 0.6, 0.7, 0.9, 1.0) for k in (0, 100)]
+    assert all(kept_count(x, 1.0, r["top_k"], r["min_p"]) == 1 for r in s)
+    say("sample min-p among equal logits")
+    check_draw(dev, np.tile(x, (len(s), 1)), s)
+    x = np.array([0.0, -2.005, -2.01, -10.0, -40.0], np.float32)
+    s = [dict(u=u, top_k=k, min_p=float(np.exp(-2.0075))) for u in (0.5, 0.999, 1.0) for k in (3, 4)]
+    assert all(kept_count(x, 1.0, r["top_k"], r["min_p"]) == 2 for r in s)
+    check_draw(dev, np.tile(x, (len(s), 1)), s)
+
+
+@pytest.mark.parametrize("vocab,rows", [(700, 40), (9001, 30), (50304, 1), (50304, 20), (9001, 300)])
+@pytest.mark.parametrize("crowded", [False, True])
+def test_sample_min_p_beside_top_k(dev, vocab, rows, crowded):
+    """The border of min-p between two logits from well above the k-th to below it: in the
+    same step of 2047 equal ones as the k-th, the steps beside it and others, with the order's
+    beginning kept aside (top-k of at most about 1000) and not.  Crowded: the best logit is far
+    above the others, which then share few steps.  One workgroup per row and several."""
+    rng = np.random.default_rng(vocab + rows + crowded)
+    T = 6.0
+    x = rng.normal(0, 2.5, (rows, vocab)).astype(np.float32)
+    if crowded:
+        x[np.arange(rows), rng.integers(0, vocab, rows)] = 40.0
+    s, same, cut = [], 0, 0
+    for r in range(rows):
+        y = -np.sort(-x[r].astype(np.float64))
+        w = np.exp((y - y[0]) / T)
+        bounds = (y[0] - np.maximum(y[-1], y[0] - 45.5 * np.log(2) * T)) / 2047
+        step = np.floor((y[0] - y) / bounds)
+        top_k = int(np.exp(rng.uniform(np.log(2), np.log(min(vocab - 2, 3000)))))
+        # logits j - 1 and j are parted (their weights differ by more than an f32's half step
+        # and what the places of an f64 exponent are off)
+        away = int(rng.choice([-200, -3, -2, -1, 0, 0, 1, 2]))
+        j = min(max(1, top_k + away), vocab - 1)
+        while j > 1 and not w[j - 1] > w[j] * (1 + 2.0 ** -20):
+            j -= 1
+        min_p = float(np.float32(math.sqrt(w[j - 1] * w[j])))
+        assert w[j - 1] > min_p > w[j]
+        s.append(dict(u=float(np.float32(rng.choice([rng.random(), 0.999, 1.0]))), T=T, top_k=top_k, min_p=min_p))
+        if rng.random() < 0.3:
+            s[-1]["top_p"] = float(rng.uniform(0.8, 1.0))
+        fewer = kept_count(x[r], T, top_k, min_p) < kept_count(x[r], T, top_k)
+        assert fewer == (j < top_k)
+        cut += fewer
+        same += fewer and step[j] == step[top_k - 1]
+    # (rows that min-p cuts, and those where it does so in the k-th logit's own step)
+    assert rows == 1 or (cut >= rows // 4 and (same >= 2 or not crowded))
+    say(f"sample min-p beside top-k {vocab} x {rows} {crowded}")
+    check_draw(dev, x, s)
+
+
+def test_sample_min_p_in_dense_steps(dev):
+    """Settings as in test_sample_dense_steps with a border that cuts: alone, with top-p, and
+    with top-k above, inside and below the k-th logit's step."""
+    rng = np.random.default_rng(45)
+    V, T = 30000, 300.0
+    x = rng.normal(0, 1, (12, V)).astype(np.float32)
+    x[:, 777] = 1000.0
+    ks = [0, 0, 0, 5, 5, 300, 300, 900, 900, 2000, 2000, 40]
+    at = [10, 700, 9000, 3, 9, 290, 400, 20, 880, 1500, 1990, 39]     # logits that the border leaves
+    s = []
+    for r in range(12):
+        y = -np.sort(-x[r].astype(np.float64))
+        w = np.exp((y - y[0]) / T)
+        j = at[r]
+        while not w[j - 1] > w[j] * (1 + 2.0 ** -20):
+            j -= 1
+        s.append(dict(u=(0.3, 0.95, 1.0)[r % 3], T=T, top_k=ks[r], min_p=float(np.float32(math.sqrt(w[j - 1] * w[j])))))
+        assert kept_count(x[r], T, ks[r], s[-1]["min_p"]) == min(j, ks[r] or V)
+    s[1]["top_p"], s[2]["top_p"] = 0.1, 0.01
+    say("sample min-p in dense steps")
+    check_draw(dev, x, s)
+
+
 def test_sample_settings_at_their_ends(dev):
     rng = np.random.default_rng(41)
     V = 9000
