@@ -171,15 +171,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // out = sum_p e^(s_p - m) v_p / sum_p e^(s_p - m), s_p = q . k_p / sqrt(head_dim), over the
 // positions p up to the row's own, in one pass over them with a running m.  Scores and
 // weighted sums are MFMAs of bf16 operands with f32 sums.  bf16 queries and
-// cache: the weights are rounded to bf16 (few rows: to two parts), as v is, and summed as
-// rounded, so that what rounding adds to them all cancels.  f32 ones are taken
+// cache: the weights are rounded to two bf16 parts and summed as rounded.  f32 ones are taken
 // apart into three bf16 parts, whose products down to 2^-16 of the largest are formed, so
 // that the result is as good as f32 arithmetic's.
 //
 // Steps are bound by reading the cache once (32 heads over 8, f32 queries, bf16 cache:
 // 32 tokens behind 60 to 8100 positions 80.6 us, 4.5 TB/s; 16 heads, all bf16: 48 behind
 // 100 to 4000 117 us, 4.8 TB/s), prompts and turns by a SIMD's two waves, whose MFMAs,
-// softmax and LDS reads overlap only in part (2500 positions, all bf16: 79 us, 650 TFLOP/s;
+// softmax and LDS reads overlap only in part (2500 positions, all bf16: 95 us, 535 TFLOP/s;
 // six turns of 9 to 400 tokens behind up to 4000, f32 queries: 73 us, of which 55 are
 // the three products at a large matrix product's rate), one token behind few positions by
 // the chain launch - lengths - page - rows - join (14.8 us).
@@ -490,11 +489,10 @@ __device__ __forceinline__ bool row_at(const PagedAttnArgs& a, const Work& w, in
 template <int HD, int QP, int NT, bool SPREAD>
 struct Rows {
     static constexpr int NS = HD / 32, VD = HD / 16;
-    // Parts of a weight.  bf16 queries: two for few rows, where the MFMAs of the second cost
-    // nothing beside the loads (48 steps: 116.5 us with one, 116.9 with two, the error
-    // against 64 bits 2.1e-3 and 1.7e-3, the output's own rounding), else one (a prompt of 2500:
-    // 79 us with one, 96 with two).
-    static constexpr int PP = QP == 1 && SPREAD ? 2 : QP;
+    // Parts of a weight.  bf16 queries: two, whose rest of 2^-16 is nothing beside the output's own
+    // rounding, however many rows arrive together (one: a prompt of 2500 79 us, its error
+    // against 64 bits 2.0e-3 where the output's rounding is 1.6e-3).
+    static constexpr int PP = QP == 1 ? 2 : QP;
     bf16x8 q[NT][QP][NS];
     f32x4v acc[NT][VD];
     float m[NT], l[NT];
@@ -673,7 +671,7 @@ struct Rows {
             }
             const float mc = m[t] == -INFINITY ? 0.f : m[t];   // (no key seen yet: all weights 0)
             // (bf16 queries: one rounding more, of the row's largest exponent, against the 2^-8
-            // of the weights or the output)
+            // of the output)
             const float mu = mc * unit;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -686,15 +684,9 @@ struct Rows {
                 if constexpr (QP == 1) {
                     const bf16x8 ones = __builtin_bit_cast(
                         bf16x8, make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u));
-                    if constexpr (PP == 1) {
-                        pp[b][t][0] =
-                            __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]),
-                                                                  pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])));
-                    } else {
-                        const Parts8 r = parts8(x);
-                        pp[b][t][0] = r.h;
-                        pp[b][t][PP - 1] = r.m;
-                    }
+                    const Parts8 r = parts8(x);
+                    pp[b][t][0] = r.h;
+                    pp[b][t][PP - 1] = r.m;
 #pragma unroll
                     for (int y = PP - 1; y >= 0; --y) lv[t] = mfma(ones, pp[b][t][y], lv[t]);
                 } else {

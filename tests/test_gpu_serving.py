@@ -457,6 +457,30 @@ def test_attention_most_heads(dev, types, heads, kv_heads, hd):
     check_close(got, ref, bound, types[0])
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,rows,past,prefix", [
+    (4, 2, 64, [60, 9, 1], [300, 900, 40], 0), (2, 2, 128, [200], [1500], 0), (8, 2, 128, [70, 5, 30], [10, 2000, 0], 0),
+    (3, 1, 256, [40, 21], [700, 3], 0), (4, 4, 128, [90, 2, 1, 30], [800, 650, 640, 700], 600),
+])
+def test_attention_bf16_error_beyond_the_rounding(dev, heads, kv_heads, hd, rows, past, prefix):
+    """bf16 rows, many of a sequence or few: what the softmax's weights lose beside the rounding of
+    the output is two bf16 parts' rest, 2^-16 of each weight and of their sum."""
+    b = Batch(np.random.default_rng(72), rows, past, 16, prefix=prefix)
+    say(f"attention bf16 weights {heads}/{kv_heads}x{hd} {rows}")
+    ctx, ops = dev
+    rng = np.random.default_rng(73)
+    q = bf16(rng.normal(0, 1, (b.T, heads * hd)))
+    kc, vc = cache_of(rng, b, kv_heads, hd, "bf16")
+    d = Held(ctx, b, kc, vc, "bf16", kv_heads, hd)
+    out = d.up(np.zeros((b.T, heads * hd), np.uint16))
+    ops.paged_attention(d.kv, d.batch, d.up(q), heads * hd, out, heads * hd, "bf16", heads)
+    ctx.sync()
+    got = f64(out.download(np.uint16)).reshape(-1, heads, hd)
+    d.free()
+    ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
+    before = attention_bound(ref, mag, top, hd, "f32") + 2 * 2.0 ** -16 * mag
+    assert np.all(np.abs(got - ref) <= before + 2.0 ** -8 * (np.abs(ref) + before))
+
+
 def test_two_graphs_share_the_partials(dev):
     """Graphs of two batches captured on one context and replayed in turn, eager calls of
     a third between them: all use the context's partials and counters."""
