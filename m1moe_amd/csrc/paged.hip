@@ -1655,7 +1655,20 @@ __device__ __forceinline__ void prefix_piece(const PagedAttnArgs& a, int id, flo
     const PagedView& p = a.p;
     const int TT = tile_rows<HD, QP>() / a.share, tiles = (p.num_rows + TT - 1) / TT;
     const int head = id / tiles % p.kv_heads, piece = id / tiles / p.kv_heads;
-    const int rows = min(p.row_start[p.num_seqs], p.num_rows), blocks = (p.prefix_len + 31) / 32;
+    const int blocks = (p.prefix_len + 31) / 32;
+    // the end of the rows: of the last sequence that is computed (the last start may be wrong)
+    int* s_end = reinterpret_cast<int*>(s_buf);
+    int rows = 0;
+    for (int s = threadIdx.x; s < p.num_seqs; s += 256) {
+        const int lo = p.row_start[s], hi = p.row_start[s + 1];
+        if (seq_ok(p, lo, hi, p.kv_len[s]) && hi > lo) rows = max(rows, hi);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) rows = max(rows, __shfl_xor(rows, m));
+    if ((threadIdx.x & 63) == 0) s_end[threadIdx.x >> 6] = rows;
+    __syncthreads();
+    rows = max(max(s_end[0], s_end[1]), max(s_end[2], s_end[3]));
+    __syncthreads();   // (s_buf is the tile's)
     Work w;
     w.token0 = id % tiles * TT;
     w.tokens = min(TT, rows - w.token0);

@@ -326,6 +326,36 @@ def test_bad_batches_are_reported(dev, breakage):
         assert np.all(got[1:3] == 3.0)
 
 
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("end", [30, 0, -5, 1 << 30])
+def test_bad_last_start_behind_a_prefix(dev, types, end):
+    """The last sequence's end lies before its start (or past the rows): it is skipped, and the
+    other sequences' rows are right, those past that end too."""
+    ctx, ops = dev
+    rng = np.random.default_rng(74)
+    heads, kv_heads, hd, prefix = 4, 2, 64, 200
+    x, cache = types
+    b = Batch(rng, [40, 1, 2], [prefix + 3, prefix + 50, prefix + 9], 16, prefix=prefix)
+    kc, vc = cache_of(rng, b, kv_heads, hd, cache)
+    d = Held(ctx, b, kc, vc, cache, kv_heads, hd)
+    out = d.up(as_dtype(np.full((b.T, heads * hd), 3.0), x))
+    q = as_dtype(rng.normal(0, 1, (b.T, heads * hd)), x)
+    say(f"attention bad last start {end} {types}")
+    # (what the workspace holds: another call's)
+    ops.paged_attention(d.kv, d.batch, d.up(as_dtype(f64(q)[::-1], x)), heads * hd, d.up(np.zeros_like(q)), heads * hd, x, heads)
+    starts = b.row_start.copy()
+    starts[3] = end
+    d.start.upload(starts)
+    ops.paged_attention(d.kv, d.batch, d.up(q), heads * hd, out, heads * hd, x, heads)
+    with pytest.raises(M1MoEError, match="paged batch"):
+        ctx.sync()
+    got = f64(out.download(np.uint16 if x == "bf16" else np.float32)).reshape(-1, heads, hd)
+    d.free()
+    ref, mag, top = attention_ref(b, q, kc, vc, heads, kv_heads, hd)
+    assert np.all(got[41:] == 3.0)
+    check_close(got[:41], ref[:41], attention_bound(ref, mag, top, hd, x)[:41], x)
+
+
 def test_attention_in_a_graph(dev):
     """One captured call serves later lengths: replays with other lengths, eager
     calls between them."""
