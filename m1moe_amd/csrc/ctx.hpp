@@ -128,6 +128,20 @@ inline int32_t device_alloc(void** p, uint64_t bytes, const char* what) {
     return M1MOE_OK;
 }
 
+// Cleared on the stream, too; *p stays as it was if either fails, so that memory which was
+// never cleared is not taken for ready by the next call.
+inline int32_t device_alloc_zeroed(void** p, uint64_t bytes, const char* what, hipStream_t stream) {
+    void* q = nullptr;
+    if (int32_t rc = device_alloc(&q, bytes, what)) return rc;
+    hipError_t e = hipMemsetAsync(q, 0, bytes, stream);
+    if (e != hipSuccess) {
+        (void)hipFree(q);
+        return fail(M1MOE_ERR_HIP, "clearing the %s failed: %s", what, hipGetErrorString(e));
+    }
+    *p = q;
+    return M1MOE_OK;
+}
+
 // Scratch that must grow is reallocated (synchronise, free, allocate): not
 // possible while the stream is being captured into a graph, and a graph
 // captured earlier would point at the freed buffers.  Growth under capture is

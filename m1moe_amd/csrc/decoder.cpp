@@ -38,9 +38,8 @@ int32_t ensure_attn_scratch(m1moe_ctx_t ctx, uint64_t floats, uint64_t reserve) 
     if (!ctx->attn_cnt || floats > ctx->attn_part_floats)
         if (int32_t rc = refuse_growth_in_capture(ctx->stream, "the attention scratch")) return rc;
     if (!ctx->attn_cnt) {
-        int32_t rc = device_alloc((void**)&ctx->attn_cnt, kAttnCntWords * 4, "attention counters");
+        int32_t rc = device_alloc_zeroed((void**)&ctx->attn_cnt, kAttnCntWords * 4, "attention counters", ctx->stream);
         if (rc) return rc;
-        HIP_TRY(hipMemsetAsync(ctx->attn_cnt, 0, kAttnCntWords * 4, ctx->stream));
     }
     if (floats <= ctx->attn_part_floats) return M1MOE_OK;
     floats = std::max(floats, reserve);

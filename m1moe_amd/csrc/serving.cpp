@@ -101,9 +101,8 @@ int32_t ensure_paged_scratch(m1moe_ctx_t ctx, uint64_t floats) {
     if (int32_t rc = refuse_growth_in_capture(ctx->stream, "the paged attention scratch")) return rc;
     if (!ctx->paged_cnt) {
         const uint64_t bytes = 4 * (2 * (uint64_t)ctx->cus + 8);   // the largest grid
-        int32_t rc = device_alloc((void**)&ctx->paged_cnt, bytes, "paged attention counters");
-        if (rc) return rc;
-        HIP_TRY(hipMemsetAsync(ctx->paged_cnt, 0, bytes, ctx->stream));
+        if (int32_t rc = device_alloc_zeroed((void**)&ctx->paged_cnt, bytes, "paged attention counters", ctx->stream))
+            return rc;
         if (floats <= ctx->paged_part_floats) return M1MOE_OK;
     }
     HIP_TRY(hipStreamSynchronize(ctx->stream));
@@ -125,11 +124,8 @@ int32_t ensure_sample_scratch(m1moe_ctx_t ctx) {
     HIP_TRY(hipStreamIsCapturing(ctx->stream, &cs));
     if (cs != hipStreamCaptureStatusNone) return M1MOE_OK;
     const uint64_t bytes = (uint64_t)sample_part_words(ctx->cus) * 4;
-    int32_t rc = device_alloc((void**)&ctx->sample_part, bytes, "sampling scratch");
-    if (rc) return rc;
-    // (the counters; on the launches' own stream)
-    HIP_TRY(hipMemsetAsync(ctx->sample_part, 0, bytes, ctx->stream));
-    return M1MOE_OK;
+    // (its counters start at zero; cleared on the launches' own stream)
+    return device_alloc_zeroed((void**)&ctx->sample_part, bytes, "sampling scratch", ctx->stream);
 }
 
 }  // namespace
