@@ -464,7 +464,8 @@ typedef struct {
     const void* d_q;         /* [num_rows][num_heads * head_dim], or NULL: k and v only */
     const void* d_k;         /* [num_rows][num_kv_heads * head_dim] */
     const void* d_v;         /* the same */
-    void* d_q_out;           /* as d_q (may be d_q itself, with its stride); NULL with d_q */
+    void* d_q_out;           /* as d_q; d_q itself, with its stride, or rows that share no
+                              * memory with those of d_q, d_k and d_v; NULL with d_q */
     int64_t q_stride, k_stride, v_stride, q_out_stride;
     const uint16_t* d_q_norm;  /* bf16 [head_dim] per-head RMSNorm weights, or NULL: no norm */
     const uint16_t* d_k_norm;
@@ -500,11 +501,12 @@ int32_t m1moe_kv_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
 /* Attention of every row of the batch over its own sequence's positions up to
  * its own: out_h = sum_p softmax_p(q_h . k_p / sqrt(head_dim)) v_p, kv head
  * h / (num_heads / num_kv_heads).  q and out [num_rows][num_heads * head_dim]
- * in dtype (row strides in elements, as above; they must not overlap); scores,
- * softmax and sums in f32 (dtype M1MOE_BF16: the softmax numerators that
- * multiply v are rounded to two bf16 parts, 16 bits).  dtype M1MOE_BF16 needs a
- * bf16 cache; num_heads is a multiple of num_kv_heads, at most 64 times it, and
- * num_heads * head_dim <= 65536.
+ * in dtype (row strides in elements, as above; their rows must not share memory,
+ * with different strides not their ranges either); scores, softmax and sums in
+ * f32 (dtype M1MOE_BF16: the softmax numerators that multiply v are rounded to
+ * two bf16 parts, 16 bits).  dtype M1MOE_BF16 needs a bf16 cache; num_heads is a
+ * multiple of num_kv_heads, at most 64 times it, and num_heads * head_dim <=
+ * 65536.
  * Later positions take no part, whatever they hold.  The first call of a
  * larger batch may grow the context's workspace (make it before capturing). */
 int32_t m1moe_paged_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,

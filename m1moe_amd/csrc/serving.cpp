@@ -75,6 +75,16 @@ int32_t check_rows(const void* p, int64_t stride, int64_t n, int32_t dtype, cons
     return M1MOE_OK;
 }
 
+// Whether rows of xn bytes at x, xs bytes apart, share memory with as many of yn bytes at y, ys
+// bytes apart (xn <= xs, yn <= ys).  Of different strides: whether their ranges do.
+bool rows_overlap(const void* x, int64_t xs, int64_t xn, const void* y, int64_t ys, int64_t yn, int64_t rows) {
+    const int64_t d = reinterpret_cast<intptr_t>(y) - reinterpret_cast<intptr_t>(x);
+    if (d >= (rows - 1) * xs + xn || -d >= (rows - 1) * ys + yn) return false;
+    if (rows == 1 || xs != ys) return true;
+    const int64_t at = (d % xs + xs) % xs;   // y's columns from x's on
+    return at < xn || at + yn > xs;
+}
+
 PagedView view(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m1moe_paged_batch* b) {
     PagedView v{};
     v.k = kv->d_k;
@@ -165,7 +175,15 @@ int32_t m1moe_kv_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m1moe_p
     if (g->rotary_dim > 0 && (rc = check_i32_ptr(g->d_inv_freq, "d_inv_freq"))) return rc;
     if (g->rotary_dim > 0 && !(std::fabs(g->rope_amplitude) <= 3.4e38f))
         return fail(M1MOE_ERR_INVALID, "rope_amplitude must be finite");
-    if ((rc = check_ctx(ctx)) || (rc = set_device(ctx))) return rc;
+    if ((rc = check_ctx(ctx))) return rc;
+    const int64_t es = g->dtype == M1MOE_BF16 ? 2 : 4;
+    const auto clash = [&](const void* p, int64_t stride, int64_t n) {
+        return rows_overlap(g->d_q_out, es * g->q_out_stride, es * qd, p, es * stride, es * n, batch->num_rows);
+    };
+    if (g->d_q && ((g->d_q_out != g->d_q && clash(g->d_q, g->q_stride, qd)) || clash(g->d_k, g->k_stride, kvd) ||
+                   clash(g->d_v, g->v_stride, kvd)))
+        return fail(M1MOE_ERR_INVALID, "d_q_out overlaps rows of d_q, d_k or d_v and is not d_q itself");
+    if ((rc = set_device(ctx))) return rc;
     AppendArgs a{};
     a.p = view(ctx, kv, batch);
     a.q = g->d_q;
@@ -204,7 +222,11 @@ int32_t m1moe_paged_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m
         (rc = check_rows(d_out, out_stride, qd, dtype, "d_out")))
         return rc;
     if (d_q == d_out) return fail(M1MOE_ERR_INVALID, "d_out must not overlap d_q");
-    if ((rc = check_ctx(ctx)) || (rc = set_device(ctx))) return rc;
+    if ((rc = check_ctx(ctx))) return rc;
+    const int64_t es = dtype == M1MOE_BF16 ? 2 : 4;
+    if (rows_overlap(d_q, es * q_stride, es * qd, d_out, es * out_stride, es * qd, batch->num_rows))
+        return fail(M1MOE_ERR_INVALID, "d_out must not overlap rows of d_q");
+    if ((rc = set_device(ctx))) return rc;
     PagedAttnArgs a{};
     a.p = view(ctx, kv, batch);
     a.q = d_q;
