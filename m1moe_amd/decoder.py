@@ -14,6 +14,7 @@ compose their own layers.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from dataclasses import dataclass
 from typing import Optional
@@ -234,6 +235,16 @@ class Decoder:
             for layer in layers:
                 self.upload(which, layer, weights(which, layer))
 
+    @staticmethod
+    @contextlib.contextmanager
+    def _held():
+        """hold(buffer): freed at the end of the block, also when it raises."""
+        with contextlib.ExitStack() as stack:
+            def hold(buf):
+                stack.callback(buf.free)
+                return buf
+            yield hold
+
     def reset(self) -> None:
         """InferenceEngine.reset (InferenceEngine.swift:159-163)."""
         check(self.lib.m1moe_dec_reset(self.handle), "m1moe_dec_reset")
@@ -265,10 +276,10 @@ class Decoder:
         """The prompt at once from the current position; returns the greedy
         token after its last token (and that token's logits when asked)."""
         prompt = np.ascontiguousarray(prompt, dtype=np.int32)
-        d = self.ctx.to_device(prompt)
-        self.prefill_device(d, prompt.size, self._tok, self._logits)
-        self.ctx.sync()
-        d.free()
+        with self._held() as hold:
+            d = hold(self.ctx.to_device(prompt))
+            self.prefill_device(d, prompt.size, self._tok, self._logits)
+            self.ctx.sync()
         nxt = int(self._tok.download(np.int32, 1)[0])
         if return_logits:
             return nxt, self._logits.download(np.float32, self.shape.vocab)
@@ -280,15 +291,14 @@ class Decoder:
         n_gen + 1 greedy tokens (the prompt's own prediction first)."""
         prompt = np.ascontiguousarray(prompt, dtype=np.int32)
         P, cap = prompt.size, prompt.size + n_gen + 1
-        seq = self.ctx.alloc(4 * cap)
-        seq.upload(np.concatenate([prompt, np.zeros(cap - P, np.int32)]))
-        self.reset()
-        for _ in range(P + n_gen):
-            self.step_seq(seq, P, cap)
-        self.ctx.sync()
-        out = seq.download(np.int32)[P:]
-        seq.free()
-        return out
+        with self._held() as hold:
+            seq = hold(self.ctx.alloc(4 * cap))
+            seq.upload(np.concatenate([prompt, np.zeros(cap - P, np.int32)]))
+            self.reset()
+            for _ in range(P + n_gen):
+                self.step_seq(seq, P, cap)
+            self.ctx.sync()
+            return seq.download(np.int32)[P:]
 
     def _sample_params(self, buf: DeviceBuffer, u, temperature, top_k, top_p, min_p):
         """Copies n draws and the settings (one each) to buf, 4 + n words; what makes
@@ -313,20 +323,18 @@ class Decoder:
         if np.size(u) != n:
             raise ValueError(f"{np.size(u)} random numbers for {n} tokens")
         ops = DenseOps(self.ctx)
-        buf = self.ctx.alloc(4 * (4 + n))
-        params = self._sample_params(buf, u, temperature, top_k, top_p, min_p)
-        toks, d = self.ctx.alloc(4 * n), self.ctx.to_device(prompt)
-        self.reset()
-        self.prefill_device(d, prompt.size, self._tok, self._logits)
-        for i in range(n):
-            if i:
-                self.step_device(toks.addr + 4 * (i - 1), self._tok, self._logits)
-            ops.sample(self._logits, 1, V, (V + 3) // 4 * 4, params(i), toks.addr + 4 * i)
-        self.ctx.sync()
-        out = toks.download(np.int32)
-        for b in (buf, toks, d):
-            b.free()
-        return out
+        with self._held() as hold:
+            buf, toks = hold(self.ctx.alloc(4 * (4 + n))), hold(self.ctx.alloc(4 * n))
+            d = hold(self.ctx.to_device(prompt))
+            params = self._sample_params(buf, u, temperature, top_k, top_p, min_p)
+            self.reset()
+            self.prefill_device(d, prompt.size, self._tok, self._logits)
+            for i in range(n):
+                if i:
+                    self.step_device(toks.addr + 4 * (i - 1), self._tok, self._logits)
+                ops.sample(self._logits, 1, V, (V + 3) // 4 * 4, params(i), toks.addr + 4 * i)
+            self.ctx.sync()
+            return toks.download(np.int32)
 
     def forward(self, token: int, return_logits: bool = False, temperature: float = 0.0,
                 top_p: float = 1.0, rng: Optional[np.random.Generator] = None, top_k: int = 0,

@@ -56,3 +56,70 @@ def test_rope_frequencies():
 def test_rope_frequencies_refusals(args):
     with pytest.raises(ValueError):
         rope_frequencies(*args)
+
+
+class FakeBuffer:
+    addr = 0x1000
+
+    def __init__(self, ctx, nbytes):
+        self.ctx, self.nbytes = ctx, nbytes
+        ctx.live += 1
+
+    def upload(self, a):
+        assert a.nbytes <= self.nbytes
+        return self
+
+    def download(self, dtype, count=None):
+        return np.zeros(self.nbytes // 4 if count is None else count, dtype)
+
+    def free(self):
+        self.ctx.live -= 1
+
+
+class FakeContext:
+    """Counts its live buffers; sync fails when asked to."""
+    lib, handle, live, fail_sync = None, None, 0, False
+
+    def alloc(self, n):
+        return FakeBuffer(self, n)
+
+    def to_device(self, a):
+        return FakeBuffer(self, a.nbytes)
+
+    def sync(self):
+        if self.fail_sync:
+            raise RuntimeError("sync")
+
+
+@pytest.mark.parametrize("where", ["", "prefill", "step", "sample", "sync", "top_k"])
+@pytest.mark.parametrize("call", ["generate_sampled", "generate", "prefill"])
+def test_buffers_are_freed_when_a_call_raises(monkeypatch, call, where):
+    """A refused prompt, a full cache, a device error: the call's own buffers go all the same."""
+    from m1moe_amd import decoder
+
+    def step(name):
+        def f(*a, **k):
+            if where == name:
+                raise RuntimeError(name)
+        return f
+    dec = decoder.Decoder.__new__(decoder.Decoder)
+    dec.ctx, dec.handle = FakeContext(), None
+    dec.ctx.fail_sync = where == "sync"
+    dec.shape = type("Shape", (), {"vocab": 100})
+    dec._tok = dec._logits = FakeBuffer(dec.ctx, 16)
+    dec.reset, dec.prefill_device = lambda: None, step("prefill")
+    dec.step_device = dec.step_seq = step("step")
+    monkeypatch.setattr(decoder.DenseOps, "__init__", lambda self, ctx: None)
+    monkeypatch.setattr(decoder.DenseOps, "sample", step("sample"))
+    reached = {"generate_sampled": ("prefill", "step", "sample", "sync", "top_k"), "generate": ("step", "sync"),
+               "prefill": ("prefill", "sync")}[call]
+    args = {"generate_sampled": ([1, 2], 3, 0.7), "generate": ([1, 2], 3), "prefill": ([1, 2],)}[call]
+    more = dict(top_k=1 << 40) if call == "generate_sampled" and where == "top_k" else {}
+    before = dec.ctx.live
+    if where in reached:
+        with pytest.raises((RuntimeError, OverflowError, ValueError)):
+            getattr(dec, call)(*args, **more)
+    else:
+        got = getattr(dec, call)(*args)
+        assert call == "prefill" or len(got) == 4
+    assert dec.ctx.live == before
