@@ -443,7 +443,8 @@ typedef struct {
  * page_size, d_kv_len[s] - n >= prefix_len where n > 0.  A sequence that
  * breaks this is skipped, a page outside the cache is not touched (attention
  * reads page 0 in its place); either sets the device error flag, reported by
- * the next m1moe_sync. */
+ * the next m1moe_sync.  (Rows that starts out of order give to two sequences
+ * hold either's result.) */
 typedef struct {
     int32_t num_seqs;
     int32_t num_rows;

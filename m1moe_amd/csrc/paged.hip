@@ -52,9 +52,9 @@ __device__ __forceinline__ void store_vec(void* base, int64_t at, const float (&
 // weight), pairs of their dims are turned by the position's angles, then k and v go
 // to the row's place in the cache, q to its output: every element is read and
 // written once.  Prompts are bound by memory (five of 37 to 1900 tokens, 32 + 2 x 8 heads
-// of 128, bf16: 28.8 us, of which 26.4 at the rate of a large copy), steps by the
-// launch and the chain sequence - page - store (64 tokens 4.3 us; one workgroup for all
-// heads of a row 5.9).
+// of 128, bf16: 28.8 us, of which 26.4 at the rate of a large copy; 20.8 where the same rows
+// come again and the device's last-level cache still has them), steps by the launch and the
+// chain sequence - page - store (64 tokens 4.4 us; one workgroup for all heads of a row 5.9).
 //
 // Workgroup = (row, a share of its q, k and v heads).  A lane holds VEC
 // neighbouring dims (16 bytes) of a head; the head's sum of squares and, in
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // 32 tokens behind 60 to 8100 positions 80.6 us, 4.5 TB/s; 16 heads, all bf16: 48 behind
 // 100 to 4000 117 us, 4.8 TB/s), prompts and turns by a SIMD's two waves, whose MFMAs,
 // softmax and LDS reads overlap only in part (2500 positions, all bf16: 95 us, 535 TFLOP/s;
-// six turns of 9 to 400 tokens behind up to 4000, f32 queries: 73 us, of which 55 are
+// six turns of 9 to 400 tokens behind up to 4000, f32 queries: 73 us, of which 42.5 are
 // the three products at a large matrix product's rate), one token behind few positions by
 // the chain launch - lengths - page - rows - join (14.8 us).
 
@@ -256,8 +256,8 @@ constexpr int kTileKeys = 128;   // what a tile costs besides its keys, in keys
 // place per key; the line is cut into equal shares, one per workgroup, the cuts
 // moved down to a multiple of kCut keys inside their tile, or to its start where it has
 // at most kWhole keys: to join two pieces of one takes longer than to read it (a prompt of
-// 2500 and turns behind up to 4000: 104 and 88 us with every tile cut, 98 and 79 with
-// 512 whole; later 84.2 and 73.2, with 768 whole 87.2 and 83.5).  (Without the places
+// 2500 (one part per weight) and turns behind up to 4000: 104 and 88 us with every tile cut,
+// 98 and 79 with 512 whole; later 84.2 and 73.2, with 768 whole 87.2 and 83.5).  (Without the places
 // per tile the workgroups with the shortest sequences ended last: 32 steps of 60 to
 // 8100 positions, 8 kv heads, median 61 us, last 116.)
 struct Tile {
@@ -1461,7 +1461,7 @@ struct Cut {
 };
 
 // True if a cut tile is done: all its other workgroups had ended, so that this one's rows
-// need not go through memory (a prompt of 2500 positions 83.9 -> 79.9 us).  Joined in the
+// need not go through memory (a prompt of 2500 positions, one part per weight, 83.9 -> 79.9 us).  Joined in the
 // order of the pieces, as join_tile does.
 template <int HD, int QP, int KP, int NT>
 __device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,

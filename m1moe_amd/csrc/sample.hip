@@ -10,10 +10,11 @@
 // multiples of 2^-44, so that their sums are integer sums: exact, whatever their
 // order (2^18 logits of weight 1 stay below 2^63).
 //
-// Bound by the chain of steps on a row: of 28.4 us for one of 50304 at a temperature
-// and a top-p 3.8 are its largest logit, 4.2 the histogram, 5.3 its joining and sums,
-// 9.6 the end of the top-p and 6.5 the draw, each a pass over the row and a few barriers of 16
-// waves; 64 rows with settings of their own and many equal logits take 47 us.  While rows
+// Bound by the chain of steps on a row: of the 28.7 us that one of 50304 at a temperature
+// and a top-p takes from its first clock to its last (one run with clocks between the steps)
+// 3.3 are its largest logit, 4.2 the histogram, 5.4 its joining and sums,
+// 9.5 the end of the top-p and 6.3 the draw, each a pass over the row and a few barriers of 16
+// waves; 64 rows with settings of their own and many equal logits take 46 us.  While rows
 // are fewer than CUs several workgroups share a row's histogram, and the last of
 // them to end adds the others' up and searches.
 #include <hip/hip_runtime.h>

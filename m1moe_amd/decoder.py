@@ -113,10 +113,13 @@ def weight_count(which: int, hidden: int, s: DecShape) -> int:
 def rope_frequencies(theta: float, rotary_dim: int, factor: float = 1.0, kind: str = "parts",
                      trained_len: int = 0, slow: float = 1.0, fast: float = 32.0):
     """(inv_freq f32 [rotary_dim / 2], amplitude) for KVAppend: theta^(-2i / rotary_dim),
-    for contexts `factor` times the trained one: "linear" divides every frequency by it,
-    "base" raises theta so that only the slowest pair's is, "parts" divides those of pairs
-    with at most `slow` turns over trained_len positions, keeps those with `fast` or more,
-    blends between, and scales cos and sin by 0.1 ln(factor) + 1."""
+    for contexts `factor` times the trained one: "linear" divides every frequency by it
+    (position interpolation), "base" raises theta so that only the slowest pair's is (a
+    scaled base), "parts" divides those of pairs with at most `slow` turns over trained_len
+    positions, keeps those with `fast` or more, blends between and scales cos and sin by
+    0.1 ln(factor) + 1: the formulas of the YaRN paper, whose blend is linear in the turns.
+    A checkpoint whose own blend is linear in the pair's index, or with another amplitude, needs
+    frequencies of its own.  No published values are at hand to compare with: parity unpinned."""
     if rotary_dim <= 0 or rotary_dim % 2 or not theta > 0 or not factor >= 1:
         raise ValueError(f"rotary_dim {rotary_dim} / theta {theta} / factor {factor}: need an even "
                          "positive rotary_dim, theta > 0 and factor >= 1")
