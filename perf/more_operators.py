@@ -321,8 +321,9 @@ def prepare(case, seed):
     if c["kind"] == "accept":
         st["kv"] = _layers(c, seed, pages)
         draft, drawn = _tokens(c, seed)
-        st["draft"], st["drawn"] = _dev(draft), _dev(drawn)
-        st["path"] = torch.zeros((st["nodes"],), dtype=torch.int32, device=DEV)
+        pad = np.zeros(c["pad"], np.int64)
+        st["draft"], st["drawn"] = (_dev(np.concatenate([t, pad])) for t in (draft, drawn))
+        st["path"] = torch.zeros((n,), dtype=torch.int32, device=DEV)
         st["some"] = torch.zeros((3, c["seqs"]), dtype=torch.int32, device=DEV)
         return st
     st["kc"], st["vc"] = _cache(c, seed, pages, st["table"])
@@ -463,7 +464,7 @@ def _plain_accept(st):
     at, to, table = base[seq] + src, (base[:, None] + i)[real], st["table"].long()
     moved = st["kv"][:, :, table[seq, at // c["page"]], at % c["page"]]
     st["kv"][:, :, table[seq, to // c["page"]], to % c["page"]] = moved
-    st["path"].copy_(path[real])
+    st["path"][:st["nodes"]] = path[real].int()
     st["some"][0], st["some"][1] = count, drawn.gather(1, last)[:, 0]
     st["some"][2] = base + count
     return st["path"], st["some"], st["kv"]
@@ -677,7 +678,8 @@ def _exact_accept(c, seed):
     start, _, parent = _tree(c, seed)
     draft, drawn = _tokens(c, seed)
     length, tab, kv, ps = _batch(c)[1], st["table"].long(), st["kv"].double(), c["page"]
-    path, some = np.full(int(start[-1]), -1, np.int32), np.zeros((3, c["seqs"]), np.int32)
+    path, some = np.zeros(int(start[-1]) + c["pad"], np.int32), np.zeros((3, c["seqs"]), np.int32)
+    path[:start[-1]] = -1
     for s in range(c["seqs"]):
         lo, hi = int(start[s]), int(start[s + 1])
         base, way = length[s] - (hi - lo), [0]
