@@ -532,6 +532,90 @@ int32_t m1moe_sample(m1moe_ctx_t ctx, const float* d_logits, int32_t rows,
                      const m1moe_sample_params* params, int32_t* d_tokens,
                      float* d_probs);
 
+/* ---- drafted tokens ------------------------------------------------------
+ * A step that verifies drafts runs a tree of tokens per sequence through the
+ * layers: the rows of a sequence in an m1moe_paged_batch are its tree, row 0 the
+ * last token that is certain, every other row a drafted one that hangs on an
+ * earlier row, its parent.  Their keys and values are stored row by row behind
+ * the conversation's kv_len - n positions; a row sees those and its own
+ * ancestors, and its angle is that of its depth.  Then a token is drawn at every
+ * row (m1moe_sample), and the drafts that were drawn are taken over.  All
+ * asynchronous on the context stream, without a workspace of their own but
+ * m1moe_tree_attention's, which is m1moe_paged_attention's.  A tree has at most
+ * 256 rows. */
+
+/* Who sees whom, and depths, from every row's parent: d_parents[row] is the
+ * parent's number in the same tree (0 its first row), -1 for none, and lower than
+ * the row's own (one that is not counts as none and sets the device error flag,
+ * reported by the next m1moe_sync).  Row i of a tree gets in d_mask[row]
+ * [mask_words] bit j (word j / 64, bit j % 64) for itself and every ancestor j, in
+ * d_depth[row] the number of its ancestors.  Rows outside every sequence are left
+ * as they were; a sequence whose starts are out of range or that has more than
+ * 64 * mask_words rows is skipped and sets the flag.
+ * 1 <= num_seqs <= 1024, 1 <= num_rows <= 1048576, 1 <= mask_words <= 4. */
+int32_t m1moe_tree_plan(m1moe_ctx_t ctx, int32_t num_seqs, int32_t num_rows,
+                        const int32_t* d_row_start, const int32_t* d_parents,
+                        int32_t mask_words, uint64_t* d_mask, int32_t* d_depth);
+
+/* m1moe_kv_append for the rows of trees: a row is stored at its own slot, d_kv_len
+ * - n + i for row i, and rotated by the position d_kv_len - n + d_depth[row]. */
+int32_t m1moe_tree_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
+                          const m1moe_paged_batch* batch,
+                          const m1moe_kv_append_args* args, const int32_t* d_depth);
+
+/* m1moe_paged_attention for the rows of trees: row i sees the d_kv_len - n
+ * positions before its tree and, of its tree, the rows j <= i whose bit is set in
+ * d_mask[row][mask_words] (its own among them only if set).  A row that sees
+ * nothing gives zeros, as one whose scores are all -inf does.  A sequence of more
+ * than 64 * mask_words rows is skipped and sets the device error flag. */
+int32_t m1moe_tree_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
+                             const m1moe_paged_batch* batch, const uint64_t* d_mask,
+                             int32_t mask_words, const void* d_q, int64_t q_stride,
+                             void* d_out, int64_t out_stride, int32_t dtype,
+                             int32_t num_heads);
+
+/* What a sequence keeps of its tree.  From row 0 on the path goes to the lowest
+ * child whose token d_drafts[row] is the one drawn at the path's row,
+ * d_drawn[row].  The path's rows, in all num_caches caches (the layers', alike in
+ * type and sizes, 1 to 64, sharing no memory), move to the places base, base + 1,
+ * .. (base = d_kv_len - n); what stood at other places of the tree stays.  Per
+ * row: d_path[row_start + i] = the path's row i, -1 past its end.  Per sequence:
+ * d_accepted = rows of the path, d_next = the token drawn at its last row (the
+ * next tree's row 0), d_past = base + accepted; 0, -1 and d_kv_len for a sequence
+ * without rows.  One that is out of range or has more than 256 rows is skipped
+ * with the same results, a move from or to a page outside the cache is left out
+ * and a parent that is not lower than its row counts as none: each sets the
+ * device error flag.  Outputs must not overlap inputs or each other. */
+int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs,
+                          int32_t num_caches, const m1moe_paged_batch* batch,
+                          const int32_t* d_parents, const int32_t* d_drafts,
+                          const int32_t* d_drawn, int32_t* d_path,
+                          int32_t* d_accepted, int32_t* d_next, int32_t* d_past);
+
+/* Weights as m1moe_quantize_4bit makes them: [rows][cols / 8] words, column 8w + j
+ * in bits 4j..4j+3 of word w, and bf16 scales and biases [rows][cols / group_size];
+ * weight = nibble * scale + bias.  group_size is 32, 64 or 128 and divides cols;
+ * rows <= 1048576, cols <= 65536; pointers are 16-byte aligned. */
+typedef struct {
+    const uint32_t* d_w;
+    const uint16_t* d_scales;
+    const uint16_t* d_biases;
+    int32_t rows;
+    int32_t cols;
+    int32_t group_size;
+} m1moe_q4_weights;
+
+/* y[t][r] = sum_c x[t][c] W[r][c] (+ residual[t][r]) for 1 to 65536 tokens t.  x
+ * [tokens][cols] in x_dtype, y and residual (NULL: none; d_y itself: in place)
+ * [tokens][rows] in y_dtype, y_stride elements apart; row strides are multiples of
+ * 16 bytes.  f32 rows give an f32 y, bf16 ones either.  Products are exact and
+ * summed in f32, a group's first; a row of x that holds an infinity or a NaN, or
+ * an f32 above the largest bf16, gives results that are not finite. */
+int32_t m1moe_matmul_q4(m1moe_ctx_t ctx, const m1moe_q4_weights* weights,
+                        const void* d_x, int32_t x_dtype, int64_t x_stride,
+                        int32_t tokens, const void* d_residual, void* d_y,
+                        int32_t y_dtype, int64_t y_stride);
+
 /* ---- the converted model directory on disk (host-side) -----------------
  * scripts/extract_olmoe.py writes model_weights.bin (non-expert tensors,
  * 4-byte aligned) + model_weights.json ({name: {offset, shape, dtype}}) and

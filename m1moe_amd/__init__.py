@@ -7,7 +7,7 @@ around it (decoder.py: InferenceEngine.forward on the GPU), plus the seeded
 synthetic workloads (synth.py).
 """
 from ._lib import (KVAppend, M1MOE_BF16, M1MOE_F32, M1MoEError, MoEShape, PROJ_DOWN, PROJ_GATE,
-                   PROJ_UP, PagedBatch, PagedKV, SampleParams, load)
+                   PROJ_UP, PagedBatch, PagedKV, Q4Weights, SampleParams, load)
 from .engine import (DeviceBuffer, HIPContext, MoEBlock, ModelSpec, check_shape, expert_bytes,
                      expert_offsets, make_shape)
 from .decoder import AttentionSpec, Decoder, DecoderSpec, DenseOps, rope_frequencies
@@ -16,6 +16,6 @@ __all__ = [
     "M1MOE_BF16", "M1MOE_F32", "M1MoEError", "MoEShape", "PROJ_DOWN", "PROJ_GATE", "PROJ_UP",
     "load", "DeviceBuffer", "HIPContext", "MoEBlock", "ModelSpec", "check_shape",
     "expert_bytes", "expert_offsets", "make_shape", "AttentionSpec", "Decoder", "DecoderSpec",
-    "DenseOps", "KVAppend", "PagedBatch", "PagedKV", "SampleParams",
+    "DenseOps", "KVAppend", "PagedBatch", "PagedKV", "Q4Weights", "SampleParams",
     "rope_frequencies",
 ]

@@ -89,6 +89,11 @@ class PagedKV(ctypes.Structure):
         return PagedKV(_address(k), _address(v), dtype_code(dtype), num_pages, page_size,
                        num_kv_heads, head_dim)
 
+    @staticmethod
+    def array(caches):
+        """Several caches (a model's layers) as one call takes them."""
+        return (PagedKV * len(caches))(*caches)
+
 
 class PagedBatch(ctypes.Structure):
     """m1moe_paged_batch: the rows, lengths and page tables of one call."""
@@ -159,6 +164,23 @@ class SampleParams(ctypes.Structure):
     def make(u, temperature=None, top_k=None, top_p=None, min_p=None) -> "SampleParams":
         return SampleParams(_address(u), _address(temperature), _address(top_k), _address(top_p),
                             _address(min_p))
+
+
+class Q4Weights(ctypes.Structure):
+    """m1moe_q4_weights: a matrix in 4 bits with a scale and a bias per group of columns."""
+
+    _fields_ = [
+        ("d_w", c_void_p),
+        ("d_scales", c_void_p),
+        ("d_biases", c_void_p),
+        ("rows", c_int32),
+        ("cols", c_int32),
+        ("group_size", c_int32),
+    ]
+
+    @staticmethod
+    def make(w, scales, biases, rows: int, cols: int, group_size: int) -> "Q4Weights":
+        return Q4Weights(_address(w), _address(scales), _address(biases), rows, cols, group_size)
 
 
 # dtypes of the on-disk manifest (m1moe_store_tensor)
@@ -244,6 +266,19 @@ _PROTOTYPES = [
     ("m1moe_sample", c_int32,
      [c_void_p, c_void_p, c_int32, c_int32, ctypes.c_int64, POINTER(SampleParams), c_void_p,
       c_void_p]),
+    ("m1moe_tree_plan", c_int32,
+     [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
+    ("m1moe_tree_append", c_int32,
+     [c_void_p, POINTER(PagedKV), POINTER(PagedBatch), POINTER(KVAppend), c_void_p]),
+    ("m1moe_tree_attention", c_int32,
+     [c_void_p, POINTER(PagedKV), POINTER(PagedBatch), c_void_p, c_int32, c_void_p,
+      ctypes.c_int64, c_void_p, ctypes.c_int64, c_int32, c_int32]),
+    ("m1moe_tree_accept", c_int32,
+     [c_void_p, POINTER(PagedKV), c_int32, POINTER(PagedBatch), c_void_p, c_void_p, c_void_p,
+      c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("m1moe_matmul_q4", c_int32,
+     [c_void_p, POINTER(Q4Weights), c_void_p, c_int32, ctypes.c_int64, c_int32, c_void_p,
+      c_void_p, c_int32, ctypes.c_int64]),
     ("m1moe_store_open", c_int32, [c_char_p, c_char_p, POINTER(c_void_p)]),
     ("m1moe_store_close", None, [c_void_p]),
     ("m1moe_store_count", c_int32, [c_void_p, POINTER(c_int32)]),

@@ -787,6 +787,11 @@ int32_t m1moe_sync(m1moe_ctx_t ctx) {
             return fail(M1MOE_ERR_DEVICE,
                         "a paged batch names a page outside the cache; nothing was stored there "
                         "(device flag 0x%x)", flag);
+        if (flag & kErrTree)
+            return fail(M1MOE_ERR_DEVICE,
+                        "a tree of drafted tokens has a parent that does not come before its row (it "
+                        "counts as none), or more rows than its masks cover (it was skipped; device "
+                        "flag 0x%x)", flag);
         return fail(M1MOE_ERR_DEVICE,
                     "a decode hand-off wait timed out (device flag 0x%x); state was reset", flag);
     }

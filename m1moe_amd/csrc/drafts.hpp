@@ -1,0 +1,49 @@
+// drafts.hpp — kernel arguments of the drafted tokens' trees (tree.hip) and of the
+// products with 4-bit weights (q4.hip).
+#pragma once
+
+#include <cstdint>
+
+#include "paged.hpp"
+
+namespace m1moe {
+
+constexpr int kTreeWords = 4;                 // most 64-bit words of a row's mask
+constexpr int kTreeRows = 64 * kTreeWords;    // most rows of a tree
+constexpr int kMostCaches = 64;               // caches of one accept
+
+struct TreePlanArgs {
+    int32_t num_seqs, num_rows, words;
+    const int32_t *row_start, *parents;
+    uint64_t* mask;
+    int32_t* depth;
+    uint32_t* err;
+};
+
+struct TreeAcceptArgs {
+    PagedView p;              // (k and v: not used)
+    void* planes[2 * kMostCaches];   // every cache's k and v
+    int32_t num_planes;
+    int32_t row_units;        // 16-byte units of a position
+    const int32_t *parents, *drafts, *drawn;
+    int32_t *path, *accepted, *next, *past;
+};
+
+struct Q4Args {
+    const uint32_t* w;
+    const uint16_t *scales, *biases;
+    int32_t rows, cols, group;
+    const void* x;
+    int64_t x_stride;
+    int32_t tokens;
+    const void* residual;     // as y, or null
+    void* y;
+    int64_t y_stride;
+    int32_t x_bf16, y_bf16;
+};
+
+int launch_tree_plan(const TreePlanArgs& a, void* stream);
+int launch_tree_accept(const TreeAcceptArgs& a, void* stream);
+int launch_matmul_q4(const Q4Args& a, int cus, void* stream);
+
+}  // namespace m1moe

@@ -85,8 +85,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     if (place == ~0ull) return;
     const int seq = (int)(place >> 32), pos = (int)(uint32_t)place;
     const int page = p.pages[(int64_t)seq * p.table_stride + (pos >> p.page_shift)];
+    const int row0 = a.depth ? p.row_start[seq] : 0;
     if (tid < a.rotary / 2) {
-        const double ang = (double)pos * (double)a.inv_freq[tid];
+        // (a drafted token: the position of its depth in the tree, not of its slot)
+        const double at = a.depth ? (double)(pos - (row - row0)) + (double)a.depth[row] : (double)pos;
+        const double ang = at * (double)a.inv_freq[tid];
         const double k = rint(ang * 0.15915494309189533577);
         const double rest = fma(-k, 2.4492935982947064e-16, fma(-k, 6.283185307179586232, ang));
         // (what its rounding to f32 leaves, up to 2^-23, turns the pair once more)
@@ -167,7 +170,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 }
 
 // ---- attention -----------------------------------------------------------------------
-//
+
+// A sequence that is computed: of a tree, one whose rows the masks cover.
+template <bool TREE>
+__device__ __forceinline__ bool attn_ok(const PagedAttnArgs& a, int lo, int hi, int len) {
+    return seq_ok(a.p, lo, hi, len) && (!TREE || hi - lo <= 64 * a.mask_words);
+}
+
 // out = sum_p e^(s_p - m) v_p / sum_p e^(s_p - m), s_p = q . k_p / sqrt(head_dim), over the
 // positions p up to the row's own, in one pass over them with a running m.  Scores and
 // weighted sums are MFMAs of bf16 operands with f32 sums.  bf16 queries and
@@ -342,7 +351,9 @@ struct Line {
 };
 
 // Fills cum and the line: the whole workgroup of 256.  tmp: LDS, 4 values.
-__device__ __forceinline__ void make_line(const PagedView& p, Line& ln, int64_t* tmp, int grid, bool flag) {
+template <bool TREE>
+__device__ __forceinline__ void make_line(const PagedAttnArgs& a, Line& ln, int64_t* tmp, int grid, bool flag) {
+    const PagedView& p = a.p;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     int64_t carry = 0;
     for (int b0 = 0; b0 < p.num_seqs; b0 += 256) {
@@ -352,6 +363,8 @@ __device__ __forceinline__ void make_line(const PagedView& p, Line& ln, int64_t*
             const int lo = p.row_start[s], hi = p.row_start[s + 1], len = p.kv_len[s], n = hi - lo;
             if (!seq_ok(p, lo, hi, len)) {
                 if (flag) flag_error(p.err, kErrPagedBatch);
+            } else if (!attn_ok<TREE>(a, lo, hi, len)) {
+                if (flag) flag_error(p.err, kErrTree);
             } else if (n > 0) {
                 keys = ln.kv_heads * ln.head_places(len - n, n, (n + ln.TT - 1) / ln.TT);
             }
@@ -411,12 +424,13 @@ struct Work {
     int head0;                // first query head
     int lo, hi;               // keys [lo, hi), lo a multiple of 32
     int first, last;          // positions that may be read and seen (others are not)
+    int tree0;                // of a tree: its first row's position, from which on masks say who is seen
     int head;                 // kv head
     const int32_t* table;
 
     // (the same in every lane: into scalar registers)
     __device__ __forceinline__ void uniform() {
-        for (int* x : {&token0, &tokens, &pos0, &head0, &lo, &hi, &last, &head}) *x = __builtin_amdgcn_readfirstlane(*x);
+        for (int* x : {&token0, &tokens, &pos0, &head0, &lo, &hi, &last, &tree0, &head}) *x = __builtin_amdgcn_readfirstlane(*x);
         const uint64_t t = reinterpret_cast<uint64_t>(table);
         table = reinterpret_cast<const int32_t*>(
             (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 32)) << 32 |
@@ -470,6 +484,16 @@ struct Cache {
     }
 };
 
+// Bits 0 .. 7: whether row `token` of a tree sees the positions j .. j + 7 of it, j < 0 being
+// before the tree (all seen), those past the mask's words not seen.
+__device__ __forceinline__ uint32_t tree_bits(const PagedAttnArgs& a, int token, int j) {
+    const int n = 2 * a.mask_words, w = j >> 5;
+    const __attribute__((address_space(1))) uint32_t* m =
+        (const __attribute__((address_space(1))) uint32_t*)(a.mask + (int64_t)token * a.mask_words);
+    const uint32_t x = m[min(max(w, 0), n - 1)], y = m[min(max(w + 1, 0), n - 1)];
+    return __builtin_amdgcn_alignbit(w + 1 < 0 ? ~0u : w + 1 < n ? y : 0u, w < 0 ? ~0u : w < n ? x : 0u, j & 31);
+}
+
 // The (token, query head) of row rho of the work; false past its rows.
 __device__ __forceinline__ bool row_at(const PagedAttnArgs& a, const Work& w, int rho, int& token, int& head) {
     const int t = rho / a.share;
@@ -486,7 +510,7 @@ __device__ __forceinline__ bool row_at(const PagedAttnArgs& a, const Work& w, in
 // other one.  Row 4 g + v of output MFMA j is dim VD (4 g + v) + j where a lane
 // loads the VD = HD / 16 neighbouring dims VD c .. of eight keys itself (SPREAD),
 // else dim 16 j + 4 g + v.
-template <int HD, int QP, int NT, bool SPREAD>
+template <int HD, int QP, int NT, bool SPREAD, bool TREE>
 struct Rows {
     static constexpr int NS = HD / 32, VD = HD / 16;
     // Parts of a weight.  bf16 queries: two, whose rest of 2^-16 is nothing beside the output's own
@@ -529,7 +553,7 @@ struct Rows {
             int token, head;
             const bool on = row_at(a, w, rho0 + 16 * t + c, token, head);
             qpos[t] = w.pos0 + (token - w.token0) * w.row_pos;
-            see = min(see, qpos[t]);
+            see = min(see, TREE ? min(qpos[t], w.tree0 - 1) : qpos[t]);
             most = max(most, qpos[t]);
             const int64_t at = (int64_t)token * a.q_stride + (int64_t)head * HD + 8 * g;
             const f32x4v* x = QP == 1 ? reinterpret_cast<const f32x4v*>(static_cast<const uint16_t*>(a.q) + at)
@@ -632,7 +656,7 @@ struct Rows {
     // is above 2^kGrown, and all are rounded relative to themselves.
     static constexpr float kGrown = 8.f;
     template <int NB>
-    __device__ __forceinline__ void softmax(const Work& w, int kb, f32x4v (&s)[NB][NT][2], float unit,
+    __device__ __forceinline__ void softmax(const PagedAttnArgs& a, const Work& w, int kb, f32x4v (&s)[NB][NT][2], float unit,
                                             bf16x8 (&pp)[NB][NT][PP]) {
         const bool whole = kb >= w.first && kb + 32 * NB - 1 <= see && kb + 32 * NB <= w.hi;
         if (!whole) {
@@ -640,11 +664,16 @@ struct Rows {
             for (int t = 0; t < NT; ++t) {
                 const int top = min(min(qpos[t], w.last), w.hi - 1) - kb - 8 * g, low = w.first - kb - 8 * g;
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t seen = 0xFFu;
+                    if constexpr (TREE)
+                        seen = tree_bits(a, w.token0 + qpos[t] - w.pos0, kb + 32 * b + 8 * g - w.tree0);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        s[b][t][e >> 2][e & 3] =
-                            32 * b + e >= low && 32 * b + e <= top ? s[b][t][e >> 2][e & 3] : -INFINITY;
+                    for (int e = 0; e < 8; ++e) {
+                        const bool in = 32 * b + e >= low && 32 * b + e <= top && (!TREE || (seen >> e & 1));
+                        s[b][t][e >> 2][e & 3] = in ? s[b][t][e >> 2][e & 3] : -INFINITY;
+                    }
+                }
             }
         }
 #pragma unroll
@@ -752,6 +781,7 @@ struct Rows {
             }
             for (int kb = lo; kb <= top; kb += step)
                 for (int k = max(kb, w.first); k <= min(kb + 31, top); ++k) {
+                    if (TREE && k >= w.tree0 && !(tree_bits(a, token, k - w.tree0) & 1)) continue;
                     const int64_t at = kv.at(kv.known(kv.page_of(k), bad), k) + PL * lane * kv.ES;
                     float s = 0.f, v[PL];
 #pragma unroll
@@ -793,9 +823,9 @@ struct Rows {
 // block is computed the next one's rows are on their way, K's from the moment the
 // scores have used the last, V's from the end of the block, and the page numbers
 // of the one after.
-template <int HD, int QP, int KP>
-struct Deep : Rows<HD, QP, 1, true> {
-    typedef Rows<HD, QP, 1, true> R;
+template <int HD, int QP, int KP, bool TREE>
+struct Deep : Rows<HD, QP, 1, true, TREE> {
+    typedef Rows<HD, QP, 1, true, TREE> R;
     static constexpr int NS = R::NS, VD = R::VD;
     using R::acc;
     using R::c;
@@ -924,7 +954,7 @@ struct Deep : Rows<HD, QP, 1, true> {
                 R::total(part, s[0]);
                 if (nb < hi) load_k(kv, nb, kv.known(pk, bad));
                 bf16x8 pp[1][1][R::PP];
-                this->template softmax<1>(w, kb, s, unit, pp);
+                this->template softmax<1>(a, w, kb, s, unit, pp);
                 if (kv.edge(kb, 32)) clear_v(kv, kb);
                 constexpr int JG = KP == 1 ? 4 : 2;
 #pragma unroll
@@ -1152,9 +1182,9 @@ struct Stage<HD, 3> {
     }
 };
 
-template <int HD, int QP, int KP, int NT>
-struct Wide : Rows<HD, QP, NT, false> {
-    typedef Rows<HD, QP, NT, false> R;
+template <int HD, int QP, int KP, int NT, bool TREE>
+struct Wide : Rows<HD, QP, NT, false, TREE> {
+    typedef Rows<HD, QP, NT, false, TREE> R;
     typedef Stage<HD, KP> S;
     static constexpr int NS = R::NS, VD = R::VD;
     // 32-key blocks a softmax takes at once: two halve its maxima and rescalings
@@ -1163,7 +1193,7 @@ struct Wide : Rows<HD, QP, NT, false> {
     // between(i): called in the course of it, i = 0 .. kBreaks - 1
     static constexpr int kBreaks = NB + 1;
     template <class F>
-    __device__ __forceinline__ void blocks(const Work& w, int kb, int b0, float unit, const uint8_t* s_kv,
+    __device__ __forceinline__ void blocks(const PagedAttnArgs& a, const Work& w, int kb, int b0, float unit, const uint8_t* s_kv,
                                            F&& between) {
         const int g = this->g, c = this->c;
         f32x4v s[NB][NT][2];
@@ -1189,7 +1219,7 @@ struct Wide : Rows<HD, QP, NT, false> {
         }
         __builtin_amdgcn_s_setprio(0);
         bf16x8 pp[NB][NT][R::PP];
-        this->template softmax<NB>(w, kb, s, unit, pp);
+        this->template softmax<NB>(a, w, kb, s, unit, pp);
         between(NB);
         __builtin_amdgcn_s_setprio(1);
         constexpr int JG = KP == 1 ? 4 : 2;
@@ -1213,7 +1243,8 @@ struct Wide : Rows<HD, QP, NT, false> {
         __builtin_amdgcn_s_setprio(0);
     }
     // `rows`: whether the wave has some (those without take part in the staging)
-    __device__ __forceinline__ void run(const PagedView& p, const Work& w, bool rows, float unit, uint8_t* s_kv) {
+    __device__ __forceinline__ void run(const PagedAttnArgs& a, const Work& w, bool rows, float unit, uint8_t* s_kv) {
+        const PagedView& p = a.p;
         const Cache<HD, KP> kv(p, w);
         const int hi = rows ? min(w.hi, min(this->most, w.last) + 1) : 0;
         bool bad = false;
@@ -1247,10 +1278,10 @@ struct Wide : Rows<HD, QP, NT, false> {
                 const bool on = k0 < hi;
                 rest(0, on ? 1 : S::N);
                 if (on)
-                    blocks(w, k0, 0, unit, buf, [&](int i) { rest(i + 1, i + 1 < kBreaks ? i + 2 : S::N); });
+                    blocks(a, w, k0, 0, unit, buf, [&](int i) { rest(i + 1, i + 1 < kBreaks ? i + 2 : S::N); });
 #pragma unroll
                 for (int b = NB; b < S::SK / 32; b += NB)
-                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, buf, [](int) {});
+                    if (k0 + 32 * b < hi) blocks(a, w, k0 + 32 * b, b, unit, buf, [](int) {});
             }
         } else {
             st.load(kv, w.lo, bad);
@@ -1266,7 +1297,7 @@ struct Wide : Rows<HD, QP, NT, false> {
                 }
 #pragma unroll
                 for (int b = 0; b < S::SK / 32; b += NB)
-                    if (k0 + 32 * b < hi) blocks(w, k0 + 32 * b, b, unit, s_kv, [](int) {});
+                    if (k0 + 32 * b < hi) blocks(a, w, k0 + 32 * b, b, unit, s_kv, [](int) {});
             }
         }
         if (bad) flag_error(p.err, kErrPagedPage);
@@ -1319,6 +1350,12 @@ __device__ __forceinline__ void load8_coh(const float* const (&p)[8], f32x4v (&v
         : "memory");
 }
 
+// One over a row's sum of weights.  (A row of a tree may see nothing: zeros.)
+template <bool TREE>
+__device__ __forceinline__ float over(float l) {
+    return TREE && l == 0.f ? 0.f : 1.0f / l;
+}
+
 // Where a finished tile's rows go: divided by their sums to out, or as they are, with
 // their maxima and sums, to a piece of the batch's rows (token, head) or, row by row, to
 // a workgroup's slot, which another workgroup reads.
@@ -1366,15 +1403,15 @@ constexpr int wgs_per_cu(int hd) { return hd <= 128 ? 2 : 1; }
 template <int HD, int KP>
 constexpr int work_lds() {
     return std::max({Stage<HD, KP>::kBuffers * Stage<HD, KP>::kBytes, (4 * 16 * HD + 128) * 4,
-                     16 * HD + 4 * Deep<HD, 3, KP>::kQueries});
+                     16 * HD + 4 * Deep<HD, 3, KP, false>::kQueries});
 }
 
-template <int HD, int QP, int KP>
+template <int HD, int QP, int KP, bool TREE>
 __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
                                          const Sink<HD>& sink) {
     constexpr int kWave = 16 * HD, VD = HD / 16;
     const int tid = thread_id(), wave = tid >> 6, lane = tid & 63;
-    Deep<HD, QP, KP> r;
+    Deep<HD, QP, KP, TREE> r;
     // (the queries behind what run_plain of another wave may write)
     r.run(a, w, w.lo + 32 * wave, 128, unit, s_buf + 16 * HD + wave * r.kQueries);
     float* s = reinterpret_cast<float*>(s_buf);      // [4 waves][VD][64][4]
@@ -1402,7 +1439,7 @@ __device__ __forceinline__ void few_rows(const PagedAttnArgs& a, const Work& w, 
     }
     if (!on) return;
     // lane (g, c) of wave v: of row c the dims VD (4 g + v) .. + VD - 1
-    const float inv = 1.0f / l;
+    const float inv = over<TREE>(l);
 #pragma unroll
     for (int j0 = 0; j0 < VD; j0 += 4) {
         float x[4];
@@ -1435,7 +1472,7 @@ __device__ __forceinline__ Sink<HD> piece_of(const PagedAttnArgs& a, int i) {
     return {kToPiece, a.pre + i * rows * HD, a.pre + (a.splits + 1) * rows * HD + i * rows * 2};
 }
 
-template <int HD, int QP, class R>
+template <int HD, int QP, bool TREE, class R>
 __device__ __forceinline__ void many_out(const PagedAttnArgs& a, const Work& w, int rho0, const R& r,
                                          const Sink<HD>& sink) {
 #pragma unroll
@@ -1443,7 +1480,7 @@ __device__ __forceinline__ void many_out(const PagedAttnArgs& a, const Work& w, 
         const int rho = rho0 + 16 * t + r.c;
         int token, head;
         if (!row_at(a, w, rho, token, head)) continue;
-        const float f = 1.0f / r.l[t];
+        const float f = over<TREE>(r.l[t]);
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
             sink.put(a, QP == 1, rho, token, head, 16 * j + 4 * r.g, r.m[t], r.l[t], f, r.acc[t][j][0],
@@ -1463,17 +1500,17 @@ struct Cut {
 // True if a cut tile is done: all its other workgroups had ended, so that this one's rows
 // need not go through memory (a prompt of 2500 positions, one part per weight, 83.9 -> 79.9 us).  Joined in the
 // order of the pieces, as join_tile does.
-template <int HD, int QP, int KP, int NT>
+template <int HD, int QP, int KP, int NT, bool TREE>
 __device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
                                           const Sink<HD>& sink, const Cut<HD>& cut) {
     const int wave = thread_id() >> 6, rho0 = wave * 16 * NT;
     const bool rows = rho0 < w.tokens * a.share;
-    Wide<HD, QP, KP, NT> r;
+    Wide<HD, QP, KP, NT, TREE> r;
     r.lanes();
-    f32x4v raw[NT][HD / 32][Wide<HD, QP, KP, NT>::R::kRaw];
+    f32x4v raw[NT][HD / 32][Wide<HD, QP, KP, NT, TREE>::R::kRaw];
     r.read(a, w, rho0, raw);
     r.split(raw);
-    r.run(a.p, w, rows, unit, s_buf);
+    r.run(a, w, rows, unit, s_buf);
     if (rows && r.odd())
         r.template run_plain<KP>(a, w, rho0, w.lo, 32, unit, reinterpret_cast<float*>(s_buf) + wave * HD);
     if (cut.counter) {
@@ -1527,26 +1564,26 @@ __device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w,
                     r.m[t] = m;
                     r.l[t] = l;
                 }
-                many_out<HD, QP>(a, w, rho0, r, cut.done);
+                many_out<HD, QP, TREE>(a, w, rho0, r, cut.done);
             }
             return true;
         }
     }
-    if (rows) many_out<HD, QP>(a, w, rho0, r, sink);
+    if (rows) many_out<HD, QP, TREE>(a, w, rho0, r, sink);
     return false;
 }
 
-template <int HD, int QP, int KP>
+template <int HD, int QP, int KP, bool TREE>
 __device__ __forceinline__ bool compute(const PagedAttnArgs& a, const Work& w, float unit, uint8_t* s_buf,
                                         const Sink<HD>& sink, const Cut<HD>& cut) {
     const int n = w.tokens * a.share;
     if (n <= 16) {
-        few_rows<HD, QP, KP>(a, w, unit, s_buf, sink);
+        few_rows<HD, QP, KP, TREE>(a, w, unit, s_buf, sink);
         return false;
     }
-    if (tile_groups<HD, QP>() == 1 || n <= 64) return many_rows<HD, QP, KP, 1>(a, w, unit, s_buf, sink, cut);
+    if (tile_groups<HD, QP>() == 1 || n <= 64) return many_rows<HD, QP, KP, 1, TREE>(a, w, unit, s_buf, sink, cut);
     if constexpr (tile_groups<HD, QP>() > 1)
-        return many_rows<HD, QP, KP, tile_groups<HD, QP>()>(a, w, unit, s_buf, sink, cut);
+        return many_rows<HD, QP, KP, tile_groups<HD, QP>(), TREE>(a, w, unit, s_buf, sink, cut);
     return false;
 }
 
@@ -1554,7 +1591,7 @@ __device__ __forceinline__ bool compute(const PagedAttnArgs& a, const Work& w, f
 // Few values: the threads that they leave share the pieces, eight loads of each in
 // flight, and join theirs through LDS.  Many: eight values of a thread in flight, piece
 // after piece.  Either way in an order that does not depend on who is last.
-template <int HD, int QP>
+template <int HD, int QP, bool TREE>
 __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w, int first, int last, float unit,
                                           uint8_t* s_buf, const Sink<HD>& sink) {
     constexpr int NV = tile_rows<HD, QP>() * HD / 4 / 256;
@@ -1603,7 +1640,7 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
                 join(m, l, y[4], y[5], unit, f0, f1);
                 o = mix(o, f0, *reinterpret_cast<const f32x4v*>(y), f1);
             }
-            sink.put(a, QP == 1, rho, token, head, d, m, l, 1.0f / l, o[0], o[1], o[2], o[3]);
+            sink.put(a, QP == 1, rho, token, head, d, m, l, over<TREE>(l), o[0], o[1], o[2], o[3]);
         }
         return;
     }
@@ -1642,7 +1679,7 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
             const int i = tid + 256 * (k0 + k), rho = i / (HD / 4);
             int token, head;
             if (rho < rows && row_at(a, w, rho, token, head))
-                sink.put(a, QP == 1, rho, token, head, 4 * (i % (HD / 4)), m[k], l[k], 1.0f / l[k], o[k][0], o[k][1],
+                sink.put(a, QP == 1, rho, token, head, 4 * (i % (HD / 4)), m[k], l[k], over<TREE>(l[k]), o[k][0], o[k][1],
                          o[k][2], o[k][3]);
         }
     }
@@ -1650,7 +1687,7 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
 
 // The prefix, for all rows of the batch: workgroup = (tile of rows, kv head, piece of
 // the prefix).
-template <int HD, int QP, int KP>
+template <int HD, int QP, int KP, bool TREE>
 __device__ __forceinline__ void prefix_piece(const PagedAttnArgs& a, int id, float unit, uint8_t* s_buf) {
     const PagedView& p = a.p;
     const int TT = tile_rows<HD, QP>() / a.share, tiles = (p.num_rows + TT - 1) / TT;
@@ -1661,7 +1698,7 @@ __device__ __forceinline__ void prefix_piece(const PagedAttnArgs& a, int id, flo
     int rows = 0;
     for (int s = threadIdx.x; s < p.num_seqs; s += 256) {
         const int lo = p.row_start[s], hi = p.row_start[s + 1];
-        if (seq_ok(p, lo, hi, p.kv_len[s]) && hi > lo) rows = max(rows, hi);
+        if (attn_ok<TREE>(a, lo, hi, p.kv_len[s]) && hi > lo) rows = max(rows, hi);
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) rows = max(rows, __shfl_xor(rows, m));
@@ -1681,16 +1718,17 @@ __device__ __forceinline__ void prefix_piece(const PagedAttnArgs& a, int id, flo
     w.hi = min(p.prefix_len, 32 * (int)((int64_t)blocks * (piece + 1) / a.splits));
     w.first = 0;
     w.last = p.prefix_len - 1;
+    w.tree0 = p.prefix_len;
     w.table = p.prefix_pages;
     w.uniform();
-    compute<HD, QP, KP>(a, w, unit, s_buf, piece_of<HD>(a, piece), Cut<HD>{});
+    compute<HD, QP, KP, TREE>(a, w, unit, s_buf, piece_of<HD>(a, piece), Cut<HD>{});
 }
 
 // The first workgroups take a share each of the line of the sequences' own positions, the
 // others a piece each of the prefix.  A tile that several workgroups have a share of is
 // joined by the last of them to end: their partials are stored past the L2s and complete
 // before the workgroup is counted.
-template <int HD, int QP, int KP>
+template <int HD, int QP, int KP, bool TREE>
 __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAttnArgs a) {
     __shared__ int64_t s_cum[kPagedMaxSeqs + 1];
     __shared__ int64_t s_tmp[4];
@@ -1700,7 +1738,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAt
     const float unit = a.scale * 1.44269504f;
     const int id = (int)blockIdx.x;
     if (id >= a.grid) {
-        prefix_piece<HD, QP, KP>(a, id - a.grid, unit, s_buf);
+        prefix_piece<HD, QP, KP, TREE>(a, id - a.grid, unit, s_buf);
         return;
     }
     Line ln;
@@ -1708,7 +1746,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAt
     ln.org = p.prefix_len & ~31;
     ln.TT = tile_rows<HD, QP>() / a.share;
     ln.kv_heads = p.kv_heads;
-    make_line(p, ln, s_tmp, a.grid, id == 0);
+    make_line<TREE>(a, ln, s_tmp, a.grid, id == 0);
     if (ln.total == 0) return;
     // neighbouring shares on one XCD (workgroup id mod 8)
     const int per = (ln.wgs + 7) / 8, wg = (id & 7) * per + (id >> 3);
@@ -1738,6 +1776,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAt
         w.hi = ln.org + ln.key(t, end);
         w.first = p.prefix_len;
         w.last = w.pos0 + w.tokens - 1;
+        w.tree0 = t.base;
         w.table = p.pages + (int64_t)t.seq * p.table_stride;
         w.uniform();
         const Sink<HD> done = a.splits ? piece_of<HD>(a, a.splits) : Sink<HD>{kToOut, nullptr, nullptr};
@@ -1751,7 +1790,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAt
         }
         const Cut<HD> cut{whole ? nullptr : a.counters + first, first, last, wg, done};
         const bool joined =
-            compute<HD, QP, KP>(a, w, unit, s_buf, whole ? done : piece_slot<HD, QP>(a, wg, first), cut);
+            compute<HD, QP, KP, TREE>(a, w, unit, s_buf, whole ? done : piece_slot<HD, QP>(a, wg, first), cut);
         if (!whole && !joined) {
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
@@ -1763,7 +1802,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAt
                     __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
-            if (s_last) join_tile<HD, QP>(a, w, first, last, unit, s_buf, done);
+            if (s_last) join_tile<HD, QP, TREE>(a, w, first, last, unit, s_buf, done);
         }
         __syncthreads();   // (s_buf and s_last are the next tile's)
         x = end;
@@ -1776,7 +1815,7 @@ __global__ __launch_bounds__(256, wgs_per_cu(HD)) void paged_attn_kernel(PagedAt
 }
 
 // A row's pieces of the prefix and its own part: out.  Workgroup = (token, some heads).
-template <int HD, int QP>
+template <int HD, int QP, bool TREE>
 __global__ __launch_bounds__(256) void paged_pieces_kernel(PagedAttnArgs a) {
     __shared__ int s_in;
     const PagedView& p = a.p;
@@ -1790,7 +1829,7 @@ __global__ __launch_bounds__(256) void paged_pieces_kernel(PagedAttnArgs a) {
     __syncthreads();
     for (int s = tid; s < p.num_seqs; s += 256) {
         const int lo = p.row_start[s], hi = p.row_start[s + 1];
-        if (token >= lo && token < hi && seq_ok(p, lo, hi, p.kv_len[s])) s_in = 1;
+        if (token >= lo && token < hi && attn_ok<TREE>(a, lo, hi, p.kv_len[s])) s_in = 1;
     }
     // (eight pieces in flight)
     float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1829,23 +1868,34 @@ __global__ __launch_bounds__(256) void paged_pieces_kernel(PagedAttnArgs a) {
            {o[0] * f, o[1] * f, o[2] * f, o[3] * f});
 }
 
-template <int HD, int QP, int KP>
+template <int HD, int QP, int KP, bool TREE>
 void launch_attn(const PagedAttnArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((paged_attn_kernel<HD, QP, KP>), dim3((unsigned)(a.grid + a.prefix_wgs)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<HD, QP, KP, TREE>), dim3((unsigned)(a.grid + a.prefix_wgs)), dim3(256), 0, st, a);
     if (a.splits)
-        hipLaunchKernelGGL((paged_pieces_kernel<HD, QP>),
+        hipLaunchKernelGGL((paged_pieces_kernel<HD, QP, TREE>),
                            dim3((unsigned)a.p.num_rows, (unsigned)((a.heads + 1024 / HD - 1) / (1024 / HD))),
                            dim3(256), 0, st, a);
 }
 
-template <int HD>
+template <int HD, bool TREE>
 void launch_attn_hd(const PagedAttnArgs& a, hipStream_t st) {
     if (a.x_bf16)
-        launch_attn<HD, 1, 1>(a, st);
+        launch_attn<HD, 1, 1, TREE>(a, st);
     else if (a.cache_bf16)
-        launch_attn<HD, 3, 1>(a, st);
+        launch_attn<HD, 3, 1, TREE>(a, st);
     else
-        launch_attn<HD, 3, 3>(a, st);
+        launch_attn<HD, 3, 3, TREE>(a, st);
+}
+
+template <bool TREE>
+int launch_any(const PagedAttnArgs& a, hipStream_t st) {
+    switch (a.head_dim) {
+        case 64: launch_attn_hd<64, TREE>(a, st); break;
+        case 128: launch_attn_hd<128, TREE>(a, st); break;
+        case 256: launch_attn_hd<256, TREE>(a, st); break;
+        default: return (int)hipErrorInvalidValue;
+    }
+    return (int)hipGetLastError();
 }
 
 template <int HD>
@@ -1879,13 +1929,7 @@ int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats) {
 
 int launch_paged_attention(const PagedAttnArgs& a, void* stream) {
     hipStream_t st = static_cast<hipStream_t>(stream);
-    switch (a.head_dim) {
-        case 64: launch_attn_hd<64>(a, st); break;
-        case 128: launch_attn_hd<128>(a, st); break;
-        case 256: launch_attn_hd<256>(a, st); break;
-        default: return (int)hipErrorInvalidValue;
-    }
-    return (int)hipGetLastError();
+    return a.mask ? launch_any<true>(a, st) : launch_any<false>(a, st);
 }
 
 int launch_kv_append(const AppendArgs& a, int cus, void* stream) {

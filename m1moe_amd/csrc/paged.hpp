@@ -8,7 +8,7 @@ namespace m1moe {
 
 constexpr int kPagedMaxSeqs = 1024;
 constexpr int kPagedMaxShare = 64;   // query heads per kv head
-constexpr uint32_t kErrPagedBatch = 256u, kErrPagedPage = 512u;   // device error flags
+constexpr uint32_t kErrPagedBatch = 256u, kErrPagedPage = 512u, kErrTree = 1024u;   // device error flags
 
 // The cache and the batch (m1moe_paged_kv, m1moe_paged_batch).
 struct PagedView {
@@ -29,6 +29,7 @@ struct AppendArgs {
     float eps, amp;
     int32_t heads, head_dim, rotary, interleaved;
     int32_t x_bf16, cache_bf16;
+    const int32_t* depth;   // of a tree's rows, or null: rows at their own positions
 };
 
 struct PagedAttnArgs {
@@ -45,6 +46,9 @@ struct PagedAttnArgs {
     float* part;         // partials: the workgroups' slots
     float* pre;          // and the prefix' pieces, [splits + 1][num_rows * heads][head_dim + 2]
     uint32_t* counters;  // [grid], zero between launches
+    // of trees: who sees whom, [num_rows][mask_words] (null: every row sees the earlier ones)
+    const uint64_t* mask;
+    int32_t mask_words;
 };
 
 struct SampleArgs {

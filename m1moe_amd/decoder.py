@@ -22,7 +22,7 @@ from typing import Optional
 import numpy as np
 
 from . import _lib
-from ._lib import (DecShape, KVAppend, PagedBatch, PagedKV, SampleParams, W_EMBED, W_FINAL_NORM, W_IN_NORM, W_K, W_K_NORM, W_LM_HEAD, W_O,
+from ._lib import (DecShape, KVAppend, PagedBatch, PagedKV, Q4Weights, SampleParams, W_EMBED, W_FINAL_NORM, W_IN_NORM, W_K, W_K_NORM, W_LM_HEAD, W_O,
                    W_PER_LAYER, W_POST_NORM, W_Q, W_Q_NORM, W_V, check, dtype_code)
 from .engine import DeviceBuffer, HIPContext, _ptr
 from .sampling import sample_token
@@ -185,6 +185,43 @@ class DenseOps:
         check(self.lib.m1moe_sample(self.ctx.handle, _ptr(logits), rows, vocab, stride,
                                     ctypes.byref(params), _ptr(tokens), _ptr(probs)),
               "m1moe_sample")
+
+    # drafted tokens: a tree of rows per sequence of a PagedBatch
+    def tree_plan(self, num_seqs: int, num_rows: int, row_start, parents, mask_words: int, mask,
+                  depth) -> None:
+        """Who sees whom (64-bit words of bits) and depths, from every row's parent."""
+        check(self.lib.m1moe_tree_plan(self.ctx.handle, num_seqs, num_rows, _ptr(row_start),
+                                       _ptr(parents), mask_words, _ptr(mask), _ptr(depth)),
+              "m1moe_tree_plan")
+
+    def tree_append(self, kv: PagedKV, batch: PagedBatch, args: KVAppend, depth) -> None:
+        """kv_append with every row rotated by the position of its depth in its tree."""
+        check(self.lib.m1moe_tree_append(self.ctx.handle, ctypes.byref(kv), ctypes.byref(batch),
+                                         ctypes.byref(args), _ptr(depth)), "m1moe_tree_append")
+
+    def tree_attention(self, kv: PagedKV, batch: PagedBatch, mask, mask_words: int, q,
+                       q_stride: int, out, out_stride: int, dtype, num_heads: int) -> None:
+        """Every row against the positions before its tree and the rows that its mask names."""
+        check(self.lib.m1moe_tree_attention(
+            self.ctx.handle, ctypes.byref(kv), ctypes.byref(batch), _ptr(mask), mask_words,
+            _ptr(q), q_stride, _ptr(out), out_stride, dtype_code(dtype), num_heads),
+            "m1moe_tree_attention")
+
+    def tree_accept(self, caches, batch: PagedBatch, parents, drafts, drawn, path, accepted, next,
+                    past) -> None:
+        """The path of drafts that were drawn at their parents, its rows moved together in all
+        caches (PagedKV.array)."""
+        check(self.lib.m1moe_tree_accept(
+            self.ctx.handle, caches, len(caches), ctypes.byref(batch), _ptr(parents),
+            _ptr(drafts), _ptr(drawn), _ptr(path), _ptr(accepted), _ptr(next), _ptr(past)),
+            "m1moe_tree_accept")
+
+    def matmul_q4(self, weights: Q4Weights, x, x_dtype, x_stride: int, tokens: int, y, y_dtype,
+                  y_stride: int, residual=None) -> None:
+        """y = x W^T (+ residual) with W in 4 bits (m1moe_amd.quant.quantize_4bit)."""
+        check(self.lib.m1moe_matmul_q4(
+            self.ctx.handle, ctypes.byref(weights), _ptr(x), dtype_code(x_dtype), x_stride, tokens,
+            _ptr(residual), _ptr(y), dtype_code(y_dtype), y_stride), "m1moe_matmul_q4")
 
 
 class Decoder:
