@@ -484,7 +484,7 @@ void m1moe_destroy(m1moe_ctx_t ctx) {
                      ctx->pf_xq,   ctx->pf_xinv,  ctx->pf_pos,  ctx->pf_sorted, ctx->pf_eoff,
                      ctx->pf_toff, ctx->pf_tdesc,  ctx->pf_act,  ctx->pf_y,     ctx->pf_aexp,
                      ctx->pf_aflag, ctx->attn_part, ctx->attn_cnt, ctx->paged_part,
-                     ctx->paged_cnt, ctx->sample_part};
+                     ctx->paged_cnt, ctx->q4_part, ctx->q4_cnt, ctx->sample_part};
     for (void* p : owned)
         if (p) (void)hipFree(p);
     share_leave(ctx);

@@ -104,6 +104,10 @@ struct m1moe_ctx {
     float* paged_part = nullptr;
     uint64_t paged_part_floats = 0;
     uint32_t* paged_cnt = nullptr;   // its workgroups' counters, zero between launches
+    // x in parts and partials of m1moe_matmul_q4, grown on demand
+    float* q4_part = nullptr;
+    uint64_t q4_part_floats = 0;
+    uint32_t* q4_cnt = nullptr;      // its workgroups' counters, zero between launches
     // m1moe_sample's workgroups' histograms, made by its first call
     uint32_t* sample_part = nullptr;
     std::set<void*> allocs;

@@ -42,6 +42,27 @@ int32_t check_mask(const uint64_t* mask, int32_t words) {
     return M1MOE_OK;
 }
 
+// At least `floats` of the products' workspace.
+int32_t ensure_q4_scratch(m1moe_ctx_t ctx, uint64_t floats) {
+    ctx->capture_uses_scratch = true;
+    if (ctx->q4_cnt && floats <= ctx->q4_part_floats) return M1MOE_OK;
+    if (int32_t rc = refuse_growth_in_capture(ctx->stream, "the 4-bit products' scratch")) return rc;
+    if (!ctx->q4_cnt) {
+        const uint64_t bytes = 4 * (uint64_t)ctx->cus;   // (split workgroups number no more than the CUs)
+        if (int32_t rc = device_alloc_zeroed((void**)&ctx->q4_cnt, bytes, "4-bit products' counters", ctx->stream))
+            return rc;
+        if (floats <= ctx->q4_part_floats) return M1MOE_OK;
+    }
+    HIP_TRY(hipStreamSynchronize(ctx->stream));
+    if (ctx->q4_part) ++ctx->scratch_gen;  // earlier graphs hold the old buffer
+    if (ctx->q4_part) HIP_TRY(hipFree(ctx->q4_part));
+    ctx->q4_part = nullptr;
+    ctx->q4_part_floats = 0;
+    if (int32_t rc = device_alloc((void**)&ctx->q4_part, floats * 4, "4-bit products' scratch")) return rc;
+    ctx->q4_part_floats = floats;
+    return M1MOE_OK;
+}
+
 int64_t row_bytes(int64_t stride, int64_t n, int64_t rows, int64_t es) { return ((rows - 1) * stride + n) * es; }
 
 }  // namespace
@@ -218,7 +239,14 @@ int32_t m1moe_matmul_q4(m1moe_ctx_t ctx, const m1moe_q4_weights* w, const void* 
     a.y_stride = y_stride;
     a.x_bf16 = x_dtype == M1MOE_BF16;
     a.y_bf16 = y_dtype == M1MOE_BF16;
-    return launched(launch_matmul_q4(a, ctx->cus, ctx->stream), "matmul_q4");
+    const int64_t floats = matmul_q4_plan(a, ctx->cus);
+    if (floats) {
+        if ((rc = ensure_q4_scratch(ctx, (uint64_t)floats))) return rc;
+        a.xparts = reinterpret_cast<uint8_t*>(ctx->q4_part);
+        a.part = ctx->q4_part + a.part_at;
+        a.counters = ctx->q4_cnt;
+    }
+    return launched(launch_matmul_q4(a, ctx->stream), "matmul_q4");
 }
 
 }  // extern "C"

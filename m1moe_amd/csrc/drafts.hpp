@@ -40,10 +40,20 @@ struct Q4Args {
     void* y;
     int64_t y_stride;
     int32_t x_bf16, y_bf16;
+    // set by matmul_q4_plan
+    int32_t grid, grid_y, waves;   // workgroups, of so many waves
+    int32_t wave_split, split;     // waves, and workgroups, that share a tile's columns
+    int32_t chunk, lds;            // units of columns staged at once, bytes of LDS
+    int32_t tiles;                 // of 16 tokens, of a workgroup
+    int64_t part_at;               // floats of x in parts, before the partials
+    uint8_t* xparts;               // x in parts
+    float* part;                   // partials of split workgroups
+    uint32_t* counters;            // [grid / split * grid_y], zero between launches
 };
 
 int launch_tree_plan(const TreePlanArgs& a, void* stream);
 int launch_tree_accept(const TreeAcceptArgs& a, void* stream);
-int launch_matmul_q4(const Q4Args& a, int cus, void* stream);
+int64_t matmul_q4_plan(Q4Args& a, int cus);   // the floats of workspace needed
+int launch_matmul_q4(const Q4Args& a, void* stream);
 
 }  // namespace m1moe

@@ -1330,26 +1330,6 @@ __device__ __forceinline__ void store4(const PagedAttnArgs& a, bool bf16, int64_
         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// Sixteen bytes to memory, past this XCD's L2 (sc1: for a workgroup on any XCD).  (The
-// s_nop: a store of more than 8 bytes may still read its registers when the next
-// instruction writes them, and the compiler does not see a store here.)
-__device__ __forceinline__ void store4_coh(float* p, const float (&x)[4]) {
-    const f32x4v v = {x[0], x[1], x[2], x[3]};
-    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
-}
-// Eight times sixteen bytes from there, waited for.
-__device__ __forceinline__ void load8_coh(const float* const (&p)[8], f32x4v (&v)[8]) {
-    asm volatile(
-        "global_load_dwordx4 %0, %8, off sc1\n\tglobal_load_dwordx4 %1, %9, off sc1\n\t"
-        "global_load_dwordx4 %2, %10, off sc1\n\tglobal_load_dwordx4 %3, %11, off sc1\n\t"
-        "global_load_dwordx4 %4, %12, off sc1\n\tglobal_load_dwordx4 %5, %13, off sc1\n\t"
-        "global_load_dwordx4 %6, %14, off sc1\n\tglobal_load_dwordx4 %7, %15, off sc1\n\t"
-        "s_waitcnt vmcnt(0)"
-        : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
-        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7])
-        : "memory");
-}
-
 // One over a row's sum of weights.  (A row of a tree may see nothing: zeros.)
 template <bool TREE>
 __device__ __forceinline__ float over(float l) {

@@ -98,12 +98,13 @@ def q4_bound(x, size, y, group, dtype):
     most 2 group products, cut rather than rounded where a matrix instruction adds them, is off by
     (2 group + 2) 2^-23 of the sum of their sizes, and so is the group's sum of x that the bias
     multiplies; groups, the residual and what a power of two scales come on top with one rounding
-    each.  Values of x that are below 2^-25 of their row's largest are kept to 2^-40 of that one.
+    each.  f16 parts of x end at steps of 2^-24 where the row's largest is 2^14 at least: half a
+    step is 2^-39 of that one.
     bf16: the result's own rounding."""
     mag = np.abs(x) @ size.T
     groups = size.shape[1] // group
     bound = mag * (2.0 ** -22 + (2 * group + groups + 8) * 2.0 ** -23)
-    bound += np.abs(x).max(1, keepdims=True) * 2.0 ** -40 * size.sum(1)[None] + np.abs(y) * 2.0 ** -22
+    bound += np.abs(x).max(1, keepdims=True) * 2.0 ** -39 * size.sum(1)[None] + np.abs(y) * 2.0 ** -22
     if dtype == "bf16":
         bound = bound + 2.0 ** -8 * np.abs(y)
     return bound + 1e-37
