@@ -48,7 +48,7 @@ int32_t ensure_q4_scratch(m1moe_ctx_t ctx, uint64_t floats) {
     if (ctx->q4_cnt && floats <= ctx->q4_part_floats) return M1MOE_OK;
     if (int32_t rc = refuse_growth_in_capture(ctx->stream, "the 4-bit products' scratch")) return rc;
     if (!ctx->q4_cnt) {
-        const uint64_t bytes = 4 * (uint64_t)ctx->cus;   // (split workgroups number no more than the CUs)
+        const uint64_t bytes = 4 * (uint64_t)ctx->cus;   // (more blocks than CUs are not split)
         if (int32_t rc = device_alloc_zeroed((void**)&ctx->q4_cnt, bytes, "4-bit products' counters", ctx->stream))
             return rc;
         if (floats <= ctx->q4_part_floats) return M1MOE_OK;
@@ -243,6 +243,7 @@ int32_t m1moe_matmul_q4(m1moe_ctx_t ctx, const m1moe_q4_weights* w, const void* 
     if (floats) {
         if ((rc = ensure_q4_scratch(ctx, (uint64_t)floats))) return rc;
         a.xparts = reinterpret_cast<uint8_t*>(ctx->q4_part);
+        a.down = ctx->q4_part + a.down_at;
         a.part = ctx->q4_part + a.part_at;
         a.counters = ctx->q4_cnt;
     }

@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device.hpp"
 #include "drafts.hpp"
@@ -13,7 +14,9 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 
-constexpr int kFewTokens = 8;
+// Most tokens that every workgroup stages for itself, and the rows of LDS that it takes for r.
+constexpr int kFewTokens = 32;
+__host__ __device__ constexpr int few_rows(int r) { return r | 1; }
 
 // With the columns' groups G, y = sum_G (s_G sum_{k in G} x_k (q_k - 8) + (b_G + 8 s_G) X_G),
 // X_G = sum_{k in G} x_k: the inner sum is an MFMA of f16 operands, exact products in f32
@@ -44,54 +47,84 @@ struct Unit {
     uint32_t s[kGroups / 2], b[kGroups / 2];            // bf16 pairs
 };
 
+// A lane's row of W.
 struct Weights {
-    const uint8_t* w;                  // the lane's row, at its 32 columns of the first block
-    const uint16_t *s, *b;             // its scales and biases
+    const uint8_t* w;                  // at the lane's 32 columns of the first block
+    const uint16_t *s, *b;             // all rows' scales and biases,
+    int64_t at, total;                 // where the row's begin and how many there are
     int cols, groups, g;
-    bool whole;                        // units' scales are whole aligned vectors
 
     Weights() = default;
-    __device__ __forceinline__ Weights(const Q4Args& a, int row, int lane_g, int unit_groups) {
+    __device__ __forceinline__ Weights(const Q4Args& a, int row, int lane_g) {
         cols = a.cols;
         groups = a.cols / a.group;
         g = lane_g;
         w = reinterpret_cast<const uint8_t*>(a.w) + (int64_t)row * (a.cols / 2) + 16 * g;
-        s = a.scales + (int64_t)row * groups;
-        b = a.biases + (int64_t)row * groups;
-        whole = groups % unit_groups == 0;
+        s = a.scales;
+        b = a.biases;
+        at = (int64_t)row * groups;
+        total = (int64_t)a.rows * groups;
     }
-
+    // A unit's N values (N <= total), the first `left` of which belong to it, `late` of them before
+    // the place that was read from.
+    template <int N>
+    struct __attribute__((packed, aligned(2))) Halves {
+        uint32_t x[N / 2];
+    };
+    template <int N>
+    __device__ __forceinline__ static void shift(uint32_t (&x)[N / 2], int late, int left) {
+        uint64_t v[2] = {x[0] | (uint64_t)x[1] << 32, 0};
+        if (N == 8) v[1] = x[N / 2 - 2] | (uint64_t)x[N / 2 - 1] << 32;
+        if (late >= 4) v[0] = v[1], v[1] = 0;
+        const int bits = 16 * (late & 3);
+        v[0] = v[0] >> bits | (bits ? v[1] << (64 - bits) : 0);
+        v[1] >>= bits;
+        v[0] &= left >= 4 ? ~0ull : (1ull << 16 * left) - 1;
+        v[1] &= left >= 8 ? ~0ull : left <= 4 ? 0ull : (1ull << 16 * (left - 4)) - 1;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) x[i] = (uint32_t)(v[i >> 1] >> 32 * (i & 1));
+    }
+    // A unit that ends in the row (all without a test: what a load may need would be kept in
+    // registers beside the units).
+    template <int G>
+    __device__ __forceinline__ void load_whole(int u, Unit<G>& x) const {
+        typedef Unit<G> U;
+        constexpr int N = U::kGroups;
+#pragma unroll
+        for (int i = 0; i < U::NQ; ++i) x.w[i] = *reinterpret_cast<const uint4*>(w + (u * U::kCols / 2 + 64 * i));
+        const int64_t from = at + u * N;
+        const Halves<N> p = *reinterpret_cast<const Halves<N>*>(s + from), q = *reinterpret_cast<const Halves<N>*>(b + from);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) x.s[i] = p.x[i], x.b[i] = q.x[i];
+    }
+    // Any unit.
     template <int G>
     __device__ __forceinline__ void load(int u, Unit<G>& x) const {
         typedef Unit<G> U;
+        constexpr int N = U::kGroups;
+        const int left = groups - u * N;
+        if (left >= N) return load_whole<G>(u, x);
 #pragma unroll
         for (int i = 0; i < U::NQ; ++i) {
             // (past the row: its last columns again, which meet x = 0 and scales of 0)
             const int col = min(u * U::kCols + 128 * i, cols - 32 * (g + 1));
             x.w[i] = *reinterpret_cast<const uint4*>(w + (col >> 1));
         }
-        const int q0 = u * U::kGroups;
-        if (whole) {
-            if constexpr (U::kGroups == 8) {
-                const uint4 p = *reinterpret_cast<const uint4*>(s + q0), q = *reinterpret_cast<const uint4*>(b + q0);
-                x.s[0] = p.x, x.s[1] = p.y, x.s[2] = p.z, x.s[3] = p.w;
-                x.b[0] = q.x, x.b[1] = q.y, x.b[2] = q.z, x.b[3] = q.w;
-            } else {
-                const uint2 p = *reinterpret_cast<const uint2*>(s + q0), q = *reinterpret_cast<const uint2*>(b + q0);
-                x.s[0] = p.x, x.s[1] = p.y;
-                x.b[0] = q.x, x.b[1] = q.y;
-            }
-            return;
-        }
+        const int64_t want = at + u * N, from = min(want, total - N);
+        const Halves<N> p = *reinterpret_cast<const Halves<N>*>(s + from), q = *reinterpret_cast<const Halves<N>*>(b + from);
 #pragma unroll
-        for (int i = 0; i < U::kGroups; i += 2) {
-            const int i0 = min(q0 + i, groups - 1), i1 = min(q0 + i + 1, groups - 1);
-            const uint32_t s0 = s[i0], s1 = s[i1], b0 = b[i0], b1 = b[i1];
-            x.s[i / 2] = (q0 + i < groups ? s0 : 0u) | (q0 + i + 1 < groups ? s1 << 16 : 0u);
-            x.b[i / 2] = (q0 + i < groups ? b0 : 0u) | (q0 + i + 1 < groups ? b1 << 16 : 0u);
-        }
+        for (int i = 0; i < N / 2; ++i) x.s[i] = p.x[i], x.b[i] = q.x[i];
+        shift<N>(x.s, (int)(want - from), left);
+        shift<N>(x.b, (int)(want - from), left);
     }
 };
+
+// The same number, but addresses made of it are made where they are used (or the compiler keeps
+// 90 registers of them over a loop's rounds).
+__device__ __forceinline__ int opaque(int u) {
+    asm volatile("" : "+s"(u));
+    return u;
+}
 
 __device__ __forceinline__ float bf16_pair(const uint32_t* p, int i) {
     return __uint_as_float(i & 1 ? p[i >> 1] & 0xFFFF0000u : p[i >> 1] << 16);
@@ -140,11 +173,14 @@ __device__ __forceinline__ void place(int o, int& i, int& g) {
     }
 }
 
-// The largest of eight values over the wave: 2^e brings it to 2^14 .. 2^15 (zeros: as 2^-112).
-__device__ __forceinline__ int scale_of(const float (&v)[8]) {
+__device__ __forceinline__ float largest(const float (&v)[8]) {
     float m = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+    return m;
+}
+// e such that 2^e brings the largest value of the wave to 2^14 .. 2^15 (zeros: as 2^-112).
+__device__ __forceinline__ int scale_of(float m) {
     return 14 - max((int)(__float_as_uint(wave_max(m)) >> 23) - 127, -112);
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -184,79 +220,119 @@ __device__ __forceinline__ float group_sum(const float (&v)[8]) {
     return sum;
 }
 
-// A unit's sums into the whole: acc += unit 2^-e, row by row.
-__device__ __forceinline__ void flush(f32x4v& acc, f32x4v unit, f32x4v down) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = fmaf(unit[e], down[e], acc[e]);
-}
-
-// RT: operand rows of a token.
-template <int G, bool XB>
+// NT operand tiles of 16 rows, P operands of a tile (an f32 x with one: its parts are rows 2 t
+// and 2 t + 1 of the tile).
+template <int G, int NT, int P, bool XB>
 struct Few {
     typedef Unit<G> U;
-    static constexpr int kTokens = 8, RT = XB ? 1 : 2;
+    static constexpr int RT = !XB && P == 1 ? 2 : 1;     // rows of a token
+    static constexpr int kSteps = 4 * U::NQ;             // of a unit
 
     const Q4Args& a;
-    int t0, tn, R;               // tokens, rows staged
-    uint8_t* s_x;                // [units][4 NQ steps][4][R] 16 bytes
-    float* s_sum;                // [units][groups][16]: X_G 2^e, row 2 t (or t)
-    float* s_down;               // [units][16]: 2^-e
+    int t0, tn;
+    int R, rows;                 // rows staged, and those apart of a step's lanes in LDS: an odd number
+    uint8_t* s_x;                // [units][P][steps][4][R] 16 bytes
+    float* s_sum;                // [units][groups][16 NT]: X_G 2^e, rows as above (their second: 0)
+    float* s_down;               // [units][16 NT]: 2^-e
 
-    __device__ __forceinline__ uint8_t* at(int u, int step, int g, int row) const {
-        return s_x + 16 * (((u * 4 * U::NQ + step) * 4 + g) * R + row);
+    __host__ __device__ static constexpr int unit_bytes(int r) {
+        return P * kSteps * 64 * r + (U::kGroups + 1) * 64 * NT;
+    }
+    __device__ __forceinline__ Few(const Q4Args& a, uint8_t* s) : a(a) {
+        t0 = (int)blockIdx.y * (16 * NT / RT);
+        tn = min(a.tokens - t0, 16 * NT / RT);
+        rows = RT * tn;
+        R = few_rows(RT * min(a.tokens, 16 * NT / RT));
+        s_x = s;
+        s_sum = reinterpret_cast<float*>(s + a.chunk * P * kSteps * 64 * R);
+        s_down = s_sum + a.chunk * U::kGroups * 16 * NT;
     }
 
-    // n units from column k0 on, by all waves, a token's unit each.
+    // n units from column k0 on, by all waves, four of a token's units each at a time.
     __device__ __forceinline__ void stage(int k0, int n) {
-        const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, waves = (int)blockDim.x >> 6;
-        for (int i = wave; i < tn * n; i += waves) {
-            const int t = i / n, u = i - t * n, row = RT * t, at0 = 8 * lane, col = k0 + u * U::kCols + at0;
-            float v[8] = {};
-            if (at0 < U::kCols && col < a.cols) read8<XB>(a, (int64_t)(t0 + t) * a.x_stride + col, v);
-            const int e = scale_of(v);
-            const float up = power(e), sum = group_sum<G>(v);
-            if (lane < RT) s_down[16 * u + row + lane] = power(-e);
-            if (at0 >= U::kCols) continue;
-            if (at0 % G == 0) {
-                float* to = s_sum + (u * U::kGroups + at0 / G) * 16 + row;
-                to[0] = sum * up;
-                if (RT == 2) to[1] = 0.f;
+        const int lane = (int)threadIdx.x & 63, waves = (int)blockDim.x >> 6;
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), at0 = 8 * lane;
+        for (int i0 = wave; i0 < tn * n; i0 += 4 * waves) {
+            float v[4][8] = {};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * waves, t = i / n, col = k0 + (i - t * n) * U::kCols + at0;
+                if (i < tn * n && at0 < U::kCols && col < a.cols)
+                    read8<XB>(a, (int64_t)(t0 + t) * a.x_stride + col, v[k]);
             }
-            f16x8 hi, lo;
-            parts(v, up, hi, lo);
-            int step, g;
-            place<G>(lane & 15, step, g);
-            step += 4 * (lane >> 4);
-            *reinterpret_cast<f16x8*>(at(u, step, g, row)) = hi;
-            if (RT == 2) *reinterpret_cast<f16x8*>(at(u, step, g, row + 1)) = lo;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * waves, t = i / n, u = i - t * n, row = RT * t;
+                if (i >= tn * n) break;
+                const int e = scale_of(largest(v[k]));
+                const float up = power(e), sum = group_sum<G>(v[k]);
+                if (lane < RT) s_down[16 * NT * u + row + lane] = power(-e);
+                if (at0 >= U::kCols) continue;
+                if (at0 % G == 0) {
+                    float* to = s_sum + (u * U::kGroups + at0 / G) * 16 * NT + row;
+                    to[0] = sum * up;
+                    if (RT == 2) to[1] = 0.f;
+                }
+                f16x8 hi, lo;
+                parts(v[k], up, hi, lo);
+                int step, g;
+                place<G>(lane & 15, step, g);
+                step += 4 * (lane >> 4);
+                uint8_t* to = s_x + 16 * (((u * P * kSteps + step) * 4 + g) * R + row);
+                *reinterpret_cast<f16x8*>(to) = hi;
+                if (RT == 2) *reinterpret_cast<f16x8*>(to + 16) = lo;
+                if (P == 2) *reinterpret_cast<f16x8*>(to + 64 * kSteps * R) = lo;
+            }
         }
     }
 
     // Unit x, unit u of the chunk.
-    __device__ __forceinline__ void add(const U& x, int u, int c, int g, f32x4v& acc) const {
-        constexpr int kSteps = G / 32;                 // of a group
-        const int row = min(c, R - 1);
+    __device__ __forceinline__ void add(const U& x, int u, int c, int g, f32x4v (&acc)[NT]) const {
+        const uint8_t* y[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            y[t] = s_x + 16 * ((u * P * kSteps * 4 + g) * R + min(16 * t + c, rows - 1));
         const NibK k = nib_consts();
-        f32x4v unit = {0.f, 0.f, 0.f, 0.f}, part;
+        f32x4v unit[NT], part[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) unit[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < U::NQ; ++i) {
+            __builtin_amdgcn_sched_barrier(0);   // (a block's operands at a time)
             uint32_t v[4];
             steps<G>(x.w[i], v);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (j % kSteps == 0) part = f32x4v{0.f, 0.f, 0.f, 0.f};
-                part = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    *reinterpret_cast<const f16x8*>(at(u, 4 * i + j, g, row)), nibbles(v[j], k), part, 0, 0, 0);
-                if (j % kSteps == kSteps - 1) {
-                    const int q = (4 * i + j) / kSteps;     // group of the unit
-                    const float s = bf16_pair(x.s, q), b = fmaf(8.f, s, bf16_pair(x.b, q));
-                    const f32x4v sum = *reinterpret_cast<const f32x4v*>(s_sum + (u * U::kGroups + q) * 16 + 4 * g);
+                const f16x8 w = nibbles(v[j], k);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) unit[e] = fmaf(b, sum[e], fmaf(s, part[e], unit[e]));
+                for (int t = 0; t < NT; ++t) {
+                    if (j % (G / 32) == 0) part[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p)
+                        part[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            *reinterpret_cast<const f16x8*>(y[t] + p * 64 * kSteps * R), w, part[t], 0, 0, 0);
+                    y[t] += 64 * R;
+                }
+                if (j % (G / 32) == G / 32 - 1) {
+                    const int q = (4 * i + j) / (G / 32);     // group of the unit
+                    const float s = bf16_pair(x.s, q), b = fmaf(8.f, s, bf16_pair(x.b, q));
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const f32x4v sum =
+                            *reinterpret_cast<const f32x4v*>(s_sum + (u * U::kGroups + q) * 16 * NT + 16 * t + 4 * g);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) unit[t][e] = fmaf(b, sum[e], fmaf(s, part[t][e], unit[t][e]));
+                        asm volatile("" : "+v"(unit[t]));   // (here and now: or all parts are kept for later)
+                    }
                 }
             }
         }
-        flush(acc, unit, *reinterpret_cast<const f32x4v*>(s_down + 16 * u + 4 * g));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const f32x4v down = *reinterpret_cast<const f32x4v*>(s_down + 16 * NT * u + 16 * t + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(unit[t][e], down[e], acc[t][e]);
+        }
     }
 };
 
@@ -271,87 +347,179 @@ __device__ __forceinline__ void put(const Q4Args& a, int t, int n, float y) {
     }
 }
 
-template <int G, bool XB>
-__global__ __launch_bounds__(512) void q4_few_kernel(Q4Args a) {
-    typedef Few<G, XB> F;
+// Weights of fewer groups in all than a unit of one row has (a unit's scales are one load): a
+// wave per token and row.
+template <bool XB>
+__global__ __launch_bounds__(64) void q4_tiny_kernel(Q4Args a) {
+    const int lane = (int)threadIdx.x, n = (int)blockIdx.x, t = (int)blockIdx.y, groups = a.cols / a.group;
+    float sum = 0.f;
+    for (int k = lane; k < a.cols; k += 64) {
+        const int64_t at = (int64_t)t * a.x_stride + k, g = (int64_t)n * groups + k / a.group;
+        const float x = XB ? bf16_to_f32(static_cast<const uint16_t*>(a.x)[at]) : static_cast<const float*>(a.x)[at];
+        const float q = (float)(a.w[((int64_t)n * a.cols + k) / 8] >> 4 * (k & 7) & 15);
+        sum = fmaf(x, fmaf(q, bf16_to_f32(a.scales[g]), bf16_to_f32(a.biases[g])), sum);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) put(a, t, n, sum);
+}
+
+// KW workgroups share a block's columns, this one kw: the last of them to end joins their sums,
+// N tiles of a wave, and goes on alone (true).  id: of the block.
+template <int N>
+__device__ __forceinline__ bool join_split(const Q4Args& a, int id, int KW, int kw, int waves, int wave, bool mine,
+                                           f32x4v (&acc)[N], int* s_flag) {
+    const int lane = (int)threadIdx.x & 63;
+    const int64_t wg = (int64_t)waves * N * 256;
+    float* part = a.part + (int64_t)id * KW * wg + (int64_t)wave * N * 256 + 4 * lane;   // [KW][waves][N][64][4]
+    if (mine)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float y[4] = {acc[i][0], acc[i][1], acc[i][2], acc[i][3]};
+            store4_coh(part + kw * wg + i * 256, y);
+        }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        *s_flag = __hip_atomic_fetch_add(a.counters + id, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                  (uint32_t)(KW - 1);
+        if (*s_flag) __hip_atomic_store(a.counters + id, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!*s_flag) return false;
+    // (in the order of the columns, whoever is last)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        f32x4v sum = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < KW; k0 += 8) {
+            const float* at[8];
+            f32x4v y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) at[k] = part + min(k0 + k, KW - 1) * wg + i * 256;
+            load8_coh(at, y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k0 + k < KW) sum += y[k];
+        }
+        acc[i] = sum;
+    }
+    return true;
+}
+
+template <int G, int NT, int P, bool XB>
+__global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
+    typedef Few<G, NT, P, XB> F;
     typedef Unit<G> U;
     extern __shared__ __attribute__((aligned(16))) uint8_t s_buf[];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = (int)blockDim.x >> 6;
-    const int c = lane & 15, g = lane >> 4, KS = a.wave_split, ks = wave % KS;
-    const int tile = (int)blockIdx.x * (waves / KS) + wave / KS;
-    F f{a};
-    f.t0 = 0;
-    f.tn = a.tokens;
-    f.R = F::RT * f.tn;
-    f.s_x = s_buf;
-    f.s_sum = reinterpret_cast<float*>(s_buf + a.chunk * (4 * U::NQ) * 64 * f.R);
-    f.s_down = f.s_sum + a.chunk * U::kGroups * 16;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int waves = (int)blockDim.x >> 6, c = lane & 15, g = lane >> 4, KS = a.wave_split, ks = wave % KS;
+    const int KW = a.split, kw = (int)blockIdx.x % KW, block = (int)blockIdx.x / KW;
+    const int tile = block * (waves / KS) + wave / KS;
+    F f(a, s_buf);
     const int units = (a.cols + U::kCols - 1) / U::kCols;
+    const int u0 = (int)((int64_t)units * kw / KW), u1 = (int)((int64_t)units * (kw + 1) / KW);
     const bool on = 16 * tile < a.rows;
     const int n = 16 * tile + c;
-    const Weights w(a, min(n, a.rows - 1), g, U::kGroups);
-    f32x4v acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < units; k += a.chunk) {
-        const int nu = min(a.chunk, units - k), lo = nu * ks / KS, hi = nu * (ks + 1) / KS;
+    const Weights w(a, min(n, a.rows - 1), g);
+    f32x4v acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    for (int k = u0; k < u1; k += a.chunk) {
+        const int nu = min(a.chunk, u1 - k), lo = nu * ks / KS, end = nu * (ks + 1) / KS;
+        const int hi = min(end, a.cols / U::kCols - k);    // (a last unit in part: behind the others)
         U x[2];
-        if (on && lo < hi) w.load<G>(k + lo, x[0]);
-        if (k) __syncthreads();
+        if (on && lo < hi) w.load_whole<G>(k + lo, x[0]);
+        if (k != u0) __syncthreads();
         f.stage(k * U::kCols, nu);
         __syncthreads();
         if (!on) continue;
-        for (int u = lo; u < hi; u += 2) {
-            if (u + 1 < hi) w.load<G>(k + u + 1, x[1]);
+        if (lo < hi) {
+            int u = lo;
+            for (; u + 2 < hi; u += 2) {   // (no load under a condition: its unit would be held twice)
+                w.load_whole<G>(k + opaque(u) + 1, x[1]);
+                f.add(x[0], opaque(u), c, g, acc);
+                w.load_whole<G>(k + opaque(u) + 2, x[0]);
+                f.add(x[1], opaque(u) + 1, c, g, acc);
+            }
+            if (u + 1 < hi) {
+                w.load_whole<G>(k + u + 1, x[1]);
+                f.add(x[0], u, c, g, acc);
+                x[0] = x[1];
+                ++u;
+            }
             f.add(x[0], u, c, g, acc);
-            if (u + 1 >= hi) break;
-            if (u + 2 < hi) w.load<G>(k + u + 2, x[0]);
-            f.add(x[1], u + 1, c, g, acc);
+        }
+        if (max(lo, hi) < end) {
+            w.load<G>(k + end - 1, x[0]);
+            f.add(x[0], end - 1, c, g, acc);
         }
     }
     // the waves of a tile, in their order
     if (KS > 1) {
         f32x4v* s = reinterpret_cast<f32x4v*>(s_buf);
         __syncthreads();
-        s[tid] = acc;
-        __syncthreads();
-        if (ks) return;
-        for (int i = 1; i < KS; ++i) acc += s[tid + 64 * i];
-    }
-    if (!on || n >= a.rows) return;
-    if constexpr (F::RT == 2) {
-        if (2 * g < f.tn) put(a, 2 * g, n, acc[0] + acc[1]);
-        if (2 * g + 1 < f.tn) put(a, 2 * g + 1, n, acc[2] + acc[3]);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (4 * g + i < f.tn) put(a, 4 * g + i, n, acc[i]);
+        for (int t = 0; t < NT; ++t) s[(wave * NT + t) * 64 + lane] = acc[t];
+        __syncthreads();
+        if (ks == 0) {
+            for (int i = 1; i < KS; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t] += s[((wave + i) * NT + t) * 64 + lane];
+        }
+    }
+    if (KW > 1) {
+        __syncthreads();
+        const int id = (int)blockIdx.y * ((int)gridDim.x / KW) + block;
+        if (!join_split<NT>(a, id, KW, kw, waves, wave, ks == 0, acc, reinterpret_cast<int*>(s_buf))) return;
+    }
+    if (ks || !on || n >= a.rows) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        if constexpr (F::RT == 2) {
+            if (2 * g < f.tn) put(a, f.t0 + 2 * g, n, acc[t][0] + acc[t][1]);
+            if (2 * g + 1 < f.tn) put(a, f.t0 + 2 * g + 1, n, acc[t][2] + acc[t][3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (16 * t + 4 * g + i < f.tn) put(a, f.t0 + 16 * t + 4 * g + i, n, acc[t][i]);
+        }
     }
 }
 
 // ---- many tokens -----------------------------------------------------------------------
 //
 // x is made into f16 parts once, by a kernel of its own: records of 16 tokens' 128 columns, [P
-// parts][4 steps][64 lanes] 16 bytes, as the MFMAs take them, then the groups' sums [4][16]
-// and 2^-e [16] (e: of a token's unit of columns).
-constexpr int record_bytes(int p) { return 4096 * p + 512; }
+// parts][4 steps][64 lanes] 16 bytes, as the MFMAs take them, then the groups' sums X_G 2^e
+// [4][16]; 2^-e of the tokens (e: of a token's whole row) behind all records.
+constexpr int record_bytes(int p) { return 4096 * p + 256; }
 
-// Workgroup = (16 tokens, unit of columns), a wave per token.
+// Workgroup = (16 tokens, a share of the units of columns), a wave per token, which reads its
+// whole row for the largest value.
 template <int G, bool XB>
 __global__ __launch_bounds__(1024) void q4_parts_kernel(Q4Args a) {
     typedef Unit<G> U;
     constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P);
-    __shared__ __attribute__((aligned(16))) uint8_t s_rec[U::NQ * kRecord];
-    const int tid = (int)threadIdx.x, lane = tid & 63, row = tid >> 6;
-    const int tile = (int)blockIdx.y, u = (int)blockIdx.x, blocks = (int)gridDim.x * U::NQ;
-    const int t = 16 * tile + row, at0 = 8 * lane, col = u * U::kCols + at0;
-    float v[8] = {};
-    if (t < a.tokens && at0 < U::kCols && col < a.cols) read8<XB>(a, (int64_t)t * a.x_stride + col, v);
-    const int e = scale_of(v);
-    const float up = power(e), sum = group_sum<G>(v);
-    if (at0 < U::kCols) {
-        uint8_t* rec = s_rec + (lane >> 4) * kRecord;
-        float* tail = reinterpret_cast<float*>(rec + 4096 * P);
-        if (at0 % G == 0) tail[(at0 & 127) / G * 16 + row] = sum * up;
-        if ((lane & 15) == 0) tail[64 + row] = power(-e);
+    const int lane = (int)threadIdx.x & 63, row = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), tile = (int)blockIdx.y;
+    const int units = (a.cols + U::kCols - 1) / U::kCols, blocks = units * U::NQ, t = 16 * tile + row;
+    const int64_t from = (int64_t)min(t, a.tokens - 1) * a.x_stride;
+    float m = 0.f;
+#pragma unroll 4
+    for (int col = 8 * lane; col < a.cols; col += 512) {
+        float v[8];
+        read8<XB>(a, from + col, v);
+        m = fmaxf(m, largest(v));
+    }
+    const int e = scale_of(m);
+    const float up = power(e);
+    if (blockIdx.x == 0 && lane == 0) a.down[t] = power(-e);
+    const int b0 = (int)((int64_t)blocks * blockIdx.x / gridDim.x), b1 = (int)((int64_t)blocks * (blockIdx.x + 1) / gridDim.x);
+    for (int b = b0 + (lane >> 4); b < (b1 + 3) / 4 * 4; b += 4) {   // (four records a wave; all lanes take part)
+        const int col = 128 * b + 8 * (lane & 15);
+        float v[8] = {};
+        if (t < a.tokens && b < b1 && col < a.cols) read8<XB>(a, from + col, v);
+        const float sum = group_sum<G>(v);
+        if (b >= b1) continue;
+        uint8_t* rec = a.xparts + ((int64_t)tile * blocks + b) * kRecord;
+        if (col % G == 0) reinterpret_cast<float*>(rec + 4096 * P)[(col & 127) / G * 16 + row] = sum * up;
         f16x8 hi, lo;
         parts(v, up, hi, lo);
         int step, g;
@@ -359,24 +527,22 @@ __global__ __launch_bounds__(1024) void q4_parts_kernel(Q4Args a) {
         *reinterpret_cast<f16x8*>(rec + 16 * (64 * step + 16 * g + row)) = hi;
         if (P == 2) *reinterpret_cast<f16x8*>(rec + 4096 + 16 * (64 * step + 16 * g + row)) = lo;
     }
-    __syncthreads();
-    uint4* to = reinterpret_cast<uint4*>(a.xparts + ((int64_t)tile * blocks + u * U::NQ) * kRecord);
-    for (int i = tid; i < U::NQ * kRecord / 16; i += 1024) to[i] = reinterpret_cast<const uint4*>(s_rec)[i];
 }
 
 // Workgroup = 16 NT tokens, 16 MW rows of W a wave; a wave's words come straight from memory as
-// above, the records through LDS, copied by the loads themselves, SB blocks of 128 columns
-// at a time, the next ones on their way while some are computed.
+// above, a unit ahead, the records through LDS, copied by the loads themselves, SB blocks of
+// 128 columns at a time, the next ones on their way while some are computed.
 template <int G, int NT, int MW, bool XB>
 struct Many {
     typedef Unit<G> U;
     static constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P);
     static constexpr int SB = std::min(U::NQ, std::max(1, 8 / (NT * P)));
     static constexpr int kStage = SB * NT * kRecord;
+    static constexpr int kLoads = MW * (U::NQ + 2);      // a unit's, at least
 };
 
 template <int G, int NT, int MW, bool XB>
-__global__ __launch_bounds__(512, 2) void q4_many_kernel(Q4Args a) {
+__global__ __launch_bounds__(512, MW * NT <= 4 ? 4 : 2) void q4_many_kernel(Q4Args a) {
     typedef Many<G, NT, MW, XB> M;
     typedef Unit<G> U;
     constexpr int P = M::P, SB = M::SB, kRecord = M::kRecord, kSteps = G / 32;
@@ -388,219 +554,211 @@ __global__ __launch_bounds__(512, 2) void q4_many_kernel(Q4Args a) {
     const int t0 = (int)blockIdx.y * 16 * NT, tile0 = (block * waves + wave) * MW;
     const int units = (a.cols + U::kCols - 1) / U::kCols, blocks = units * U::NQ;
     const int u0 = (int)((int64_t)units * kw / KW), u1 = (int)((int64_t)units * (kw + 1) / KW);
-    const bool on = 16 * tile0 < a.rows;
     const int tiles = min(NT, (a.tokens - t0 + 15) / 16);   // of tokens that there are
     int n[MW];
     Weights w[MW];
 #pragma unroll
     for (int m = 0; m < MW; ++m) {
         n[m] = 16 * (tile0 + m) + c;
-        w[m] = Weights(a, min(n[m], a.rows - 1), g, U::kGroups);
+        w[m] = Weights(a, min(n[m], a.rows - 1), g);
     }
     const uint8_t* rec = a.xparts + (int64_t)blockIdx.y * NT * blocks * kRecord;
     // SB blocks from block k on to buffer s
     const auto copy = [&](int k, int s) {
-        constexpr int kUnits = kRecord / 512;      // half-kilobytes of a record
 #pragma unroll 1
         for (int i = wave; i < NT * SB; i += waves) {
             const int t = i / SB, b = i - t * SB;
             const uint8_t* from = rec + ((int64_t)min(t, tiles - 1) * blocks + k + b) * kRecord;
             const uint32_t to = lds_addr(s_x) + s * M::kStage + (t * SB + b) * kRecord;
 #pragma unroll
-            for (int j = 0; j + 1 < kUnits; j += 2) lds_copy16(16 * lane + 512 * j, from, to + 512 * j);
-            if (lane < 32) lds_copy16(16 * lane + 512 * (kUnits - 1), from, to + 512 * (kUnits - 1));
+            for (int j = 0; j < 4 * P; ++j) lds_copy16(16 * lane + 1024 * j, from, to + 1024 * j);
+            lds_copy4(4 * lane + 4096 * P, from, to + 4096 * P);
         }
     };
-    f32x4v acc[MW][NT], unit[MW][NT];
+    f32x4v acc[MW * NT];
 #pragma unroll
-    for (int m = 0; m < MW; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[m][t] = unit[m][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    U x[2][MW];
+    for (int i = 0; i < MW * NT; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
     const NibK nk = nib_consts();
     int turn = 0;
-    // Unit u, x; the next one's words, y, are asked for behind the second stage's records.
-    const auto compute = [&](const U (&x)[MW], U (&y)[MW], int u, bool more) {
+    // Unit u, x; the next one's words, y (NEXT: 0 none, 1 a whole unit, 2 any), are asked for
+    // behind the second stage's records.
+    const auto compute = [&](auto next_unit, const U (&x)[MW], U (&y)[MW], int u) {
+        constexpr int NEXT = decltype(next_unit)::value;
 #pragma unroll
         for (int b0 = 0; b0 < U::NQ; b0 += SB) {
-            if (b0 == SB && on && more)
-                wait_vm<MW * (U::NQ + 2)>();
+            if (b0 == SB && NEXT)
+                wait_vm<M::kLoads>();
             else
                 wait_vm<0>();
             __syncthreads();      // (the stage is there, and the other one read)
-            if (b0 + SB < U::NQ || more) copy(u * U::NQ + b0 + SB, turn ^ 1);
-            if (b0 == 0 && on && more) {
+            if (b0 + SB < U::NQ || NEXT) copy(u * U::NQ + b0 + SB, turn ^ 1);
+            if (b0 == 0) {
 #pragma unroll
-                for (int m = 0; m < MW; ++m) w[m].template load<G>(u + 1, y[m]);
+                for (int m = 0; m < MW; ++m) {
+                    if (NEXT == 1) w[m].template load_whole<G>(u + 1, y[m]);
+                    if (NEXT == 2) w[m].template load<G>(u + 1, y[m]);
+                }
             }
             const uint8_t* s = s_x + turn * M::kStage;
             turn ^= 1;
-            if (!on) continue;
 #pragma unroll
             for (int b = 0; b < SB; ++b) {
+                __builtin_amdgcn_sched_barrier(0);   // (as above)
                 uint32_t v[MW][4];
 #pragma unroll
                 for (int m = 0; m < MW; ++m) steps<G>(x[m].w[b0 + b], v[m]);
-                f32x4v part[MW][NT];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f16x8 q[MW];
-#pragma unroll
-                    for (int m = 0; m < MW; ++m) q[m] = nibbles(v[m][j], nk);
-#pragma unroll
-                    for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            const f16x8 y = *reinterpret_cast<const f16x8*>(s + (t * SB + b) * kRecord + 4096 * p +
-                                                                            1024 * j + 16 * lane);
-#pragma unroll
-                            for (int m = 0; m < MW; ++m) {
-                                if (j % kSteps == 0 && p == P - 1) part[m][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
-                                part[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[m], part[m][t], 0, 0, 0);
-                            }
-                        }
-                    if (j % kSteps == kSteps - 1) {
-                        const int qb = j / kSteps, qu = (4 * (b0 + b) + j) / kSteps;   // group of the block, the unit
-                        float sc[MW], bi[MW];
-#pragma unroll
-                        for (int m = 0; m < MW; ++m) {
-                            sc[m] = bf16_pair(x[m].s, qu);
-                            bi[m] = fmaf(8.f, sc[m], bf16_pair(x[m].b, qu));
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            const f32x4v sum = *reinterpret_cast<const f32x4v*>(s + (t * SB + b) * kRecord + 4096 * P +
-                                                                                64 * qb + 16 * g);
-#pragma unroll
-                            for (int m = 0; m < MW; ++m)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    unit[m][t][e] = fmaf(bi[m], sum[e], fmaf(sc[m], part[m][t][e], unit[m][t][e]));
-                        }
-                    }
-                }
-            }
-            if (b0 + SB == U::NQ) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const f32x4v down = *reinterpret_cast<const f32x4v*>(s + t * SB * kRecord + 4096 * P + 256 + 16 * g);
+                // (a tile's sums are added while the next one's MFMAs run; here and now: or the
+                // compiler keeps all tiles' sums of a stage for later)
+                f32x4v part[2][MW], sum[2];
+                float sc[2][MW], bi[2][MW];
+                const auto flush = [&](int i) {
+                    const int t = i % NT;
 #pragma unroll
                     for (int m = 0; m < MW; ++m) {
-                        flush(acc[m][t], unit[m][t], down);
-                        unit[m][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[m * NT + t][e] = fmaf(bi[i / NT & 1][m], sum[i & 1][e],
+                                                fmaf(sc[i / NT & 1][m], part[i & 1][m][e], acc[m * NT + t][e]));
+                        asm volatile("" : "+v"(acc[m * NT + t]));
+                    }
+                };
+#pragma unroll
+                for (int qb = 0; qb < 4 / kSteps; ++qb) {     // the block's groups
+                    const int qu = (4 * (b0 + b)) / kSteps + qb;
+                    f16x8 q[MW][kSteps];
+#pragma unroll
+                    for (int m = 0; m < MW; ++m) {
+#pragma unroll
+                        for (int j = 0; j < kSteps; ++j) q[m][j] = nibbles(v[m][kSteps * qb + j], nk);
+                        sc[qb & 1][m] = bf16_pair(x[m].s, qu);
+                        bi[qb & 1][m] = fmaf(8.f, sc[qb & 1][m], bf16_pair(x[m].b, qu));
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const int i = qb * NT + t;
+                        const uint8_t* r = s + (t * SB + b) * kRecord;
+#pragma unroll
+                        for (int m = 0; m < MW; ++m) part[i & 1][m] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                            for (int j = 0; j < kSteps; ++j) {
+                                const f16x8 y = *reinterpret_cast<const f16x8*>(r + 4096 * p + 1024 * (kSteps * qb + j) +
+                                                                                16 * lane);
+#pragma unroll
+                                for (int m = 0; m < MW; ++m)
+                                    part[i & 1][m] =
+                                        __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[m][j], part[i & 1][m], 0, 0, 0);
+                            }
+                        sum[i & 1] = *reinterpret_cast<const f32x4v*>(r + 4096 * P + 64 * qb + 16 * g);
+                        if (i > 0) flush(i - 1);
                     }
                 }
+                flush(4 / kSteps * NT - 1);
             }
         }
     };
+    U x[MW], y[MW];
     copy(u0 * U::NQ, 0);
-    if (on) {
 #pragma unroll
-        for (int m = 0; m < MW; ++m) w[m].template load<G>(u0, x[0][m]);
+    for (int m = 0; m < MW; ++m) w[m].template load<G>(u0, x[m]);
+    const auto next = [&] {
+#pragma unroll
+        for (int m = 0; m < MW; ++m) x[m] = y[m];
+    };
+    int u = u0;
+    for (const int whole = min(u1, a.cols / U::kCols); u + 1 < whole; ++u) {
+        compute(std::integral_constant<int, 1>{}, x, y, u);
+        next();
     }
-    for (int u = u0; u < u1; u += 2) {
-        compute(x[0], x[1], u, u + 1 < u1);
-        if (u + 1 < u1) compute(x[1], x[0], u + 1, u + 2 < u1);
+    if (u + 1 < u1) {
+        compute(std::integral_constant<int, 2>{}, x, y, u);
+        next();
+        ++u;
     }
-    if (KW > 1) {
-        // the last of the workgroups that share a block's columns to end joins them
-        const int id = (int)blockIdx.y * ((int)gridDim.x / KW) + block;
-        const int64_t wg = (int64_t)waves * MW * NT * 256;
-        float* part = a.part + (int64_t)id * KW * wg + (int64_t)wave * MW * NT * 256 + 4 * lane;   // [KW][waves][MW][NT][64][4]
+    compute(std::integral_constant<int, 0>{}, x, y, u);
+    if (KW > 1 && !join_split<MW * NT>(a, (int)blockIdx.y * ((int)gridDim.x / KW) + block, KW, kw, waves, wave, true, acc,
+                                       &s_last))
+        return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        if (t >= tiles) break;
+        const f32x4v down = *reinterpret_cast<const f32x4v*>(a.down + t0 + 16 * t + 4 * g);
 #pragma unroll
         for (int m = 0; m < MW; ++m)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float y[4] = {acc[m][t][0], acc[m][t][1], acc[m][t][2], acc[m][t][3]};
-                store4_coh(part + kw * wg + (m * NT + t) * 256, y);
-            }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (tid == 0) {
-            s_last = __hip_atomic_fetch_add(a.counters + id, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                     (uint32_t)(KW - 1);
-            if (s_last) __hip_atomic_store(a.counters + id, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!s_last) return;
-        // (in the order of the columns, whoever is last)
-#pragma unroll
-        for (int m = 0; m < MW; ++m)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                f32x4v sum = {0.f, 0.f, 0.f, 0.f};
-                for (int i0 = 0; i0 < KW; i0 += 8) {
-                    const float* at[8];
-                    f32x4v y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) at[i] = part + min(i0 + i, KW - 1) * wg + (m * NT + t) * 256;
-                    load8_coh(at, y);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i0 + i < KW) sum += y[i];
-                }
-                acc[m][t] = sum;
-            }
-    }
-#pragma unroll
-    for (int m = 0; m < MW; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int tok = t0 + 16 * t + 4 * g + i;
-                if (n[m] < a.rows && tok < a.tokens) put(a, tok, n[m], acc[m][t][i]);
+                if (n[m] < a.rows && tok < a.tokens) put(a, tok, n[m], acc[m * NT + t][i] * down[i]);
             }
+    }
+}
+
+template <int G, int NT, int P, bool XB>
+void launch_few(const Q4Args& a, hipStream_t st) {
+    hipLaunchKernelGGL((q4_few_kernel<G, NT, P, XB>), dim3((unsigned)a.grid, (unsigned)a.grid_y),
+                       dim3((unsigned)(64 * a.waves)), (size_t)a.lds, st, a);
 }
 
 template <int G, int NT, int MW, bool XB>
 void launch_many(const Q4Args& a, hipStream_t st) {
+    hipLaunchKernelGGL((q4_parts_kernel<G, XB>), dim3((unsigned)a.part_split, (unsigned)((a.tokens + 15) / 16)), dim3(1024),
+                       0, st, a);
     hipLaunchKernelGGL((q4_many_kernel<G, NT, MW, XB>), dim3((unsigned)a.grid, (unsigned)a.grid_y),
                        dim3((unsigned)(64 * a.waves)), 0, st, a);
 }
 
 template <int G, bool XB>
 void launch_group(const Q4Args& a, hipStream_t st) {
-    if (a.tokens <= kFewTokens) {
-        hipLaunchKernelGGL((q4_few_kernel<G, XB>), dim3((unsigned)a.grid), dim3((unsigned)(64 * a.waves)), (size_t)a.lds, st, a);
-        return;
-    }
-    const int units = (a.cols + Unit<G>::kCols - 1) / Unit<G>::kCols;
-    hipLaunchKernelGGL((q4_parts_kernel<G, XB>), dim3((unsigned)units, (unsigned)((a.tokens + 15) / 16)), dim3(1024), 0, st, a);
-    switch (a.tiles) {
-        case 1: launch_many<G, 1, 2, XB>(a, st); break;
-        case 2: launch_many<G, 2, 2, XB>(a, st); break;
-        default: launch_many<G, 4, 2, XB>(a, st); break;
-    }
+    if (a.tiny)
+        hipLaunchKernelGGL((q4_tiny_kernel<XB>), dim3((unsigned)a.rows, (unsigned)a.tokens), dim3(64), 0, st, a);
+    else if (a.tokens > kFewTokens)
+        launch_many<G, 4, 1, XB>(a, st);
+    else if (a.tokens <= (XB ? 16 : 8))
+        launch_few<G, 1, 1, XB>(a, st);
+    else if (!XB && a.tokens <= 16)
+        launch_few<G, 1, XB ? 1 : 2, XB>(a, st);
+    else
+        launch_few<G, 2, XB ? 1 : 2, XB>(a, st);
 }
 
 }  // namespace
 
 int64_t matmul_q4_plan(Q4Args& a, int cus) {
-    const int unit = a.group == 32 ? 256 : 512, units = (a.cols + unit - 1) / unit;
+    const int unit = a.group == 32 ? 256 : 512, units = (a.cols + unit - 1) / unit, groups = unit / a.group;
     const int tiles = (a.rows + 15) / 16;
     a.waves = 8;
-    a.split = a.wave_split = 1;
+    a.split = a.wave_split = a.grid_y = 1;
+    a.tiny = (int64_t)a.rows * (a.cols / a.group) < groups;
+    if (a.tiny) return 0;
     if (a.tokens <= kFewTokens) {
-        const int rows = (a.x_bf16 ? 1 : 2) * a.tokens, bytes = rows * unit * 2 + unit / a.group * 64 + 64;
-        // chunks of at most 48 KB, so that three workgroups fit a CU
-        a.chunk = std::max(1, std::min(49152 / bytes, units));
-        while (a.wave_split < 8 && 2 * a.wave_split <= units && tiles * a.wave_split * 2 <= 16 * cus) a.wave_split *= 2;
-        if (a.wave_split <= 4 && tiles * a.wave_split < 8 * cus) a.waves = 4;
+        const bool flat = !a.x_bf16 && a.tokens <= 8;
+        const int nt = a.tokens <= 16 ? 1 : 2, p = a.x_bf16 || flat ? 1 : 2;
+        const int bytes = p * (unit / 32) * 64 * few_rows(flat ? 2 * a.tokens : a.tokens) + (groups + 1) * 64 * nt;
+        if (a.tokens <= 4) {
+            while (a.wave_split < 8 && 2 * a.wave_split <= units && tiles * a.wave_split * 2 <= 16 * cus) a.wave_split *= 2;
+            if (a.wave_split <= 4 && tiles * a.wave_split < 8 * cus) a.waves = 4;
+        } else {
+            a.waves = tiles >= 8 * cus ? 16 : 8;
+            a.split = std::max(1, std::min(units, cus / ((tiles + a.waves - 1) / a.waves)));
+        }
         const int per = a.waves / a.wave_split;
-        a.grid = (tiles + per - 1) / per;
-        a.lds = std::max(a.chunk * bytes, a.waves * 1024);
-        return 0;
+        // all of a workgroup's columns at once, in at most 76 KB, so that two fit a CU, of many waves 152
+        a.chunk = std::max(1, std::min((a.waves == 16 ? 152 : 76) * 1024 / bytes, (units + a.split - 1) / a.split));
+        a.grid = (tiles + per - 1) / per * a.split;
+        a.lds = std::max(a.chunk * bytes, a.wave_split > 1 ? a.waves * nt * 1024 : 16);
+        return a.split > 1 ? (int64_t)a.grid * a.waves * nt * 256 : 0;
     }
-    const int tt = (a.tokens + 15) / 16;
-    a.tiles = tt == 1 ? 1 : tt == 2 ? 2 : 4;
-    a.grid_y = (tt + a.tiles - 1) / a.tiles;
-    const int blocks = (tiles + 2 * a.waves - 1) / (2 * a.waves);
+    const int tt = (a.tokens + 15) / 16, nblocks = units * (unit / 128), nt = 4, mw = 1;
+    a.grid_y = (tt + nt - 1) / nt;
+    const int blocks = (tiles + mw * a.waves - 1) / (mw * a.waves);
     a.split = std::max(1, std::min(units, cus / (blocks * a.grid_y)));
     a.grid = blocks * a.split;
-    const int64_t record = record_bytes(a.x_bf16 ? 1 : 2), records = (int64_t)tt * units * (unit / 128) * record / 4;
-    a.part_at = records;
-    return records + (a.split > 1 ? (int64_t)a.grid * a.grid_y * a.waves * 2 * a.tiles * 256 : 0);
+    a.part_split = std::max(1, std::min(nblocks / 4, cus / tt));
+    const int64_t records = (int64_t)tt * nblocks * record_bytes(a.x_bf16 ? 1 : 2) / 4;
+    a.down_at = records;
+    a.part_at = records + 16 * tt;
+    return a.part_at + (a.split > 1 ? (int64_t)a.grid * a.grid_y * a.waves * mw * nt * 256 : 0);
 }
 
 int launch_matmul_q4(const Q4Args& a, void* stream) {
