@@ -42,15 +42,16 @@ struct Q4Args {
     int32_t x_bf16, y_bf16;
     // set by matmul_q4_plan
     int32_t tiny;                  // less than a unit's groups
-    int32_t grid, grid_y, waves;   // workgroups, of so many waves
+    int32_t grid, waves;           // workgroups, of so many waves
     int32_t wave_split, split;     // waves, and workgroups, that share a tile's columns
+    int32_t grid_x, whole;         // tiles of rows of W; tiles that are not shared
     int32_t chunk, lds;            // units of columns staged at once, bytes of LDS
     int32_t part_split;            // workgroups that make 16 tokens' parts
     int64_t down_at, part_at;      // floats of the workspace before these
     uint8_t* xparts;               // x in parts
     float* down;                   // [tokens rounded up to 16]: what x was divided by
     float* part;                   // partials of split workgroups
-    uint32_t* counters;            // [grid / split * grid_y], zero between launches
+    uint32_t* counters;            // of shared tiles, zero between launches
 };
 
 int launch_tree_plan(const TreePlanArgs& a, void* stream);

@@ -229,7 +229,6 @@ struct Few {
     static constexpr int kSteps = 4 * U::NQ;             // of a unit
 
     const Q4Args& a;
-    int t0, tn;
     int R, rows;                 // rows staged, and those apart of a step's lanes in LDS: an odd number
     uint8_t* s_x;                // [units][P][steps][4][R] 16 bytes
     float* s_sum;                // [units][groups][16 NT]: X_G 2^e, rows as above (their second: 0)
@@ -239,10 +238,8 @@ struct Few {
         return P * kSteps * 64 * r + (U::kGroups + 1) * 64 * NT;
     }
     __device__ __forceinline__ Few(const Q4Args& a, uint8_t* s) : a(a) {
-        t0 = (int)blockIdx.y * (16 * NT / RT);
-        tn = min(a.tokens - t0, 16 * NT / RT);
-        rows = RT * tn;
-        R = few_rows(RT * min(a.tokens, 16 * NT / RT));
+        rows = RT * a.tokens;
+        R = few_rows(rows);
         s_x = s;
         s_sum = reinterpret_cast<float*>(s + a.chunk * P * kSteps * 64 * R);
         s_down = s_sum + a.chunk * U::kGroups * 16 * NT;
@@ -251,14 +248,14 @@ struct Few {
     // n units from column k0 on, by all waves, four of a token's units each at a time.
     __device__ __forceinline__ void stage(int k0, int n) {
         const int lane = (int)threadIdx.x & 63, waves = (int)blockDim.x >> 6;
-        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), at0 = 8 * lane;
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), at0 = 8 * lane, tn = a.tokens;
         for (int i0 = wave; i0 < tn * n; i0 += 4 * waves) {
             float v[4][8] = {};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int i = i0 + k * waves, t = i / n, col = k0 + (i - t * n) * U::kCols + at0;
                 if (i < tn * n && at0 < U::kCols && col < a.cols)
-                    read8<XB>(a, (int64_t)(t0 + t) * a.x_stride + col, v[k]);
+                    read8<XB>(a, (int64_t)t * a.x_stride + col, v[k]);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -468,19 +465,18 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
     }
     if (KW > 1) {
         __syncthreads();
-        const int id = (int)blockIdx.y * ((int)gridDim.x / KW) + block;
-        if (!join_split<NT>(a, id, KW, kw, waves, wave, ks == 0, acc, reinterpret_cast<int*>(s_buf))) return;
+        if (!join_split<NT>(a, block, KW, kw, waves, wave, ks == 0, acc, reinterpret_cast<int*>(s_buf))) return;
     }
     if (ks || !on || n >= a.rows) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         if constexpr (F::RT == 2) {
-            if (2 * g < f.tn) put(a, f.t0 + 2 * g, n, acc[t][0] + acc[t][1]);
-            if (2 * g + 1 < f.tn) put(a, f.t0 + 2 * g + 1, n, acc[t][2] + acc[t][3]);
+            if (2 * g < a.tokens) put(a, 2 * g, n, acc[t][0] + acc[t][1]);
+            if (2 * g + 1 < a.tokens) put(a, 2 * g + 1, n, acc[t][2] + acc[t][3]);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (16 * t + 4 * g + i < f.tn) put(a, f.t0 + 16 * t + 4 * g + i, n, acc[t][i]);
+                if (16 * t + 4 * g + i < a.tokens) put(a, 16 * t + 4 * g + i, n, acc[t][i]);
         }
     }
 }
@@ -549,9 +545,11 @@ __global__ __launch_bounds__(512, MW * NT <= 4 ? 4 : 2) void q4_many_kernel(Q4Ar
     __shared__ __attribute__((aligned(16))) uint8_t s_x[2 * M::kStage];
     __shared__ int s_last;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int waves = (int)blockDim.x >> 6, c = lane & 15, g = lane >> 4, KW = a.split;
-    const int kw = (int)blockIdx.x % KW, block = (int)blockIdx.x / KW;
-    const int t0 = (int)blockIdx.y * 16 * NT, tile0 = (block * waves + wave) * MW;
+    const int waves = (int)blockDim.x >> 6, c = lane & 15, g = lane >> 4;
+    // this workgroup's tile: one of the `whole` ones, or a share of one of the others
+    const int id = (int)blockIdx.x, rest = id - a.whole, KW = rest < 0 ? 1 : a.split, kw = rest < 0 ? 0 : rest % KW;
+    const int tile = rest < 0 ? id : a.whole + rest / KW, ty = tile / a.grid_x, block = tile - ty * a.grid_x;
+    const int t0 = ty * 16 * NT, tile0 = (block * waves + wave) * MW;
     const int units = (a.cols + U::kCols - 1) / U::kCols, blocks = units * U::NQ;
     const int u0 = (int)((int64_t)units * kw / KW), u1 = (int)((int64_t)units * (kw + 1) / KW);
     const int tiles = min(NT, (a.tokens - t0 + 15) / 16);   // of tokens that there are
@@ -562,7 +560,7 @@ __global__ __launch_bounds__(512, MW * NT <= 4 ? 4 : 2) void q4_many_kernel(Q4Ar
         n[m] = 16 * (tile0 + m) + c;
         w[m] = Weights(a, min(n[m], a.rows - 1), g);
     }
-    const uint8_t* rec = a.xparts + (int64_t)blockIdx.y * NT * blocks * kRecord;
+    const uint8_t* rec = a.xparts + (int64_t)ty * NT * blocks * kRecord;
     // SB blocks from block k on to buffer s
     const auto copy = [&](int k, int s) {
 #pragma unroll 1
@@ -677,9 +675,7 @@ __global__ __launch_bounds__(512, MW * NT <= 4 ? 4 : 2) void q4_many_kernel(Q4Ar
         ++u;
     }
     compute(std::integral_constant<int, 0>{}, x, y, u);
-    if (KW > 1 && !join_split<MW * NT>(a, (int)blockIdx.y * ((int)gridDim.x / KW) + block, KW, kw, waves, wave, true, acc,
-                                       &s_last))
-        return;
+    if (KW > 1 && !join_split<MW * NT>(a, tile - a.whole, KW, kw, waves, wave, true, acc, &s_last)) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         if (t >= tiles) break;
@@ -696,16 +692,15 @@ __global__ __launch_bounds__(512, MW * NT <= 4 ? 4 : 2) void q4_many_kernel(Q4Ar
 
 template <int G, int NT, int P, bool XB>
 void launch_few(const Q4Args& a, hipStream_t st) {
-    hipLaunchKernelGGL((q4_few_kernel<G, NT, P, XB>), dim3((unsigned)a.grid, (unsigned)a.grid_y),
-                       dim3((unsigned)(64 * a.waves)), (size_t)a.lds, st, a);
+    hipLaunchKernelGGL((q4_few_kernel<G, NT, P, XB>), dim3((unsigned)a.grid), dim3((unsigned)(64 * a.waves)),
+                       (size_t)a.lds, st, a);
 }
 
 template <int G, int NT, int MW, bool XB>
 void launch_many(const Q4Args& a, hipStream_t st) {
     hipLaunchKernelGGL((q4_parts_kernel<G, XB>), dim3((unsigned)a.part_split, (unsigned)((a.tokens + 15) / 16)), dim3(1024),
                        0, st, a);
-    hipLaunchKernelGGL((q4_many_kernel<G, NT, MW, XB>), dim3((unsigned)a.grid, (unsigned)a.grid_y),
-                       dim3((unsigned)(64 * a.waves)), 0, st, a);
+    hipLaunchKernelGGL((q4_many_kernel<G, NT, MW, XB>), dim3((unsigned)a.grid), dim3((unsigned)(64 * a.waves)), 0, st, a);
 }
 
 template <int G, bool XB>
@@ -728,7 +723,7 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
     const int unit = a.group == 32 ? 256 : 512, units = (a.cols + unit - 1) / unit, groups = unit / a.group;
     const int tiles = (a.rows + 15) / 16;
     a.waves = 8;
-    a.split = a.wave_split = a.grid_y = 1;
+    a.split = a.wave_split = 1;
     a.tiny = (int64_t)a.rows * (a.cols / a.group) < groups;
     if (a.tiny) return 0;
     if (a.tokens <= kFewTokens) {
@@ -750,15 +745,20 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
         return a.split > 1 ? (int64_t)a.grid * a.waves * nt * 256 : 0;
     }
     const int tt = (a.tokens + 15) / 16, nblocks = units * (unit / 128), nt = 4, mw = 1;
-    a.grid_y = (tt + nt - 1) / nt;
-    const int blocks = (tiles + mw * a.waves - 1) / (mw * a.waves);
-    a.split = std::max(1, std::min(units, cus / (blocks * a.grid_y)));
-    a.grid = blocks * a.split;
+    // Whole tiles as long as they fill the card, two workgroups a CU; the columns of the others are
+    // shared by as many workgroups as make one more round of it (800 x 6144 x 4096, 624 tiles: all
+    // whole 136 us).
+    a.grid_x = (tiles + mw * a.waves - 1) / (mw * a.waves);
+    const int all = a.grid_x * ((tt + nt - 1) / nt), slots = 2 * cus;
+    a.whole = all / slots * slots;
+    a.split = all == a.whole ? 1 : std::max(1, std::min(units, slots / (all - a.whole)));
+    if (a.split == 1) a.whole = all;
+    a.grid = a.whole + (all - a.whole) * a.split;
     a.part_split = std::max(1, std::min(nblocks / 4, cus / tt));
     const int64_t records = (int64_t)tt * nblocks * record_bytes(a.x_bf16 ? 1 : 2) / 4;
     a.down_at = records;
     a.part_at = records + 16 * tt;
-    return a.part_at + (a.split > 1 ? (int64_t)a.grid * a.grid_y * a.waves * mw * nt * 256 : 0);
+    return a.part_at + (int64_t)(a.grid - a.whole) * a.waves * mw * nt * 256;
 }
 
 int launch_matmul_q4(const Q4Args& a, void* stream) {
