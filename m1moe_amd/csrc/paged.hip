@@ -1501,7 +1501,7 @@ __device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w,
         if (*s_there == (uint32_t)(cut.last - cut.first)) {
             if (threadIdx.x == 0) __hip_atomic_store(cut.counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (rows) {
-                constexpr int VD = HD / 16, V = VD < 8 ? VD : 8;
+                constexpr int VD = HD / 16, V = VD < 8 ? VD : 8, PP = 16 / V;   // values, pieces at once
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const int rho = rho0 + 16 * t + r.c;
@@ -1509,33 +1509,41 @@ __device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w,
 #pragma unroll
                     for (int j0 = 0; j0 < VD; j0 += V) {
                         f32x4v o[V];
-                        for (int p = cut.first; p <= cut.last; ++p) {
-                            float mp = r.m[t], lp = r.l[t];
-                            f32x4v y[8];
+                        for (int p0 = cut.first; p0 <= cut.last; p0 += PP) {
+                            const float* at[16];
+                            f32x4v y[16];
+                            unsigned long long z[PP];
 #pragma unroll
-                            for (int k = 0; k < V; ++k) y[k] = r.acc[t][j0 + k];
-                            if (p != cut.mine) {
-                                const Sink<HD> slot = piece_slot<HD, QP>(a, p, cut.first);
-                                const unsigned long long z =
-                                    __hip_atomic_load(reinterpret_cast<unsigned long long*>(slot.ml + 2 * rho),
-                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                                const float* at[8];
+                            for (int q = 0; q < PP; ++q) {
+                                const Sink<HD> slot = piece_slot<HD, QP>(a, min(p0 + q, cut.last), cut.first);
+                                const float* o0 = uniform_ptr(slot.o);
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) at[k] = slot.o + rho * HD + 16 * (j0 + k % V) + 4 * r.g;
-                                load8_coh(at, y);
-                                mp = __uint_as_float((uint32_t)z);
-                                lp = __uint_as_float((uint32_t)(z >> 32));
+                                for (int k = 0; k < V; ++k) at[q * V + k] = o0 + 16 * (j0 + k);
+                                z[q] = __hip_atomic_load(reinterpret_cast<unsigned long long*>(slot.ml + 2 * rho),
+                                                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                             }
-                            if (p == cut.first) {
-                                m = mp;
-                                l = lp;
+                            load16_coh(4u * (uint32_t)(rho * HD + 4 * r.g), at, y);
 #pragma unroll
-                                for (int k = 0; k < V; ++k) o[k] = y[k];
-                            } else {
-                                float f0, f1;
-                                join(m, l, mp, lp, unit, f0, f1);
+                            for (int q = 0; q < PP; ++q) {
+                                if (p0 + q > cut.last) break;
+                                // (this workgroup's own: not through memory)
+                                const bool own = p0 + q == cut.mine;
+                                const float mp = own ? r.m[t] : __uint_as_float((uint32_t)z[q]);
+                                const float lp = own ? r.l[t] : __uint_as_float((uint32_t)(z[q] >> 32));
 #pragma unroll
-                                for (int k = 0; k < V; ++k) o[k] = mix(o[k], f0, y[k], f1);
+                                for (int k = 0; k < V; ++k)
+                                    if (own) y[q * V + k] = r.acc[t][j0 + k];
+                                if (p0 + q == cut.first) {
+                                    m = mp;
+                                    l = lp;
+#pragma unroll
+                                    for (int k = 0; k < V; ++k) o[k] = y[q * V + k];
+                                } else {
+                                    float f0, f1;
+                                    join(m, l, mp, lp, unit, f0, f1);
+#pragma unroll
+                                    for (int k = 0; k < V; ++k) o[k] = mix(o[k], f0, y[q * V + k], f1);
+                                }
                             }
                         }
 #pragma unroll
@@ -1567,14 +1575,71 @@ __device__ __forceinline__ bool compute(const PagedAttnArgs& a, const Work& w, f
     return false;
 }
 
+// As join_tile, many values: V of a thread and 16 / V pieces at a time.
+template <int HD, int QP, bool TREE, int V>
+__device__ __forceinline__ void join_values(const PagedAttnArgs& a, const Work& w, int first, int last, float unit,
+                                            const Sink<HD>& sink) {
+    constexpr int PP = 16 / V;
+    const int rows = w.tokens * a.share, tid = thread_id(), values = rows * (HD / 4);
+#pragma unroll 1
+    for (int k0 = 0; 256 * k0 < values; k0 += V) {
+        f32x4v o[V];
+        float m[V], l[V];
+        for (int p0 = first; p0 <= last; p0 += PP) {
+            const float* at[16];
+            f32x4v y[16];
+            unsigned long long z[16];
+#pragma unroll
+            for (int q = 0; q < PP; ++q) {
+                const Sink<HD> slot = piece_slot<HD, QP>(a, min(p0 + q, last), first);
+                const float* o0 = uniform_ptr(slot.o);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const int rho = min((tid + 256 * (k0 + k)) / (HD / 4), rows - 1);
+                    at[q * V + k] = o0 + 1024 * (k0 + k);
+                    z[q * V + k] = __hip_atomic_load(reinterpret_cast<unsigned long long*>(slot.ml + 2 * rho),
+                                                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+            }
+            load16_coh(16u * tid, at, y);
+#pragma unroll
+            for (int q = 0; q < PP; ++q) {
+                if (p0 + q > last) break;
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const int i = q * V + k;
+                    const float mp = __uint_as_float((uint32_t)z[i]), lp = __uint_as_float((uint32_t)(z[i] >> 32));
+                    if (p0 + q == first) {
+                        o[k] = y[i];
+                        m[k] = mp;
+                        l[k] = lp;
+                    } else {
+                        float f0, f1;
+                        join(m[k], l[k], mp, lp, unit, f0, f1);
+                        o[k] = mix(o[k], f0, y[i], f1);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int i = tid + 256 * (k0 + k), rho = i / (HD / 4);
+            int token, head;
+            if (rho < rows && row_at(a, w, rho, token, head))
+                sink.put(a, QP == 1, rho, token, head, 4 * (i % (HD / 4)), m[k], l[k], over<TREE>(l[k]), o[k][0], o[k][1],
+                         o[k][2], o[k][3]);
+        }
+    }
+}
+
 // The pieces of a tile that workgroups first .. last have written to their slots, joined.
 // Few values: the threads that they leave share the pieces, eight loads of each in
-// flight, and join theirs through LDS.  Many: eight values of a thread in flight, piece
-// after piece.  Either way in an order that does not depend on who is last.
+// flight, and join theirs through LDS.  Many: sixteen loads of a thread in flight, of as many
+// pieces as its values leave room for (one piece of eight values at a time: 16 rows behind 3000
+// positions, 25 pieces, 39 us against TBD).  Either way in an order that does not depend on who is last.
 template <int HD, int QP, bool TREE>
 __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w, int first, int last, float unit,
                                           uint8_t* s_buf, const Sink<HD>& sink) {
-    constexpr int NV = tile_rows<HD, QP>() * HD / 4 / 256;
     const int rows = w.tokens * a.share, tid = thread_id(), values = rows * (HD / 4);
     const auto piece = [&](int p) { return piece_slot<HD, QP>(a, p, first); };
     const auto coh = [](const float* p) {
@@ -1624,45 +1689,13 @@ __device__ __forceinline__ void join_tile(const PagedAttnArgs& a, const Work& w,
         }
         return;
     }
-#pragma unroll 1
-    for (int k0 = 0; k0 < NV && 256 * k0 < values; k0 += 8) {
-        f32x4v o[8];
-        float m[8], l[8];
-        for (int p = first; p <= last; ++p) {
-            const Sink<HD> slot = piece(p);
-            const float* at[8];
-            f32x4v y[8];
-            float z[8], u[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int i = tid + 256 * (k0 + k), rho = min(i / (HD / 4), rows - 1);
-                at[k] = slot.o + rho * HD + 4 * (i % (HD / 4));
-                z[k] = coh(slot.ml + 2 * rho);
-                u[k] = coh(slot.ml + 2 * rho + 1);
-            }
-            load8_coh(at, y);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (p == first) {
-                    o[k] = y[k];
-                    m[k] = z[k];
-                    l[k] = u[k];
-                } else {
-                    float f0, f1;
-                    join(m[k], l[k], z[k], u[k], unit, f0, f1);
-                    o[k] = mix(o[k], f0, y[k], f1);
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int i = tid + 256 * (k0 + k), rho = i / (HD / 4);
-            int token, head;
-            if (rho < rows && row_at(a, w, rho, token, head))
-                sink.put(a, QP == 1, rho, token, head, 4 * (i % (HD / 4)), m[k], l[k], over<TREE>(l[k]), o[k][0], o[k][1],
-                         o[k][2], o[k][3]);
-        }
-    }
+    // (a slot holds 1024 values at least, and whole 2048 where there are more)
+    if (values <= 512)
+        join_values<HD, QP, TREE, 2>(a, w, first, last, unit, sink);
+    else if (values <= 1024)
+        join_values<HD, QP, TREE, 4>(a, w, first, last, unit, sink);
+    else
+        join_values<HD, QP, TREE, 8>(a, w, first, last, unit, sink);
 }
 
 // The prefix, for all rows of the batch: workgroup = (tile of rows, kv head, piece of

@@ -296,9 +296,11 @@ def _dtype_code(x_dtype) -> int:
     raise ValueError(f"unknown activation dtype {x_dtype!r}")
 
 
-def _ptr(buf) -> Optional[ctypes.c_void_p]:
-    if buf is None:
-        return None
+def _ptr(buf):
+    """A device address (an int, a c_void_p, a DeviceBuffer or None) as a call takes it: an int
+    goes through as it is, without an object made of it."""
+    if buf.__class__ is int or buf is None:
+        return buf
     if isinstance(buf, DeviceBuffer):
         return buf.ptr
     return ctypes.c_void_p(int(buf))
