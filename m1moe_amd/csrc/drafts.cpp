@@ -125,7 +125,7 @@ int32_t m1moe_tree_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m1
         return rc;
     a.mask = d_mask;
     a.mask_words = mask_words;
-    return launched(launch_paged_attention(a, ctx->stream), "tree_attention");
+    return launched(launch_tree_attention(a, ctx->stream), "tree_attention");
 }
 
 int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs, int32_t num_caches,
@@ -170,7 +170,7 @@ int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs, int32_t nu
     // (planes that share memory would be moved twice, by workgroups that do not wait for each other)
     void* sorted[2 * kMostCaches];
     std::copy(a.planes, a.planes + a.num_planes, sorted);
-    std::sort(sorted, sorted + a.num_planes);
+    if (!std::is_sorted(sorted, sorted + a.num_planes)) std::sort(sorted, sorted + a.num_planes);
     for (int i = 1; i < a.num_planes; ++i)
         if (static_cast<char*>(sorted[i]) - static_cast<char*>(sorted[i - 1]) < plane)
             return fail(M1MOE_ERR_INVALID, "two of the caches' d_k and d_v overlap");

@@ -46,7 +46,7 @@ struct Q4Args {
     int32_t wave_split, split;     // waves, and workgroups, that share a tile's columns
     int32_t grid_x, whole;         // tiles of rows of W; tiles that are not shared
     int32_t chunk, lds;            // units of columns staged at once, bytes of LDS
-    int32_t part_split;            // workgroups that make 16 tokens' parts
+    int32_t part_split;            // workgroups that make a token's parts
     int64_t down_at, part_at;      // floats of the workspace before these
     uint8_t* xparts;               // x in parts
     float* down;                   // [tokens rounded up to 16]: what x was divided by
@@ -55,6 +55,7 @@ struct Q4Args {
 };
 
 int launch_tree_plan(const TreePlanArgs& a, void* stream);
+int launch_tree_attention(const PagedAttnArgs& a, void* stream);
 int launch_tree_accept(const TreeAcceptArgs& a, void* stream);
 int64_t matmul_q4_plan(Q4Args& a, int cus);   // the floats of workspace needed
 int launch_matmul_q4(const Q4Args& a, void* stream);

@@ -488,36 +488,46 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
 // [4][16]; 2^-e of the tokens (e: of a token's whole row) behind all records.
 constexpr int record_bytes(int p) { return 4096 * p + 256; }
 
-// Workgroup = (16 tokens, a share of the units of columns), a wave per token, which reads its
-// whole row for the largest value.
+// Workgroup = (four tokens, a share of the columns, 4096 at most), a wave per token, which holds
+// its share in registers and reads the rest of its row for the largest value only.
 template <int G, bool XB>
-__global__ __launch_bounds__(1024) void q4_parts_kernel(Q4Args a) {
+__global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
     typedef Unit<G> U;
-    constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P);
-    const int lane = (int)threadIdx.x & 63, row = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), tile = (int)blockIdx.y;
-    const int units = (a.cols + U::kCols - 1) / U::kCols, blocks = units * U::NQ, t = 16 * tile + row;
+    constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), N = 8;
+    const int lane = (int)threadIdx.x & 63, t = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int units = (a.cols + U::kCols - 1) / U::kCols, blocks = units * U::NQ, tile = t >> 4, row = t & 15;
     const int64_t from = (int64_t)min(t, a.tokens - 1) * a.x_stride;
-    float m = 0.f;
-#pragma unroll 4
-    for (int col = 8 * lane; col < a.cols; col += 512) {
-        float v[8];
-        read8<XB>(a, from + col, v);
-        m = fmaxf(m, largest(v));
+    // four blocks, 512 columns, at a time
+    const int q = (blocks + 3) / 4, q0 = (int)((int64_t)q * blockIdx.x / gridDim.x), q1 = (int)((int64_t)q * (blockIdx.x + 1) / gridDim.x);
+    float v[N][8] = {}, m = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int col = 512 * (q0 + i) + 8 * lane;
+        if (q0 + i < q1 && col < a.cols && t < a.tokens) read8<XB>(a, from + col, v[i]);
     }
+    if (gridDim.x > 1) {
+#pragma unroll 4
+        for (int col = 8 * lane; col < a.cols; col += 512) {
+            float x[8];
+            read8<XB>(a, from + col, x);
+            m = fmaxf(m, largest(x));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, largest(v[i]));
     const int e = scale_of(m);
     const float up = power(e);
     if (blockIdx.x == 0 && lane == 0) a.down[t] = power(-e);
-    const int b0 = (int)((int64_t)blocks * blockIdx.x / gridDim.x), b1 = (int)((int64_t)blocks * (blockIdx.x + 1) / gridDim.x);
-    for (int b = b0 + (lane >> 4); b < (b1 + 3) / 4 * 4; b += 4) {   // (four records a wave; all lanes take part)
-        const int col = 128 * b + 8 * (lane & 15);
-        float v[8] = {};
-        if (t < a.tokens && b < b1 && col < a.cols) read8<XB>(a, from + col, v);
-        const float sum = group_sum<G>(v);
-        if (b >= b1) continue;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int b = 4 * (q0 + i) + (lane >> 4), col = 128 * b + 8 * (lane & 15);
+        if (q0 + i >= q1) break;
+        const float sum = group_sum<G>(v[i]);
+        if (b >= blocks) continue;
         uint8_t* rec = a.xparts + ((int64_t)tile * blocks + b) * kRecord;
         if (col % G == 0) reinterpret_cast<float*>(rec + 4096 * P)[(col & 127) / G * 16 + row] = sum * up;
         f16x8 hi, lo;
-        parts(v, up, hi, lo);
+        parts(v[i], up, hi, lo);
         int step, g;
         place<G>(lane & 15, step, g);
         *reinterpret_cast<f16x8*>(rec + 16 * (64 * step + 16 * g + row)) = hi;
@@ -698,7 +708,7 @@ void launch_few(const Q4Args& a, hipStream_t st) {
 
 template <int G, int NT, int MW, bool XB>
 void launch_many(const Q4Args& a, hipStream_t st) {
-    hipLaunchKernelGGL((q4_parts_kernel<G, XB>), dim3((unsigned)a.part_split, (unsigned)((a.tokens + 15) / 16)), dim3(1024),
+    hipLaunchKernelGGL((q4_parts_kernel<G, XB>), dim3((unsigned)a.part_split, (unsigned)((a.tokens + 15) / 16 * 4)), dim3(256),
                        0, st, a);
     hipLaunchKernelGGL((q4_many_kernel<G, NT, MW, XB>), dim3((unsigned)a.grid), dim3((unsigned)(64 * a.waves)), 0, st, a);
 }
@@ -754,7 +764,7 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
     a.split = all == a.whole ? 1 : std::max(1, std::min(units, slots / (all - a.whole)));
     if (a.split == 1) a.whole = all;
     a.grid = a.whole + (all - a.whole) * a.split;
-    a.part_split = std::max(1, std::min(nblocks / 4, cus / tt));
+    a.part_split = (nblocks + 31) / 32;
     const int64_t records = (int64_t)tt * nblocks * record_bytes(a.x_bf16 ? 1 : 2) / 4;
     a.down_at = records;
     a.part_at = records + 16 * tt;

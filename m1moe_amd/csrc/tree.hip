@@ -69,13 +69,12 @@ __global__ __launch_bounds__(64 * W) void tree_plan_kernel(TreePlanArgs a) {
 // the conversation: p_i >= i, so a place that is written is read by no later move, and a
 // thread that reads its 16 bytes of eight rows before it writes them needs no second buffer.
 //
-// Workgroup = (tree, plane of a layer's k or v, 4 KB of a position).  Every one walks for
-// itself: the walk (a thread in LDS, a level at a time) takes less than a launch would.
+// Workgroup = (tree, 4 KB of a position through all planes, the layers' k and v).  Every one walks
+// for itself: the walk (a thread in LDS, a level at a time) takes less than a launch would.
 __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptArgs a) {
     __shared__ int s_child[kTreeRows], s_drawn[kTreeRows], s_page[kTreeRows], s_path[kTreeRows], s_count;
     const PagedView& p = a.p;
     const int seq = (int)blockIdx.y, tid = (int)threadIdx.x;
-    const int slices = (a.row_units + 255) / 256, plane = (int)blockIdx.x / slices;
     const bool first = blockIdx.x == 0;
     const int lo = p.row_start[seq], hi = p.row_start[seq + 1], len = p.kv_len[seq], n = hi - lo;
     const bool rows = lo >= 0 && hi >= lo && hi <= p.num_rows && len >= n &&
@@ -125,8 +124,8 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptArgs a) {
             a.past[seq] = base + count;
         }
     }
-    const int unit = ((int)blockIdx.x - plane * slices) * 256 + tid;
-    if (unit >= a.row_units) return;
+    const int all = (int)blockIdx.x * 256 + tid, plane = all / a.row_units, unit = all - plane * a.row_units;
+    if (plane >= a.num_planes) return;
     uint4* cells = static_cast<uint4*>(a.planes[plane]);
     const auto cell = [&](int row) {
         const int pos = base + row;
@@ -171,7 +170,7 @@ int launch_tree_plan(const TreePlanArgs& a, void* stream) {
 
 int launch_tree_accept(const TreeAcceptArgs& a, void* stream) {
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)(a.num_planes * ((a.row_units + 255) / 256)), (unsigned)a.p.num_seqs);
+    const dim3 grid((unsigned)((a.num_planes * a.row_units + 255) / 256), (unsigned)a.p.num_seqs);
     hipLaunchKernelGGL(tree_accept_kernel, grid, dim3(256), 0, st, a);
     return (int)hipGetLastError();
 }

@@ -8,6 +8,11 @@ extern "C" long stub_drafts(void) { return g_drafts; }
 
 namespace m1moe {
 int launch_tree_plan(const TreePlanArgs&, void*) { return ++g_drafts, 0; }
+int launch_tree_attention(const PagedAttnArgs& a, void*) {
+    for (int i = 0; i < a.grid; ++i)
+        if (a.counters[i]) abort();
+    return ++g_drafts, 0;
+}
 int launch_tree_accept(const TreeAcceptArgs&, void*) { return ++g_drafts, 0; }
 int64_t matmul_q4_plan(Q4Args& a, int cus) {
     a.split = 2;
