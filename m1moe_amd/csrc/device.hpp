@@ -510,38 +510,23 @@ __device__ __forceinline__ void load8_coh(const float* const (&p)[8], vf4 (&v)[8
         : "memory");
 }
 
-// Sixteen times sixteen bytes from there, the lane's `at` bytes behind sixteen places that are the same
-// in all lanes, waited for.
-__device__ __forceinline__ void load16_coh(uint32_t at, const float* const (&p)[16], vf4 (&v)[16]) {
+// Sixteen times.
+__device__ __forceinline__ void load16_coh(const float* const (&p)[16], vf4 (&v)[16]) {
     asm volatile(
-        "global_load_dwordx4 %0, %16, %17 sc1\n\t"
-        "global_load_dwordx4 %1, %16, %18 sc1\n\t"
-        "global_load_dwordx4 %2, %16, %19 sc1\n\t"
-        "global_load_dwordx4 %3, %16, %20 sc1\n\t"
-        "global_load_dwordx4 %4, %16, %21 sc1\n\t"
-        "global_load_dwordx4 %5, %16, %22 sc1\n\t"
-        "global_load_dwordx4 %6, %16, %23 sc1\n\t"
-        "global_load_dwordx4 %7, %16, %24 sc1\n\t"
-        "global_load_dwordx4 %8, %16, %25 sc1\n\t"
-        "global_load_dwordx4 %9, %16, %26 sc1\n\t"
-        "global_load_dwordx4 %10, %16, %27 sc1\n\t"
-        "global_load_dwordx4 %11, %16, %28 sc1\n\t"
-        "global_load_dwordx4 %12, %16, %29 sc1\n\t"
-        "global_load_dwordx4 %13, %16, %30 sc1\n\t"
-        "global_load_dwordx4 %14, %16, %31 sc1\n\t"
-        "global_load_dwordx4 %15, %16, %32 sc1\n\t"
+        "global_load_dwordx4 %0, %16, off sc1\n\tglobal_load_dwordx4 %1, %17, off sc1\n\t"
+        "global_load_dwordx4 %2, %18, off sc1\n\tglobal_load_dwordx4 %3, %19, off sc1\n\t"
+        "global_load_dwordx4 %4, %20, off sc1\n\tglobal_load_dwordx4 %5, %21, off sc1\n\t"
+        "global_load_dwordx4 %6, %22, off sc1\n\tglobal_load_dwordx4 %7, %23, off sc1\n\t"
+        "global_load_dwordx4 %8, %24, off sc1\n\tglobal_load_dwordx4 %9, %25, off sc1\n\t"
+        "global_load_dwordx4 %10, %26, off sc1\n\tglobal_load_dwordx4 %11, %27, off sc1\n\t"
+        "global_load_dwordx4 %12, %28, off sc1\n\tglobal_load_dwordx4 %13, %29, off sc1\n\t"
+        "global_load_dwordx4 %14, %30, off sc1\n\tglobal_load_dwordx4 %15, %31, off sc1\n\t"
         "s_waitcnt vmcnt(0)"
         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]),
           "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]), "=&v"(v[14]), "=&v"(v[15])
-        : "v"(at), "s"(p[0]), "s"(p[1]), "s"(p[2]), "s"(p[3]), "s"(p[4]), "s"(p[5]), "s"(p[6]), "s"(p[7]),
-          "s"(p[8]), "s"(p[9]), "s"(p[10]), "s"(p[11]), "s"(p[12]), "s"(p[13]), "s"(p[14]), "s"(p[15])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]),
+          "v"(p[8]), "v"(p[9]), "v"(p[10]), "v"(p[11]), "v"(p[12]), "v"(p[13]), "v"(p[14]), "v"(p[15])
         : "memory");
-}
-// The same address in every lane, as the scalar it is.
-__device__ __forceinline__ const float* uniform_ptr(const float* p) {
-    const uint64_t x = reinterpret_cast<uint64_t>(p);
-    return reinterpret_cast<const float*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
-                                          (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
 }
 
 __device__ __forceinline__ void flag_error(uint32_t* err, uint32_t code) {

