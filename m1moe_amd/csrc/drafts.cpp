@@ -243,6 +243,7 @@ int32_t m1moe_matmul_q4(m1moe_ctx_t ctx, const m1moe_q4_weights* w, const void* 
     if (floats) {
         if ((rc = ensure_q4_scratch(ctx, (uint64_t)floats))) return rc;
         a.xparts = reinterpret_cast<uint8_t*>(ctx->q4_part);
+        a.xsums = reinterpret_cast<uint8_t*>(ctx->q4_part + a.sums_at);
         a.down = ctx->q4_part + a.down_at;
         a.part = ctx->q4_part + a.part_at;
         a.counters = ctx->q4_cnt;

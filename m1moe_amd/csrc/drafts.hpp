@@ -47,8 +47,8 @@ struct Q4Args {
     int32_t grid_x, whole;         // tiles of rows of W; tiles that are not shared
     int32_t chunk, lds;            // units of columns staged at once, bytes of LDS
     int32_t part_split;            // workgroups that make a token's parts
-    int64_t down_at, part_at;      // floats of the workspace before these
-    uint8_t* xparts;               // x in parts
+    int64_t sums_at, down_at, part_at;   // floats of the workspace before these
+    uint8_t *xparts, *xsums;       // x in parts, its groups' sums in parts
     float* down;                   // [tokens rounded up to 16]: what x was divided by
     float* part;                   // partials of split workgroups
     uint32_t* counters;            // of shared tiles, zero between launches

@@ -14,6 +14,8 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 
+// Of a workgroup of many tokens: tiles of 16 of them, tiles of 16 rows of a wave.
+constexpr int kManyTiles = 2, kManyRows = 2;
 // Most tokens that every workgroup stages for itself, and the rows of LDS that it takes for r.
 constexpr int kFewTokens = 32;
 __host__ __device__ constexpr int few_rows(int r) { return r | 1; }
@@ -97,25 +99,31 @@ struct Weights {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) x.s[i] = p.x[i], x.b[i] = q.x[i];
     }
+    // The words of any 128-column block (past the row its last columns again, which meet x = 0 and
+    // scales of 0).
+    __device__ __forceinline__ uint4 words(int block) const {
+        return *reinterpret_cast<const uint4*>(w + (min(128 * block, cols - 32 * (g + 1)) >> 1));
+    }
+    // N of the row's scales or biases from group q on, past its last one 0.
+    template <int N>
+    __device__ __forceinline__ void halves(const uint16_t* from_all, int q, uint32_t (&x)[N / 2]) const {
+        const int left = max(groups - q, 0);
+        const int64_t want = at + q, from = min(want, total - N);
+        const Halves<N> p = *reinterpret_cast<const Halves<N>*>(from_all + from);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) x[i] = p.x[i];
+        if (left < N) shift<N>(x, (int)(want - from), left);
+    }
     // Any unit.
     template <int G>
     __device__ __forceinline__ void load(int u, Unit<G>& x) const {
         typedef Unit<G> U;
         constexpr int N = U::kGroups;
-        const int left = groups - u * N;
-        if (left >= N) return load_whole<G>(u, x);
+        if (groups - u * N >= N) return load_whole<G>(u, x);
 #pragma unroll
-        for (int i = 0; i < U::NQ; ++i) {
-            // (past the row: its last columns again, which meet x = 0 and scales of 0)
-            const int col = min(u * U::kCols + 128 * i, cols - 32 * (g + 1));
-            x.w[i] = *reinterpret_cast<const uint4*>(w + (col >> 1));
-        }
-        const int64_t want = at + u * N, from = min(want, total - N);
-        const Halves<N> p = *reinterpret_cast<const Halves<N>*>(s + from), q = *reinterpret_cast<const Halves<N>*>(b + from);
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) x.s[i] = p.x[i], x.b[i] = q.x[i];
-        shift<N>(x.s, (int)(want - from), left);
-        shift<N>(x.b, (int)(want - from), left);
+        for (int i = 0; i < U::NQ; ++i) x.w[i] = words(u * U::NQ + i);
+        halves<N>(s, u * N, x.s);
+        halves<N>(b, u * N, x.b);
     }
 };
 
@@ -483,22 +491,32 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
 
 // ---- many tokens -----------------------------------------------------------------------
 //
-// x is made into f16 parts once, by a kernel of its own: records of 16 tokens' 128 columns, [P
-// parts][4 steps][64 lanes] 16 bytes, as the MFMAs take them, then the groups' sums X_G 2^e
-// [4][16]; 2^-e of the tokens (e: of a token's whole row) behind all records.
-constexpr int record_bytes(int p) { return 4096 * p + 256; }
+// x is made into operands once, by a kernel of its own: f16 parts in records of 16 tokens' 128
+// columns, [P parts][4 steps][64 lanes] 16 bytes, as the MFMAs take them; the groups' sums
+// X_G 2^e as three bf16 parts, 32 groups together, [3][64 lanes] 16 bytes; and the tokens' 2^-e
+// (e: of a token's whole row).
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+constexpr int record_bytes(int p) { return 4096 * p; }
+constexpr int kSumBytes = 3072;
+
+// x as three bf16 parts.
+__device__ __forceinline__ void bf16_parts(float x, __bf16 (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        p[i] = (__bf16)x;
+        x -= (float)p[i];
+    }
+}
 
 // Workgroup = (four tokens, a share of the columns, 4096 at most), a wave per token, which holds
 // its share in registers and reads the rest of its row for the largest value only.
 template <int G, bool XB>
 __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
-    typedef Unit<G> U;
     constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), N = 8;
     const int lane = (int)threadIdx.x & 63, t = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int units = (a.cols + U::kCols - 1) / U::kCols, blocks = units * U::NQ, tile = t >> 4, row = t & 15;
+    const int quads = (a.cols + 511) / 512, tile = t >> 4, row = t & 15, sums = (a.cols / G + 31) / 32;
     const int64_t from = (int64_t)min(t, a.tokens - 1) * a.x_stride;
-    // four blocks, 512 columns, at a time
-    const int q = (blocks + 3) / 4, q0 = (int)((int64_t)q * blockIdx.x / gridDim.x), q1 = (int)((int64_t)q * (blockIdx.x + 1) / gridDim.x);
+    const int q0 = (int)((int64_t)quads * blockIdx.x / gridDim.x), q1 = (int)((int64_t)quads * (blockIdx.x + 1) / gridDim.x);
     float v[N][8] = {}, m = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -518,14 +536,20 @@ __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
     const int e = scale_of(m);
     const float up = power(e);
     if (blockIdx.x == 0 && lane == 0) a.down[t] = power(-e);
+    const auto put_sum = [&](int q, float x) {      // group q's
+        __bf16 p[3];
+        bf16_parts(x, p);
+        uint8_t* to = a.xsums + ((int64_t)tile * sums + (q >> 5)) * kSumBytes + 16 * (16 * (q >> 3 & 3) + row) + 2 * (q & 7);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<__bf16*>(to + 1024 * k) = p[k];
+    };
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int b = 4 * (q0 + i) + (lane >> 4), col = 128 * b + 8 * (lane & 15);
         if (q0 + i >= q1) break;
         const float sum = group_sum<G>(v[i]);
-        if (b >= blocks) continue;
-        uint8_t* rec = a.xparts + ((int64_t)tile * blocks + b) * kRecord;
-        if (col % G == 0) reinterpret_cast<float*>(rec + 4096 * P)[(col & 127) / G * 16 + row] = sum * up;
+        uint8_t* rec = a.xparts + ((int64_t)tile * 4 * quads + b) * kRecord;
+        if (col % G == 0) put_sum(col / G, sum * up);
         f16x8 hi, lo;
         parts(v[i], up, hi, lo);
         int step, g;
@@ -533,35 +557,29 @@ __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
         *reinterpret_cast<f16x8*>(rec + 16 * (64 * step + 16 * g + row)) = hi;
         if (P == 2) *reinterpret_cast<f16x8*>(rec + 4096 + 16 * (64 * step + 16 * g + row)) = lo;
     }
+    if (blockIdx.x == 0)
+        for (int q = 512 * quads / G + lane; q < 32 * sums; q += 64) put_sum(q, 0.f);
 }
 
-// Workgroup = 16 NT tokens, 16 MW rows of W a wave; a wave's words come straight from memory as
-// above, a unit ahead, the records through LDS, copied by the loads themselves, SB blocks of
-// 128 columns at a time, the next ones on their way while some are computed.
+// Workgroup = 16 NT tokens, 16 MW rows of W a wave.  A wave's words come straight from memory,
+// two blocks of 128 columns ahead, its scales four; the records through LDS, copied by the
+// loads themselves, a block ahead.  The biases' part, sum_G b'_G X_G with b' = b + 8 s, is a
+// product of its own before the others, of bf16 parts, six MFMAs for 32 groups (as a
+// multiply-add per value, group and lane, with its sums read from LDS, 800 x 6144 x 4096: 122 us).
 template <int G, int NT, int MW, bool XB>
-struct Many {
-    typedef Unit<G> U;
-    static constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P);
-    static constexpr int SB = std::min(U::NQ, std::max(1, 8 / (NT * P)));
-    static constexpr int kStage = SB * NT * kRecord;
-    static constexpr int kLoads = MW * (U::NQ + 2);      // a unit's, at least
-};
-
-template <int G, int NT, int MW, bool XB>
-__global__ __launch_bounds__(512, MW * NT <= 4 ? 4 : 2) void q4_many_kernel(Q4Args a) {
-    typedef Many<G, NT, MW, XB> M;
-    typedef Unit<G> U;
-    constexpr int P = M::P, SB = M::SB, kRecord = M::kRecord, kSteps = G / 32;
-    __shared__ __attribute__((aligned(16))) uint8_t s_x[2 * M::kStage];
+__global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
+    constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), kStage = NT * kRecord, kSteps = G / 32, kWaves = 8;
+    constexpr int kGroups = 512 / G, N = kGroups < 8 ? kGroups : 8;    // of a unit of four blocks, of one load
+    __shared__ __attribute__((aligned(16))) uint8_t s_x[2 * kStage];
     __shared__ int s_last;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int waves = (int)blockDim.x >> 6, c = lane & 15, g = lane >> 4;
+    const int c = lane & 15, g = lane >> 4;
     // this workgroup's tile: one of the `whole` ones, or a share of one of the others
     const int id = (int)blockIdx.x, rest = id - a.whole, KW = rest < 0 ? 1 : a.split, kw = rest < 0 ? 0 : rest % KW;
     const int tile = rest < 0 ? id : a.whole + rest / KW, ty = tile / a.grid_x, block = tile - ty * a.grid_x;
-    const int t0 = ty * 16 * NT, tile0 = (block * waves + wave) * MW;
-    const int units = (a.cols + U::kCols - 1) / U::kCols, blocks = units * U::NQ;
-    const int u0 = (int)((int64_t)units * kw / KW), u1 = (int)((int64_t)units * (kw + 1) / KW);
+    const int t0 = ty * 16 * NT, tile0 = (block * kWaves + wave) * MW;
+    const int units = (a.cols + 511) / 512, sums = (a.cols / G + 31) / 32;
+    const int u0 = (int)((int64_t)units * kw / KW), u1 = (int)((int64_t)units * (kw + 1) / KW), last = 4 * u1 - 1;
     const int tiles = min(NT, (a.tokens - t0 + 15) / 16);   // of tokens that there are
     int n[MW];
     Weights w[MW];
@@ -570,122 +588,137 @@ __global__ __launch_bounds__(512, MW * NT <= 4 ? 4 : 2) void q4_many_kernel(Q4Ar
         n[m] = 16 * (tile0 + m) + c;
         w[m] = Weights(a, min(n[m], a.rows - 1), g);
     }
-    const uint8_t* rec = a.xparts + (int64_t)ty * NT * blocks * kRecord;
-    // SB blocks from block k on to buffer s
+    const uint8_t* rec = a.xparts + (int64_t)ty * NT * 4 * units * kRecord;
+    // block k's records to buffer s
     const auto copy = [&](int k, int s) {
-#pragma unroll 1
-        for (int i = wave; i < NT * SB; i += waves) {
-            const int t = i / SB, b = i - t * SB;
-            const uint8_t* from = rec + ((int64_t)min(t, tiles - 1) * blocks + k + b) * kRecord;
-            const uint32_t to = lds_addr(s_x) + s * M::kStage + (t * SB + b) * kRecord;
 #pragma unroll
-            for (int j = 0; j < 4 * P; ++j) lds_copy16(16 * lane + 1024 * j, from, to + 1024 * j);
-            lds_copy4(4 * lane + 4096 * P, from, to + 4096 * P);
+        for (int i = 0; i < NT * 4 * P; i += kWaves) {
+            if (NT * 4 * P % kWaves && i + wave >= NT * 4 * P) break;
+            const int t = (i + wave) / (4 * P), j = (i + wave) % (4 * P);
+            const uint8_t* from = rec + ((int64_t)min(t, tiles - 1) * 4 * units + k) * kRecord + 1024 * j;
+            lds_copy16(16 * lane, from, lds_addr(s_x) + s * kStage + t * kRecord + 1024 * j);
         }
+    };
+    const auto scales = [&](int u, uint32_t (&x)[MW][kGroups / 2]) {
+#pragma unroll
+        for (int m = 0; m < MW; ++m)
+#pragma unroll
+            for (int i = 0; i < kGroups / N; ++i)
+                w[m].template halves<N>(w[m].s, u * kGroups + N * i, reinterpret_cast<uint32_t(&)[N / 2]>(x[m][i * N / 2]));
     };
     f32x4v acc[MW * NT];
 #pragma unroll
     for (int i = 0; i < MW * NT; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    const NibK nk = nib_consts();
-    int turn = 0;
-    // Unit u, x; the next one's words, y (NEXT: 0 none, 1 a whole unit, 2 any), are asked for
-    // behind the second stage's records.
-    const auto compute = [&](auto next_unit, const U (&x)[MW], U (&y)[MW], int u) {
-        constexpr int NEXT = decltype(next_unit)::value;
+    if (kw == 0) {
+        for (int k = 0; k < sums; ++k) {
+            bf16x8 x[NT][3], b[MW][3];
 #pragma unroll
-        for (int b0 = 0; b0 < U::NQ; b0 += SB) {
-            if (b0 == SB && NEXT)
-                wait_vm<M::kLoads>();
-            else
-                wait_vm<0>();
-            __syncthreads();      // (the stage is there, and the other one read)
-            if (b0 + SB < U::NQ || NEXT) copy(u * U::NQ + b0 + SB, turn ^ 1);
-            if (b0 == 0) {
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    x[t][p] = *reinterpret_cast<const bf16x8*>(
+                        a.xsums + (((int64_t)ty * NT + min(t, tiles - 1)) * sums + k) * kSumBytes + 1024 * p + 16 * lane);
+#pragma unroll
+            for (int m = 0; m < MW; ++m) {
+                constexpr int H = G == 128 ? 4 : 8;     // (a row has as many groups at least, or all rows together)
+                uint32_t sv[4], bv[4];
+#pragma unroll
+                for (int i = 0; i < 8 / H; ++i) {
+                    w[m].template halves<H>(w[m].s, 32 * k + 8 * g + H * i, reinterpret_cast<uint32_t(&)[H / 2]>(sv[i * H / 2]));
+                    w[m].template halves<H>(w[m].b, 32 * k + 8 * g + H * i, reinterpret_cast<uint32_t(&)[H / 2]>(bv[i * H / 2]));
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    __bf16 p[3];
+                    bf16_parts(fmaf(8.f, bf16_pair(sv, i), bf16_pair(bv, i)), p);
+                    b[m][0][i] = p[0], b[m][1][i] = p[1], b[m][2][i] = p[2];
+                }
+            }
+#pragma unroll
+            for (int o = 2; o >= 0; --o)      // (small products first)
+#pragma unroll
+                for (int p = 0; p <= o; ++p)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int m = 0; m < MW; ++m)
+                            acc[m * NT + t] =
+                                __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[t][p], b[m][o - p], acc[m * NT + t], 0, 0, 0);
+        }
+    }
+    uint4 x[4][MW];
+    uint32_t s_now[MW][kGroups / 2], s_next[MW][kGroups / 2];
+    const auto words = [&](int k, uint4 (&y)[MW]) {
+#pragma unroll
+        for (int m = 0; m < MW; ++m) y[m] = w[m].words(k);
+    };
+    scales(u0, s_now);
+    words(4 * u0, x[0]);
+    copy(4 * u0, 0);
+    words(4 * u0 + 1, x[1]);
+    const NibK nk = nib_consts();
+    for (int u = u0; u < u1; ++u) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int k = 4 * opaque(u) + b;
+            wait_vm<MW>();        // (but for the next block's words)
+            __syncthreads();      // (the block's records are there, and the other buffer read)
+            uint32_t v[MW][4];
+#pragma unroll
+            for (int m = 0; m < MW; ++m) steps<G>(x[b][m], v[m]);
+            // (past the last block: that one again, into a buffer that is not read)
+            if (b == 2) scales(min(u + 1, u1 - 1), s_next);
+            copy(min(k + 1, last), ~b & 1);
+            words(min(k + 2, last), x[(b + 2) & 3]);
+            const uint8_t* s = s_x + (b & 1) * kStage;
+            // (a tile's sums are added while the next one's MFMAs run; here and now: or the
+            // compiler keeps all tiles' sums of a block for later)
+            f32x4v part[2][MW];
+            float sc[2][MW];
+            const auto flush = [&](int i) {
 #pragma unroll
                 for (int m = 0; m < MW; ++m) {
-                    if (NEXT == 1) w[m].template load_whole<G>(u + 1, y[m]);
-                    if (NEXT == 2) w[m].template load<G>(u + 1, y[m]);
+                    f32x4v& y = acc[m * NT + i % NT];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = fmaf(sc[i / NT & 1][m], part[i & 1][m][e], y[e]);
+                    asm volatile("" : "+v"(y));
+                }
+            };
+#pragma unroll
+            for (int qb = 0; qb < 4 / kSteps; ++qb) {     // the block's groups
+                f16x8 q[MW][kSteps];
+#pragma unroll
+                for (int m = 0; m < MW; ++m) {
+#pragma unroll
+                    for (int j = 0; j < kSteps; ++j) q[m][j] = nibbles(v[m][kSteps * qb + j], nk);
+                    sc[qb & 1][m] = bf16_pair(s_now[m], 4 / kSteps * b + qb);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int i = qb * NT + t;
+#pragma unroll
+                    for (int m = 0; m < MW; ++m) part[i & 1][m] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+                        for (int j = 0; j < kSteps; ++j) {
+                            const f16x8 y = *reinterpret_cast<const f16x8*>(s + t * kRecord + 4096 * p +
+                                                                            1024 * (kSteps * qb + j) + 16 * lane);
+#pragma unroll
+                            for (int m = 0; m < MW; ++m)
+                                part[i & 1][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[m][j], part[i & 1][m], 0, 0, 0);
+                        }
+                    if (i > 0) flush(i - 1);
                 }
             }
-            const uint8_t* s = s_x + turn * M::kStage;
-            turn ^= 1;
-#pragma unroll
-            for (int b = 0; b < SB; ++b) {
-                __builtin_amdgcn_sched_barrier(0);   // (as above)
-                uint32_t v[MW][4];
-#pragma unroll
-                for (int m = 0; m < MW; ++m) steps<G>(x[m].w[b0 + b], v[m]);
-                // (a tile's sums are added while the next one's MFMAs run; here and now: or the
-                // compiler keeps all tiles' sums of a stage for later)
-                f32x4v part[2][MW], sum[2];
-                float sc[2][MW], bi[2][MW];
-                const auto flush = [&](int i) {
-                    const int t = i % NT;
-#pragma unroll
-                    for (int m = 0; m < MW; ++m) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            acc[m * NT + t][e] = fmaf(bi[i / NT & 1][m], sum[i & 1][e],
-                                                fmaf(sc[i / NT & 1][m], part[i & 1][m][e], acc[m * NT + t][e]));
-                        asm volatile("" : "+v"(acc[m * NT + t]));
-                    }
-                };
-#pragma unroll
-                for (int qb = 0; qb < 4 / kSteps; ++qb) {     // the block's groups
-                    const int qu = (4 * (b0 + b)) / kSteps + qb;
-                    f16x8 q[MW][kSteps];
-#pragma unroll
-                    for (int m = 0; m < MW; ++m) {
-#pragma unroll
-                        for (int j = 0; j < kSteps; ++j) q[m][j] = nibbles(v[m][kSteps * qb + j], nk);
-                        sc[qb & 1][m] = bf16_pair(x[m].s, qu);
-                        bi[qb & 1][m] = fmaf(8.f, sc[qb & 1][m], bf16_pair(x[m].b, qu));
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const int i = qb * NT + t;
-                        const uint8_t* r = s + (t * SB + b) * kRecord;
-#pragma unroll
-                        for (int m = 0; m < MW; ++m) part[i & 1][m] = f32x4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-                            for (int j = 0; j < kSteps; ++j) {
-                                const f16x8 y = *reinterpret_cast<const f16x8*>(r + 4096 * p + 1024 * (kSteps * qb + j) +
-                                                                                16 * lane);
-#pragma unroll
-                                for (int m = 0; m < MW; ++m)
-                                    part[i & 1][m] =
-                                        __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[m][j], part[i & 1][m], 0, 0, 0);
-                            }
-                        sum[i & 1] = *reinterpret_cast<const f32x4v*>(r + 4096 * P + 64 * qb + 16 * g);
-                        if (i > 0) flush(i - 1);
-                    }
-                }
-                flush(4 / kSteps * NT - 1);
-            }
+            flush(4 / kSteps * NT - 1);
         }
-    };
-    U x[MW], y[MW];
-    copy(u0 * U::NQ, 0);
 #pragma unroll
-    for (int m = 0; m < MW; ++m) w[m].template load<G>(u0, x[m]);
-    const auto next = [&] {
+        for (int m = 0; m < MW; ++m)
 #pragma unroll
-        for (int m = 0; m < MW; ++m) x[m] = y[m];
-    };
-    int u = u0;
-    for (const int whole = min(u1, a.cols / U::kCols); u + 1 < whole; ++u) {
-        compute(std::integral_constant<int, 1>{}, x, y, u);
-        next();
+            for (int i = 0; i < kGroups / 2; ++i) s_now[m][i] = s_next[m][i];
     }
-    if (u + 1 < u1) {
-        compute(std::integral_constant<int, 2>{}, x, y, u);
-        next();
-        ++u;
-    }
-    compute(std::integral_constant<int, 0>{}, x, y, u);
-    if (KW > 1 && !join_split<MW * NT>(a, tile - a.whole, KW, kw, waves, wave, true, acc, &s_last)) return;
+    if (KW > 1 && !join_split<MW * NT>(a, tile - a.whole, KW, kw, kWaves, wave, true, acc, &s_last)) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         if (t >= tiles) break;
@@ -718,7 +751,7 @@ void launch_group(const Q4Args& a, hipStream_t st) {
     if (a.tiny)
         hipLaunchKernelGGL((q4_tiny_kernel<XB>), dim3((unsigned)a.rows, (unsigned)a.tokens), dim3(64), 0, st, a);
     else if (a.tokens > kFewTokens)
-        launch_many<G, 4, 1, XB>(a, st);
+        launch_many<G, kManyTiles, kManyRows, XB>(a, st);
     else if (a.tokens <= (XB ? 16 : 8))
         launch_few<G, 1, 1, XB>(a, st);
     else if (!XB && a.tokens <= 16)
@@ -754,20 +787,21 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
         a.lds = std::max(a.chunk * bytes, a.wave_split > 1 ? a.waves * nt * 1024 : 16);
         return a.split > 1 ? (int64_t)a.grid * a.waves * nt * 256 : 0;
     }
-    const int tt = (a.tokens + 15) / 16, nblocks = units * (unit / 128), nt = 4, mw = 1;
+    constexpr int nt = kManyTiles, mw = kManyRows;
+    const int tt = (a.tokens + 15) / 16, quads = (a.cols + 511) / 512, sums = (a.cols / a.group + 31) / 32;
     // Whole tiles as long as they fill the card, two workgroups a CU; the columns of the others are
     // shared by as many workgroups as make one more round of it (800 x 6144 x 4096, 624 tiles: all
     // whole 136 us).
     a.grid_x = (tiles + mw * a.waves - 1) / (mw * a.waves);
     const int all = a.grid_x * ((tt + nt - 1) / nt), slots = 2 * cus;
     a.whole = all / slots * slots;
-    a.split = all == a.whole ? 1 : std::max(1, std::min(units, slots / (all - a.whole)));
+    a.split = all == a.whole ? 1 : std::max(1, std::min(quads, slots / (all - a.whole)));
     if (a.split == 1) a.whole = all;
     a.grid = a.whole + (all - a.whole) * a.split;
-    a.part_split = (nblocks + 31) / 32;
-    const int64_t records = (int64_t)tt * nblocks * record_bytes(a.x_bf16 ? 1 : 2) / 4;
-    a.down_at = records;
-    a.part_at = records + 16 * tt;
+    a.part_split = (quads + 7) / 8;
+    a.sums_at = (int64_t)tt * quads * record_bytes(a.x_bf16 ? 1 : 2);
+    a.down_at = a.sums_at + (int64_t)tt * sums * kSumBytes / 4;
+    a.part_at = a.down_at + 16 * tt;
     return a.part_at + (int64_t)(a.grid - a.whole) * a.waves * mw * nt * 256;
 }
 
