@@ -174,6 +174,13 @@ int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs, int32_t nu
     for (int i = 1; i < a.num_planes; ++i)
         if (static_cast<char*>(sorted[i]) - static_cast<char*>(sorted[i - 1]) < plane)
             return fail(M1MOE_ERR_INVALID, "two of the caches' d_k and d_v overlap");
+    // (apart and in order: of those that begin before an output's end, the last one ends last)
+    for (const Range& o : {Range{d_path, rows, "d_path"}, Range{d_accepted, seqs, "d_accepted"},
+                           Range{d_next, seqs, "d_next"}, Range{d_past, seqs, "d_past"}}) {
+        void** after = std::lower_bound(sorted, sorted + a.num_planes, const_cast<char*>(static_cast<const char*>(o.p)) + o.bytes);
+        if (after != sorted && overlap(o, {after[-1], plane, ""}))
+            return fail(M1MOE_ERR_INVALID, "%s must not overlap a cache's d_k or d_v", o.what);
+    }
     if ((rc = set_device(ctx))) return rc;
     a.p = view(ctx, kvs, batch);
     a.row_units = (int32_t)(position / 16);

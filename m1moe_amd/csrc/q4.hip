@@ -16,8 +16,11 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 
 // Of a workgroup of many tokens: tiles of 16 of them, tiles of 16 rows of a wave.
 constexpr int kManyTiles = 2, kManyRows = 2;
-// Most tokens that every workgroup stages for itself, and the rows of LDS that it takes for r.
-constexpr int kFewTokens = 32;
+// Most tokens that every workgroup stages for itself (with 16, 17 to 32 tokens as many: 6144 x 4096
+// f32, 17 tokens 16.6 us as few, 25.5 as many, 32 tokens 20.6 and 27.0; 50304 x 2048 26.2 and
+// 33.4, 33.0 and 35.4), the LDS that it does so in, so that two fit a CU, and the rows of LDS
+// that it takes for r.
+constexpr int kFewTokens = 32, kFewLds = 76 * 1024;
 __host__ __device__ constexpr int few_rows(int r) { return r | 1; }
 
 // With the columns' groups G, y = sum_G (s_G sum_{k in G} x_k (q_k - 8) + (b_G + 8 s_G) X_G),
@@ -207,12 +210,17 @@ __device__ __forceinline__ void read8(const Q4Args& a, int64_t at, float (&v)[8]
         v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
     }
 }
-// They times 2^e as f16 parts, in the order of a word's nibbles.
-__device__ __forceinline__ void parts(const float (&v)[8], float up, f16x8& hi, f16x8& lo) {
+// They, times 2^e (before they are summed, or large ones would pass the largest float).
+__device__ __forceinline__ void scale(float (&v)[8], float up) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= up;
+}
+// As f16 parts, in the order of a word's nibbles.
+__device__ __forceinline__ void parts(const float (&v)[8], f16x8& hi, f16x8& lo) {
     constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float x = v[order[j]] * up;
+        const float x = v[order[j]];
         hi[j] = (_Float16)x;
         lo[j] = (_Float16)(x - (float)hi[j]);
     }
@@ -270,16 +278,17 @@ struct Few {
                 const int i = i0 + k * waves, t = i / n, u = i - t * n, row = RT * t;
                 if (i >= tn * n) break;
                 const int e = scale_of(largest(v[k]));
-                const float up = power(e), sum = group_sum<G>(v[k]);
+                scale(v[k], power(e));
+                const float sum = group_sum<G>(v[k]);
                 if (lane < RT) s_down[16 * NT * u + row + lane] = power(-e);
                 if (at0 >= U::kCols) continue;
                 if (at0 % G == 0) {
                     float* to = s_sum + (u * U::kGroups + at0 / G) * 16 * NT + row;
-                    to[0] = sum * up;
+                    to[0] = sum;
                     if (RT == 2) to[1] = 0.f;
                 }
                 f16x8 hi, lo;
-                parts(v[k], up, hi, lo);
+                parts(v[k], hi, lo);
                 int step, g;
                 place<G>(lane & 15, step, g);
                 step += 4 * (lane >> 4);
@@ -356,7 +365,7 @@ __device__ __forceinline__ void put(const Q4Args& a, int t, int n, float y) {
 // wave per token and row.
 template <bool XB>
 __global__ __launch_bounds__(64) void q4_tiny_kernel(Q4Args a) {
-    const int lane = (int)threadIdx.x, n = (int)blockIdx.x, t = (int)blockIdx.y, groups = a.cols / a.group;
+    const int lane = (int)threadIdx.x, t = (int)blockIdx.x, n = (int)blockIdx.y, groups = a.cols / a.group;
     float sum = 0.f;
     for (int k = lane; k < a.cols; k += 64) {
         const int64_t at = (int64_t)t * a.x_stride + k, g = (int64_t)n * groups + k / a.group;
@@ -547,11 +556,12 @@ __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
     for (int i = 0; i < N; ++i) {
         const int b = 4 * (q0 + i) + (lane >> 4), col = 128 * b + 8 * (lane & 15);
         if (q0 + i >= q1) break;
+        scale(v[i], up);
         const float sum = group_sum<G>(v[i]);
         uint8_t* rec = a.xparts + ((int64_t)tile * 4 * quads + b) * kRecord;
-        if (col % G == 0) put_sum(col / G, sum * up);
+        if (col % G == 0) put_sum(col / G, sum);
         f16x8 hi, lo;
-        parts(v[i], up, hi, lo);
+        parts(v[i], hi, lo);
         int step, g;
         place<G>(lane & 15, step, g);
         *reinterpret_cast<f16x8*>(rec + 16 * (64 * step + 16 * g + row)) = hi;
@@ -718,6 +728,7 @@ __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
 #pragma unroll
             for (int i = 0; i < kGroups / 2; ++i) s_now[m][i] = s_next[m][i];
     }
+    wait_vm<0>();     // (the last copy into LDS, before the LDS may be another workgroup's)
     if (KW > 1 && !join_split<MW * NT>(a, tile - a.whole, KW, kw, kWaves, wave, true, acc, &s_last)) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -749,7 +760,7 @@ void launch_many(const Q4Args& a, hipStream_t st) {
 template <int G, bool XB>
 void launch_group(const Q4Args& a, hipStream_t st) {
     if (a.tiny)
-        hipLaunchKernelGGL((q4_tiny_kernel<XB>), dim3((unsigned)a.rows, (unsigned)a.tokens), dim3(64), 0, st, a);
+        hipLaunchKernelGGL((q4_tiny_kernel<XB>), dim3((unsigned)a.tokens, (unsigned)a.rows), dim3(64), 0, st, a);
     else if (a.tokens > kFewTokens)
         launch_many<G, kManyTiles, kManyRows, XB>(a, st);
     else if (a.tokens <= (XB ? 16 : 8))
@@ -773,16 +784,24 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
         const bool flat = !a.x_bf16 && a.tokens <= 8;
         const int nt = a.tokens <= 16 ? 1 : 2, p = a.x_bf16 || flat ? 1 : 2;
         const int bytes = p * (unit / 32) * 64 * few_rows(flat ? 2 * a.tokens : a.tokens) + (groups + 1) * 64 * nt;
-        if (a.tokens <= 4) {
+        // A tile's columns are shared by the waves of a workgroup, which need no second pass, as long as
+        // staging x costs little: 4 tokens, all of whose columns fit the LDS at once; behind that by
+        // workgroups, each of which stages its share only (2048 x 2048: 1 token 5.4 us so, 7.8 by
+        // workgroups, 8 tokens 8.6 and 8.4; 6144 x 4096: 1 token 9.4 and 11.3, 4 bf16 ones 11.5 and
+        // 11.7, 4 f32 ones, whose columns do not fit, 13.7 and 11.6, 8 16.5 and 12.1).
+        if (a.tokens <= 4 && units * bytes <= kFewLds) {
             while (a.wave_split < 8 && 2 * a.wave_split <= units && tiles * a.wave_split * 2 <= 16 * cus) a.wave_split *= 2;
+            // (workgroups of 4 while there are few: 2048 x 2048, 1 token 5.5 us, of 8 waves 5.9)
             if (a.wave_split <= 4 && tiles * a.wave_split < 8 * cus) a.waves = 4;
         } else {
+            // (x is staged once for 16 waves where these still fill the card: 50304 x 2048, 16 f32 tokens
+            // 21.2 us, of 8 waves 24.7; 2048 x 2048 9.2, of 16 waves 11.5)
             a.waves = tiles >= 8 * cus ? 16 : 8;
             a.split = std::max(1, std::min(units, cus / ((tiles + a.waves - 1) / a.waves)));
         }
         const int per = a.waves / a.wave_split;
-        // all of a workgroup's columns at once, in at most 76 KB, so that two fit a CU, of many waves 152
-        a.chunk = std::max(1, std::min((a.waves == 16 ? 152 : 76) * 1024 / bytes, (units + a.split - 1) / a.split));
+        // all of a workgroup's columns at once, of 16 waves in the LDS of two workgroups of 8
+        a.chunk = std::max(1, std::min((a.waves == 16 ? 2 : 1) * kFewLds / bytes, (units + a.split - 1) / a.split));
         a.grid = (tiles + per - 1) / per * a.split;
         a.lds = std::max(a.chunk * bytes, a.wave_split > 1 ? a.waves * nt * 1024 : 16);
         return a.split > 1 ? (int64_t)a.grid * a.waves * nt * 256 : 0;

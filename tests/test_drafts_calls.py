@@ -29,7 +29,7 @@ def lib(tmp_path_factory):
             getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
     lib.stub_ctx.restype = ctypes.c_void_p
     lib.stub_free.argtypes = [ctypes.c_void_p]
-    lib.stub_launches.restype = lib.stub_drafts.restype = ctypes.c_long
+    lib.stub_launches.restype = lib.stub_drafts.restype = lib.stub_live.restype = ctypes.c_long
     lib.stub_message.restype = ctypes.c_char_p
     return lib
 
@@ -143,3 +143,27 @@ def test_q4_outputs(lib, ctx, change, bad):
     n = lib.stub_drafts()
     told(lib, q4(lib, ctx, **change), bad is None, *([bad, "overlap"] if bad else []))
     assert lib.stub_drafts() == n + (bad is None)
+
+
+# (planes of 160 KB; 28 bytes of path, 12 of the others)
+@pytest.mark.parametrize("out", OUTS)
+def test_accept_outputs_and_planes(lib, ctx, out):
+    plane, size = 10 * 16 * 4 * 128 * 2, 28 if out == "d_path" else 12
+    caches = PagedKV.array([kv(96 * MB, 64 * MB), kv(64 * MB + plane, 128 * MB)])
+    for at, ok in ((64 * MB, False), (64 * MB - size, True), (64 * MB - size + 4, False), (64 * MB + 2 * plane - 4, False),
+                   (64 * MB + 2 * plane, True), (96 * MB + plane // 2, False), (128 * MB + plane - 4, False),
+                   (128 * MB + plane, True), (MB + 1024, True)):
+        rc = lib.m1moe_tree_accept(ctx, caches, 2, batch(), *INS.values(), *{**OUTS, out: at}.values())
+        told(lib, rc, ok, *([] if ok else [out, "overlap"]))
+
+
+def test_q4_counters_that_could_not_be_cleared_are_not_used(lib, ctx):
+    """(the stand-in's launch ends the process if a counter is not zero)"""
+    live, n = lib.stub_live(), lib.stub_drafts()
+    lib.stub_fail_memset(1)
+    assert q4(lib, ctx) not in (_lib.M1MOE_OK, _lib.M1MOE_ERR_INVALID)
+    assert lib.stub_live() == live and lib.stub_drafts() == n
+    lib.stub_fail_memset(0)
+    for _ in range(2):
+        told(lib, q4(lib, ctx), True)
+    assert lib.stub_drafts() == n + 2 and lib.stub_live() == live + 2

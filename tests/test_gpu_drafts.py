@@ -615,6 +615,120 @@ def test_q4_what_is_not_finite_stays_in_its_row(dev, tokens, what):
     check_product(y[np.ix_(fine_t, fine_n)], x[fine_t], w[fine_n], s[fine_n], b[fine_n], 64, "f32")
 
 
+@pytest.mark.parametrize("kinds", KINDS)
+@pytest.mark.parametrize("tokens,rows,cols,group", [(500, 9000, 1216, 64), (33, 5000, 1024, 128), (290, 9300, 544, 32),
+                                                    (12, 700, 4736, 64), (32, 260, 8192, 128)])
+def test_q4_shared_columns(dev, tokens, rows, cols, group, kinds):
+    """Tiles behind the last whole round, and tiles too few for the card, whose columns workgroups
+    share: in one order whoever is last."""
+    rng = np.random.default_rng(tokens)
+    w, s, b = q4_weights(rng, rows, cols, group)
+    x = as_dtype(rng.normal(0, 1, (tokens, cols)), kinds[0])
+    say(f"q4 shared {kinds} {tokens} x {rows} x {cols}")
+    y = product(dev, x, w, s, b, group, *kinds)
+    check_product(y, x, w, s, b, group, kinds[1])
+    for _ in range(3):
+        assert np.array_equal(product(dev, x, w, s, b, group, *kinds), y)
+
+
+@pytest.mark.parametrize("tokens", [2, 7, 14, 30, 45])
+def test_q4_sums_past_the_largest_float(dev, tokens):
+    """Groups whose x add up to more than an f32 holds, with results that one does."""
+    rng = np.random.default_rng(tokens)
+    w, s, b = q4_weights(rng, 70, 640, 64, sigma=0.002)
+    x = np.full((tokens, 640), 3e38, np.float32) * (1 - 0.1 * rng.random((tokens, 640))).astype(np.float32)
+    ref = f64(x) @ q4_dense(w, s, b, 64)[0].T
+    assert np.abs(ref).max() < 3.3e38 and f64(x)[:, :64].sum() > 1e40
+    say(f"q4 large sums, {tokens} tokens")
+    check_product(product(dev, x, w, s, b, 64), x, w, s, b, 64, "f32")
+
+
+@pytest.mark.parametrize("rows,cols,group", [(3, 128, 64), (5, 64, 64), (1, 128, 128)])
+def test_q4_of_most_tokens(dev, rows, cols, group):
+    """Less than a unit's groups, and a little more."""
+    rng = np.random.default_rng(rows)
+    w, s, b = q4_weights(rng, rows, cols, group)
+    x = rng.normal(0, 1, (65536, cols)).astype(np.float32)
+    say(f"q4 65536 tokens {rows} x {cols}")
+    check_product(product(dev, x, w, s, b, group), x, w, s, b, group, "f32")
+
+
+class Product:
+    """A call whose operands stay on the device."""
+
+    def __init__(self, dev, tokens, rows, cols, group=64):
+        self.ctx, self.ops = dev
+        rng = np.random.default_rng(tokens)
+        self.w, self.s, self.b = q4_weights(rng, rows, cols, group)
+        self.x = rng.normal(0, 1, (tokens, cols)).astype(np.float32)
+        self.shape, self.group = (tokens, rows), group
+        self.held = [self.ctx.to_device(a) for a in (self.w, self.s, self.b, self.x, np.zeros((tokens, rows), np.float32))]
+        self.weights = Q4Weights.make(*self.held[:3], rows, cols, group)
+
+    def __call__(self):
+        (t, n), k = self.shape, self.x.shape[1]
+        self.ops.matmul_q4(self.weights, self.held[3], "f32", k, t, self.held[4], "f32", n)
+
+    def result(self):
+        """y, and zeros in its place."""
+        self.ctx.sync()
+        y = self.held[4].download(np.float32).reshape(self.shape)
+        self.held[4].upload(np.zeros(self.shape, np.float32))
+        return y
+
+    def free(self):
+        for h in self.held:
+            h.free()
+
+
+def test_q4_graphs_share_a_workspace():
+    """Two graphs and eager calls on one context's workspace, in turns; a call that needs more of it
+    is refused in a capture, and behind it the graphs of the smaller one are."""
+    ctx = m.HIPContext(m.make_shape(64, 1, 1, 64))
+    dev = ctx, DenseOps(ctx)
+    big, small, few, huge, alone = (Product(dev, *a) for a in ((100, 512, 1024), (40, 96, 2048), (10, 48, 4096),
+                                                               (400, 512, 1024), (1, 48, 256)))
+    say("q4 capture without a workspace")
+    ctx.graph_begin()
+    with pytest.raises(M1MoEError) as e:
+        big()
+    assert e.value.code == _lib.M1MOE_ERR_INVALID and "capture" in str(e.value)
+    alone()                             # (needs none)
+    one = ctx.graph_end()
+    one.launch()
+    want = []
+    check_product(alone.result(), alone.x, alone.w, alone.s, alone.b, 64, "f32")
+    for p in (big, small, few):
+        p()
+        want.append(p.result())
+        check_product(want[-1], p.x, p.w, p.s, p.b, p.group, "f32")
+    say("q4 two graphs")
+    ctx.graph_begin()
+    big(), few()
+    one = ctx.graph_end()
+    ctx.graph_begin()
+    few(), small(), few()
+    two = ctx.graph_end()
+    for i in range(3):
+        one.launch(), two.launch()
+        assert np.array_equal(big.result(), want[0]) and np.array_equal(small.result(), want[1]), i
+        assert np.array_equal(few.result(), want[2]), i
+        two.launch(), small(), one.launch()
+        assert np.array_equal(small.result(), want[1]) and np.array_equal(few.result(), want[2]), i
+        assert np.array_equal(big.result(), want[0]), i
+    huge()
+    check_product(huge.result(), huge.x, huge.w, huge.s, huge.b, 64, "f32")
+    with pytest.raises(M1MoEError) as e:
+        one.launch()
+    assert "capture it again" in str(e.value)
+    big()
+    assert np.array_equal(big.result(), want[0])
+    del one, two
+    for p in (big, small, few, huge, alone):
+        p.free()
+    ctx.close()
+
+
 def test_q4_rows_past_32_bits(dev):
     """x and y whose last rows lie past 2^32 bytes."""
     ctx, ops = dev
