@@ -110,12 +110,21 @@ struct Weights {
     // N of the row's scales or biases from group q on, past its last one 0.
     template <int N>
     __device__ __forceinline__ void halves(const uint16_t* from_all, int q, uint32_t (&x)[N / 2]) const {
-        const int left = max(groups - q, 0);
-        const int64_t want = at + q, from = min(want, total - N);
-        const Halves<N> p = *reinterpret_cast<const Halves<N>*>(from_all + from);
+        raw_halves<N>(from_all, q, x);
+        settle<N>(q, x);
+    }
+    // Their load, and what puts them in place where it could not begin at group q: apart, as a test
+    // behind each load would wait for it.
+    template <int N>
+    __device__ __forceinline__ void raw_halves(const uint16_t* from_all, int q, uint32_t (&x)[N / 2]) const {
+        const Halves<N> p = *reinterpret_cast<const Halves<N>*>(from_all + min(at + q, total - N));
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) x[i] = p.x[i];
-        if (left < N) shift<N>(x, (int)(want - from), left);
+    }
+    template <int N>
+    __device__ __forceinline__ void settle(int q, uint32_t (&x)[N / 2]) const {
+        const int left = max(groups - q, 0);
+        if (left < N) shift<N>(x, (int)(at + q - min(at + q, total - N)), left);
     }
     // Any unit.
     template <int G>
@@ -400,21 +409,24 @@ __device__ __forceinline__ bool join_split(const Q4Args& a, int id, int KW, int 
     }
     __syncthreads();
     if (!*s_flag) return false;
-    // (in the order of the columns, whoever is last)
+    // (in the order of the columns, whoever is last; as many loads at once as pay)
+    constexpr int L = N > 1 ? 16 : 8, K = L / N;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        f32x4v sum = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = 0; k0 < KW; k0 += 8) {
-            const float* at[8];
-            f32x4v y[8];
+    for (int i = 0; i < N; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < KW; k0 += K) {
+        const float* at[L];
+        f32x4v y[L];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) at[k] = part + min(k0 + k, KW - 1) * wg + i * 256;
-            load8_coh(at, y);
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k0 + k < KW) sum += y[k];
-        }
-        acc[i] = sum;
+            for (int i = 0; i < N; ++i) at[k * N + i] = part + min(k0 + k, KW - 1) * wg + i * 256;
+        if constexpr (L == 16) load16_coh(at, y);
+        else load8_coh(at, y);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k0 + k < KW)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] += y[k * N + i];
     }
     return true;
 }
@@ -614,47 +626,57 @@ __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
         for (int m = 0; m < MW; ++m)
 #pragma unroll
             for (int i = 0; i < kGroups / N; ++i)
-                w[m].template halves<N>(w[m].s, u * kGroups + N * i, reinterpret_cast<uint32_t(&)[N / 2]>(x[m][i * N / 2]));
+                w[m].template raw_halves<N>(w[m].s, u * kGroups + N * i, reinterpret_cast<uint32_t(&)[N / 2]>(x[m][i * N / 2]));
+    };
+    const auto settle = [&](int u, uint32_t (&x)[MW][kGroups / 2]) {
+#pragma unroll
+        for (int m = 0; m < MW; ++m)
+#pragma unroll
+            for (int i = 0; i < kGroups / N; ++i)
+                w[m].template settle<N>(u * kGroups + N * i, reinterpret_cast<uint32_t(&)[N / 2]>(x[m][i * N / 2]));
     };
     f32x4v acc[MW * NT];
 #pragma unroll
     for (int i = 0; i < MW * NT; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    if (kw == 0) {
-        for (int k = 0; k < sums; ++k) {
-            bf16x8 x[NT][3], b[MW][3];
+    for (int k = (sums * kw + KW - 1) / KW; k < (sums * (kw + 1) + KW - 1) / KW; ++k) {   // (the first shares have fewer units)
+        constexpr int H = G == 128 ? 4 : 8;     // (a row has as many groups at least, or all rows together)
+        bf16x8 y[NT][3], b[MW][3];
+        uint32_t sv[MW][8 / H][H / 2], bv[MW][8 / H][H / 2];
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    x[t][p] = *reinterpret_cast<const bf16x8*>(
-                        a.xsums + (((int64_t)ty * NT + min(t, tiles - 1)) * sums + k) * kSumBytes + 1024 * p + 16 * lane);
+            for (int p = 0; p < 3; ++p)
+                y[t][p] = *reinterpret_cast<const bf16x8*>(
+                    a.xsums + (((int64_t)ty * NT + min(t, tiles - 1)) * sums + k) * kSumBytes + 1024 * p + 16 * lane);
 #pragma unroll
-            for (int m = 0; m < MW; ++m) {
-                constexpr int H = G == 128 ? 4 : 8;     // (a row has as many groups at least, or all rows together)
-                uint32_t sv[4], bv[4];
+        for (int m = 0; m < MW; ++m)
 #pragma unroll
-                for (int i = 0; i < 8 / H; ++i) {
-                    w[m].template halves<H>(w[m].s, 32 * k + 8 * g + H * i, reinterpret_cast<uint32_t(&)[H / 2]>(sv[i * H / 2]));
-                    w[m].template halves<H>(w[m].b, 32 * k + 8 * g + H * i, reinterpret_cast<uint32_t(&)[H / 2]>(bv[i * H / 2]));
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    __bf16 p[3];
-                    bf16_parts(fmaf(8.f, bf16_pair(sv, i), bf16_pair(bv, i)), p);
-                    b[m][0][i] = p[0], b[m][1][i] = p[1], b[m][2][i] = p[2];
-                }
+            for (int i = 0; i < 8 / H; ++i) {
+                w[m].template raw_halves<H>(w[m].s, 32 * k + 8 * g + H * i, sv[m][i]);
+                w[m].template raw_halves<H>(w[m].b, 32 * k + 8 * g + H * i, bv[m][i]);
             }
 #pragma unroll
-            for (int o = 2; o >= 0; --o)      // (small products first)
+        for (int m = 0; m < MW; ++m)
 #pragma unroll
-                for (int p = 0; p <= o; ++p)
+            for (int i = 0; i < 8; ++i) {
+                if (i % H == 0) {
+                    w[m].template settle<H>(32 * k + 8 * g + i, sv[m][i / H]);
+                    w[m].template settle<H>(32 * k + 8 * g + i, bv[m][i / H]);
+                }
+                __bf16 p[3];
+                bf16_parts(fmaf(8.f, bf16_pair(sv[m][i / H], i % H), bf16_pair(bv[m][i / H], i % H)), p);
+                b[m][0][i] = p[0], b[m][1][i] = p[1], b[m][2][i] = p[2];
+            }
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+        for (int o = 2; o >= 0; --o)      // (small products first)
 #pragma unroll
-                        for (int m = 0; m < MW; ++m)
-                            acc[m * NT + t] =
-                                __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[t][p], b[m][o - p], acc[m * NT + t], 0, 0, 0);
-        }
+            for (int p = 0; p <= o; ++p)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int m = 0; m < MW; ++m)
+                        acc[m * NT + t] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[t][p], b[m][o - p], acc[m * NT + t], 0, 0, 0);
     }
     uint4 x[4][MW];
     uint32_t s_now[MW][kGroups / 2], s_next[MW][kGroups / 2];
@@ -662,10 +684,11 @@ __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
 #pragma unroll
         for (int m = 0; m < MW; ++m) y[m] = w[m].words(k);
     };
-    scales(u0, s_now);
     words(4 * u0, x[0]);
+    scales(u0, s_now);
     copy(4 * u0, 0);
     words(4 * u0 + 1, x[1]);
+    settle(u0, s_now);
     const NibK nk = nib_consts();
     for (int u = u0; u < u1; ++u) {
 #pragma unroll
@@ -677,7 +700,7 @@ __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
 #pragma unroll
             for (int m = 0; m < MW; ++m) steps<G>(x[b][m], v[m]);
             // (past the last block: that one again, into a buffer that is not read)
-            if (b == 2) scales(min(u + 1, u1 - 1), s_next);
+            if (b == 2) scales(min(u + 1, u1 - 1), s_next), settle(min(u + 1, u1 - 1), s_next);
             copy(min(k + 1, last), ~b & 1);
             words(min(k + 2, last), x[(b + 2) & 3]);
             const uint8_t* s = s_x + (b & 1) * kStage;
