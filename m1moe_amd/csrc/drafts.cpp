@@ -48,7 +48,7 @@ int32_t ensure_q4_scratch(m1moe_ctx_t ctx, uint64_t floats) {
     if (ctx->q4_cnt && floats <= ctx->q4_part_floats) return M1MOE_OK;
     if (int32_t rc = refuse_growth_in_capture(ctx->stream, "the 4-bit products' scratch")) return rc;
     if (!ctx->q4_cnt) {
-        const uint64_t bytes = 4 * (uint64_t)ctx->cus;   // (shared tiles are fewer: two workgroups at least of two a CU)
+        const uint64_t bytes = 4 * (uint64_t)ctx->cus;   // (tiles that are shared are fewer than the CUs)
         if (int32_t rc = device_alloc_zeroed((void**)&ctx->q4_cnt, bytes, "4-bit products' counters", ctx->stream))
             return rc;
         if (floats <= ctx->q4_part_floats) return M1MOE_OK;

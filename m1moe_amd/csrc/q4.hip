@@ -831,13 +831,17 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
     }
     constexpr int nt = kManyTiles, mw = kManyRows;
     const int tt = (a.tokens + 15) / 16, quads = (a.cols + 511) / 512, sums = (a.cols / a.group + 31) / 32;
-    // Whole tiles as long as they fill the card, two workgroups a CU; the columns of the others are
-    // shared by as many workgroups as make one more round of it (800 x 6144 x 4096, 624 tiles: all
-    // whole 136 us).
+    // Whole tiles as long as there is one for every CU (two workgroups fit one); the columns of the
+    // rest are shared by as many workgroups as there are CUs.  A join costs as much as two units of
+    // columns, a second workgroup on a CU 0.6 of its time: f32, 4096 columns, n tiles, whole
+    // and shared, 16 45.6 and 23.6 us, 64 47.1 and 28.9 (by twice as many 36.9), 112 48.4 and 37.9,
+    // 208 50.3 and 53.7, 312 (256 of them whole) 78.3 and 61.4.  By twice as many where these are three
+    // a tile and have units enough (168, 8 units: 48.4 and 43.4, 4 units: 28.1 and 28.9).
     a.grid_x = (tiles + mw * a.waves - 1) / (mw * a.waves);
-    const int all = a.grid_x * ((tt + nt - 1) / nt), slots = 2 * cus;
-    a.whole = all / slots * slots;
-    a.split = all == a.whole ? 1 : std::max(1, std::min(quads, slots / (all - a.whole)));
+    const int all = a.grid_x * ((tt + nt - 1) / nt);
+    a.whole = all / cus * cus;
+    const int rest = all - a.whole;
+    if (rest) a.split = std::min(quads, cus / rest > 1 ? cus / rest : 2 * cus / rest == 3 && quads >= 8 ? 3 : 1);
     if (a.split == 1) a.whole = all;
     a.grid = a.whole + (all - a.whole) * a.split;
     a.part_split = (quads + 7) / 8;
