@@ -540,9 +540,9 @@ int32_t m1moe_sample(m1moe_ctx_t ctx, const float* d_logits, int32_t rows,
  * the conversation's kv_len - n positions; a row sees those and its own
  * ancestors, and its angle is that of its depth.  Then a token is drawn at every
  * row (m1moe_sample), and the drafts that were drawn are taken over.  All
- * asynchronous on the context stream, without a workspace of their own but
- * m1moe_tree_attention's, which is m1moe_paged_attention's.  A tree has at most
- * 256 rows. */
+ * asynchronous on the context stream.  m1moe_tree_attention uses
+ * m1moe_paged_attention's workspace, m1moe_matmul_q4 one of its own, both the
+ * context's; the other calls need none.  A tree has at most 256 rows. */
 
 /* Who sees whom, and depths, from every row's parent: d_parents[row] is the
  * parent's number in the same tree (0 its first row), -1 for none, and lower than
@@ -585,7 +585,7 @@ int32_t m1moe_tree_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
  * without rows.  One that is out of range or has more than 256 rows is skipped
  * with the same results, a move from or to a page outside the cache is left out
  * and a parent that is not lower than its row counts as none: each sets the
- * device error flag.  Outputs must not overlap inputs or each other. */
+ * device error flag.  Outputs must not overlap inputs, caches or each other. */
 int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs,
                           int32_t num_caches, const m1moe_paged_batch* batch,
                           const int32_t* d_parents, const int32_t* d_drafts,
@@ -608,9 +608,15 @@ typedef struct {
 /* y[t][r] = sum_c x[t][c] W[r][c] (+ residual[t][r]) for 1 to 65536 tokens t.  x
  * [tokens][cols] in x_dtype, y and residual (NULL: none; d_y itself: in place)
  * [tokens][rows] in y_dtype, y_stride elements apart; row strides are multiples of
- * 16 bytes.  f32 rows give an f32 y, bf16 ones either.  Products are exact and
- * summed in f32, a group's first; a row of x that holds an infinity or a NaN, or
- * an f32 above the largest bf16, gives results that are not finite. */
+ * 16 bytes.  f32 rows give an f32 y, bf16 ones either.  An f32 x is taken to 22
+ * bits, and to 2^-39 of its row's largest where that is more; products are exact
+ * and summed in f32, a group's first.  A row of x that holds an infinity or a NaN
+ * gives results that are not finite, the other rows are what they were.  A result
+ * does not depend on what else runs, but its last bits may on the number of tokens.
+ * Calls of more than 32 tokens, or of so few rows of W that their columns are
+ * shared by workgroups, use a workspace of the context's, which the first such
+ * call of a larger size makes: do that before capturing (in a capture it is
+ * refused, and graphs from before it are refused afterwards). */
 int32_t m1moe_matmul_q4(m1moe_ctx_t ctx, const m1moe_q4_weights* weights,
                         const void* d_x, int32_t x_dtype, int64_t x_stride,
                         int32_t tokens, const void* d_residual, void* d_y,

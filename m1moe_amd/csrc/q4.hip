@@ -43,7 +43,11 @@ __host__ __device__ constexpr int few_rows(int r) { return r | 1; }
 // a unit of columns ahead; v_permlane swaps bring the words of one group together.  x is staged
 // in LDS as the other operand, a chunk of columns at a time; its rows are the tokens, or
 // of f32 tokens the two parts of each, which fill the rows of one MFMA for up to 8 tokens.
-// KS waves of a workgroup share a tile's columns.
+// KS waves of a workgroup share a tile's columns, or KW workgroups.
+//
+// Group 64, us (at the rate of a large copy): 2048 x 2048, 1 token 5.2 (0.5), the launch, x, a row's
+// words and the join in turn; 50304 x 2048, 1 token 16.6 (11.4), 16 f32 21.2, 26 bf16 24.7 (12.2), where
+// a tile's nibbles, MFMAs and LDS reads of x follow each other in a wave and 16 waves fill a CU.
 template <int G>
 struct Unit {
     static constexpr int NQ = G == 32 ? 2 : 4;          // 128-column blocks
@@ -321,7 +325,7 @@ struct Few {
         for (int t = 0; t < NT; ++t) unit[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < U::NQ; ++i) {
-            __builtin_amdgcn_sched_barrier(0);   // (a block's operands at a time)
+            __builtin_amdgcn_sched_barrier(0);   // (a block's operands at a time: registers)
             uint32_t v[4];
             steps<G>(x.w[i], v);
 #pragma unroll
@@ -530,7 +534,8 @@ __device__ __forceinline__ void bf16_parts(float x, __bf16 (&p)[3]) {
 }
 
 // Workgroup = (four tokens, a share of the columns, 4096 at most), a wave per token, which holds
-// its share in registers and reads the rest of its row for the largest value only.
+// its share in registers and reads the rest of its row for the largest value only.  (800 x 4096
+// f32: 9.3 us; 64 x 4096 5.7, a row and its largest value in turn.)
 template <int G, bool XB>
 __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
     constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), N = 8;
@@ -586,8 +591,14 @@ __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
 // Workgroup = 16 NT tokens, 16 MW rows of W a wave.  A wave's words come straight from memory,
 // two blocks of 128 columns ahead, its scales four; the records through LDS, copied by the
 // loads themselves, a block ahead.  The biases' part, sum_G b'_G X_G with b' = b + 8 s, is a
-// product of its own before the others, of bf16 parts, six MFMAs for 32 groups (as a
-// multiply-add per value, group and lane, with its sums read from LDS, 800 x 6144 x 4096: 122 us).
+// product of its own before the others, of bf16 parts, six MFMAs for 32 groups: per value and
+// group, with the sums read from LDS, it took as many instructions as the nibbles.
+//
+// Bound by a SIMD's two waves, whose MFMAs (30%), vector work (36%: nibbles, scales) and LDS
+// reads (37%) overlap only in part; setting them one beside the other by hand, operands a
+// group ahead, changed nothing (122 us and 124).  800 x 6144 x 4096 f32, group 64: 105 us, 384 TFLOP/s
+// and, with both parts of x, 768 of the 1174 that a large f16 product reaches; 800 x 50304 x 2048
+// 399 us, of bf16 rows 319.
 template <int G, int NT, int MW, bool XB>
 __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
     constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), kStage = NT * kRecord, kSteps = G / 32, kWaves = 8;

@@ -18,7 +18,8 @@ namespace {
 // until no row has an ancestor left above: as many rounds as the depth has bits.
 //
 // Workgroup = tree, a thread per row.  A few KB are read and written: bound by the launch and
-// the chain start - parents - rounds.
+// the chain start - parents - rounds (one tree of 26 rows and 64 of 1 to 64 alike 4.4 us, as
+// fast as the calls are made).
 template <int W>
 __global__ __launch_bounds__(64 * W) void tree_plan_kernel(TreePlanArgs a) {
     constexpr int N = 64 * W;
@@ -71,6 +72,8 @@ __global__ __launch_bounds__(64 * W) void tree_plan_kernel(TreePlanArgs a) {
 //
 // Workgroup = (tree, 4 KB of a position through all planes, the layers' k and v).  Every one walks
 // for itself: the walk (a thread in LDS, a level at a time) takes less than a launch would.
+// 32 trees of 8 to 64, 32 layers of 8 heads of 128 in bf16: 12.5 us, 2.7 TB/s, half of a large
+// copy's rate; one tree, 16 layers: 7.7 us, the chain lengths - parents - walk - rows.
 __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptArgs a) {
     __shared__ int s_child[kTreeRows], s_drawn[kTreeRows], s_page[kTreeRows], s_path[kTreeRows], s_count;
     const PagedView& p = a.p;
