@@ -823,19 +823,26 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
         // workgroups, each of which stages its share only (2048 x 2048: 1 token 5.4 us so, 7.8 by
         // workgroups, 8 tokens 8.6 and 8.4; 6144 x 4096: 1 token 9.4 and 11.3, 4 bf16 ones 11.5 and
         // 11.7, 4 f32 ones, whose columns do not fit, 13.7 and 11.6, 8 16.5 and 12.1).
+        // Tiles for every wave that the CUs hold: waves of workgroups that share them evenly, one a CU,
+        // where that is a wave of a SIMD less than the 16 that fit (2048 columns, f32: 33000 rows, 9 waves,
+        // 1 token 13.3 us, of 8 waves 16.5, 8 tokens 15.1, of 16 17.3; 50304 rows, 13 waves, 26 tokens 33.2,
+        // of 16 31.5; 100000, twice 13, 1 token 34.8, of 8 32.2).
+        const int rounds = (tiles + 16 * cus - 1) / (16 * cus), even = (tiles + rounds * cus - 1) / (rounds * cus);
+        const bool apart = tiles > 8 * cus && even <= 12;
         if (a.tokens <= 4 && units * bytes <= kFewLds) {
             while (a.wave_split < 8 && 2 * a.wave_split <= units && tiles * a.wave_split * 2 <= 16 * cus) a.wave_split *= 2;
             // (workgroups of 4 while there are few: 2048 x 2048, 1 token 5.5 us, of 8 waves 5.9)
             if (a.wave_split <= 4 && tiles * a.wave_split < 8 * cus) a.waves = 4;
+            if (apart) a.waves = std::max(8, even);
         } else {
             // (x is staged once for 16 waves where these still fill the card: 50304 x 2048, 16 f32 tokens
             // 21.2 us, of 8 waves 24.7; 2048 x 2048 9.2, of 16 waves 11.5)
-            a.waves = tiles >= 8 * cus ? 16 : 8;
+            a.waves = apart ? std::max(8, even) : tiles >= 8 * cus ? 16 : 8;
             a.split = std::max(1, std::min(units, cus / ((tiles + a.waves - 1) / a.waves)));
         }
         const int per = a.waves / a.wave_split;
         // all of a workgroup's columns at once, of 16 waves in the LDS of two workgroups of 8
-        a.chunk = std::max(1, std::min((a.waves == 16 ? 2 : 1) * kFewLds / bytes, (units + a.split - 1) / a.split));
+        a.chunk = std::max(1, std::min((a.waves > 8 ? 2 : 1) * kFewLds / bytes, (units + a.split - 1) / a.split));
         a.grid = (tiles + per - 1) / per * a.split;
         a.lds = std::max(a.chunk * bytes, a.wave_split > 1 ? a.waves * nt * 1024 : 16);
         return a.split > 1 ? (int64_t)a.grid * a.waves * nt * 256 : 0;

@@ -631,6 +631,17 @@ def test_q4_shared_columns(dev, tokens, rows, cols, group, kinds):
         assert np.array_equal(product(dev, x, w, s, b, group, *kinds), y)
 
 
+@pytest.mark.parametrize("tokens,kinds", [(1, KINDS[0]), (4, KINDS[2]), (6, KINDS[0]), (20, KINDS[1]), (32, KINDS[0])])
+@pytest.mark.parametrize("rows", [32790, 49150, 66001])
+def test_q4_rows_for_every_wave(dev, rows, tokens, kinds):
+    """Workgroups of 9 to 16 waves."""
+    rng = np.random.default_rng(rows + tokens)
+    w, s, b = q4_weights(rng, rows, 192, 64)
+    x = as_dtype(rng.normal(0, 1, (tokens, 192)), kinds[0])
+    say(f"q4 {kinds} {rows} rows, {tokens} tokens")
+    check_product(product(dev, x, w, s, b, 64, *kinds), x, w, s, b, 64, kinds[1])
+
+
 @pytest.mark.parametrize("tokens", [2, 7, 14, 30, 45])
 def test_q4_sums_past_the_largest_float(dev, tokens):
     """Groups whose x add up to more than an f32 holds, with results that one does."""
