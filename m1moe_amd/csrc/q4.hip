@@ -608,7 +608,9 @@ __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     // this workgroup's tile: one of the `whole` ones, or a share of one of the others
-    const int id = (int)blockIdx.x, rest = id - a.whole, KW = rest < 0 ? 1 : a.split, kw = rest < 0 ? 0 : rest % KW;
+    const int id = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+    if (id >= a.grid) return;
+    const int rest = id - a.whole, KW = rest < 0 ? 1 : a.split, kw = rest < 0 ? 0 : rest % KW;
     const int tile = rest < 0 ? id : a.whole + rest / KW, ty = tile / a.grid_x, block = tile - ty * a.grid_x;
     const int t0 = ty * 16 * NT, tile0 = (block * kWaves + wave) * MW;
     const int units = (a.cols + 511) / 512, sums = (a.cols / G + 31) / 32;
@@ -788,7 +790,10 @@ template <int G, int NT, int MW, bool XB>
 void launch_many(const Q4Args& a, hipStream_t st) {
     hipLaunchKernelGGL((q4_parts_kernel<G, XB>), dim3((unsigned)a.part_split, (unsigned)((a.tokens + 15) / 16 * 4)), dim3(256),
                        0, st, a);
-    hipLaunchKernelGGL((q4_many_kernel<G, NT, MW, XB>), dim3((unsigned)a.grid), dim3((unsigned)(64 * a.waves)), 0, st, a);
+    // (a dimension of a grid holds less than 2^32 threads)
+    const int x = std::min(a.grid, 1 << 14);
+    hipLaunchKernelGGL((q4_many_kernel<G, NT, MW, XB>), dim3((unsigned)x, (unsigned)((a.grid + x - 1) / x)),
+                       dim3((unsigned)(64 * a.waves)), 0, st, a);
 }
 
 template <int G, bool XB>

@@ -664,6 +664,21 @@ def test_q4_of_most_tokens(dev, rows, cols, group):
     check_product(product(dev, x, w, s, b, group), x, w, s, b, group, "f32")
 
 
+def test_q4_of_many_tiles(dev):
+    """More workgroups than one dimension of a grid takes here (17262), the last of them shared."""
+    rng = np.random.default_rng(9)
+    T, N, K = 2001, 70001, 64
+    w, s, b = q4_weights(rng, N, K, 32)
+    x = as_dtype(rng.normal(0, 1, (T, K)), "bf16")
+    say(f"q4 {T} x {N} x {K}")
+    y = product(dev, x, w, s, b, 32, "bf16", "bf16")
+    t = np.r_[0:40, 1000:1040, 1960:2001]
+    n = np.r_[0:300, 35000:35300, 69700:70001]
+    check_product(y[np.ix_(t, n)], x[t], w[n], s[n], b[n], 32, "bf16")
+    sums = np.abs(y).sum(1), np.abs(y).sum(0)
+    assert sums[0].min() > 0 and sums[1].min() > 0
+
+
 class Product:
     """A call whose operands stay on the device."""
 
