@@ -598,7 +598,7 @@ __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
 // reads (37%) overlap only in part; setting them one beside the other by hand, operands a
 // group ahead, changed nothing (122 us and 124).  800 x 6144 x 4096 f32, group 64: 105 us, 384 TFLOP/s
 // and, with both parts of x, 768 of the 1174 that a large f16 product reaches; 800 x 50304 x 2048
-// 399 us, of bf16 rows 319.
+// 400 us, of bf16 rows 311.
 template <int G, int NT, int MW, bool XB>
 __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
     constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), kStage = NT * kRecord, kSteps = G / 32, kWaves = 8;
@@ -611,7 +611,11 @@ __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
     const int id = (int)(blockIdx.y * gridDim.x + blockIdx.x);
     if (id >= a.grid) return;
     const int rest = id - a.whole, KW = rest < 0 ? 1 : a.split, kw = rest < 0 ? 0 : rest % KW;
-    const int tile = rest < 0 ? id : a.whole + rest / KW, ty = tile / a.grid_x, block = tile - ty * a.grid_x;
+    const int tile = rest < 0 ? id : a.whole + rest / KW;
+    // all tokens of 32 blocks of rows, then of the next: an XCD's L2 keeps four blocks' words (800 x
+    // 50304 x 2048 400 us, row by row of tiles 422; 800 x 50304 x 4096 786 and 851; of 16 blocks 405, 797)
+    const int tall = (a.tokens + 16 * NT - 1) / (16 * NT), group = tile / (32 * tall), in = tile - group * 32 * tall;
+    const int wide = min(32, a.grid_x - 32 * group), ty = in / wide, block = 32 * group + in - ty * wide;
     const int t0 = ty * 16 * NT, tile0 = (block * kWaves + wave) * MW;
     const int units = (a.cols + 511) / 512, sums = (a.cols / G + 31) / 32;
     const int u0 = (int)((int64_t)units * kw / KW), u1 = (int)((int64_t)units * (kw + 1) / KW), last = 4 * u1 - 1;
