@@ -522,7 +522,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
 // (e: of a token's whole row).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr int record_bytes(int p) { return 4096 * p; }
-constexpr int kSumBytes = 3072;
+constexpr int kSumBytes = 3 * 1024;
 
 // x as three bf16 parts.
 __device__ __forceinline__ void bf16_parts(float x, __bf16 (&p)[3]) {
