@@ -535,7 +535,7 @@ __device__ __forceinline__ void bf16_parts(float x, __bf16 (&p)[3]) {
 
 // Workgroup = (four tokens, a share of the columns, 4096 at most), a wave per token, which holds
 // its share in registers and reads the rest of its row for the largest value only.  (800 x 4096
-// f32: 9.3 us; 64 x 4096 5.7, a row and its largest value in turn.)
+// f32: 9.3 us.)
 template <int G, bool XB>
 __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
     constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), N = 8;
@@ -871,7 +871,9 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
     if (rest) a.split = std::min(quads, cus / rest > 1 ? cus / rest : 2 * cus / rest == 3 && quads >= 8 ? 3 : 1);
     if (a.split == 1) a.whole = all;
     a.grid = a.whole + (all - a.whole) * a.split;
-    a.part_split = (quads + 7) / 8;
+    // (as many workgroups as CUs where there are few tokens, though each reads whole rows for their
+    // largest: 64 x 6144 x 4096 bf16 23.2 us, by the fewest 25.7)
+    a.part_split = std::max((quads + 7) / 8, std::min(quads, cus / (4 * tt)));
     a.sums_at = (int64_t)tt * quads * record_bytes(a.x_bf16 ? 1 : 2);
     a.down_at = a.sums_at + (int64_t)tt * sums * kSumBytes / 4;
     a.part_at = a.down_at + 16 * tt;
