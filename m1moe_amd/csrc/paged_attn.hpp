@@ -1764,7 +1764,7 @@ __global__ __launch_bounds__(256) void paged_pieces_kernel(PagedAttnArgs a) {
     }
     __syncthreads();
     if (!s_in || head >= a.heads) return;
-    const float f = 1.0f / l;
+    const float f = over<TREE>(l);
     store4(a, QP == 1, (int64_t)token * a.out_stride + (int64_t)head * HD + d,
            {o[0] * f, o[1] * f, o[2] * f, o[3] * f});
 }
