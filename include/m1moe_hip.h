@@ -615,8 +615,10 @@ typedef struct {
  * does not depend on what else runs, but its last bits may on the number of tokens.
  * Calls of more than 32 tokens, or of so few rows of W that their columns are
  * shared by workgroups, use a workspace of the context's, which the first such
- * call of a larger size makes: do that before capturing (in a capture it is
- * refused, and graphs from before it are refused afterwards). */
+ * call of more tokens or longer rows of x makes (behind one of more than 32 tokens
+ * none of as many tokens and bytes of a row or fewer needs more): do that before
+ * capturing (in a capture it is refused, and graphs from before it are refused
+ * afterwards). */
 int32_t m1moe_matmul_q4(m1moe_ctx_t ctx, const m1moe_q4_weights* weights,
                         const void* d_x, int32_t x_dtype, int64_t x_stride,
                         int32_t tokens, const void* d_residual, void* d_y,

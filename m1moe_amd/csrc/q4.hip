@@ -816,6 +816,12 @@ void launch_group(const Q4Args& a, hipStream_t st) {
 
 }  // namespace
 
+// Floats of the most partials that a call has: workgroups that share columns are at most two a CU, of 8
+// waves with kManyRows by kManyTiles tiles, or one of 16 waves with two.  (This call's own would be
+// fewer, but more than those of some calls of more tokens: a program that has run its largest step
+// captures any other.)
+static int64_t most_partials(int cus) { return (int64_t)2 * cus * 8 * kManyRows * kManyTiles * 256; }
+
 int64_t matmul_q4_plan(Q4Args& a, int cus) {
     const int unit = a.group == 32 ? 256 : 512, units = (a.cols + unit - 1) / unit, groups = unit / a.group;
     const int tiles = (a.rows + 15) / 16;
@@ -854,7 +860,7 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
         a.chunk = std::max(1, std::min((a.waves > 8 ? 2 : 1) * kFewLds / bytes, (units + a.split - 1) / a.split));
         a.grid = (tiles + per - 1) / per * a.split;
         a.lds = std::max(a.chunk * bytes, a.wave_split > 1 ? a.waves * nt * 1024 : 16);
-        return a.split > 1 ? (int64_t)a.grid * a.waves * nt * 256 : 0;
+        return a.split > 1 ? most_partials(cus) : 0;
     }
     constexpr int nt = kManyTiles, mw = kManyRows;
     const int tt = (a.tokens + 15) / 16, quads = (a.cols + 511) / 512, sums = (a.cols / a.group + 31) / 32;
@@ -877,7 +883,7 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
     a.sums_at = (int64_t)tt * quads * record_bytes(a.x_bf16 ? 1 : 2);
     a.down_at = a.sums_at + (int64_t)tt * sums * kSumBytes / 4;
     a.part_at = a.down_at + 16 * tt;
-    return a.part_at + (int64_t)(a.grid - a.whole) * a.waves * mw * nt * 256;
+    return a.part_at + most_partials(cus);
 }
 
 int launch_matmul_q4(const Q4Args& a, void* stream) {

@@ -1,0 +1,44 @@
+"""What calls need of a context's workspaces, and the pieces of a shared prefix: the library's own
+plans, which run on the host (plans_probe.cpp, linked against the built library)."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from m1moe_amd import _lib
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+CSRC = os.path.join(os.path.dirname(HERE), "m1moe_amd", "csrc")
+CUS = 256
+
+
+@pytest.fixture(scope="module")
+def probe(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("plans") / "libplans.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I" + CSRC, os.path.join(HERE, "plans_probe.cpp"),
+                    _lib.LIB_PATH, "-Wl,-rpath," + os.path.dirname(_lib.LIB_PATH), "-o", out], check=True)
+    lib = ctypes.CDLL(out)
+    lib.probe_q4.restype = lib.probe_paged.restype = ctypes.c_int64
+    return lib
+
+
+def q4(probe, rows, cols, group, tokens, bf16):
+    """Floats a call makes sure of, no fewer than it uses."""
+    used, shared = ctypes.c_int64(), ctypes.c_int()
+    n = probe.probe_q4(rows, cols, group, tokens, bf16, CUS, ctypes.byref(used), ctypes.byref(shared))
+    assert used.value <= n and shared.value <= CUS
+    return n
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("rows,cols,group", [(6144, 4096, 64), (50304, 2048, 64), (2048, 2048, 64), (2048, 1024, 32),
+                                             (48, 4096, 128), (129, 352, 32), (70, 65536, 64)])
+def test_products_of_fewer_tokens_need_no_more(probe, rows, cols, group, bf16):
+    need = [q4(probe, rows, cols, group, t, bf16) for t in range(1, 2101)]
+    assert all(a <= b for a, b in zip(need, need[1:]))
+    assert need[-1] > 0
+    # (nor do those of smaller weights, behind a call of more than 32 tokens)
+    for n, k in ((rows // 2 + 1, cols), (rows, cols - cols // 2 // group * group), (40, group)):
+        assert all(q4(probe, n, k, group, t, bf16) <= need[t - 1] for t in range(33, 700))
+        assert max(q4(probe, n, k, group, t, bf16) for t in range(1, 33)) <= need[32]
