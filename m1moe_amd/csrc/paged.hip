@@ -175,17 +175,24 @@ int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats) {
     a.splits = a.prefix_wgs = 0;
     *own_floats = (int64_t)a.grid * 2 * R * (a.head_dim + 2);
     if (a.p.prefix_len == 0) return *own_floats;
-    // at least one workgroup per CU takes the prefix, pieces of at least 64 keys; up to three times as
-    // many pieces where that many leave CUs without one at the end (144 tiles on 256 CUs, 24 trees
-    // behind 4096 positions: 98 us with 2 pieces, 84 with 3)
+    // Pieces of at least 64 keys, so many that one workgroup per CU takes the prefix, and up to three
+    // times as many where a last round would leave CUs without one (144 tiles on 256 CUs, 24 trees behind
+    // 4096 positions: 98 us with 2 pieces, 84 with 3; 2100 rows, 32 heads over 8, bf16, 304 and 262).
+    // That is weighed against a piece's rows, which are written and read once more: about 256 keys'
+    // time a round (behind 500 positions 5 pieces of 800 such rows in place of 2: 54.8 us and 44.9).  By that
+    // count more pieces have to save a twentieth, and past four rounds they do not (of 78 batches of 64 to
+    // 2100 rows behind 500 and 4096 positions none is slower than with the fewest; 16 heads, f32 cache,
+    // 24 turns behind 500, 65.8 us, would be 67.5).
     const int TT = R / a.share, tiles = (a.p.num_rows + TT - 1) / TT;
-    const int64_t wgs = (int64_t)tiles * a.p.kv_heads, most = std::min(a.p.prefix_len / 64, 32);
-    const int64_t least = (cus + wgs - 1) / wgs;
-    const auto idle = [&](int64_t s) { return (double)((wgs * s + cus - 1) / cus * cus) / (double)(wgs * s); };
+    const int64_t wgs = (int64_t)tiles * a.p.kv_heads, most = std::max(1, std::min(a.p.prefix_len / 64, 32));
+    const int64_t least = std::min((cus + wgs - 1) / wgs, most);
+    const auto keys = [&](int64_t s) {
+        return (double)((wgs * s + cus - 1) / cus) * a.p.prefix_len / s + 256.0 * wgs * s / cus;
+    };
     int64_t splits = least;
-    for (int64_t s = least; s <= 3 * least && idle(splits) > 1.25; ++s)
-        if (idle(s) < idle(splits)) splits = s;
-    a.splits = (int)std::max<int64_t>(1, std::min(most, splits));
+    for (int64_t s = least + 1; wgs <= 4 * (int64_t)cus && s <= std::min(3 * least, most); ++s)
+        if (keys(s) < keys(splits) * (splits == least ? 0.95 : 1.0)) splits = s;
+    a.splits = (int)splits;
     a.prefix_wgs = (int)(wgs * a.splits);
     return *own_floats + (int64_t)(a.splits + 1) * a.p.num_rows * a.heads * (a.head_dim + 2);
 }

@@ -23,6 +23,13 @@ def probe(tmp_path_factory):
     return lib
 
 
+def paged(probe, rows, heads, kv_heads, hd, bf16, prefix):
+    """(floats a call makes sure of, those it uses, pieces of the prefix)"""
+    splits, used = ctypes.c_int(), ctypes.c_int64()
+    n = probe.probe_paged(rows, heads, kv_heads, hd, bf16, prefix, CUS, ctypes.byref(splits), ctypes.byref(used))
+    return n, used.value, splits.value
+
+
 def q4(probe, rows, cols, group, tokens, bf16):
     """Floats a call makes sure of, no fewer than it uses."""
     used, shared = ctypes.c_int64(), ctypes.c_int()
@@ -42,3 +49,16 @@ def test_products_of_fewer_tokens_need_no_more(probe, rows, cols, group, bf16):
     for n, k in ((rows // 2 + 1, cols), (rows, cols - cols // 2 // group * group), (40, group)):
         assert all(q4(probe, n, k, group, t, bf16) <= need[t - 1] for t in range(33, 700))
         assert max(q4(probe, n, k, group, t, bf16) for t in range(1, 33)) <= need[32]
+
+
+# (measured: 32/8 heads, bf16, 800 rows behind 500, 2 pieces 44.9 us, 5 54.8; behind 4096, 513 rows
+# 2 pieces 106, 3 and 5 87)
+@pytest.mark.parametrize("rows,heads,kv_heads,bf16,prefix,splits", [
+    (800, 32, 8, 1, 500, (2, 2)), (513, 32, 8, 1, 500, (2, 2)), (2100, 16, 16, 1, 500, (1, 1)),
+    (513, 32, 8, 0, 500, (1, 1)), (513, 32, 8, 1, 4096, (3, 5)), (513, 32, 8, 0, 4096, (3, 5)),
+    (800, 16, 16, 1, 4096, (4, 4)), (2100, 32, 8, 1, 4096, (2, 4)), (64, 32, 8, 0, 4096, (8, 8)),
+    (115, 16, 16, 1, 500, (7, 7)), (1, 8, 8, 1, 63, (1, 1)), (1, 8, 8, 1, 1, (1, 1)), (1, 1, 1, 1, 1 << 20, (32, 32)),
+    (1 << 20, 1, 1, 1, 4096, (1, 1))])
+def test_pieces_of_a_prefix(probe, rows, heads, kv_heads, bf16, prefix, splits):
+    """More pieces where that fills the card's CUs, and none that cost more than they give."""
+    assert splits[0] <= paged(probe, rows, heads, kv_heads, 128, bf16, prefix)[2] <= splits[1]
