@@ -1,7 +1,11 @@
 """GPU: attention of trees of drafted tokens at its edges: rows without a finite score behind a shared
-prefix, other head counts and sizes behind one.  References and bounds as in test_gpu_drafts.py."""
+prefix, other head counts and sizes behind one, repeated calls.  References and bounds as in
+test_gpu_drafts.py."""
 import numpy as np
 import pytest
+
+import m1moe_amd as m
+from m1moe_amd.decoder import DenseOps
 
 from cases import say
 from draft_cases import tree_attention_ref
@@ -56,3 +60,63 @@ def test_attention_prefix_of_other_heads(dev, types, heads, kv_heads, hd, page):
     got, rest, ref, bound = attend(dev, b, mask, heads, kv_heads, hd, types, heads + 1)
     check_close(got, ref, bound, types[0])
     assert np.all(rest == 7.0)
+
+
+class Attention:
+    """A call, tree or plain, whose operands stay on the device."""
+
+    def __init__(self, dev, b, types, heads, kv_heads, hd, seed, tree=True):  # noqa: F811
+        self.ctx, self.ops = dev
+        rng = np.random.default_rng(seed)
+        self.x, cache = types
+        self.b, self.heads, self.n, self.tree = b, heads, heads * hd, tree
+        _, mask, _ = trees(rng, b, 0.6) if tree else (0, np.zeros((b.num_rows, 1), np.uint64), 0)
+        kc, vc = cache_of(rng, b, kv_heads, hd, cache)
+        self.d = d = Held(self.ctx, b, kc, vc, cache, kv_heads, hd)
+        self.words, self.mask = mask.shape[1], d.up(mask)
+        self.q = d.up(as_dtype(rng.normal(0, 1, (b.num_rows, self.n)), self.x))
+        self.zero = as_dtype(np.zeros((b.num_rows, self.n)), self.x)
+        self.out = d.up(self.zero)
+
+    def __call__(self):
+        d, o = self.d, self.ops
+        if self.tree:
+            o.tree_attention(d.kv, d.batch, self.mask, self.words, self.q, self.n, self.out, self.n, self.x, self.heads)
+        else:
+            o.paged_attention(d.kv, d.batch, self.q, self.n, self.out, self.n, self.x, self.heads)
+
+    def result(self):
+        """The bits of out, and zeros in its place."""
+        self.ctx.sync()
+        y = self.out.download(self.zero.dtype)
+        self.out.upload(self.zero)
+        return y
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd", [(16, 16, 128), (32, 8, 128), (8, 2, 64), (4, 2, 256)])
+def test_calls_repeat_bit_for_bit(dev, types, heads, kv_heads, hd):  # noqa: F811
+    """Cut tiles, shared prefixes, other batches in between and the first call of a context: one
+    order of every sum, whoever ends last."""
+    rng = np.random.default_rng(hd + heads)
+    rows = [1, 100, 64, 17, 3, 40, 90, 16, 33]
+    kinds = [Batch(rng, rows, [p + 900 for p in (20, 600, 300, 900, 5, 60, 420, 2000, 0)], 64, prefix=900, pad=3),
+             Batch(rng, rows, [20, 600, 300, 2900, 5, 60, 420, 2000, 0], 64, pad=3)]
+    ctx = m.HIPContext(m.make_shape(64, 1, 1, 64))
+    fresh = ctx, DenseOps(ctx)
+    firsts = []
+    for where in (fresh, dev):
+        a, c = (Attention(where, b, types, heads, kv_heads, hd, i) for i, b in enumerate(kinds))
+        say(f"repeated calls {types} {heads}/{kv_heads}x{hd}")
+        a()
+        want = [a.result()]
+        c()
+        want.append(c.result())
+        for i in range(5):
+            a(), c(), a()
+            assert np.array_equal(a.result(), want[0]) and np.array_equal(c.result(), want[1]), i
+        firsts.append(want)
+        a.d.free()
+        c.d.free()
+    ctx.close()
+    assert all(np.array_equal(x, y) for x, y in zip(*firsts))
