@@ -509,7 +509,9 @@ int32_t m1moe_kv_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
  * multiple of num_kv_heads, at most 64 times it, and num_heads * head_dim <=
  * 65536.
  * Later positions take no part, whatever they hold.  The first call of a
- * larger batch may grow the context's workspace (make it before capturing). */
+ * larger batch may grow the context's workspace (make it before capturing: of
+ * the same heads and types, one of as many rows and as long a prefix or less
+ * needs no more). */
 int32_t m1moe_paged_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
                               const m1moe_paged_batch* batch, const void* d_q,
                               int64_t q_stride, void* d_out, int64_t out_stride,

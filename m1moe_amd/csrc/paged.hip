@@ -171,9 +171,11 @@ int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats) {
     // takes the prefix' at the same time, which computes while that one loads (two for
     // the own positions after the prefix': 64 steps of 20 to 600 positions behind 4096,
     // 45.6 us against 39.5; 8 turns behind 500, 41.3 against 40.2)
-    a.grid = ((a.p.prefix_len ? 1 : per) * cus + 7) / 8 * 8;
+    const auto grid = [&](int wgs) { return (wgs * cus + 7) / 8 * 8; };
+    const auto slots = [&](int wgs) { return (int64_t)wgs * 2 * R * (a.head_dim + 2); };
+    a.grid = grid(a.p.prefix_len ? 1 : per);
     a.splits = a.prefix_wgs = 0;
-    *own_floats = (int64_t)a.grid * 2 * R * (a.head_dim + 2);
+    *own_floats = slots(a.grid);
     if (a.p.prefix_len == 0) return *own_floats;
     // Pieces of at least 64 keys, so many that one workgroup per CU takes the prefix, and up to three
     // times as many where a last round would leave CUs without one (144 tiles on 256 CUs, 24 trees behind
@@ -194,7 +196,14 @@ int64_t paged_attention_plan(PagedAttnArgs& a, int cus, int64_t* own_floats) {
         if (keys(s) < keys(splits) * (splits == least ? 0.95 : 1.0)) splits = s;
     a.splits = (int)splits;
     a.prefix_wgs = (int)(wgs * a.splits);
-    return *own_floats + (int64_t)(a.splits + 1) * a.p.num_rows * a.heads * (a.head_dim + 2);
+    // What is asked for never falls with the rows or the prefix, so that a program that has run its largest
+    // batch captures any other of its model: the slots of a call without a prefix, and the most rows of
+    // pieces that some batch of as many rows or fewer has: pieces x rows is at most most x rows, and
+    // with wgs >= rows kv_heads / TT at most cus TT / kv_heads + rows for the fewest pieces, three times
+    // that for as many more, which up to 4 cus workgroups have.
+    const int64_t rows = a.p.num_rows, one = ((int64_t)cus * TT + a.p.kv_heads - 1) / a.p.kv_heads;
+    const int64_t pieces = std::min(most * rows, std::max(one + rows, 3 * (one + std::min(rows, 4 * one))));
+    return slots(grid(per)) + (pieces + rows) * a.heads * (a.head_dim + 2);
 }
 
 int launch_paged_attention(const PagedAttnArgs& a, void* stream) {

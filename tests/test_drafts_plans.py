@@ -51,6 +51,18 @@ def test_products_of_fewer_tokens_need_no_more(probe, rows, cols, group, bf16):
         assert max(q4(probe, n, k, group, t, bf16) for t in range(1, 33)) <= need[32]
 
 
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(32, 8, 128), (16, 16, 128), (32, 4, 128), (8, 8, 64), (40, 1, 128), (4, 2, 256)])
+def test_attention_of_fewer_rows_needs_no_more(probe, heads, kv_heads, hd, bf16):
+    before = None
+    for prefix in (0, 1, 64, 500, 777, 1024, 4096):
+        need, used, _ = zip(*(paged(probe, r, heads, kv_heads, hd, bf16, prefix) for r in range(1, 2200)))
+        assert all(u <= n for u, n in zip(used, need))
+        assert all(a <= b for a, b in zip(need, need[1:])), prefix
+        assert before is None or all(a <= b for a, b in zip(before, need)), prefix
+        before = need
+
+
 # (measured: 32/8 heads, bf16, 800 rows behind 500, 2 pieces 44.9 us, 5 54.8; behind 4096, 513 rows
 # 2 pieces 106, 3 and 5 87)
 @pytest.mark.parametrize("rows,heads,kv_heads,bf16,prefix,splits", [
