@@ -560,7 +560,8 @@ int32_t m1moe_tree_plan(m1moe_ctx_t ctx, int32_t num_seqs, int32_t num_rows,
                         int32_t mask_words, uint64_t* d_mask, int32_t* d_depth);
 
 /* m1moe_kv_append for the rows of trees: a row is stored at its own slot, d_kv_len
- * - n + i for row i, and rotated by the position d_kv_len - n + d_depth[row]. */
+ * - n + i for row i, and rotated by the position d_kv_len - n + d_depth[row].  The
+ * cache and d_q_out share no memory with d_depth and the batch's arrays. */
 int32_t m1moe_tree_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
                           const m1moe_paged_batch* batch,
                           const m1moe_kv_append_args* args, const int32_t* d_depth);
@@ -569,7 +570,8 @@ int32_t m1moe_tree_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
  * positions before its tree and, of its tree, the rows j <= i whose bit is set in
  * d_mask[row][mask_words] (its own among them only if set).  A row that sees
  * nothing gives zeros, as one whose scores are all -inf does.  A sequence of more
- * than 64 * mask_words rows is skipped and sets the device error flag. */
+ * than 64 * mask_words rows is skipped and sets the device error flag.  d_out shares
+ * no memory with d_mask, the batch's arrays and the cache. */
 int32_t m1moe_tree_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
                              const m1moe_paged_batch* batch, const uint64_t* d_mask,
                              int32_t mask_words, const void* d_q, int64_t q_stride,
@@ -587,7 +589,8 @@ int32_t m1moe_tree_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv,
  * without rows.  One that is out of range or has more than 256 rows is skipped
  * with the same results, a move from or to a page outside the cache is left out
  * and a parent that is not lower than its row counts as none: each sets the
- * device error flag.  Outputs must not overlap inputs, caches or each other. */
+ * device error flag.  Outputs must not overlap inputs, caches or each other, inputs
+ * not the caches. */
 int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs,
                           int32_t num_caches, const m1moe_paged_batch* batch,
                           const int32_t* d_parents, const int32_t* d_drafts,

@@ -24,14 +24,17 @@ bool overlap(const Range& a, const Range& b) {
 }
 
 // Every output apart from every input and from the other outputs.
-int32_t check_apart(std::initializer_list<Range> outs, std::initializer_list<Range> ins) {
-    for (auto o = outs.begin(); o != outs.end(); ++o) {
-        for (const Range& i : ins)
-            if (overlap(*o, i)) return fail(M1MOE_ERR_INVALID, "%s must not overlap %s", o->what, i.what);
-        for (auto x = outs.begin(); x != o; ++x)
+int32_t check_apart(const Range* outs, const Range* outs_end, const Range* ins, const Range* ins_end) {
+    for (const Range* o = outs; o != outs_end; ++o) {
+        for (const Range* i = ins; i != ins_end; ++i)
+            if (overlap(*o, *i)) return fail(M1MOE_ERR_INVALID, "%s must not overlap %s", o->what, i->what);
+        for (const Range* x = outs; x != o; ++x)
             if (overlap(*o, *x)) return fail(M1MOE_ERR_INVALID, "%s must not overlap %s", o->what, x->what);
     }
     return M1MOE_OK;
+}
+int32_t check_apart(std::initializer_list<Range> outs, std::initializer_list<Range> ins) {
+    return check_apart(outs.begin(), outs.end(), ins.begin(), ins.end());
 }
 
 int32_t check_mask(const uint64_t* mask, int32_t words) {
@@ -64,6 +67,18 @@ int32_t ensure_q4_scratch(m1moe_ctx_t ctx, uint64_t floats) {
 }
 
 int64_t row_bytes(int64_t stride, int64_t n, int64_t rows, int64_t es) { return ((rows - 1) * stride + n) * es; }
+
+// Of a cache: bytes of a position, and of all of k (or v).
+int64_t position_bytes(const m1moe_paged_kv* kv) {
+    return (int64_t)kv->num_kv_heads * kv->head_dim * (kv->dtype == M1MOE_BF16 ? 2 : 4);
+}
+int64_t plane_bytes(const m1moe_paged_kv* kv) { return position_bytes(kv) * kv->page_size * kv->num_pages; }
+
+Range starts_of(const m1moe_paged_batch* b) { return {b->d_row_start, 4 * ((int64_t)b->num_seqs + 1), "d_row_start"}; }
+Range lengths_of(const m1moe_paged_batch* b) { return {b->d_kv_len, 4 * (int64_t)b->num_seqs, "d_kv_len"}; }
+Range pages_of(const m1moe_paged_batch* b) {
+    return {b->d_pages, 4 * (int64_t)b->num_seqs * b->table_stride, "d_pages"};
+}
 
 }  // namespace
 
@@ -104,9 +119,10 @@ int32_t m1moe_tree_append(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m1moe
     AppendArgs a{};
     if ((rc = append_args(ctx, kv, batch, args, a))) return rc;
     const int64_t qd = (int64_t)args->num_heads * kv->head_dim, es = args->dtype == M1MOE_BF16 ? 2 : 4;
-    if (args->d_q &&
-        (rc = check_apart({{args->d_q_out, row_bytes(args->q_out_stride, qd, batch->num_rows, es), "d_q_out"}},
-                          {{d_depth, 4 * (int64_t)batch->num_rows, "d_depth"}})))
+    const Range q{args->d_q ? args->d_q_out : nullptr, row_bytes(args->q_out_stride, qd, batch->num_rows, es), "d_q_out"};
+    if ((rc = check_apart({q, {kv->d_k, plane_bytes(kv), "the cache's d_k"}, {kv->d_v, plane_bytes(kv), "the cache's d_v"}},
+                          {{d_depth, 4 * (int64_t)batch->num_rows, "d_depth"}, starts_of(batch), lengths_of(batch),
+                           pages_of(batch)})))
         return rc;
     a.depth = d_depth;
     return launched(launch_kv_append(a, ctx->cus, ctx->stream), "tree_append");
@@ -121,7 +137,14 @@ int32_t m1moe_tree_attention(m1moe_ctx_t ctx, const m1moe_paged_kv* kv, const m1
     if ((rc = attention_args(ctx, kv, batch, d_q, q_stride, d_out, out_stride, dtype, num_heads, a))) return rc;
     const int64_t qd = (int64_t)num_heads * kv->head_dim, es = dtype == M1MOE_BF16 ? 2 : 4;
     if ((rc = check_apart({{d_out, row_bytes(out_stride, qd, batch->num_rows, es), "d_out"}},
-                          {{d_mask, 8 * (int64_t)batch->num_rows * mask_words, "d_mask"}})))
+                          {{d_mask, 8 * (int64_t)batch->num_rows * mask_words, "d_mask"},
+                           starts_of(batch),
+                           lengths_of(batch),
+                           pages_of(batch),
+                           {batch->prefix_len ? batch->d_prefix_pages : nullptr,
+                            4 * (((int64_t)batch->prefix_len + kv->page_size - 1) / kv->page_size), "d_prefix_pages"},
+                           {kv->d_k, plane_bytes(kv), "the cache's d_k"},
+                           {kv->d_v, plane_bytes(kv), "the cache's d_v"}})))
         return rc;
     a.mask = d_mask;
     a.mask_words = mask_words;
@@ -150,18 +173,12 @@ int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs, int32_t nu
         return rc;
     if ((rc = check_ctx(ctx))) return rc;
     const int64_t rows = 4 * (int64_t)batch->num_rows, seqs = 4 * (int64_t)batch->num_seqs;
-    if ((rc = check_apart({{d_path, rows, "d_path"}, {d_accepted, seqs, "d_accepted"}, {d_next, seqs, "d_next"},
-                           {d_past, seqs, "d_past"}},
-                          {{d_parents, rows, "d_parents"},
-                           {d_drafts, rows, "d_drafts"},
-                           {d_drawn, rows, "d_drawn"},
-                           {batch->d_row_start, seqs + 4, "d_row_start"},
-                           {batch->d_kv_len, seqs, "d_kv_len"},
-                           {batch->d_pages, seqs * batch->table_stride, "d_pages"}})))
-        return rc;
+    const Range outs[4] = {{d_path, rows, "d_path"}, {d_accepted, seqs, "d_accepted"}, {d_next, seqs, "d_next"}, {d_past, seqs, "d_past"}};
+    const Range ins[6] = {{d_parents, rows, "d_parents"}, {d_drafts, rows, "d_drafts"}, {d_drawn, rows, "d_drawn"},
+                          starts_of(batch), lengths_of(batch), pages_of(batch)};
+    if ((rc = check_apart(outs, outs + 4, ins, ins + 6))) return rc;
     TreeAcceptArgs a{};
-    const int64_t position = (int64_t)kvs->num_kv_heads * kvs->head_dim * (kvs->dtype == M1MOE_BF16 ? 2 : 4);
-    const int64_t plane = position * kvs->page_size * kvs->num_pages;
+    const int64_t position = position_bytes(kvs), plane = plane_bytes(kvs);
     for (int i = 0; i < num_caches; ++i) {
         a.planes[2 * i] = kvs[i].d_k;
         a.planes[2 * i + 1] = kvs[i].d_v;
@@ -174,13 +191,16 @@ int32_t m1moe_tree_accept(m1moe_ctx_t ctx, const m1moe_paged_kv* kvs, int32_t nu
     for (int i = 1; i < a.num_planes; ++i)
         if (static_cast<char*>(sorted[i]) - static_cast<char*>(sorted[i - 1]) < plane)
             return fail(M1MOE_ERR_INVALID, "two of the caches' d_k and d_v overlap");
-    // (apart and in order: of those that begin before an output's end, the last one ends last)
-    for (const Range& o : {Range{d_path, rows, "d_path"}, Range{d_accepted, seqs, "d_accepted"},
-                           Range{d_next, seqs, "d_next"}, Range{d_past, seqs, "d_past"}}) {
+    // (apart and in order: of those that begin before a range's end, the last one ends last.  The inputs
+    // too: every workgroup walks for itself, while others move rows already)
+    const auto in_plane = [&](const Range& o) {
         void** after = std::lower_bound(sorted, sorted + a.num_planes, const_cast<char*>(static_cast<const char*>(o.p)) + o.bytes);
-        if (after != sorted && overlap(o, {after[-1], plane, ""}))
-            return fail(M1MOE_ERR_INVALID, "%s must not overlap a cache's d_k or d_v", o.what);
-    }
+        return after != sorted && overlap(o, {after[-1], plane, ""});
+    };
+    for (const Range& o : outs)
+        if (in_plane(o)) return fail(M1MOE_ERR_INVALID, "%s must not overlap a cache's d_k or d_v", o.what);
+    for (const Range& i : ins)
+        if (in_plane(i)) return fail(M1MOE_ERR_INVALID, "%s must not overlap a cache's d_k or d_v", i.what);
     if ((rc = set_device(ctx))) return rc;
     a.p = view(ctx, kvs, batch);
     a.row_units = (int32_t)(position / 16);
