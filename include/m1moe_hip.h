@@ -613,11 +613,14 @@ typedef struct {
 /* y[t][r] = sum_c x[t][c] W[r][c] (+ residual[t][r]) for 1 to 65536 tokens t.  x
  * [tokens][cols] in x_dtype, y and residual (NULL: none; d_y itself: in place)
  * [tokens][rows] in y_dtype, y_stride elements apart; row strides are multiples of
- * 16 bytes.  f32 rows give an f32 y, bf16 ones either.  An f32 x is taken to 22
- * bits, and to 2^-39 of its row's largest where that is more; products are exact
- * and summed in f32, a group's first.  A row of x that holds an infinity or a NaN
- * gives results that are not finite, the other rows are what they were.  A result
- * does not depend on what else runs, but its last bits may on the number of tokens.
+ * 16 bytes.  f32 rows give an f32 y, bf16 ones either.  Where it meets the nibbles an
+ * f32 x is taken to 22 bits, and x of either type to 2^-39 of the largest value of
+ * its row (of at most 32 tokens: of 256 columns for groups of 32, else 512) where that
+ * is more: in an f32 row that is what is below 2^-16 of its largest, in a bf16 row
+ * below 2^-31.  Products are exact and summed in f32, a group's first.  A row of x that
+ * holds an infinity or a NaN gives results that are not finite, the other rows are what
+ * they were.  A result does not depend on what else runs, but with the number of tokens
+ * its last bits may change, and within those 2^-39 how small values are kept.
  * Calls of more than 32 tokens, or of so few rows of W that their columns are
  * shared by workgroups, use a workspace of the context's, which the first such
  * call of more tokens or longer rows of x makes (behind one of more than 32 tokens
