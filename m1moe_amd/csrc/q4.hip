@@ -132,12 +132,11 @@ struct Weights {
         const int left = max(groups - q, 0);
         if (left < N) shift<N>(x, (int)(at + q - min(at + q, total - N)), left);
     }
-    // Any unit.
+    // A last unit that the row has only some groups of.
     template <int G>
-    __device__ __forceinline__ void load(int u, Unit<G>& x) const {
+    __device__ __forceinline__ void load_part(int u, Unit<G>& x) const {
         typedef Unit<G> U;
         constexpr int N = U::kGroups;
-        if (groups - u * N >= N) return load_whole<G>(u, x);
 #pragma unroll
         for (int i = 0; i < U::NQ; ++i) x.w[i] = words(u * U::NQ + i);
         halves<N>(s, u * N, x.s);
@@ -481,7 +480,7 @@ __global__ __launch_bounds__(1024) void q4_few_kernel(Q4Args a) {
             f.add(x[0], u, c, g, acc);
         }
         if (max(lo, hi) < end) {
-            w.load<G>(k + end - 1, x[0]);
+            w.load_part<G>(k + end - 1, x[0]);
             f.add(x[0], end - 1, c, g, acc);
         }
     }
