@@ -17,9 +17,9 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 // Of a workgroup of many tokens: tiles of 16 of them, tiles of 16 rows of a wave.
 constexpr int kManyTiles = 2, kManyRows = 2;
 // Most tokens that every workgroup stages for itself (with 16, 17 to 32 tokens as many: 6144 x 4096
-// f32, 17 tokens 16.6 us as few, 25.5 as many, 32 tokens 20.6 and 27.0; 50304 x 2048 26.2 and
-// 33.4, 33.0 and 35.4), the LDS that it does so in, so that two fit a CU, and the rows of LDS
-// that it takes for r.
+// f32, 17 tokens 16.1 us as few, 21.9 as many, 32 tokens 19.3 and 23.5; 50304 x 2048, whose rows fill the
+// card either way, 25.6 and 25.6, 32.0 and 27.2), the LDS that it does so in, so that two fit a CU,
+// and the rows of LDS that it takes for r.
 constexpr int kFewTokens = 32, kFewLds = 76 * 1024;
 __host__ __device__ constexpr int few_rows(int r) { return r | 1; }
 
@@ -47,9 +47,10 @@ __host__ __device__ constexpr int few_rows(int r) { return r | 1; }
 // of f32 tokens the two parts of each, which fill the rows of one MFMA for up to 8 tokens.
 // KS waves of a workgroup share a tile's columns, or KW workgroups.
 //
-// Group 64, us (at the rate of a large copy): 2048 x 2048, 1 token 5.2 (0.5), the launch, x, a row's
-// words and the join in turn; 50304 x 2048, 1 token 16.6 (11.4), 16 f32 21.2, 26 bf16 24.7 (12.2), where
-// a tile's nibbles, MFMAs and LDS reads of x follow each other in a wave and 16 waves fill a CU.
+// Group 64, us (at the rate of a large copy): 2048 x 2048, 1 token 5.1 (0.5), the launch, x, a row's
+// words and the join in turn; 6144 x 4096 8.0 (2.7); 50304 x 2048, 1 token 15.4 (11.4), 16 f32 20.6, 26
+// bf16 24.4 (12.2), where a tile's nibbles, MFMAs and LDS reads of x follow each other in a wave,
+// 16 waves fill a CU and 197 such workgroups leave 59 CUs without one.
 template <int G>
 struct Unit {
     static constexpr int NQ = G == 32 ? 2 : 4;          // 128-column blocks
@@ -595,11 +596,11 @@ __global__ __launch_bounds__(256) void q4_parts_kernel(Q4Args a) {
 // product of its own before the others, of bf16 parts, six MFMAs for 32 groups: per value and
 // group, with the sums read from LDS, it took as many instructions as the nibbles.
 //
-// Bound by a SIMD's two waves, whose MFMAs (30%), vector work (36%: nibbles, scales) and LDS
-// reads (37%) overlap only in part; setting them one beside the other by hand, operands a
-// group ahead, changed nothing (122 us and 124).  800 x 6144 x 4096 f32, group 64: 105 us, 384 TFLOP/s
-// and, with both parts of x, 768 of the 1174 that a large f16 product reaches; 800 x 50304 x 2048
-// 400 us, of bf16 rows 311.
+// Bound by a SIMD's two waves, whose MFMAs (35% of the time), vector work (37%: nibbles, scales) and LDS
+// reads (34%, no bank conflicts) overlap only in part; setting them one beside the other by hand,
+// operands a group ahead, changed nothing (122 us and 124).  800 x 6144 x 4096 f32, group 64: 107 us, 376
+// TFLOP/s and, with both parts of x, 753 of the 1174 that a large f16 product reaches; 800 x 50304 x 2048
+// 380 to 400 us (on different cards), of bf16 rows 294 to 311.
 template <int G, int NT, int MW, bool XB>
 __global__ __launch_bounds__(512, 4) void q4_many_kernel(Q4Args a) {
     constexpr int P = XB ? 1 : 2, kRecord = record_bytes(P), kStage = NT * kRecord, kSteps = G / 32, kWaves = 8;
@@ -836,23 +837,23 @@ int64_t matmul_q4_plan(Q4Args& a, int cus) {
         const int bytes = p * (unit / 32) * 64 * few_rows(flat ? 2 * a.tokens : a.tokens) + (groups + 1) * 64 * nt;
         // A tile's columns are shared by the waves of a workgroup, which need no second pass, as long as
         // staging x costs little: 4 tokens, all of whose columns fit the LDS at once; behind that by
-        // workgroups, each of which stages its share only (2048 x 2048: 1 token 5.4 us so, 7.8 by
-        // workgroups, 8 tokens 8.6 and 8.4; 6144 x 4096: 1 token 9.4 and 11.3, 4 bf16 ones 11.5 and
-        // 11.7, 4 f32 ones, whose columns do not fit, 13.7 and 11.6, 8 16.5 and 12.1).
+        // workgroups, each of which stages its share only (2048 x 2048: 1 token 5.3 us so, 7.5 by
+        // workgroups, 8 tokens 8.2 and 8.0; 6144 x 4096: 1 token 8.0 and 9.9, 4 bf16 ones 10.6 and
+        // 11.0, 4 f32 ones, whose columns do not fit, 12.4 and 10.5, 8 15.3 and 11.3).
         // Tiles for every wave that the CUs hold: waves of workgroups that share them evenly, one a CU,
         // where that is a wave of a SIMD less than the 16 that fit (2048 columns, f32: 33000 rows, 9 waves,
-        // 1 token 13.3 us, of 8 waves 16.5, 8 tokens 15.1, of 16 17.3; 50304 rows, 13 waves, 26 tokens 33.2,
-        // of 16 31.5; 100000, twice 13, 1 token 34.8, of 8 32.2).
+        // 1 token 11.8 us, of 8 waves 14.8, 8 tokens 14.3, of 16 16.5; 50304 rows, 13 waves, 26 tokens 31.9,
+        // of 16 30.5; 100000, twice 13, 1 token 28.6, of 8 26.4).
         const int rounds = (tiles + 16 * cus - 1) / (16 * cus), even = (tiles + rounds * cus - 1) / (rounds * cus);
         const bool apart = tiles > 8 * cus && even <= 12;
         if (a.tokens <= 4 && units * bytes <= kFewLds) {
             while (a.wave_split < 8 && 2 * a.wave_split <= units && tiles * a.wave_split * 2 <= 16 * cus) a.wave_split *= 2;
-            // (workgroups of 4 while there are few: 2048 x 2048, 1 token 5.5 us, of 8 waves 5.9)
+            // (workgroups of 4 while there are few: 2048 x 2048, 1 token 5.3 us, of 8 waves 5.6)
             if (a.wave_split <= 4 && tiles * a.wave_split < 8 * cus) a.waves = 4;
             if (apart) a.waves = std::max(8, even);
         } else {
             // (x is staged once for 16 waves where these still fill the card: 50304 x 2048, 16 f32 tokens
-            // 21.2 us, of 8 waves 24.7; 2048 x 2048 9.2, of 16 waves 11.5)
+            // 20.6 us, of 8 waves 23.9; 2048 x 2048 8.9, of 16 waves 10.9)
             a.waves = apart ? std::max(8, even) : tiles >= 8 * cus ? 16 : 8;
             a.split = std::max(1, std::min(units, cus / ((tiles + a.waves - 1) / a.waves)));
         }

@@ -72,8 +72,8 @@ __global__ __launch_bounds__(64 * W) void tree_plan_kernel(TreePlanArgs a) {
 //
 // Workgroup = (tree, 4 KB of a position through all planes, the layers' k and v).  Every one walks
 // for itself: the walk (a thread in LDS, a level at a time) takes less than a launch would.
-// 32 trees of 8 to 64, 32 layers of 8 heads of 128 in bf16: 12.5 us, 2.7 TB/s, half of a large
-// copy's rate; one tree, 16 layers: 5.9 us in a trace, the chain lengths - parents - walk - rows (7.4
+// 32 trees of 8 to 64, 32 layers of 8 heads of 128 in bf16: 12.4 us, 2.7 TB/s, half of a large
+// copy's rate; one tree, 16 layers: 5.9 us in a trace, the chain lengths - parents - walk - rows (7.6
 // as fast as the calls are made).
 __global__ __launch_bounds__(256) void tree_accept_kernel(TreeAcceptArgs a) {
     __shared__ int s_child[kTreeRows], s_drawn[kTreeRows], s_page[kTreeRows], s_path[kTreeRows], s_count;
